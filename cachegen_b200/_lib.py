@@ -15,6 +15,8 @@ CG_MAX_DECODE_JOBS = 40
 CG_MAX_ENCODE_LEVELS = 4
 CG_MAX_OFFSET_GROUPS = 96000
 CG_S_STREAM_OVERFLOW, CG_S_BAD_LENGTHS, CG_S_BAD_SYMBOL, CG_S_COUNT_OVERFLOW, CG_S_BAD_TABLE = 1, 2, 4, 8, 16
+CG_S_BAD_PAGE, CG_S_TIMEOUT = 32, 64
+CG_MAX_REQUESTS = 4096
 CG_TABLES_CDF, CG_TABLES_COUNTS, CG_TABLES_SPARSE = 0, 1, 2
 CG_LENGTHS_I32, CG_LENGTHS_U16 = 0, 1
 CG_E_CUDA = -8
@@ -72,6 +74,33 @@ class HostSegment(ctypes.Structure):
     _fields_ = [("host", ctypes.c_void_p), ("device", ctypes.c_void_p), ("bytes", ctypes.c_int64)]
 
 
+def _fields(kinds):
+    """Structure fields from (type, names, length or None) runs."""
+    return [(n, t * length if length else t) for t, names, length in kinds for n in names.split()]
+
+
+class RowsJob(ctypes.Structure):
+    """cg_rows_job"""
+    _fields_ = _fields([
+        (ctypes.c_void_p, "q q_out k v k_out pages_k pages_v positions slots turns status", None),
+        (ctypes.c_int64, "q_strides q_out_strides k_strides v_strides k_out_strides", 3),
+        (ctypes.c_int64, "pages_k_strides pages_v_strides", 4),
+        (ctypes.c_int64, "num_pages pos_layer", None),
+        (ctypes.c_int32, "dtype nlayers ntokens q_heads heads head_size rotary_dims interleaved inverse page_size "
+                         "wide_positions wide_slots", None)])
+
+
+class AttentionJob(ctypes.Structure):
+    """cg_attention_job"""
+    _fields_ = _fields([
+        (ctypes.c_void_p, "q pages_k pages_v out lse table kv_lens q_starts workspace status", None),
+        (ctypes.c_int64, "workspace_bytes table_row num_pages", None),
+        (ctypes.c_int64, "q_strides out_strides", 2),
+        (ctypes.c_int64, "pages_k_strides pages_v_strides", 3),
+        (ctypes.c_int32, "dtype nrequests nrows q_heads heads head_size page_size table_width causal window max_q", None),
+        (ctypes.c_float, "scale", None)])
+
+
 EXPORTS = [
     "cg_host_upload", "cg_host_stage", "cg_host_stage_ahead", "cg_host_stage_send", "cg_host_stage_end", "cg_host_download", "cg_decode_kv",
     "cg_stream_sizes", "cg_decode_packed", "cg_wait_word",
@@ -82,6 +111,7 @@ EXPORTS = [
     "cg_quantize_cdf", "cg_pack_sparse_tables", "cg_encode_chunk", "cg_compact_streams",
     "cg_decode_offsets", "cg_decode_dequant", "cg_decode_dequant_static",
     "cg_quantize_cdf_delta", "cg_decode_dequant_delta",
+    "cg_rotary", "cg_append_paged", "cg_gather_paged", "cg_paged_attention_workspace", "cg_paged_attention",
 ]
 CG_STATIC_OFFSET_ENTRIES = 131072
 
@@ -141,11 +171,16 @@ def lib():
     L.cg_host_stage_send.argtypes = [p, ctypes.POINTER(HostSegment), i, p]
     L.cg_host_stage_end.argtypes = [p]
     L.cg_host_download.argtypes = [ctypes.POINTER(HostSegment), i, p, i64, i, p]
+    rows, attention = ctypes.POINTER(RowsJob), ctypes.POINTER(AttentionJob)
+    for name in ("cg_rotary", "cg_append_paged", "cg_gather_paged"):
+        getattr(L, name).argtypes = [rows, p]
+    L.cg_paged_attention_workspace.argtypes = [attention]
+    L.cg_paged_attention.argtypes = [attention, p]
     for name in EXPORTS:
         fn = getattr(L, name)
         if name not in ("cg_version", "cg_status_string", "cg_last_cuda_error"):
             fn.restype = i
-    L.cg_encode_kv_workspace.restype = i64
+    L.cg_encode_kv_workspace.restype = L.cg_paged_attention_workspace.restype = i64
     _lib = L
     return L
 
@@ -219,4 +254,8 @@ def status_text(bits):
         names.append("a histogram count does not fit the byte-count tables")
     if bits & CG_S_BAD_TABLE:
         names.append("sparse table offsets reach past the table set")
+    if bits & CG_S_BAD_PAGE:
+        names.append("a slot, page or length does not fit the paged cache")
+    if bits & CG_S_TIMEOUT:
+        names.append("a kernel gave up waiting; its output is not valid")
     return "; ".join(names) if names else "ok"

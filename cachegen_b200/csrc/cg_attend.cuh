@@ -1,0 +1,295 @@
+// What the two attention kernels share: how the work of a batch is divided, and what is left where a tile is divided.
+//
+// A tile is up to M query rows of one request that read the same key/value head: row r of a request is token r / group, query head
+// r % group of the head's group, so that a key that is read serves all of them.  A tile's work is counted in units, blocks of BK keys
+// that one of its rows sees (one unit at least).  All units of a call stand in one line, (request, head, tile, block), and every
+// CTA takes an equal run of it: whatever the batch's lengths, the CTAs end together.  A tile that two CTAs or more share leaves
+// a maximum, a sum and a product a row from each of them in the workspace, and combine_kernel joins those.  Lengths stay on the
+// GPU, so that one captured graph serves all of them: each CTA works out its own run.
+#pragma once
+
+#include "cg_common.cuh"
+
+namespace cg {
+
+struct AttendArgs {
+    const char *q, *k, *v;
+    char *out;
+    float *lse;
+    const int32_t *table, *kv_lens, *q_starts;
+    char *parts;    // [ctas][2] rows of sums, see part_bytes
+    int4 *joins;    // [ctas]: request, head, tile of the divided tile that begins in this CTA, CTAs that share it (0: none)
+    int32_t *status;
+    int64_t q_token, q_head, out_token, out_head, k_page, k_token, k_head, v_page, v_token, v_head;  // bytes
+    int64_t table_row, num_pages;
+    int32_t nrequests, nrows, q_heads, heads, group, head_size, page_size, table_width, causal, window;
+    float scale;    // of the scores, times log2(e)
+};
+
+constexpr float kNegInf = -INFINITY;
+
+// bytes of one CTA's share of a tile: float sums[M][DP], then float2 (maximum, sum of weights)[M]
+__host__ __device__ constexpr int64_t part_bytes(int M, int DP) { return static_cast<int64_t>(M) * (DP * 4 + 8); }
+
+struct Lengths {
+    int first, n, kv;  // first row of q, rows, keys
+};
+__device__ __forceinline__ Lengths lengths_of(const AttendArgs &a, int b, bool report = false) {
+    Lengths r;
+    int last;
+    r.first = b, last = b + 1;
+    if (a.q_starts) r.first = __ldg(a.q_starts + b), last = __ldg(a.q_starts + b + 1);
+    r.kv = __ldg(a.kv_lens + b);
+    const int64_t room = static_cast<int64_t>(a.table_width) * a.page_size;
+    const bool bad = r.first < 0 || last < r.first || last > a.nrows || r.kv < 0 || r.kv > room;
+    if (bad) {
+        r.first = min(max(r.first, 0), a.nrows);
+        last = min(max(last, r.first), a.nrows);
+        r.kv = r.kv < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(r.kv), room));
+        if (report && a.status) atomicOr(a.status, CG_S_BAD_PAGE);
+    }
+    r.n = last - r.first;
+    return r;
+}
+
+// keys [lo, hi) that token i of n sees
+__device__ __forceinline__ int first_key(const AttendArgs &a, const Lengths &r, int i) {
+    return a.window > 0 ? max(0, r.kv - r.n + i - a.window + 1) : 0;
+}
+__device__ __forceinline__ int last_key(const AttendArgs &a, const Lengths &r, int i) {
+    return a.causal ? min(r.kv, max(0, r.kv - r.n + i + 1)) : r.kv;
+}
+
+struct Tile {
+    int lo, hi;          // keys that a row of the tile sees
+    int block0, units;   // first block of BK keys, blocks
+};
+template <int M, int BK> __device__ __forceinline__ Tile tile_of(const AttendArgs &a, const Lengths &r, int t) {
+    const int last = min(r.n * a.group, (t + 1) * M) - 1;
+    Tile x;
+    x.hi = last_key(a, r, last / a.group);
+    x.lo = min(first_key(a, r, t * M / a.group), x.hi);
+    x.block0 = x.lo / BK;
+    x.units = max(1, (x.hi + BK - 1) / BK - x.block0);
+    return x;
+}
+template <int M> __device__ __forceinline__ int tiles_of(const AttendArgs &a, const Lengths &r) { return (r.n * a.group + M - 1) / M; }
+
+// The part of a tile that a CTA has.
+struct Piece {
+    Lengths r;
+    Tile tile;
+    int request, head, t;
+    int begin, end;      // blocks of BK keys
+    bool whole, starts;  // the tile is all here; its first block is here
+    int sharers;         // CTAs that share a tile that starts here
+};
+
+// A CTA's run through the line of units.  init is called by all threads of the block, with room in shared memory for
+// nrequests + 1 numbers; next by any of them, as often, all with the same result.
+template <int M, int BK> struct Run {
+    int64_t at, to, total;
+    int ctas;
+    int b, h, t, tiles, skip;
+    Lengths r;
+
+    // by requests a thread (TILES false: most have one tile) or by requests a warp, tiles a lane
+    template <int THREADS, bool MANY_TILES>
+    __device__ __forceinline__ void init(const AttendArgs &a, int64_t *before) {
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+        if (MANY_TILES) {
+            for (int i = warp; i < a.nrequests; i += THREADS / 32) {
+                const Lengths x = lengths_of(a, i, blockIdx.x == 0 && lane == 0);
+                const int n = tiles_of<M>(a, x);
+                int units = 0;
+                for (int k = lane; k < n; k += 32) units += tile_of<M, BK>(a, x, k).units;
+                units = __reduce_add_sync(0xffffffffu, units);
+                if (lane == 0) before[i + 1] = static_cast<int64_t>(units) * a.heads;
+            }
+        } else {
+            for (int i = tid; i < a.nrequests; i += THREADS) {
+                const Lengths x = lengths_of(a, i, blockIdx.x == 0);
+                const int n = tiles_of<M>(a, x);
+                int units = 0;
+                for (int k = 0; k < n; ++k) units += tile_of<M, BK>(a, x, k).units;
+                before[i + 1] = static_cast<int64_t>(units) * a.heads;
+            }
+        }
+        __syncthreads();
+        if (warp == 0) {
+            int64_t carry = 0;
+            for (int i = 0; i < a.nrequests; i += 32) {
+                int64_t s = i + lane < a.nrequests ? before[i + lane + 1] : 0;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int64_t o = __shfl_up_sync(0xffffffffu, s, d);
+                    if (lane >= d) s += o;
+                }
+                s += carry;
+                if (i + lane < a.nrequests) before[i + lane + 1] = s;
+                carry = __shfl_sync(0xffffffffu, s, 31);
+            }
+            if (lane == 0) before[0] = 0;
+        }
+        __syncthreads();
+        total = before[a.nrequests];
+        ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+        const int c = blockIdx.x;
+        at = to = 0;
+        if (c < ctas) {
+            at = total * c / ctas;
+            to = total * (c + 1) / ctas;
+            int lo = 0, hi = a.nrequests - 1;  // the last request that begins at or before `at` and has rows
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (before[mid] <= at) lo = mid;
+                else hi = mid - 1;
+            }
+            b = lo;
+            r = lengths_of(a, b);
+            tiles = tiles_of<M>(a, r);
+            const int64_t per_head = (before[b + 1] - before[b]) / a.heads;
+            int64_t rest = at - before[b];
+            h = static_cast<int>(rest / per_head);
+            rest -= h * per_head;
+            for (t = 0;; ++t) {
+                const int u = tile_of<M, BK>(a, r, t).units;
+                if (rest < u) break;
+                rest -= u;
+            }
+            skip = static_cast<int>(rest);
+        }
+        __syncthreads();  // the numbers' memory is free again
+    }
+
+    __device__ __forceinline__ bool next(const AttendArgs &a, Piece &p) {
+        if (at >= to) return false;
+        while (t >= tiles) {
+            t = 0;
+            if (++h >= a.heads) {
+                h = 0;
+                do {
+                    r = lengths_of(a, ++b);
+                    tiles = tiles_of<M>(a, r);
+                } while (tiles == 0);
+            }
+        }
+        p.r = r;
+        p.request = b, p.head = h, p.t = t;
+        p.tile = tile_of<M, BK>(a, r, t);
+        const int left = p.tile.units - skip, take = static_cast<int>(min(static_cast<int64_t>(left), to - at));
+        p.begin = p.tile.block0 + skip;
+        p.end = p.begin + take;
+        p.starts = skip == 0;
+        p.whole = p.starts && take == left;
+        p.sharers = 0;
+        if (p.starts && !p.whole) p.sharers = static_cast<int>(((at + left) * ctas - 1) / total) - static_cast<int>(blockIdx.x) + 1;
+        at += take;
+        skip = 0;
+        ++t;
+        return true;
+    }
+};
+
+// Where a page of a request lies, or -1.
+__device__ __forceinline__ int page_of(const AttendArgs &a, int b, int index) {
+    const int page = __ldg(a.table + b * a.table_row + index);
+    if (page >= 0 && page < a.num_pages) return page;
+    if (a.status) atomicOr(a.status, CG_S_BAD_PAGE);
+    return -1;
+}
+
+// 2^x to 2 units of the last place (0 for -infinity); a weight that is too small for a normal number is 0
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// One row over keys [k0, k1) by a warp, straight from memory: for tiles in which a key that some rows do not see has values that
+// are not finite, since a weight of zero does not keep those out of a product.  sums[i] is value lane + 32 i of the head.
+template <int DT, int DP>
+__device__ __noinline__ void slow_row(const AttendArgs &a, const Lengths &r, int b, int head, int row, int k0, int k1,
+                                      float (&sums)[DP / 32], float &top, float &total) {
+    const int lane = threadIdx.x & 31, token = row / a.group;
+    const char *q = a.q + (r.first + token) * a.q_token + (head * a.group + row % a.group) * a.q_head;
+    float x[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+        const int d = lane + 32 * i;
+        x[i] = d < a.head_size ? Half16<DT>::to_float(reinterpret_cast<const uint16_t *>(q)[d]) : 0.0f;
+        sums[i] = 0.0f;
+    }
+    top = kNegInf, total = 0.0f;
+    k0 = max(k0, first_key(a, r, token)), k1 = min(k1, last_key(a, r, token));
+    for (int j = k0; j < k1; ++j) {
+        const int page = page_of(a, b, j / a.page_size), in_page = j % a.page_size;
+        const char *k = a.k + page * a.k_page + in_page * a.k_token + head * a.k_head;
+        const char *v = a.v + page * a.v_page + in_page * a.v_token + head * a.v_head;
+        float s = 0.0f, y[DP / 32];
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+            const int d = lane + 32 * i;
+            const bool there = d < a.head_size && page >= 0;
+            s += there ? x[i] * Half16<DT>::to_float(reinterpret_cast<const uint16_t *>(k)[d]) : 0.0f;
+            y[i] = there ? Half16<DT>::to_float(reinterpret_cast<const uint16_t *>(v)[d]) : 0.0f;
+        }
+        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        s *= a.scale;
+        const float now = fmaxf(top, s), base = now == kNegInf ? 0.0f : now;
+        const float keep = exp2_approx(top - base), w = exp2_approx(s - base);
+        total = total * keep + w;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) sums[i] = sums[i] * keep + w * y[i];
+        top = now;
+    }
+}
+
+// Joins what the CTAs of a divided tile have left.  Block (i, j): rows j * ROWS .. of the tile that begins in CTA i.  COLUMNS: sums are stored
+// [DP / 4][M][4], as a kernel with a row a thread writes them side by side; else [M][DP].
+template <int DT, int M, int DP, bool COLUMNS>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttendArgs a) {
+    constexpr int kRows = 256 / (DP / 4);
+    wait_for_launch_before();
+    const int c = blockIdx.x;
+    const int4 join = __ldcg(a.joins + c);
+    if (join.w == 0) return;
+    const int tid = threadIdx.x;
+    const int row = blockIdx.y * kRows + (COLUMNS ? tid % kRows : tid / (DP / 4)), col = 4 * (COLUMNS ? tid / kRows : tid % (DP / 4));
+    const Lengths r = lengths_of(a, join.x);
+    const int64_t at = static_cast<int64_t>(join.z) * M + row;
+    if (at >= static_cast<int64_t>(r.n) * a.group) return;
+    const char *part = a.parts + (2 * c + 1) * part_bytes(M, DP);
+    float top = kNegInf;
+    for (int i = 0; i < join.w; ++i) {
+        const char *p = i ? a.parts + 2 * (c + i) * part_bytes(M, DP) : part;
+        top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(p + M * DP * 4) + row).x);
+    }
+    const float base = top == kNegInf ? 0.0f : top;
+    float total = 0.0f;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = 0; i < join.w; ++i) {
+        const char *p = i ? a.parts + 2 * (c + i) * part_bytes(M, DP) : part;
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + M * DP * 4) + row);
+        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p) + (COLUMNS ? col / 4 * M + row : row * (DP / 4) + col / 4));
+        const float w = exp2_approx(ml.x - base);
+        total += w * ml.y;
+        sum.x += w * x.x, sum.y += w * x.y, sum.z += w * x.z, sum.w += w * x.w;
+    }
+    const int token = static_cast<int>(at / a.group), head = join.y * a.group + static_cast<int>(at % a.group);
+    const bool sees = last_key(a, r, token) > first_key(a, r, token);
+    const float inv = sees ? 1.0f / total : 0.0f;
+    if (col < a.head_size) {
+        uint16_t h[4] = {Half16<DT>::from_float(sees ? sum.x * inv : 0.0f), Half16<DT>::from_float(sees ? sum.y * inv : 0.0f),
+                         Half16<DT>::from_float(sees ? sum.z * inv : 0.0f), Half16<DT>::from_float(sees ? sum.w * inv : 0.0f)};
+        *reinterpret_cast<uint2 *>(a.out + (r.first + token) * a.out_token + head * a.out_head + 2 * col) = *reinterpret_cast<uint2 *>(h);
+    }
+    if (a.lse && col == 0)
+        a.lse[static_cast<int64_t>(r.first + token) * a.q_heads + head] = sees ? (base + log2f(total)) * 0.693147180559945f : kNegInf;
+}
+
+// cg_attend_tiles.cu
+int launch_attend_tiles(const AttendArgs &a, int dtype, int ctas, cudaStream_t st);
+constexpr int kTileRows = 256, kTileKeys = 128;
+
+}  // namespace cg

@@ -96,6 +96,8 @@ extern "C" {
 #define CG_S_BAD_SYMBOL 4      /* a symbol outside [0, Lp-2] was met while encoding */
 #define CG_S_COUNT_OVERFLOW 8  /* a histogram count above 255: the byte-count tables are not usable */
 #define CG_S_BAD_TABLE 16     /* CG_TABLES_SPARSE offsets reach past the table set (read as zero counts) */
+#define CG_S_BAD_PAGE 32      /* a slot or page outside the cache, or lengths that its tables have no room for */
+#define CG_S_TIMEOUT 64       /* a kernel gave up waiting for its own copies or products; its output is not valid */
 
 /*
  * Sizes in bytes of the buffers a caller allocates for the fused calls, for one chunk of
@@ -477,6 +479,78 @@ int cg_host_stage_ahead(const void *host, int64_t bytes, void *staging, int64_t 
                         void **handle_host);
 int cg_host_stage_send(void *handle_host, const cg_host_segment *segments_host, int nsegments, void *stream);
 int cg_host_stage_end(void *handle_host);
+
+/* ------------------------------------------------------------------------------------------
+ * a paged KV cache: where decoded contexts are used (no counterpart in the reference, whose engine copies blobs)
+ * ------------------------------------------------------------------------------------------ */
+
+/*
+ * Rows of 16-bit values [nlayers, ntokens, heads, head_size], innermost stride 1, other strides in elements
+ * {layer, token, head}; pages [nlayers, num_pages, page_size, heads, head_size] with strides {layer, page, token, head}.
+ * Slot s is token s % page_size of page s / page_size.  A token with slot -1 is padding: nothing of it, its query
+ * included, is read or written.  Any other slot outside the cache is treated the same way and raises CG_S_BAD_PAGE.  A slot
+ * that two tokens of a call name holds one or the other afterwards, or pieces of both.
+ *
+ * Rotation of the first rotary_dims (even, 0: none) values of a head at position p: pair i, i < rotary_dims / 2, turns by
+ * p * turns[i] / 2^64 whole turns; the pair is values i and i + rotary_dims / 2, or 2i and 2i + 1 when `interleaved`.
+ * positions: int64 (wide_positions) or int32 [ntokens], any sign; pos_layer != 0: [nlayers, ntokens], layers pos_layer apart
+ * (cg_rotary only).  Products are 32-bit floats, each value rounded once.  Rows that are not rotated are copied bit for bit.
+ *
+ * cg_rotary: k to k_out, which is k itself or does not overlap it; inverse: turned back.
+ * cg_append_paged: keys rotated and values to the slots of their tokens; q (nlayers 1, q_heads 0: none) rotated to q_out.
+ * cg_gather_paged: the slots' values to v, and the keys turned back to k (inverse is implied).
+ * head_size <= 512, 2 * heads + q_heads <= 65,536.  ntokens or nlayers 0: nothing is done.
+ */
+typedef struct cg_rows_job {
+    const void *q;
+    void *q_out, *k, *v, *k_out, *pages_k, *pages_v;
+    const void *positions, *slots;
+    const uint64_t *turns;
+    int32_t *status; /* may be NULL */
+    int64_t q_strides[3], q_out_strides[3], k_strides[3], v_strides[3], k_out_strides[3];
+    int64_t pages_k_strides[4], pages_v_strides[4];
+    int64_t num_pages, pos_layer;
+    int32_t dtype, nlayers, ntokens, q_heads, heads, head_size, rotary_dims, interleaved, inverse, page_size;
+    int32_t wide_positions, wide_slots;
+} cg_rows_job;
+int cg_rotary(const cg_rows_job *job_host, void *stream);
+int cg_append_paged(const cg_rows_job *job_host, void *stream);
+int cg_gather_paged(const cg_rows_job *job_host, void *stream);
+
+/*
+ * Attention of the newest tokens of nrequests requests over their pages.
+ *
+ * q, out: 16-bit [nrows, q_heads, head_size], strides {token, head}; rows q_starts[b] .. q_starts[b + 1] - 1 are the newest
+ * tokens of request b (int32 [nrequests + 1], rising from 0 or more; NULL: one row a request).  Rows in no request are left as they
+ * were.  Query head h uses key/value head h / (q_heads / heads).  pages_k, pages_v: strides {page, token, head}, multiples of 8,
+ * addresses of 16 bytes (q and out too).  table: int32 [nrequests, table_width], rows table_row apart: the pages of a request in order;
+ * kv_lens: int32 [nrequests], its tokens in the cache, the newest included.  Entries of the table behind those are not read.
+ *
+ * Row i of n, at place p = kv - n + i, sees the keys at j <= p (causal; else all kv), and with window > 0 only j > p - window:
+ *     s_j = scale * <q_i, k_j>,  out_i = sum_j exp(s_j) v_j / sum_j exp(s_j),  lse_i = log sum_j exp(s_j)
+ * in 32-bit floats but for the weights of the second product, rounded to the cache's type.  A row that sees no key gets
+ * 0 and -infinity.  What a row does not see does not enter its result, whatever values stand there.
+ * lse: float32 [nrows, q_heads] or NULL.  max_q: the most rows of a request, or 0; it only chooses between two kernels.
+ *
+ * A page outside the cache counts as zeros, lengths that do not fit the table or the rows are cut; both raise CG_S_BAD_PAGE.
+ * head_size: a multiple of 8 up to 128; nrequests <= CG_MAX_REQUESTS.  workspace: cg_paged_attention_workspace(job) bytes of device memory
+ * (16-byte aligned; 0: none), which calls on one stream may share.  nrows or nrequests 0: nothing is done.
+ */
+#define CG_MAX_REQUESTS 4096
+typedef struct cg_attention_job {
+    const void *q, *pages_k, *pages_v;
+    void *out;
+    float *lse;
+    const int32_t *table, *kv_lens, *q_starts;
+    void *workspace;
+    int32_t *status; /* may be NULL */
+    int64_t workspace_bytes, table_row, num_pages;
+    int64_t q_strides[2], out_strides[2], pages_k_strides[3], pages_v_strides[3];
+    int32_t dtype, nrequests, nrows, q_heads, heads, head_size, page_size, table_width, causal, window, max_q;
+    float scale;
+} cg_attention_job;
+int64_t cg_paged_attention_workspace(const cg_attention_job *job_host); /* bytes, or CG_E_* */
+int cg_paged_attention(const cg_attention_job *job_host, void *stream);
 
 #ifdef __cplusplus
 }
