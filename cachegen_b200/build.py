@@ -14,7 +14,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libcachegen_b200.so")
 SOURCES = ["cg_api.cu", "cg_quant.cu", "cg_tables.cu", "cg_encode.cu", "cg_store.cu", "cg_decode.cu", "cg_host.cu", "cg_paged.cu",
-           "cg_attend.cu"]
+           "cg_attend.cu", "cg_attend_tiles.cu"]
 HEADERS = [os.path.join(CSRC, "cg_common.cuh"), os.path.join(CSRC, "cg_coder.cuh"), os.path.join(CSRC, "cg_hostcopy.h"),
            os.path.join(CSRC, "cg_attend.cuh"),
            os.path.join(PKG, "..", "include", "cachegen_b200.h")]

@@ -290,8 +290,7 @@ int plan_of(const cg_attention_job &j, Plan &p) {
     if (j.nrequests > CG_MAX_REQUESTS) return CG_E_CAPACITY;
     const int64_t group = j.q_heads / j.heads;
     const int most = !j.q_starts ? 1 : j.max_q > 0 ? j.max_q : j.nrows;
-    (void)most;
-    p.tiles = false;
+    p.tiles = most * group > kRowsM && j.scale > 0.0f;  // (its maxima are those of unscaled scores)
     p.dp = j.head_size > 64 ? 128 : 64;
     const int M = p.tiles ? kTileRows : kRowsM, BK = p.tiles ? kTileKeys : kRowsBK;
     const int64_t keys = static_cast<int64_t>(j.table_width) * j.page_size;
@@ -345,6 +344,7 @@ extern "C" int cg_paged_attention(const cg_attention_job *job, void *stream) {
     a.head_size = j.head_size, a.page_size = j.page_size, a.table_width = j.table_width, a.causal = j.causal, a.window = j.window;
     a.scale = j.scale * 1.44269504088896340736f;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p.tiles) return launch_attend_tiles(a, j.dtype, p.ctas, st);
     if (p.dp == 64) return j.dtype == CG_F16 ? launch_attend_rows<CG_F16, 64>(a, p.ctas, st) : launch_attend_rows<CG_BF16, 64>(a, p.ctas, st);
     return j.dtype == CG_F16 ? launch_attend_rows<CG_F16, 128>(a, p.ctas, st) : launch_attend_rows<CG_BF16, 128>(a, p.ctas, st);
 }

@@ -1,0 +1,491 @@
+// Attention over a paged KV cache for many query rows a key/value head: chunks of new tokens and whole prompts.
+//
+// Here the products bound the kernel, so they go to the tensor cores' own memory: a CTA has up to 256 query rows, two halves of 128,
+// whose scores S and results O are accumulators in tensor memory (128 columns each: all 512), and whose weights P overwrite
+// the scores they came from.  While one half's softmax works on its scores, the tensor cores work on the other's:
+//
+//     warps 0-3, 4-7   softmax of one half each: a thread has a row, so there are no exchanges for maxima and sums
+//     warps 8-11       copies of Q, K and V to shared memory, 16 bytes at a time, through the page table
+//     warp 12          one thread issues the products: S = Q K^T from shared memory, O += P V with P from tensor memory
+//
+// A row's maximum is only raised when a score is more than 2^8 times beyond it in weight: weights up to 2^8 lose nothing as 16-bit or
+// 32-bit floats, and O, which has to be multiplied in tensor memory for every raise, is then left alone in nearly every block.
+//
+// Copies are asynchronous 16-byte copies and not TMA: pages may have any size and stride, a block's last keys may lie in the middle of a
+// page, and what lies behind them has to arrive as zeros (a weight of zero does not keep NaN out of a product).
+#include "cg_attend.cuh"
+
+namespace cg {
+namespace {
+
+constexpr int kTileThreads = 512;
+constexpr int kTileStages128 = 5;  // K or V tiles of 128 keys x 128 values
+constexpr uint64_t kGiveUpNs = 10ull * 1000 * 1000 * 1000;  // a wait takes microseconds, or the length of a slow row
+
+// ---- barriers in shared memory --------------------------------------------------------------
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done;
+}
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+// Whether the phase ended.  If it does not within kGiveUpNs, or another wait of the block gave up, the block is told to end.
+__device__ __forceinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
+    const uint64_t start = now_ns();
+    while (true) {
+        for (int i = 0; i < 256; ++i)
+            if (bar_try(bar, parity)) return true;
+        if (*failed) return false;
+        if (now_ns() - start > kGiveUpNs) {
+            *failed = 1;
+            if (status) atomicOr(status, CG_S_TIMEOUT);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
+    for (int i = 0; i < 16; ++i)
+        if (bar_try(bar, parity)) return true;
+    return bar_wait_long(bar, parity, failed, status);
+}
+// the same for a whole warp, with one result
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
+    return __all_sync(0xffffffffu, bar_wait(bar, parity, failed, status));
+}
+
+// ---- tensor memory and products ---------------------------------------------------------------
+__device__ __forceinline__ void tmem_alloc(uint32_t dst, int columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, int columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"(add ? 1 : 0) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+                 "r"(add ? 1 : 0) : "memory");
+}
+// an operand in shared memory, rows (of queries, of keys) of 64 values that are swizzled in groups of 8 rows, 1024 bytes; `panel`: bytes
+// from 64 values of a row to the next 64, where they are the operand's outer axis
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t panel) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | static_cast<uint64_t>((panel >> 4) & 0x3FFF) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
+           1ull << 46 | 2ull << 61;
+}
+// 32-bit sums of products of 16-bit values, 128 rows, n columns; b_outer: the second operand's rows are the summed axis
+__host__ __device__ constexpr uint32_t product(int dtype, int n, bool b_outer) {
+    const uint32_t type = dtype == CG_BF16 ? 1u : 0u;
+    return 1u << 4 | type << 7 | type << 10 | (b_outer ? 1u << 16 : 0u) | static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
+}
+
+__device__ __forceinline__ void tmem_load32(uint32_t (&x)[32], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]),
+                   "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]),
+                   "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]),
+                   "=r"(x[31]) : "r"(at));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&x)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::"r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]),
+                   "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15]), "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&x)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+                 ::"r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]),
+                   "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15]), "r"(x[16]), "r"(x[17]), "r"(x[18]), "r"(x[19]), "r"(x[20]),
+                   "r"(x[21]), "r"(x[22]), "r"(x[23]), "r"(x[24]), "r"(x[25]), "r"(x[26]), "r"(x[27]), "r"(x[28]), "r"(x[29]), "r"(x[30]),
+                   "r"(x[31]), "r"(at) : "memory");
+}
+// (the registers are named so that nothing reads them in front of the wait)
+__device__ __forceinline__ void tmem_load_wait(uint32_t (&x)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), "+r"(x[9]), "+r"(x[10]),
+                   "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15]), "+r"(x[16]), "+r"(x[17]), "+r"(x[18]), "+r"(x[19]), "+r"(x[20]),
+                   "+r"(x[21]), "+r"(x[22]), "+r"(x[23]), "+r"(x[24]), "+r"(x[25]), "+r"(x[26]), "+r"(x[27]), "+r"(x[28]), "+r"(x[29]), "+r"(x[30]),
+                   "+r"(x[31]) :: "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- shared memory ------------------------------------------------------------------------------
+// Q [2 halves][DP / 64 panels][128 rows][128 bytes], then the ring of K and V tiles [DP / 64][128 keys][128 bytes]; the 16-byte piece p of a
+// row lies at p ^ row % 8, which is the swizzle that the products expect.
+template <int DP> constexpr int kTileBytes = 128 * DP * 2;
+template <int DP> constexpr int kTileStages = kTileStages128 * 128 / DP;
+template <int DP> constexpr int kBarsAt = (2 + kTileStages<DP>)*kTileBytes<DP>;
+template <int DP> constexpr int kTilesSmem = kBarsAt<DP> + 256 + 1024;  // and what it takes to begin at a multiple of 1024
+enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 2, kOFull = kPFull + 2, kKvFull = kOFull + 2 };  // two each of S, P and O
+
+template <int DT, int DP>
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __grid_constant__ AttendArgs a) {
+    extern __shared__ unsigned char raw[];
+    constexpr int kStages = kTileStages<DP>, kPieces = DP / 8, kRowsAtOnce = 32 / kPieces;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+    unsigned char *mem = raw + (base - smem_addr(raw));
+    const uint32_t tiles_at = base + 2 * kTileBytes<DP>, bars = base + kBarsAt<DP>;
+    const auto bar = [&](int i) { return bars + 8 * i; };
+    const auto full = [&](int s) { return bar(kKvFull + s); };
+    const auto empty = [&](int s) { return bar(kKvFull + kStages + s); };
+    static_assert(8 * (kKvFull + 2 * kStages) <= 240, "room for the barriers");
+    volatile int *words = reinterpret_cast<volatile int *>(mem + kBarsAt<DP> + 240);  // tensor memory, failed, odd[2]
+    volatile int *failed = words + 1;
+
+    Run<kTileRows, kTileKeys> run;
+    run.template init<kTileThreads, true>(a, reinterpret_cast<int64_t *>(mem));
+    let_next_launch_start();
+    if (tid == 0) {
+        bar_init(bar(kQFull), 4);
+        bar_init(bar(kQEmpty), 1);
+        for (int i = 0; i < 2; ++i) {
+            bar_init(bar(kSFull + i), 1);
+            bar_init(bar(kPFull + i), 4);
+            bar_init(bar(kOFull + i), 1);
+            words[2 + i] = 0;
+        }
+        for (int s = 0; s < kStages; ++s) bar_init(full(s), 4), bar_init(empty(s), 1);
+        *failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) tmem_alloc(base + kBarsAt<DP> + 240, 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = words[0];
+    // columns: S (and P) of the halves, then O
+    const auto s_at = [&](int half) { return tmem + 128 * half; };
+    const auto o_at = [&](int half) { return tmem + 256 + 128 * half; };
+    int4 join = make_int4(0, 0, 0, 0);
+    Piece p;
+
+    if (warp < 8) {
+        // ================================================================ softmax: a row a thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");  // 256 threads of 168 and 256 of 88 registers: the 512 x 128 of the launch
+        const int half = warp >> 2, in_half = tid & 127;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_mine = s_at(half) + lanes, o_mine = o_at(half) + lanes;
+        uint32_t s_phase = 0, o_phase = 0;
+        int tile_count = 0, pieces = 0;  // K and V tiles so far, and pieces: the word `odd` names the last piece that it was set in
+        bool ok = true;
+        while (ok && run.next(a, p)) {
+            const Lengths r = p.r;
+            const int blocks = p.end - p.begin, row0 = p.t * kTileRows, rows = min(kTileRows, r.n * a.group - row0);
+            const int row = half * 128 + in_half, first_tile = tile_count;
+            tile_count += 2 * blocks;
+            ++pieces;
+            if (p.sharers) join = make_int4(p.request, p.head, p.t, p.sharers);
+            if (half * 128 >= rows) continue;
+            const bool there = row < rows;
+            const int token = there ? (row0 + row) / a.group : 0, head = p.head * a.group + (there ? (row0 + row) % a.group : 0);
+            // (rows behind the last see everything: they ask for no masks)
+            const int lo = there ? first_key(a, r, token) : 0, hi = there ? last_key(a, r, token) : INT32_MAX;
+            const int half_lo = first_key(a, r, (row0 + min(rows, half * 128 + 128) - 1) / a.group), half_hi = last_key(a, r, (row0 + half * 128) / a.group);
+            float m = kNegInf, l = 0.0f;
+            for (int j = 0; j < blocks; ++j) {
+                const int key = (p.begin + j) * kTileKeys;
+                ok = warp_wait(bar(kSFull + half), s_phase, failed, a.status);
+                s_phase ^= 1;
+                if (!ok) break;
+                fence_after();
+                const bool masked = key < half_lo || key + kTileKeys > half_hi;  // for one of the half's rows
+                float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+                // the scores are read twice, for the maximum and for the weights: 128 of them would not fit beside the rest
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t x[32];
+                    tmem_load32(x, s_mine + 32 * c);
+                    tmem_load_wait(x);
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            top[i & 3] = fmaxf(top[i & 3], key + 32 * c + i >= lo && key + 32 * c + i < hi ? __uint_as_float(x[i]) : kNegInf);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
+                    }
+                }
+                if (masked) {
+                    // values of keys that some rows do not see: are they all finite?
+                    const int t = first_tile + 2 * j + 1;
+                    ok = warp_wait(full(t % kStages), (t / kStages) & 1, failed, a.status);
+                    if (!ok) break;
+                    const unsigned char *v = mem + (2 + t % kStages) * kTileBytes<DP>;
+                    bool odd = false;
+                    constexpr uint32_t e = DT == CG_F16 ? 0x7C00u : 0x7F80u;
+                    for (int i = in_half; i < kTileBytes<DP> / 16; i += 128) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(v + 16 * i);
+                        for (const uint32_t y : {w.x, w.y, w.z, w.w}) odd = odd || (y & e) == e || ((y >> 16) & e) == e;
+                    }
+                    if (odd) words[2 + half] = pieces;
+                }
+                const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale;
+                const bool raise = high > m + 8.0f || (m == kNegInf && high > m);
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float keep = raise ? (m == kNegInf ? 0.0f : exp2_approx(m - high)) : 1.0f;
+                    if (raise) m = high;
+                    l *= keep;
+                    if (j > 0) {  // the products of the block before are done: this block's scores came behind them
+                        uint32_t y[32];
+#pragma unroll
+                        for (int c = 0; c < DP / 32; ++c) {
+                            tmem_load32(y, o_mine + 32 * c);
+                            tmem_load_wait(y);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * keep);
+                            tmem_store32(o_mine + 32 * c, y);
+                        }
+                    }
+                }
+                const float down = m == kNegInf ? 0.0f : -m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {  // (weights take half the columns of the scores that they come from: these have been read)
+                    uint32_t x[32], w[16];
+                    tmem_load32(x, s_mine + 32 * c);
+                    tmem_load_wait(x);
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (key + 32 * c + i < lo || key + 32 * c + i >= hi) x[i] = __float_as_uint(kNegInf);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float w0 = exp2_approx(fmaf(__uint_as_float(x[2 * i]), a.scale, down));
+                        const float w1 = exp2_approx(fmaf(__uint_as_float(x[2 * i + 1]), a.scale, down));
+                        sum[i & 1] += w0, sum[2 + (i & 1)] += w1;
+                        // weights are rounded to the cache's type for the product: off by half a step each, without bias
+                        w[i] = Half16<DT>::from_float(w0) | static_cast<uint32_t>(Half16<DT>::from_float(w1)) << 16;
+                    }
+                    tmem_store16(s_mine + 16 * c, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_store_wait();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar(kPFull + half));
+            }
+            ok = ok && warp_wait(bar(kOFull + half), o_phase, failed, a.status);
+            o_phase ^= 1;
+            if (!ok) break;
+            fence_after();
+            char *part = a.parts + (2 * blockIdx.x + (p.starts ? 1 : 0)) * part_bytes(kTileRows, DP);
+            float2 *part_ml = reinterpret_cast<float2 *>(part + kTileRows * DP * 4);
+            const bool sees = hi > lo;
+            // (all four warps of the half have passed their last block: its barrier came after their arrivals)
+            if (words[2 + half] != pieces) {
+                const float inv = sees ? 1.0f / l : 0.0f;
+                char *to = a.out + (r.first + token) * a.out_token + head * a.out_head;
+                uint32_t y[32];
+#pragma unroll
+                for (int c = 0; c < DP / 32; ++c) {
+                    tmem_load32(y, o_mine + 32 * c);
+                    tmem_load_wait(y);
+                    if (there && p.whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                h[k] = Half16<DT>::from_float(__uint_as_float(y[8 * i + 2 * k]) * inv) |
+                                       static_cast<uint32_t>(Half16<DT>::from_float(__uint_as_float(y[8 * i + 2 * k + 1]) * inv)) << 16;
+                            if (32 * c + 8 * i < a.head_size)
+                                *reinterpret_cast<uint4 *>(to + 2 * (32 * c + 8 * i)) = sees ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(0, 0, 0, 0);
+                        }
+                    } else if (there) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<uint4 *>(part + ((8 * c + i) * kTileRows + row) * 16) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                    }
+                }
+                if (there && p.whole && a.lse)
+                    a.lse[static_cast<int64_t>(r.first + token) * a.q_heads + head] = sees ? (m + log2f(l)) * 0.693147180559945f : kNegInf;
+                if (there && !p.whole) part_ml[row] = make_float2(m, l);
+            } else {
+                for (int i = half * 128 + (warp & 3); i < min(rows, half * 128 + 128); i += 4) {
+                    float x[DP / 32], top, total;
+                    slow_row<DT, DP>(a, r, p.request, p.head, row0 + i, p.begin * kTileKeys, p.end * kTileKeys, x, top, total);
+                    const int tok = (row0 + i) / a.group, hd = p.head * a.group + (row0 + i) % a.group;
+                    const bool any = last_key(a, r, tok) > first_key(a, r, tok);
+#pragma unroll
+                    for (int c = 0; c < DP / 32; ++c) {
+                        const int d = lane + 32 * c;
+                        if (!p.whole) reinterpret_cast<float *>(part)[(d / 4 * kTileRows + i) * 4 + d % 4] = x[c];
+                        else if (d < a.head_size)
+                            reinterpret_cast<uint16_t *>(a.out + (r.first + tok) * a.out_token + hd * a.out_head)[d] = any ? Half16<DT>::from_float(x[c] / total) : 0;
+                    }
+                    if (lane == 0 && !p.whole) part_ml[i] = make_float2(top, total);
+                    if (lane == 0 && p.whole && a.lse)
+                        a.lse[static_cast<int64_t>(r.first + tok) * a.q_heads + hd] = any ? (top + log2f(total)) * 0.693147180559945f : kNegInf;
+                }
+            }
+            fence_before();  // O has been read: the next piece's products follow an arrival of this warp
+        }
+        if (tid == 0 && a.joins) {
+            // (pieces that this half has no rows of are counted above all the same)
+            a.joins[blockIdx.x] = join;
+        }
+    } else if (warp < 12) {
+        // ================================================================ copies
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        const int w = warp - 8, piece = lane % kPieces;
+        constexpr int kLag = 2;  // tiles that are on their way when one more is begun; the ring has to be longer by two
+        static_assert(kStages >= kLag + 2, "the products may need the tile behind the one that they free");
+        const uint32_t at_piece = static_cast<uint32_t>(piece / 8) * 16384;
+        int t = 0, told = 0, q_count = 0;
+        bool ok = true;
+        const auto tell = [&](int upto) {  // tiles that have arrived
+            for (; told < upto; ++told) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(full(told % kStages));
+            }
+        };
+        const auto copy_rows = [&](uint32_t tile, const char *from, int64_t at, bool there) {  // lane i: where row 32 w + i lies
+#pragma unroll
+            for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+                const int src = i * kRowsAtOnce + lane / kPieces, row = 32 * w + src;
+                const int64_t offset = __shfl_sync(0xffffffffu, at, src);
+                const bool copy = __shfl_sync(0xffffffffu, there, src) && 8 * piece < a.head_size;
+                const uint32_t dst = tile + at_piece + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(copy ? from + offset + 16 * piece : a.q), "r"(copy ? 16 : 0) : "memory");
+            }
+        };
+        while (ok && run.next(a, p)) {
+            const Lengths r = p.r;
+            const int blocks = p.end - p.begin, row0 = p.t * kTileRows, rows = min(kTileRows, r.n * a.group - row0);
+            const auto page_for = [&](int j) {
+                const int key = (p.begin + j) * kTileKeys + 32 * w + lane;
+                return j < blocks && key >= p.tile.lo && key < p.tile.hi ? page_of(a, p.request, key / a.page_size) : -1;
+            };
+            int page = page_for(0);
+            // queries: once the last products with the ones before are done, which need the tiles that are still on their way
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            tell(t);
+            if (q_count && !(ok = warp_wait(bar(kQEmpty), (q_count - 1) & 1, failed, a.status))) break;
+            ++q_count;
+            for (int half = 0; half < 2; ++half) {
+                const int row = half * 128 + 32 * w + lane;
+                const bool there = row < rows;
+                const int token = there ? (row0 + row) / a.group : 0, head = p.head * a.group + (there ? (row0 + row) % a.group : 0);
+                copy_rows(base + half * kTileBytes<DP>, a.q, (r.first + token) * a.q_token + head * a.q_head, there);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar(kQFull));
+            for (int j = 0; ok && j < blocks; ++j) {
+                const int key = (p.begin + j) * kTileKeys + 32 * w + lane, in_page = key % a.page_size;
+                const int64_t at_k = page * a.k_page + in_page * a.k_token + p.head * a.k_head;
+                const int64_t at_v = page * a.v_page + in_page * a.v_token + p.head * a.v_head;
+                const bool there = page >= 0;
+                page = page_for(j + 1);
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    if (t >= kStages && !(ok = warp_wait(empty(t % kStages), (t / kStages - 1) & 1, failed, a.status))) break;
+                    copy_rows(tiles_at + t % kStages * kTileBytes<DP>, kv ? a.v : a.k, kv ? at_v : at_k, there);
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+                    ++t;
+                    tell(t - kLag);
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        tell(ok ? t : told);
+    } else {
+        // ================================================================ products
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 12 && lane == 0) {
+            constexpr uint32_t qk = product(DT, kTileKeys, false), pv = product(DT, DP, true);
+            uint32_t p_phase[2] = {0, 0};
+            int t = 0, q_count = 0;
+            bool ok = true;
+            const auto scores = [&](int half, int tile) {
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    const uint32_t at = (k / 4) * 16384 + (k % 4) * 32;
+                    mma_ss(s_at(half), operand(base + half * kTileBytes<DP> + at, 16), operand(tiles_at + tile % kStages * kTileBytes<DP> + at, 16), qk, k > 0);
+                }
+            };
+            while (ok && run.next(a, p)) {
+                const int blocks = p.end - p.begin, rows = min(kTileRows, p.r.n * a.group - p.t * kTileRows), halves = rows > 128 ? 2 : 1;
+                if (!(ok = bar_wait(bar(kQFull), q_count & 1, failed, a.status))) break;
+                ++q_count;
+                if (!(ok = bar_wait(full(t % kStages), (t / kStages) & 1, failed, a.status))) break;
+                fence_after();
+                for (int half = 0; half < halves; ++half) {
+                    scores(half, t);
+                    commit(bar(kSFull + half));
+                }
+                commit(empty(t % kStages));
+                if (blocks == 1) commit(bar(kQEmpty));
+                for (int j = 0; ok && j < blocks; ++j) {
+                    const int v = t + 1, next = t + 2;
+                    if (!(ok = bar_wait(full(v % kStages), (v / kStages) & 1, failed, a.status))) break;
+                    for (int half = 0; half < halves; ++half) {
+                        if (!(ok = bar_wait(bar(kPFull + half), p_phase[half], failed, a.status))) break;
+                        p_phase[half] ^= 1;
+                        fence_after();
+#pragma unroll
+                        for (int k = 0; k < kTileKeys / 16; ++k)
+                            mma_ts(o_at(half), s_at(half) + 8 * k, operand(tiles_at + v % kStages * kTileBytes<DP> + k * 2048, 16384), pv, j > 0 || k > 0);
+                        if (half == halves - 1) commit(empty(v % kStages));
+                        if (j + 1 < blocks) {
+                            if (half == 0 && !(ok = bar_wait(full(next % kStages), (next / kStages) & 1, failed, a.status))) break;
+                            scores(half, next);
+                            commit(bar(kSFull + half));
+                            if (half == halves - 1) {
+                                commit(empty(next % kStages));
+                                if (j + 2 == blocks) commit(bar(kQEmpty));
+                            }
+                        } else {
+                            commit(bar(kOFull + half));
+                        }
+                    }
+                    t += 2;
+                }
+            }
+        }
+        __syncwarp();
+    }
+    // every product has been waited for (its O read), or the block has given up on one
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 12) tmem_free(tmem, 512);
+}
+
+template <int DT, int DP> int launch_tiles(const AttendArgs &a, int ctas, cudaStream_t st) {
+    constexpr int smem = kTilesSmem<DP>;
+    int rc = allow_smem(attend_tiles_kernel<DT, DP>, smem);
+    if (rc) return rc;
+    rc = launch(attend_tiles_kernel<DT, DP>, dim3(ctas), kTileThreads, smem, false, st, a);
+    if (rc || !a.joins) return rc;
+    return launch(combine_kernel<DT, kTileRows, DP, true>, dim3(ctas, kTileRows * (DP / 4) / 256), 256, 0, true, st, a);
+}
+
+}  // namespace
+
+int launch_attend_tiles(const AttendArgs &a, int dtype, int ctas, cudaStream_t st) {
+    if (a.head_size <= 64) return dtype == CG_F16 ? launch_tiles<CG_F16, 64>(a, ctas, st) : launch_tiles<CG_BF16, 64>(a, ctas, st);
+    return dtype == CG_F16 ? launch_tiles<CG_F16, 128>(a, ctas, st) : launch_tiles<CG_BF16, 128>(a, ctas, st);
+}
+
+}  // namespace cg
