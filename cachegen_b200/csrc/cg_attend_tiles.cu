@@ -123,6 +123,44 @@ __device__ __forceinline__ void tmem_load_wait(uint32_t (&x)[32]) {
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// ---- pairs of 32-bit floats, as one instruction takes them ------------------------------------------------
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+    return p;
+}
+__device__ __forceinline__ float2 parts_of(uint64_t p) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+template <int DT> __device__ __forceinline__ uint32_t round_pair(float lo, float hi) {
+    uint32_t w;
+    if (DT == CG_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+// 32 scores to weights 2^(s * scale + down), rounded to 16 bits for the product: off by half a step each, without bias
+template <int DT> __device__ __forceinline__ void weigh(const uint32_t (&x)[32], uint64_t scale, uint64_t down, uint32_t (&w)[16], uint64_t (&sum)[2]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float2 y = parts_of(pair_fma(pair_of(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale, down));
+        const float w0 = exp2_approx(y.x), w1 = exp2_approx(y.y);
+        sum[i & 1] = pair_add(sum[i & 1], pair_of(w0, w1));
+        w[i] = round_pair<DT>(w0, w1);
+    }
+}
+
 // ---- shared memory ------------------------------------------------------------------------------
 // Q [2 halves][DP / 64 panels][128 rows][128 bytes], then the ring of K and V tiles [DP / 64][128 keys][128 bytes]; the 16-byte piece p of a
 // row lies at p ^ row % 8, which is the swizzle that the products expect.
@@ -204,22 +242,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 if (!ok) break;
                 fence_after();
                 const bool masked = key < half_lo || key + kTileKeys > half_hi;  // for one of the half's rows
-                float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
-                // the scores are read twice, for the maximum and for the weights: 128 of them would not fit beside the rest
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32];
-                    tmem_load32(x, s_mine + 32 * c);
-                    tmem_load_wait(x);
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            top[i & 3] = fmaxf(top[i & 3], key + 32 * c + i >= lo && key + 32 * c + i < hi ? __uint_as_float(x[i]) : kNegInf);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
-                    }
-                }
                 if (masked) {
                     // values of keys that some rows do not see: are they all finite?
                     const int t = first_tile + 2 * j + 1;
@@ -233,7 +255,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                         for (const uint32_t y : {w.x, w.y, w.z, w.w}) odd = odd || (y & e) == e || ((y >> 16) & e) == e;
                     }
                     if (odd) words[2 + half] = pieces;
+                    // scores of keys that a row does not see go back as minus infinity: what follows knows no masks
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[32];
+                        tmem_load32(x, s_mine + 32 * c);
+                        tmem_load_wait(x);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (key + 32 * c + i < lo || key + 32 * c + i >= hi) x[i] = __float_as_uint(kNegInf);
+                        tmem_store32(s_mine + 32 * c, x);
+                    }
+                    tmem_store_wait();
                 }
+                // the scores are read twice, for the maximum and for the weights: 128 of them would not fit beside the rest.  Loops
+                // stay loops: the roles' code together has to fit the instruction caches.
+                float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+                uint32_t x[32], y[32];
+                tmem_load32(x, s_mine);
+#pragma unroll 1
+                for (int c = 0; c < 4; c += 2) {
+                    tmem_load_wait(x);
+                    tmem_load32(y, s_mine + 32 * c + 32);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
+                    tmem_load_wait(y);
+                    tmem_load32(x, s_mine + (32 * c + 64) % 128);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(y[i]));
+                }
+                tmem_load_wait(x);
                 const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale;
                 const bool raise = high > m + 8.0f || (m == kNegInf && high > m);
                 if (__any_sync(0xffffffffu, raise)) {
@@ -241,8 +292,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     if (raise) m = high;
                     l *= keep;
                     if (j > 0) {  // the products of the block before are done: this block's scores came behind them
-                        uint32_t y[32];
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < DP / 32; ++c) {
                             tmem_load32(y, o_mine + 32 * c);
                             tmem_load_wait(y);
@@ -252,29 +302,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                         }
                     }
                 }
-                const float down = m == kNegInf ? 0.0f : -m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {  // (weights take half the columns of the scores that they come from: these have been read)
-                    uint32_t x[32], w[16];
-                    tmem_load32(x, s_mine + 32 * c);
-                    tmem_load_wait(x);
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (key + 32 * c + i < lo || key + 32 * c + i >= hi) x[i] = __float_as_uint(kNegInf);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float w0 = exp2_approx(fmaf(__uint_as_float(x[2 * i]), a.scale, down));
-                        const float w1 = exp2_approx(fmaf(__uint_as_float(x[2 * i + 1]), a.scale, down));
-                        sum[i & 1] += w0, sum[2 + (i & 1)] += w1;
-                        // weights are rounded to the cache's type for the product: off by half a step each, without bias
-                        w[i] = Half16<DT>::from_float(w0) | static_cast<uint32_t>(Half16<DT>::from_float(w1)) << 16;
-                    }
+                const float base = m == kNegInf ? 0.0f : -m;
+                const uint64_t scale = pair_of(a.scale, a.scale), down = pair_of(base, base);
+                uint64_t sum[2] = {0, 0};
+                uint32_t w[16];
+#pragma unroll 1
+                for (int c = 0; c < 4; c += 2) {  // (weights take half the columns of the scores that they come from: these have been read)
+                    tmem_load32(y, s_mine + 32 * c + 32);
+                    weigh<DT>(x, scale, down, w, sum);
+                    tmem_load_wait(y);
                     tmem_store16(s_mine + 16 * c, w);
+                    if (c == 0) tmem_load32(x, s_mine + 64);
+                    weigh<DT>(y, scale, down, w, sum);
+                    if (c == 0) tmem_load_wait(x);
+                    tmem_store16(s_mine + 16 * c + 16, w);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                const float2 s0 = parts_of(sum[0]), s1 = parts_of(sum[1]);
+                l += (s0.x + s0.y) + (s1.x + s1.y);
                 tmem_store_wait();
                 fence_before();
                 __syncwarp();
@@ -292,7 +336,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 const float inv = sees ? 1.0f / l : 0.0f;
                 char *to = a.out + (r.first + token) * a.out_token + head * a.out_head;
                 uint32_t y[32];
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < DP / 32; ++c) {
                     tmem_load32(y, o_mine + 32 * c);
                     tmem_load_wait(y);
@@ -414,52 +458,59 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 12 && lane == 0) {
             constexpr uint32_t qk = product(DT, kTileKeys, false), pv = product(DT, DP, true);
-            uint32_t p_phase[2] = {0, 0};
-            int t = 0, q_count = 0;
+            const uint64_t q_desc = operand(base, 16), k_desc = operand(tiles_at, 16), v_desc = operand(tiles_at, 16384);
+            constexpr uint32_t kTile = kTileBytes<DP> >> 4;  // in units of a descriptor's address
+            uint32_t p_phase = 0, q_phase = 0, stage = 0, phase = 0;  // of the tile that is waited for next
             bool ok = true;
-            const auto scores = [&](int half, int tile) {
+            const auto scores = [&](int half, uint32_t at) {
+                const uint64_t q = q_desc + half * kTile, k = k_desc + at * kTile;
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t at = (k / 4) * 16384 + (k % 4) * 32;
-                    mma_ss(s_at(half), operand(base + half * kTileBytes<DP> + at, 16), operand(tiles_at + tile % kStages * kTileBytes<DP> + at, 16), qk, k > 0);
-                }
+                for (int i = 0; i < DP / 16; ++i) mma_ss(s_at(half), q + (i / 4) * 1024 + (i % 4) * 2, k + (i / 4) * 1024 + (i % 4) * 2, qk, i > 0);
+            };
+            const auto tile_there = [&]() {  // its stage, when it is there
+                const uint32_t at = stage;
+                ok = bar_wait(full(at), phase, failed, a.status);
+                if (++stage == kStages) stage = 0, phase ^= 1;
+                return at;
             };
             while (ok && run.next(a, p)) {
                 const int blocks = p.end - p.begin, rows = min(kTileRows, p.r.n * a.group - p.t * kTileRows), halves = rows > 128 ? 2 : 1;
-                if (!(ok = bar_wait(bar(kQFull), q_count & 1, failed, a.status))) break;
-                ++q_count;
-                if (!(ok = bar_wait(full(t % kStages), (t / kStages) & 1, failed, a.status))) break;
+                if (!(ok = bar_wait(bar(kQFull), q_phase, failed, a.status))) break;
+                q_phase ^= 1;
+                uint32_t k_stage = tile_there(), v_stage = 0;
+                if (!ok) break;
                 fence_after();
+#pragma unroll 1
                 for (int half = 0; half < halves; ++half) {
-                    scores(half, t);
+                    scores(half, k_stage);
                     commit(bar(kSFull + half));
                 }
-                commit(empty(t % kStages));
+                commit(empty(k_stage));
                 if (blocks == 1) commit(bar(kQEmpty));
-                for (int j = 0; ok && j < blocks; ++j) {
-                    const int v = t + 1, next = t + 2;
-                    if (!(ok = bar_wait(full(v % kStages), (v / kStages) & 1, failed, a.status))) break;
-                    for (int half = 0; half < halves; ++half) {
-                        if (!(ok = bar_wait(bar(kPFull + half), p_phase[half], failed, a.status))) break;
-                        p_phase[half] ^= 1;
-                        fence_after();
+#pragma unroll 1
+                for (int i = 0; ok && i < blocks * halves; ++i) {
+                    const int half = halves == 2 ? i & 1 : 0;
+                    const bool first = half == 0, last_half = half == halves - 1, more = i + halves < blocks * halves;
+                    if (first) v_stage = tile_there();
+                    if (!ok || !(ok = bar_wait(bar(kPFull + half), p_phase >> half & 1, failed, a.status))) break;
+                    p_phase ^= 1 << half;
+                    fence_after();
+                    const uint64_t v = v_desc + v_stage * kTile;
 #pragma unroll
-                        for (int k = 0; k < kTileKeys / 16; ++k)
-                            mma_ts(o_at(half), s_at(half) + 8 * k, operand(tiles_at + v % kStages * kTileBytes<DP> + k * 2048, 16384), pv, j > 0 || k > 0);
-                        if (half == halves - 1) commit(empty(v % kStages));
-                        if (j + 1 < blocks) {
-                            if (half == 0 && !(ok = bar_wait(full(next % kStages), (next / kStages) & 1, failed, a.status))) break;
-                            scores(half, next);
-                            commit(bar(kSFull + half));
-                            if (half == halves - 1) {
-                                commit(empty(next % kStages));
-                                if (j + 2 == blocks) commit(bar(kQEmpty));
-                            }
-                        } else {
-                            commit(bar(kOFull + half));
+                    for (int k = 0; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, pv, i >= halves || k > 0);
+                    if (last_half) commit(empty(v_stage));
+                    if (more) {
+                        if (first) k_stage = tile_there();
+                        if (!ok) break;
+                        scores(half, k_stage);
+                        commit(bar(kSFull + half));
+                        if (last_half) {
+                            commit(empty(k_stage));
+                            if (i + 1 + halves == blocks * halves) commit(bar(kQEmpty));
                         }
+                    } else {
+                        commit(bar(kOFull + half));
                     }
-                    t += 2;
                 }
             }
         }
