@@ -208,7 +208,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // One row over keys [k0, k1) by a warp, straight from memory: for tiles in which a key that some rows do not see has values that
 // are not finite, since a weight of zero does not keep those out of a product.  sums[i] is value lane + 32 i of the head.
 template <int DT, int DP>
-__device__ __noinline__ void slow_row(const AttendArgs &a, const Lengths &r, int b, int head, int row, int k0, int k1,
+__device__ __forceinline__ void slow_row(const AttendArgs &a, const Lengths &r, int b, int head, int row, int k0, int k1,
                                       float (&sums)[DP / 32], float &top, float &total) {
     const int lane = threadIdx.x & 31, token = row / a.group;
     const char *q = a.q + (r.first + token) * a.q_token + (head * a.group + row % a.group) * a.q_head;

@@ -36,27 +36,31 @@ __device__ __forceinline__ uint64_t now_ns() {
     return t;
 }
 // Whether the phase ended.  If it does not within kGiveUpNs, or another wait of the block gave up, the block is told to end.
-__device__ __forceinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
-    const uint64_t start = now_ns();
-    while (true) {
-        for (int i = 0; i < 256; ++i)
-            if (bar_try(bar, parity)) return true;
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
+    uint64_t start = 0;
+#pragma unroll 1
+    for (uint32_t n = 1; !bar_try(bar, parity); ++n) {
+        if (n & 255) continue;
         if (*failed) return false;
-        if (now_ns() - start > kGiveUpNs) {
+        const uint64_t now = now_ns();
+        if (!start) start = now;
+        if (now - start > kGiveUpNs) {
             *failed = 1;
             if (status) atomicOr(status, CG_S_TIMEOUT);
             return false;
         }
     }
-}
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
-    for (int i = 0; i < 16; ++i)
-        if (bar_try(bar, parity)) return true;
-    return bar_wait_long(bar, parity, failed, status);
+    return true;
 }
 // the same for a whole warp, with one result
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
     return __all_sync(0xffffffffu, bar_wait(bar, parity, failed, status));
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+    return yes;
 }
 
 // ---- tensor memory and products ---------------------------------------------------------------
@@ -144,6 +148,11 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 template <int DT> __device__ __forceinline__ uint32_t round_pair(float lo, float hi) {
     uint32_t w;
     if (DT == CG_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
@@ -174,7 +183,7 @@ template <int DT, int DP>
 __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __grid_constant__ AttendArgs a) {
     extern __shared__ unsigned char raw[];
     constexpr int kStages = kTileStages<DP>, kPieces = DP / 8, kRowsAtOnce = 32 / kPieces;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // (known to be the same in a warp)
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     unsigned char *mem = raw + (base - smem_addr(raw));
     const uint32_t tiles_at = base + 2 * kTileBytes<DP>, bars = base + kBarsAt<DP>;
@@ -214,7 +223,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
 
     if (warp < 8) {
         // ================================================================ softmax: a row a thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");  // 256 threads of 168 and 256 of 88 registers: the 512 x 128 of the launch
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int half = warp >> 2, in_half = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_mine = s_at(half) + lanes, o_mine = o_at(half) + lanes;
@@ -268,23 +277,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     }
                     tmem_store_wait();
                 }
-                // the scores are read twice, for the maximum and for the weights: 128 of them would not fit beside the rest.  Loops
-                // stay loops: the roles' code together has to fit the instruction caches.
+                uint32_t x[4][32];
+                tmem_load32(x[0], s_mine);
+                tmem_load32(x[1], s_mine + 32);
+                tmem_load_wait(x[0]);
+                tmem_load_wait(x[1]);
+                tmem_load32(x[2], s_mine + 64);
+                tmem_load32(x[3], s_mine + 96);
                 float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
-                uint32_t x[32], y[32];
-                tmem_load32(x, s_mine);
-#pragma unroll 1
-                for (int c = 0; c < 4; c += 2) {
-                    tmem_load_wait(x);
-                    tmem_load32(y, s_mine + 32 * c + 32);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
-                    tmem_load_wait(y);
-                    tmem_load32(x, s_mine + (32 * c + 64) % 128);
+                for (int i = 0; i < 64; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(x[i / 32][i % 32]), __uint_as_float(x[i / 32][i % 32 + 1]));
+                tmem_load_wait(x[2]);
+                tmem_load_wait(x[3]);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(y[i]));
-                }
-                tmem_load_wait(x);
+                for (int i = 64; i < 128; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(x[i / 32][i % 32]), __uint_as_float(x[i / 32][i % 32 + 1]));
                 const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale;
                 const bool raise = high > m + 8.0f || (m == kNegInf && high > m);
                 if (__any_sync(0xffffffffu, raise)) {
@@ -294,6 +300,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     if (j > 0) {  // the products of the block before are done: this block's scores came behind them
 #pragma unroll 1
                         for (int c = 0; c < DP / 32; ++c) {
+                            uint32_t y[32];
                             tmem_load32(y, o_mine + 32 * c);
                             tmem_load_wait(y);
 #pragma unroll
@@ -305,17 +312,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 const float base = m == kNegInf ? 0.0f : -m;
                 const uint64_t scale = pair_of(a.scale, a.scale), down = pair_of(base, base);
                 uint64_t sum[2] = {0, 0};
-                uint32_t w[16];
-#pragma unroll 1
-                for (int c = 0; c < 4; c += 2) {  // (weights take half the columns of the scores that they come from: these have been read)
-                    tmem_load32(y, s_mine + 32 * c + 32);
-                    weigh<DT>(x, scale, down, w, sum);
-                    tmem_load_wait(y);
+                // (weights take half the columns of the scores that they come from: these have been read)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+                    weigh<DT>(x[c], scale, down, w, sum);
                     tmem_store16(s_mine + 16 * c, w);
-                    if (c == 0) tmem_load32(x, s_mine + 64);
-                    weigh<DT>(y, scale, down, w, sum);
-                    if (c == 0) tmem_load_wait(x);
-                    tmem_store16(s_mine + 16 * c + 16, w);
                 }
                 const float2 s0 = parts_of(sum[0]), s1 = parts_of(sum[1]);
                 l += (s0.x + s0.y) + (s1.x + s1.y);
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         }
     } else if (warp < 12) {
         // ================================================================ copies
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         const int w = warp - 8, piece = lane % kPieces;
         constexpr int kLag = 2;  // tiles that are on their way when one more is begun; the ring has to be longer by two
         static_assert(kStages >= kLag + 2, "the products may need the tile behind the one that they free");
@@ -455,11 +457,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         tell(ok ? t : told);
     } else {
         // ================================================================ products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 12 && lane == 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 12) {
+            // the whole warp goes through the same steps, so that operands stay in uniform registers; one thread issues
             constexpr uint32_t qk = product(DT, kTileKeys, false), pv = product(DT, DP, true);
-            const uint64_t q_desc = operand(base, 16), k_desc = operand(tiles_at, 16), v_desc = operand(tiles_at, 16384);
             constexpr uint32_t kTile = kTileBytes<DP> >> 4;  // in units of a descriptor's address
+            const uint64_t q_desc = operand(base, 16), k_desc = operand(tiles_at, 16), v_desc = operand(tiles_at, 16384);
+            const bool issues = elect_one();
             uint32_t p_phase = 0, q_phase = 0, stage = 0, phase = 0;  // of the tile that is waited for next
             bool ok = true;
             const auto scores = [&](int half, uint32_t at) {
@@ -469,48 +473,61 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             };
             const auto tile_there = [&]() {  // its stage, when it is there
                 const uint32_t at = stage;
-                ok = bar_wait(full(at), phase, failed, a.status);
+                ok = warp_wait(full(at), phase, failed, a.status);
                 if (++stage == kStages) stage = 0, phase ^= 1;
                 return at;
             };
             while (ok && run.next(a, p)) {
                 const int blocks = p.end - p.begin, rows = min(kTileRows, p.r.n * a.group - p.t * kTileRows), halves = rows > 128 ? 2 : 1;
-                if (!(ok = bar_wait(bar(kQFull), q_phase, failed, a.status))) break;
+                if (!(ok = warp_wait(bar(kQFull), q_phase, failed, a.status))) break;
                 q_phase ^= 1;
                 uint32_t k_stage = tile_there(), v_stage = 0;
                 if (!ok) break;
                 fence_after();
-#pragma unroll 1
-                for (int half = 0; half < halves; ++half) {
-                    scores(half, k_stage);
-                    commit(bar(kSFull + half));
-                }
-                commit(empty(k_stage));
-                if (blocks == 1) commit(bar(kQEmpty));
-#pragma unroll 1
-                for (int i = 0; ok && i < blocks * halves; ++i) {
-                    const int half = halves == 2 ? i & 1 : 0;
-                    const bool first = half == 0, last_half = half == halves - 1, more = i + halves < blocks * halves;
-                    if (first) v_stage = tile_there();
-                    if (!ok || !(ok = bar_wait(bar(kPFull + half), p_phase >> half & 1, failed, a.status))) break;
-                    p_phase ^= 1 << half;
-                    fence_after();
-                    const uint64_t v = v_desc + v_stage * kTile;
-#pragma unroll
-                    for (int k = 0; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, pv, i >= halves || k > 0);
-                    if (last_half) commit(empty(v_stage));
-                    if (more) {
-                        if (first) k_stage = tile_there();
-                        if (!ok) break;
-                        scores(half, k_stage);
-                        commit(bar(kSFull + half));
-                        if (last_half) {
-                            commit(empty(k_stage));
-                            if (i + 1 + halves == blocks * halves) commit(bar(kQEmpty));
-                        }
-                    } else {
-                        commit(bar(kOFull + half));
+                if (issues) {
+                    scores(0, k_stage);
+                    commit(bar(kSFull));
+                    if (halves == 2) {
+                        scores(1, k_stage);
+                        commit(bar(kSFull + 1));
                     }
+                    commit(empty(k_stage));
+                    if (blocks == 1) commit(bar(kQEmpty));
+                }
+#pragma unroll 1
+                for (int j = 0; j < blocks; ++j) {
+                    v_stage = tile_there();
+                    if (!ok) break;
+                    const bool more = j + 1 < blocks;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (half == halves) break;
+                        if (!(ok = warp_wait(bar(kPFull + half), p_phase >> half & 1, failed, a.status))) break;
+                        p_phase ^= 1 << half;
+                        fence_after();
+                        const uint64_t v = v_desc + v_stage * kTile;
+                        if (issues) {
+#pragma unroll
+                            for (int k = 0; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, pv, j > 0 || k > 0);
+                            if (half == halves - 1) commit(empty(v_stage));
+                        }
+                        if (more && half == 0) k_stage = tile_there();
+                        if (!ok) break;
+                        if (issues) {
+                            if (more) {
+                                scores(half, k_stage);
+                                commit(bar(kSFull + half));
+                                if (half == halves - 1) {
+                                    commit(empty(k_stage));
+                                    if (j + 2 == blocks) commit(bar(kQEmpty));
+                                }
+                            } else {
+                                commit(bar(kOFull + half));
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    if (!ok) break;
                 }
             }
         }
