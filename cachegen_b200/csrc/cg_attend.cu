@@ -11,7 +11,7 @@ namespace cg {
 namespace {
 
 constexpr int kRowsM = 16, kWarps = 4, kStages = 3, kChunk = 16;
-constexpr int kRowsBK = kWarps * kChunk;
+constexpr int kRowsBK = kWarps * kChunk, kRowsCost = 1;
 
 template <int DT>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_rows_kernel(const __gri
     const int g = lane >> 2, q2 = 2 * (lane & 3);
     const uint32_t ring = smem_addr(smem) + warp * kRingBytes<DP>;
 
-    Run<kRowsM, kRowsBK> run;
+    Run<kRowsM, kRowsBK, kRowsCost> run;
     run.template init<kWarps * 32, false>(a, reinterpret_cast<int64_t *>(smem));
     let_next_launch_start();
     int4 join = make_int4(0, 0, 0, 0);

@@ -87,7 +87,7 @@ struct Piece {
 
 // A CTA's run through the line of units.  init is called by all threads of the block, with room in shared memory for
 // nrequests + 1 numbers; next by any of them, as often, all with the same result.
-template <int M, int BK> struct Run {
+template <int M, int BK, int COST> struct Run {
     int64_t at, to, total;
     int ctas;
     int b, h, t, tiles, skip;
@@ -102,7 +102,7 @@ template <int M, int BK> struct Run {
                 const Lengths x = lengths_of(a, i, blockIdx.x == 0 && lane == 0);
                 const int n = tiles_of<M>(a, x);
                 int units = 0;
-                for (int k = lane; k < n; k += 32) units += tile_of<M, BK>(a, x, k).units;
+                for (int k = lane; k < n; k += 32) units += tile_of<M, BK>(a, x, k).units + COST;
                 units = __reduce_add_sync(0xffffffffu, units);
                 if (lane == 0) before[i + 1] = static_cast<int64_t>(units) * a.heads;
             }
@@ -111,7 +111,7 @@ template <int M, int BK> struct Run {
                 const Lengths x = lengths_of(a, i, blockIdx.x == 0);
                 const int n = tiles_of<M>(a, x);
                 int units = 0;
-                for (int k = 0; k < n; ++k) units += tile_of<M, BK>(a, x, k).units;
+                for (int k = 0; k < n; ++k) units += tile_of<M, BK>(a, x, k).units + COST;
                 before[i + 1] = static_cast<int64_t>(units) * a.heads;
             }
         }
@@ -151,10 +151,17 @@ template <int M, int BK> struct Run {
             int64_t rest = at - before[b];
             h = static_cast<int>(rest / per_head);
             rest -= h * per_head;
-            for (t = 0;; ++t) {
-                const int u = tile_of<M, BK>(a, r, t).units;
-                if (rest < u) break;
-                rest -= u;
+            for (int first = 0;; first += 32) {  // 32 tiles at a time: how many end in front of `rest`
+                int s = first + lane < tiles ? tile_of<M, BK>(a, r, first + lane).units + COST : 0;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, s, d);
+                    if (lane >= d) s += o;
+                }
+                const int n = __popc(__ballot_sync(0xffffffffu, s <= rest && first + lane < tiles));
+                const int gone = __shfl_sync(0xffffffffu, s, n ? n - 1 : 0);
+                t = first + n;
+                if (n) rest -= gone;
+                if (n < 32) break;
             }
             skip = static_cast<int>(rest);
         }
@@ -162,31 +169,34 @@ template <int M, int BK> struct Run {
     }
 
     __device__ __forceinline__ bool next(const AttendArgs &a, Piece &p) {
-        if (at >= to) return false;
-        while (t >= tiles) {
-            t = 0;
-            if (++h >= a.heads) {
-                h = 0;
-                do {
-                    r = lengths_of(a, ++b);
-                    tiles = tiles_of<M>(a, r);
-                } while (tiles == 0);
+        while (at < to) {
+            while (t >= tiles) {
+                t = 0;
+                if (++h >= a.heads) {
+                    h = 0;
+                    do {
+                        r = lengths_of(a, ++b);
+                        tiles = tiles_of<M>(a, r);
+                    } while (tiles == 0);
+                }
             }
+            p.tile = tile_of<M, BK>(a, r, t);
+            const int length = p.tile.units + COST, left = length - skip, take = static_cast<int>(min(static_cast<int64_t>(left), to - at));
+            const int begin = max(0, skip - COST), end = max(0, skip + take - COST);
+            p.r = r;
+            p.request = b, p.head = h, p.t = t;
+            p.begin = p.tile.block0 + begin;
+            p.end = p.tile.block0 + end;
+            p.starts = begin == 0;
+            p.whole = p.starts && end == p.tile.units;
+            p.sharers = 0;
+            if (p.starts && !p.whole) p.sharers = static_cast<int>(((at + left) * ctas - 1) / total) - static_cast<int>(blockIdx.x) + 1;
+            at += take;
+            skip = 0;
+            ++t;
+            if (end > begin) return true;
         }
-        p.r = r;
-        p.request = b, p.head = h, p.t = t;
-        p.tile = tile_of<M, BK>(a, r, t);
-        const int left = p.tile.units - skip, take = static_cast<int>(min(static_cast<int64_t>(left), to - at));
-        p.begin = p.tile.block0 + skip;
-        p.end = p.begin + take;
-        p.starts = skip == 0;
-        p.whole = p.starts && take == left;
-        p.sharers = 0;
-        if (p.starts && !p.whole) p.sharers = static_cast<int>(((at + left) * ctas - 1) / total) - static_cast<int>(blockIdx.x) + 1;
-        at += take;
-        skip = 0;
-        ++t;
-        return true;
+        return false;
     }
 };
 
@@ -290,6 +300,6 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
 
 // cg_attend_tiles.cu
 int launch_attend_tiles(const AttendArgs &a, int dtype, int ctas, cudaStream_t st);
-constexpr int kTileRows = 256, kTileKeys = 128;
+constexpr int kTileRows = 256, kTileKeys = 128, kTileCost = 2;
 
 }  // namespace cg

@@ -11,9 +11,13 @@
 // A row's maximum is only raised when a score is more than 2^8 times beyond it in weight: weights up to 2^8 lose nothing as 16-bit or
 // 32-bit floats, and O, which has to be multiplied in tensor memory for every raise, is then left alone in nearly every block.
 //
-// Copies are asynchronous 16-byte copies and not TMA: pages may have any size and stride, a block's last keys may lie in the middle of a
-// page, and what lies behind them has to arrive as zeros (a weight of zero does not keep NaN out of a product).
+// Keys and values come by TMA, a box of up to 32 tokens of one page at a time, where pages allow it (8, 16 or a multiple of 32 tokens) and
+// all 32 are seen; else by 16-byte asynchronous copies: pages may have any size, a block's last keys may lie in the middle of one, and
+// what lies behind them has to arrive as zeros (a weight of zero does not keep NaN out of a product).
 #include "cg_attend.cuh"
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
 namespace cg {
 namespace {
@@ -63,6 +67,19 @@ __device__ __forceinline__ bool elect_one() {
     return yes;
 }
 
+// ---- TMA ----------------------------------------------------------------------------------------
+struct PageMaps {  // of keys and values [pages, heads, page_size, head_size]; rows 0: TMA cannot read these pages
+    CUtensorMap k, v;
+    int32_t rows;  // tokens of a box
+};
+__device__ __forceinline__ void bar_expect(uint32_t bar, int bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_box(uint32_t to, const CUtensorMap *map, int value, int token, int head, int page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map),
+                 "r"(value), "r"(token), "r"(head), "r"(page), "r"(bar) : "memory");
+}
+
 // ---- tensor memory and products ---------------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t dst, int columns) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(columns) : "memory");
@@ -76,20 +93,19 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-                 "r"(add ? 1 : 0) : "memory");
+// (descriptors by their lower halves: one addition moves an operand)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nmov.b64 x, {%1, %3};\nmov.b64 y, {%2, %3};\nsetp.ne.u32 p, %5, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n}" ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(add ? 1 : 0) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-                 "r"(add ? 1 : 0) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 y;\nmov.b64 y, {%2, %3};\nsetp.ne.u32 p, %5, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n}" ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(add ? 1 : 0) : "memory");
 }
 // an operand in shared memory, rows (of queries, of keys) of 64 values that are swizzled in groups of 8 rows, 1024 bytes; `panel`: bytes
 // from 64 values of a row to the next 64, where they are the operand's outer axis
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t panel) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | static_cast<uint64_t>((panel >> 4) & 0x3FFF) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
-           1ull << 46 | 2ull << 61;
-}
+__device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t panel) { return ((addr >> 4) & 0x3FFF) | ((panel >> 4) & 0x3FFF) << 16; }
+constexpr uint32_t kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
 // 32-bit sums of products of 16-bit values, 128 rows, n columns; b_outer: the second operand's rows are the summed axis
 __host__ __device__ constexpr uint32_t product(int dtype, int n, bool b_outer) {
     const uint32_t type = dtype == CG_BF16 ? 1u : 0u;
@@ -180,7 +196,7 @@ template <int DP> constexpr int kTilesSmem = kBarsAt<DP> + 256 + 1024;  // and w
 enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 2, kOFull = kPFull + 2, kKvFull = kOFull + 2 };  // two each of S, P and O
 
 template <int DT, int DP>
-__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ PageMaps maps) {
     extern __shared__ unsigned char raw[];
     constexpr int kStages = kTileStages<DP>, kPieces = DP / 8, kRowsAtOnce = 32 / kPieces;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // (known to be the same in a warp)
@@ -194,7 +210,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
     volatile int *words = reinterpret_cast<volatile int *>(mem + kBarsAt<DP> + 240);  // tensor memory, failed, odd[2]
     volatile int *failed = words + 1;
 
-    Run<kTileRows, kTileKeys> run;
+    Run<kTileRows, kTileKeys, kTileCost> run;
     run.template init<kTileThreads, true>(a, reinterpret_cast<int64_t *>(mem));
     let_next_launch_start();
     if (tid == 0) {
@@ -211,6 +227,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) tmem_alloc(base + kBarsAt<DP> + 240, 512);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (TMA writes where `run` has had its numbers)
     fence_before();
     __syncthreads();
     fence_after();
@@ -394,22 +411,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         static_assert(kStages >= kLag + 2, "the products may need the tile behind the one that they free");
         const uint32_t at_piece = static_cast<uint32_t>(piece / 8) * 16384;
         int t = 0, told = 0, q_count = 0;
+        uint32_t by_tma = 0;  // bit i: this warp's part of tile t - 1 - i came by TMA, whose barrier knows when it is there
         bool ok = true;
-        const auto tell = [&](int upto) {  // tiles that have arrived
+        const auto tell = [&](int upto) {  // copies that have arrived
             for (; told < upto; ++told) {
+                if (by_tma >> (t - 1 - told) & 1) continue;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) bar_arrive(full(told % kStages));
             }
         };
-        const auto copy_rows = [&](uint32_t tile, const char *from, int64_t at, bool there) {  // lane i: where row 32 w + i lies
+        // where this lane's pieces of a tile go: rows 2 i + lane / 16 (of DP 64: 4 i + lane / 8) of the warp's 32
+        constexpr int kOrders = 8 / kRowsAtOnce;  // of a row's pieces, which repeat every 8 rows
+        uint32_t place[kOrders];
+#pragma unroll
+        for (int i = 0; i < kOrders; ++i) {
+            const int row = i * kRowsAtOnce + lane / kPieces;
+            place[i] = at_piece + (32 * w + row) * 128 + (((piece & 7) ^ (row & 7)) << 4);
+        }
+        const bool in_head = 8 * piece < a.head_size;
+        const auto copy_rows = [&](uint32_t tile, const char *at, bool there) {  // lane i: where row 32 w + i lies
+            const uint32_t rows_there = __ballot_sync(0xffffffffu, there);
+            const uint64_t where = reinterpret_cast<uint64_t>(at);
 #pragma unroll
             for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
-                const int src = i * kRowsAtOnce + lane / kPieces, row = 32 * w + src;
-                const int64_t offset = __shfl_sync(0xffffffffu, at, src);
-                const bool copy = __shfl_sync(0xffffffffu, there, src) && 8 * piece < a.head_size;
-                const uint32_t dst = tile + at_piece + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(copy ? from + offset + 16 * piece : a.q), "r"(copy ? 16 : 0) : "memory");
+                const int src = i * kRowsAtOnce + lane / kPieces;
+                const uint64_t from = __shfl_sync(0xffffffffu, where, src);
+                const bool copy = in_head && (rows_there >> src & 1);
+                const uint32_t dst = tile + place[i % kOrders] + i / kOrders * 1024;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(copy ? from + 16 * piece : reinterpret_cast<uint64_t>(a.q)), "r"(copy ? 16 : 0)
+                             : "memory");
             }
         };
         while (ok && run.next(a, p)) {
@@ -420,37 +451,54 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 return j < blocks && key >= p.tile.lo && key < p.tile.hi ? page_of(a, p.request, key / a.page_size) : -1;
             };
             int page = page_for(0);
-            // queries: once the last products with the ones before are done, which need the tiles that are still on their way
+            // what the products of the piece before need and is still on its way
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             tell(t);
-            if (q_count && !(ok = warp_wait(bar(kQEmpty), (q_count - 1) & 1, failed, a.status))) break;
-            ++q_count;
-            for (int half = 0; half < 2; ++half) {
-                const int row = half * 128 + 32 * w + lane;
-                const bool there = row < rows;
-                const int token = there ? (row0 + row) / a.group : 0, head = p.head * a.group + (there ? (row0 + row) % a.group : 0);
-                copy_rows(base + half * kTileBytes<DP>, a.q, (r.first + token) * a.q_token + head * a.q_head, there);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive(bar(kQFull));
+#pragma unroll 1
             for (int j = 0; ok && j < blocks; ++j) {
-                const int key = (p.begin + j) * kTileKeys + 32 * w + lane, in_page = key % a.page_size;
-                const int64_t at_k = page * a.k_page + in_page * a.k_token + p.head * a.k_head;
-                const int64_t at_v = page * a.v_page + in_page * a.v_token + p.head * a.v_head;
-                const bool there = page >= 0;
+                const int key = (p.begin + j) * kTileKeys + 32 * w + lane, in_page = key % a.page_size, here = page;
+                const bool boxes = maps.rows && __all_sync(0xffffffffu, here >= 0);
                 page = page_for(j + 1);
-#pragma unroll
+#pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv) {
                     if (t >= kStages && !(ok = warp_wait(empty(t % kStages), (t / kStages - 1) & 1, failed, a.status))) break;
-                    copy_rows(tiles_at + t % kStages * kTileBytes<DP>, kv ? a.v : a.k, kv ? at_v : at_k, there);
+                    const uint32_t tile = tiles_at + t % kStages * kTileBytes<DP>;
+                    by_tma = by_tma << 1 | boxes;
+                    if (boxes) {
+                        if (lane == 0) bar_expect(full(t % kStages), 32 * DP * 2);
+                        __syncwarp();
+                        if (lane % maps.rows == 0) {  // the lane of a box's first token
+#pragma unroll
+                            for (int panel = 0; panel < DP / 64; ++panel)
+                                tma_box(tile + panel * 16384 + (32 * w + lane) * 128, kv ? &maps.v : &maps.k, 64 * panel, in_page, p.head, here, full(t % kStages));
+                        }
+                    } else {
+                        const char *at = kv ? a.v + here * a.v_page + in_page * a.v_token + p.head * a.v_head
+                                            : a.k + here * a.k_page + in_page * a.k_token + p.head * a.k_head;
+                        copy_rows(tile, at, here >= 0);
+                    }
                     asm volatile("cp.async.commit_group;" ::: "memory");
                     asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
                     ++t;
                     tell(t - kLag);
                 }
+                if (!ok || j > 0) continue;
+                // queries, behind the first block's tiles, which are on their way meanwhile: once the last products with the ones before are done
+                if (q_count && !(ok = warp_wait(bar(kQEmpty), (q_count - 1) & 1, failed, a.status))) break;
+                ++q_count;
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    const int row = half * 128 + 32 * w + lane;
+                    const bool there = row < rows;
+                    const int token = there ? (row0 + row) / a.group : 0, head = p.head * a.group + (there ? (row0 + row) % a.group : 0);
+                    copy_rows(base + half * kTileBytes<DP>, a.q + (r.first + token) * a.q_token + head * a.q_head, there);
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar(kQFull));
+                tell(t);
             }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -462,14 +510,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             // the whole warp goes through the same steps, so that operands stay in uniform registers; one thread issues
             constexpr uint32_t qk = product(DT, kTileKeys, false), pv = product(DT, DP, true);
             constexpr uint32_t kTile = kTileBytes<DP> >> 4;  // in units of a descriptor's address
-            const uint64_t q_desc = operand(base, 16), k_desc = operand(tiles_at, 16), v_desc = operand(tiles_at, 16384);
+            const uint32_t q_desc = operand(base, 16), k_desc = operand(tiles_at, 16), v_desc = operand(tiles_at, 16384);
             const bool issues = elect_one();
             uint32_t p_phase = 0, q_phase = 0, stage = 0, phase = 0;  // of the tile that is waited for next
             bool ok = true;
             const auto scores = [&](int half, uint32_t at) {
-                const uint64_t q = q_desc + half * kTile, k = k_desc + at * kTile;
+                const uint32_t q = q_desc + half * kTile, k = k_desc + at * kTile;
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i) mma_ss(s_at(half), q + (i / 4) * 1024 + (i % 4) * 2, k + (i / 4) * 1024 + (i % 4) * 2, qk, i > 0);
+                for (int i = 0; i < DP / 16; ++i) mma_ss(s_at(half), q + (i / 4) * 1024 + (i % 4) * 2, k + (i / 4) * 1024 + (i % 4) * 2, kOperandHigh, qk, i > 0);
             };
             const auto tile_there = [&]() {  // its stage, when it is there
                 const uint32_t at = stage;
@@ -505,10 +553,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                         if (!(ok = warp_wait(bar(kPFull + half), p_phase >> half & 1, failed, a.status))) break;
                         p_phase ^= 1 << half;
                         fence_after();
-                        const uint64_t v = v_desc + v_stage * kTile;
+                        const uint32_t v = v_desc + v_stage * kTile;
                         if (issues) {
 #pragma unroll
-                            for (int k = 0; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, pv, j > 0 || k > 0);
+                            for (int k = 0; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, j > 0 || k > 0);
                             if (half == halves - 1) commit(empty(v_stage));
                         }
                         if (more && half == 0) k_stage = tile_there();
@@ -540,11 +588,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
     if (warp == 12) tmem_free(tmem, 512);
 }
 
+// Maps of the pages, where TMA can read them: its boxes are whole runs of 8 rows in shared memory, and sizes and strides have limits.
+bool map_pages(const AttendArgs &a, int dtype, PageMaps &maps) {
+    static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }();
+    const int rows = a.page_size % 32 == 0 ? 32 : a.page_size;
+    if (!encode || (rows != 32 && rows != 16 && rows != 8) || a.num_pages == 0) return false;
+    const cuuint64_t sizes[4] = {static_cast<cuuint64_t>(a.head_size), static_cast<cuuint64_t>(a.page_size), static_cast<cuuint64_t>(a.heads),
+                                 static_cast<cuuint64_t>(a.num_pages)};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, steps[4] = {1, 1, 1, 1};
+    const auto one = [&](CUtensorMap &map, const char *at, int64_t token, int64_t head, int64_t page) {
+        cuuint64_t strides[3] = {static_cast<cuuint64_t>(token), static_cast<cuuint64_t>(head), static_cast<cuuint64_t>(page)};
+        for (int i = 0; i < 3; ++i) {
+            if (sizes[i + 1] == 1) strides[i] = 16;  // never used
+            if (strides[i] == 0 || strides[i] % 16 || strides[i] >= 1ull << 40) return false;
+        }
+        return encode(&map, dtype == CG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<char *>(at), sizes, strides, box, steps,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    if (!one(maps.k, a.k, a.k_token, a.k_head, a.k_page) || !one(maps.v, a.v, a.v_token, a.v_head, a.v_page)) return false;
+    maps.rows = rows;
+    return true;
+}
+
 template <int DT, int DP> int launch_tiles(const AttendArgs &a, int ctas, cudaStream_t st) {
     constexpr int smem = kTilesSmem<DP>;
+    PageMaps maps{};
+    if (!map_pages(a, DT, maps)) maps.rows = 0;
     int rc = allow_smem(attend_tiles_kernel<DT, DP>, smem);
     if (rc) return rc;
-    rc = launch(attend_tiles_kernel<DT, DP>, dim3(ctas), kTileThreads, smem, false, st, a);
+    rc = launch(attend_tiles_kernel<DT, DP>, dim3(ctas), kTileThreads, smem, false, st, a, maps);
     if (rc || !a.joins) return rc;
     return launch(combine_kernel<DT, kTileRows, DP, true>, dim3(ctas, kTileRows * (DP / 4) / 256), 256, 0, true, st, a);
 }
