@@ -192,8 +192,16 @@ template <int DT> __device__ __forceinline__ void weigh(const uint32_t (&x)[32],
 template <int DP> constexpr int kTileBytes = 128 * DP * 2;
 template <int DP> constexpr int kTileStages = kTileStages128 * 128 / DP;
 template <int DP> constexpr int kBarsAt = (2 + kTileStages<DP>)*kTileBytes<DP>;
-template <int DP> constexpr int kTilesSmem = kBarsAt<DP> + 256 + 1024;  // and what it takes to begin at a multiple of 1024
-enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 2, kOFull = kPFull + 2, kKvFull = kOFull + 2 };  // two each of S, P and O
+template <int DP> constexpr int kTilesSmem = kBarsAt<DP> + 512 + 1024;  // and what it takes to begin at a multiple of 1024
+enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 2, kOFull = kPFull + 2, kPieceFull = kOFull + 2, kPieceEmpty = kPieceFull + 2,
+       kKvFull = kPieceEmpty + 2 };  // two each of S, P, O and pieces
+
+// A piece as the scheduling warp hands it to the others, 48 bytes.
+struct __align__(16) Parcel {
+    int32_t first, n, kv, request;
+    int32_t head, t, begin, end;  // no blocks: there are no more pieces
+    int32_t lo, hi, starts, whole;
+};
 
 template <int DT, int DP>
 __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ PageMaps maps) {
@@ -206,11 +214,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
     const auto bar = [&](int i) { return bars + 8 * i; };
     const auto full = [&](int s) { return bar(kKvFull + s); };
     const auto empty = [&](int s) { return bar(kKvFull + kStages + s); };
-    static_assert(8 * (kKvFull + 2 * kStages) <= 240, "room for the barriers");
-    volatile int *words = reinterpret_cast<volatile int *>(mem + kBarsAt<DP> + 240);  // tensor memory, failed, odd[2]
+    static_assert(8 * (kKvFull + 2 * kStages) <= 320, "room for the barriers");
+    volatile int *words = reinterpret_cast<volatile int *>(mem + kBarsAt<DP> + 320);  // tensor memory, failed, odd[2]
+    Parcel *parcels = reinterpret_cast<Parcel *>(mem + kBarsAt<DP> + 384);  // [2]
     volatile int *failed = words + 1;
 
-    Run<kTileRows, kTileKeys, kTileCost> run;
+    Run<kTileRows, kTileKeys, kTileCost> run;  // (of warp 13; all find their run together)
     run.template init<kTileThreads, true>(a, reinterpret_cast<int64_t *>(mem));
     let_next_launch_start();
     if (tid == 0) {
@@ -220,13 +229,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             bar_init(bar(kSFull + i), 1);
             bar_init(bar(kPFull + i), 4);
             bar_init(bar(kOFull + i), 1);
+            bar_init(bar(kPieceFull + i), 1);
+            bar_init(bar(kPieceEmpty + i), 13);  // warps that read it
             words[2 + i] = 0;
         }
         for (int s = 0; s < kStages; ++s) bar_init(full(s), 4), bar_init(empty(s), 1);
         *failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) tmem_alloc(base + kBarsAt<DP> + 240, 512);
+    if (warp == 12) tmem_alloc(base + kBarsAt<DP> + 320, 512);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (TMA writes where `run` has had its numbers)
     fence_before();
     __syncthreads();
@@ -235,8 +246,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
     // columns: S (and P) of the halves, then O
     const auto s_at = [&](int half) { return tmem + 128 * half; };
     const auto o_at = [&](int half) { return tmem + 256 + 128 * half; };
-    int4 join = make_int4(0, 0, 0, 0);
-    Piece p;
+    // the next piece: every warp reads it for itself
+    Parcel p;
+    int pieces = 0;
+    const auto next_piece = [&]() {
+        if (!warp_wait(bar(kPieceFull + (pieces & 1)), pieces >> 1 & 1, failed, a.status)) return false;
+        const int4 *from = reinterpret_cast<const int4 *>(parcels + (pieces & 1));
+        int4 *to = reinterpret_cast<int4 *>(&p);
+        to[0] = from[0], to[1] = from[1], to[2] = from[2];
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar(kPieceEmpty + (pieces & 1)));
+        ++pieces;
+        return p.end > p.begin;
+    };
 
     if (warp < 8) {
         // ================================================================ softmax: a row a thread
@@ -245,15 +267,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_mine = s_at(half) + lanes, o_mine = o_at(half) + lanes;
         uint32_t s_phase = 0, o_phase = 0;
-        int tile_count = 0, pieces = 0;  // K and V tiles so far, and pieces: the word `odd` names the last piece that it was set in
+        int tile_count = 0;  // K and V tiles so far (and pieces: the word `odd` names the last piece that it was set in)
         bool ok = true;
-        while (ok && run.next(a, p)) {
-            const Lengths r = p.r;
+        while (ok && next_piece()) {
+            const Lengths r{p.first, p.n, p.kv};
             const int blocks = p.end - p.begin, row0 = p.t * kTileRows, rows = min(kTileRows, r.n * a.group - row0);
             const int row = half * 128 + in_half, first_tile = tile_count;
             tile_count += 2 * blocks;
-            ++pieces;
-            if (p.sharers) join = make_int4(p.request, p.head, p.t, p.sharers);
             if (half * 128 >= rows) continue;
             const bool there = row < rows;
             const int token = there ? (row0 + row) / a.group : 0, head = p.head * a.group + (there ? (row0 + row) % a.group : 0);
@@ -353,6 +373,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             // (all four warps of the half have passed their last block: its barrier came after their arrivals)
             if (words[2 + half] != pieces) {
                 const float inv = sees ? 1.0f / l : 0.0f;
+                const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | a.out_token | a.out_head) & 31) == 0;
                 char *to = a.out + (r.first + token) * a.out_token + head * a.out_head;
                 uint32_t y[32];
 #pragma unroll 1
@@ -360,15 +381,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     tmem_load32(y, o_mine + 32 * c);
                     tmem_load_wait(y);
                     if (there && p.whole) {
+                        // 32 bytes at a time where they are aligned: a thread's row is its own, and halves of a sector take as long
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t h[4];
+                        for (int i = 0; i < 2; ++i) {
+                            uint32_t h[8];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                h[k] = Half16<DT>::from_float(__uint_as_float(y[8 * i + 2 * k]) * inv) |
-                                       static_cast<uint32_t>(Half16<DT>::from_float(__uint_as_float(y[8 * i + 2 * k + 1]) * inv)) << 16;
-                            if (32 * c + 8 * i < a.head_size)
-                                *reinterpret_cast<uint4 *>(to + 2 * (32 * c + 8 * i)) = sees ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(0, 0, 0, 0);
+                            for (int k = 0; k < 8; ++k) {
+                                h[k] = round_pair<DT>(__uint_as_float(y[16 * i + 2 * k]) * inv, __uint_as_float(y[16 * i + 2 * k + 1]) * inv);
+                                if (!sees) h[k] = 0;
+                            }
+                            char *at = to + 2 * (32 * c + 16 * i);
+                            const int left = a.head_size - (32 * c + 16 * i);
+                            if (wide && left >= 16) {
+                                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]), "r"(h[4]),
+                                             "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                            } else {
+                                if (left >= 8) *reinterpret_cast<uint4 *>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+                                if (left >= 16) *reinterpret_cast<uint4 *>(at + 16) = make_uint4(h[4], h[5], h[6], h[7]);
+                            }
                         }
                     } else if (there) {
 #pragma unroll
@@ -398,10 +428,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 }
             }
             fence_before();  // O has been read: the next piece's products follow an arrival of this warp
-        }
-        if (tid == 0 && a.joins) {
-            // (pieces that this half has no rows of are counted above all the same)
-            a.joins[blockIdx.x] = join;
         }
     } else if (warp < 12) {
         // ================================================================ copies
@@ -443,12 +469,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                              : "memory");
             }
         };
-        while (ok && run.next(a, p)) {
-            const Lengths r = p.r;
+        while (ok && next_piece()) {
+            const Lengths r{p.first, p.n, p.kv};
             const int blocks = p.end - p.begin, row0 = p.t * kTileRows, rows = min(kTileRows, r.n * a.group - row0);
             const auto page_for = [&](int j) {
                 const int key = (p.begin + j) * kTileKeys + 32 * w + lane;
-                return j < blocks && key >= p.tile.lo && key < p.tile.hi ? page_of(a, p.request, key / a.page_size) : -1;
+                return j < blocks && key >= p.lo && key < p.hi ? page_of(a, p.request, key / a.page_size) : -1;
             };
             int page = page_for(0);
             // what the products of the piece before need and is still on its way
@@ -525,8 +551,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 if (++stage == kStages) stage = 0, phase ^= 1;
                 return at;
             };
-            while (ok && run.next(a, p)) {
-                const int blocks = p.end - p.begin, rows = min(kTileRows, p.r.n * a.group - p.t * kTileRows), halves = rows > 128 ? 2 : 1;
+            while (ok && next_piece()) {
+                const int blocks = p.end - p.begin, rows = min(kTileRows, p.n * a.group - p.t * kTileRows), halves = rows > 128 ? 2 : 1;
                 if (!(ok = warp_wait(bar(kQFull), q_phase, failed, a.status))) break;
                 q_phase ^= 1;
                 uint32_t k_stage = tile_there(), v_stage = 0;
@@ -578,6 +604,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     if (!ok) break;
                 }
             }
+        }
+        if (warp == 13) {
+            int4 join = make_int4(0, 0, 0, 0);
+            Piece x;
+            bool more = true;
+            for (int i = 0; more; ++i) {
+                more = run.next(a, x);
+                if (more && x.sharers) join = make_int4(x.request, x.head, x.t, x.sharers);
+                if (i >= 2 && !warp_wait(bar(kPieceEmpty + (i & 1)), (i / 2 - 1) & 1, failed, a.status)) break;
+                if (lane == 0) {
+                    Parcel &to = parcels[i & 1];
+                    to = more ? Parcel{x.r.first, x.r.n, x.r.kv, x.request, x.head, x.t, x.begin, x.end, x.tile.lo, x.tile.hi, x.starts, x.whole} : Parcel{};
+                    bar_arrive(bar(kPieceFull + (i & 1)));
+                }
+                __syncwarp();
+            }
+            if (lane == 0 && a.joins) a.joins[blockIdx.x] = join;
         }
         __syncwarp();
     }
