@@ -193,8 +193,9 @@ template <int DP> constexpr int kTileBytes = 128 * DP * 2;
 template <int DP> constexpr int kTileStages = kTileStages128 * 128 / DP;
 template <int DP> constexpr int kBarsAt = (2 + kTileStages<DP>)*kTileBytes<DP>;
 template <int DP> constexpr int kTilesSmem = kBarsAt<DP> + 512 + 1024;  // and what it takes to begin at a multiple of 1024
-enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 2, kOFull = kPFull + 2, kPieceFull = kOFull + 2, kPieceEmpty = kPieceFull + 2,
-       kKvFull = kPieceEmpty + 2 };  // two each of S, P, O and pieces
+enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 2, kOFull = kPFull + 4, kPieceFull = kOFull + 2, kPieceEmpty = kPieceFull + 2,
+       kKvFull = kPieceEmpty + 2 };  // two each of S, O and pieces; P: the first 64 keys' weights of a
+// half, then the others'
 
 // A piece as the scheduling warp hands it to the others, 48 bytes.
 struct __align__(16) Parcel {
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
     const auto full = [&](int s) { return bar(kKvFull + s); };
     const auto empty = [&](int s) { return bar(kKvFull + kStages + s); };
     static_assert(8 * (kKvFull + 2 * kStages) <= 320, "room for the barriers");
-    volatile int *words = reinterpret_cast<volatile int *>(mem + kBarsAt<DP> + 320);  // tensor memory, failed, odd[2]
+    volatile int *words = reinterpret_cast<volatile int *>(mem + kBarsAt<DP> + 320);  // tensor memory, failed
     Parcel *parcels = reinterpret_cast<Parcel *>(mem + kBarsAt<DP> + 384);  // [2]
     volatile int *failed = words + 1;
 
@@ -227,11 +228,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         bar_init(bar(kQEmpty), 1);
         for (int i = 0; i < 2; ++i) {
             bar_init(bar(kSFull + i), 1);
-            bar_init(bar(kPFull + i), 4);
+            bar_init(bar(kPFull + 2 * i), 4);
+            bar_init(bar(kPFull + 2 * i + 1), 4);
             bar_init(bar(kOFull + i), 1);
             bar_init(bar(kPieceFull + i), 1);
             bar_init(bar(kPieceEmpty + i), 13);  // warps that read it
-            words[2 + i] = 0;
         }
         for (int s = 0; s < kStages; ++s) bar_init(full(s), 4), bar_init(empty(s), 1);
         *failed = 0;
@@ -267,13 +268,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_mine = s_at(half) + lanes, o_mine = o_at(half) + lanes;
         uint32_t s_phase = 0, o_phase = 0;
-        int tile_count = 0;  // K and V tiles so far (and pieces: the word `odd` names the last piece that it was set in)
         bool ok = true;
         while (ok && next_piece()) {
             const Lengths r{p.first, p.n, p.kv};
             const int blocks = p.end - p.begin, row0 = p.t * kTileRows, rows = min(kTileRows, r.n * a.group - row0);
-            const int row = half * 128 + in_half, first_tile = tile_count;
-            tile_count += 2 * blocks;
+            const int row = half * 128 + in_half;
             if (half * 128 >= rows) continue;
             const bool there = row < rows;
             const int token = there ? (row0 + row) / a.group : 0, head = p.head * a.group + (there ? (row0 + row) % a.group : 0);
@@ -281,6 +280,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             const int lo = there ? first_key(a, r, token) : 0, hi = there ? last_key(a, r, token) : INT32_MAX;
             const int half_lo = first_key(a, r, (row0 + min(rows, half * 128 + 128) - 1) / a.group), half_hi = last_key(a, r, (row0 + half * 128) / a.group);
             float m = kNegInf, l = 0.0f;
+            bool any_masked = false;
             for (int j = 0; j < blocks; ++j) {
                 const int key = (p.begin + j) * kTileKeys;
                 ok = warp_wait(bar(kSFull + half), s_phase, failed, a.status);
@@ -288,32 +288,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 if (!ok) break;
                 fence_after();
                 const bool masked = key < half_lo || key + kTileKeys > half_hi;  // for one of the half's rows
-                if (masked) {
-                    // values of keys that some rows do not see: are they all finite?
-                    const int t = first_tile + 2 * j + 1;
-                    ok = warp_wait(full(t % kStages), (t / kStages) & 1, failed, a.status);
-                    if (!ok) break;
-                    const unsigned char *v = mem + (2 + t % kStages) * kTileBytes<DP>;
-                    bool odd = false;
-                    constexpr uint32_t e = DT == CG_F16 ? 0x7C00u : 0x7F80u;
-                    for (int i = in_half; i < kTileBytes<DP> / 16; i += 128) {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(v + 16 * i);
-                        for (const uint32_t y : {w.x, w.y, w.z, w.w}) odd = odd || (y & e) == e || ((y >> 16) & e) == e;
-                    }
-                    if (odd) words[2 + half] = pieces;
-                    // scores of keys that a row does not see go back as minus infinity: what follows knows no masks
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t x[32];
-                        tmem_load32(x, s_mine + 32 * c);
-                        tmem_load_wait(x);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (key + 32 * c + i < lo || key + 32 * c + i >= hi) x[i] = __float_as_uint(kNegInf);
-                        tmem_store32(s_mine + 32 * c, x);
-                    }
-                    tmem_store_wait();
-                }
+                any_masked = any_masked || masked;
                 uint32_t x[4][32];
                 tmem_load32(x[0], s_mine);
                 tmem_load32(x[1], s_mine + 32);
@@ -321,11 +296,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 tmem_load_wait(x[1]);
                 tmem_load32(x[2], s_mine + 64);
                 tmem_load32(x[3], s_mine + 96);
+                const uint32_t from = key - lo, count = max(0, hi - lo);  // key + i is seen: from + i < count, without signs
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) x[i / 32][i % 32] = from + i < count ? x[i / 32][i % 32] : __float_as_uint(kNegInf);
+                }
                 float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(x[i / 32][i % 32]), __uint_as_float(x[i / 32][i % 32 + 1]));
                 tmem_load_wait(x[2]);
                 tmem_load_wait(x[3]);
+                if (masked) {
+#pragma unroll
+                    for (int i = 64; i < 128; ++i) x[i / 32][i % 32] = from + i < count ? x[i / 32][i % 32] : __float_as_uint(kNegInf);
+                }
 #pragma unroll
                 for (int i = 64; i < 128; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(x[i / 32][i % 32]), __uint_as_float(x[i / 32][i % 32 + 1]));
                 const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale;
@@ -355,13 +339,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     uint32_t w[16];
                     weigh<DT>(x[c], scale, down, w, sum);
                     tmem_store16(s_mine + 16 * c, w);
+                    if (c & 1) {
+                        tmem_store_wait();
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(bar(kPFull + 2 * half + c / 2));
+                    }
                 }
                 const float2 s0 = parts_of(sum[0]), s1 = parts_of(sum[1]);
                 l += (s0.x + s0.y) + (s1.x + s1.y);
-                tmem_store_wait();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(bar(kPFull + half));
             }
             ok = ok && warp_wait(bar(kOFull + half), o_phase, failed, a.status);
             o_phase ^= 1;
@@ -370,62 +356,74 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             char *part = a.parts + (2 * blockIdx.x + (p.starts ? 1 : 0)) * part_bytes(kTileRows, DP);
             float2 *part_ml = reinterpret_cast<float2 *>(part + kTileRows * DP * 4);
             const bool sees = hi > lo;
-            // (all four warps of the half have passed their last block: its barrier came after their arrivals)
-            if (words[2 + half] != pieces) {
-                const float inv = sees ? 1.0f / l : 0.0f;
-                const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | a.out_token | a.out_head) & 31) == 0;
-                char *to = a.out + (r.first + token) * a.out_token + head * a.out_head;
+            // A value that is not finite, of a key that some rows do not see, is in all rows' sums: those rows are done again, from memory.
+            uint32_t again = 0;
+            if (any_masked) {
+                bool odd = false;
                 uint32_t y[32];
 #pragma unroll 1
                 for (int c = 0; c < DP / 32; ++c) {
                     tmem_load32(y, o_mine + 32 * c);
                     tmem_load_wait(y);
-                    if (there && p.whole) {
-                        // 32 bytes at a time where they are aligned: a thread's row is its own, and halves of a sector take as long
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            uint32_t h[8];
+                    for (int i = 0; i < 32; ++i) odd = odd || (y[i] & 0x7F800000u) == 0x7F800000u;
+                }
+                again = __ballot_sync(0xffffffffu, odd && there);
+            }
+            const float inv = sees ? 1.0f / l : 0.0f;
+            const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | a.out_token | a.out_head) & 31) == 0;
+            char *to = a.out + (r.first + token) * a.out_token + head * a.out_head;
+            uint32_t y[32];
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+                tmem_load32(y, o_mine + 32 * c);
+                tmem_load_wait(y);
+                if (there && p.whole) {
+                    // 32 bytes at a time where they are aligned: a thread's row is its own, and halves of a sector take as long
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                h[k] = round_pair<DT>(__uint_as_float(y[16 * i + 2 * k]) * inv, __uint_as_float(y[16 * i + 2 * k + 1]) * inv);
-                                if (!sees) h[k] = 0;
-                            }
-                            char *at = to + 2 * (32 * c + 16 * i);
-                            const int left = a.head_size - (32 * c + 16 * i);
-                            if (wide && left >= 16) {
-                                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]), "r"(h[4]),
-                                             "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
-                            } else {
-                                if (left >= 8) *reinterpret_cast<uint4 *>(at) = make_uint4(h[0], h[1], h[2], h[3]);
-                                if (left >= 16) *reinterpret_cast<uint4 *>(at + 16) = make_uint4(h[4], h[5], h[6], h[7]);
-                            }
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t h[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            h[k] = round_pair<DT>(__uint_as_float(y[16 * i + 2 * k]) * inv, __uint_as_float(y[16 * i + 2 * k + 1]) * inv);
+                            if (!sees) h[k] = 0;
                         }
-                    } else if (there) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<uint4 *>(part + ((8 * c + i) * kTileRows + row) * 16) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                        char *at = to + 2 * (32 * c + 16 * i);
+                        const int left = a.head_size - (32 * c + 16 * i);
+                        if (wide && left >= 16) {
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]), "r"(h[4]),
+                                         "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                        } else {
+                            if (left >= 8) *reinterpret_cast<uint4 *>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+                            if (left >= 16) *reinterpret_cast<uint4 *>(at + 16) = make_uint4(h[4], h[5], h[6], h[7]);
+                        }
                     }
-                }
-                if (there && p.whole && a.lse)
-                    a.lse[static_cast<int64_t>(r.first + token) * a.q_heads + head] = sees ? (m + log2f(l)) * 0.693147180559945f : kNegInf;
-                if (there && !p.whole) part_ml[row] = make_float2(m, l);
-            } else {
-                for (int i = half * 128 + (warp & 3); i < min(rows, half * 128 + 128); i += 4) {
-                    float x[DP / 32], top, total;
-                    slow_row<DT, DP>(a, r, p.request, p.head, row0 + i, p.begin * kTileKeys, p.end * kTileKeys, x, top, total);
-                    const int tok = (row0 + i) / a.group, hd = p.head * a.group + (row0 + i) % a.group;
-                    const bool any = last_key(a, r, tok) > first_key(a, r, tok);
+                } else if (there) {
 #pragma unroll
-                    for (int c = 0; c < DP / 32; ++c) {
-                        const int d = lane + 32 * c;
-                        if (!p.whole) reinterpret_cast<float *>(part)[(d / 4 * kTileRows + i) * 4 + d % 4] = x[c];
-                        else if (d < a.head_size)
-                            reinterpret_cast<uint16_t *>(a.out + (r.first + tok) * a.out_token + hd * a.out_head)[d] = any ? Half16<DT>::from_float(x[c] / total) : 0;
-                    }
-                    if (lane == 0 && !p.whole) part_ml[i] = make_float2(top, total);
-                    if (lane == 0 && p.whole && a.lse)
-                        a.lse[static_cast<int64_t>(r.first + tok) * a.q_heads + hd] = any ? (top + log2f(total)) * 0.693147180559945f : kNegInf;
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint4 *>(part + ((8 * c + i) * kTileRows + row) * 16) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
                 }
+            }
+            if (there && p.whole && a.lse)
+                a.lse[static_cast<int64_t>(r.first + token) * a.q_heads + head] = sees ? (m + log2f(l)) * 0.693147180559945f : kNegInf;
+            if (there && !p.whole) part_ml[row] = make_float2(m, l);
+            for (; again; again &= again - 1) {
+                const int i = half * 128 + 32 * (warp & 3) + __ffs(again) - 1;
+                __syncwarp();  // (the row has been written once)
+                float x[DP / 32], top, total;
+                slow_row<DT, DP>(a, r, p.request, p.head, row0 + i, p.begin * kTileKeys, p.end * kTileKeys, x, top, total);
+                const int tok = (row0 + i) / a.group, hd = p.head * a.group + (row0 + i) % a.group;
+                const bool any = last_key(a, r, tok) > first_key(a, r, tok);
+#pragma unroll
+                for (int c = 0; c < DP / 32; ++c) {
+                    const int d = lane + 32 * c;
+                    if (!p.whole) reinterpret_cast<float *>(part)[(d / 4 * kTileRows + i) * 4 + d % 4] = x[c];
+                    else if (d < a.head_size)
+                        reinterpret_cast<uint16_t *>(a.out + (r.first + tok) * a.out_token + hd * a.out_head)[d] = any ? Half16<DT>::from_float(x[c] / total) : 0;
+                }
+                if (lane == 0 && !p.whole) part_ml[i] = make_float2(top, total);
+                if (lane == 0 && p.whole && a.lse)
+                    a.lse[static_cast<int64_t>(r.first + tok) * a.q_heads + hd] = any ? (top + log2f(total)) * 0.693147180559945f : kNegInf;
             }
             fence_before();  // O has been read: the next piece's products follow an arrival of this warp
         }
@@ -576,13 +574,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         if (half == halves) break;
-                        if (!(ok = warp_wait(bar(kPFull + half), p_phase >> half & 1, failed, a.status))) break;
-                        p_phase ^= 1 << half;
-                        fence_after();
                         const uint32_t v = v_desc + v_stage * kTile;
+                        if (!(ok = warp_wait(bar(kPFull + 2 * half), p_phase >> half & 1, failed, a.status))) break;
+                        fence_after();
                         if (issues) {
 #pragma unroll
-                            for (int k = 0; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, j > 0 || k > 0);
+                            for (int k = 0; k < 4; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, j > 0 || k > 0);
+                        }
+                        if (!(ok = warp_wait(bar(kPFull + 2 * half + 1), p_phase >> half & 1, failed, a.status))) break;
+                        p_phase ^= 1 << half;
+                        fence_after();
+                        if (issues) {
+#pragma unroll
+                            for (int k = 4; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, j > 0 || k > 0);
                             if (half == halves - 1) commit(empty(v_stage));
                         }
                         if (more && half == 0) k_stage = tile_there();
