@@ -201,7 +201,8 @@ def native_calls():
         raise CacheGenLibraryMissing(f"{build.CALLS} is missing or was built for another torch: build it with "
                                      f"`python -m cachegen_b200.build --force` ({e})") from e
     module.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value
-                 for n in ("cg_decode_kv", "cg_encode_kv", "cg_encode_kv_workspace", "cg_encode_kv_wait", "cg_encode_kv_gather")})
+                 for n in ("cg_decode_kv", "cg_encode_kv", "cg_encode_kv_workspace", "cg_encode_kv_wait", "cg_encode_kv_gather",
+                           "cg_rotary", "cg_append_paged", "cg_gather_paged", "cg_paged_attention_workspace", "cg_paged_attention")})
     return module
 
 

@@ -14,6 +14,14 @@ def decode(*_):
     return None
 
 
+def _left(*_):
+    """No call is taken: cachegen_b200.paged does them all."""
+    return None
+
+
+rotary = append = gather = attend = _left
+
+
 def encode_start(job_at, kv, bins, max_bins, tail_at, workspace, row_off, counts_bytes, on, launch):
     L, _, T, H, D = kv.shape
     dev, lib, job = kv.device, _lib.lib(), _lib.EncodeKvJob.from_address(job_at)

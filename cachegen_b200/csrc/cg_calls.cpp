@@ -31,6 +31,11 @@ decltype(&cg_encode_kv) encode_kv;
 decltype(&cg_encode_kv_workspace) encode_kv_workspace;
 decltype(&cg_encode_kv_wait) encode_kv_wait;
 decltype(&cg_encode_kv_gather) encode_kv_gather;
+decltype(&cg_rotary) rotary_rows;
+decltype(&cg_append_paged) append_rows;
+decltype(&cg_gather_paged) gather_rows;
+decltype(&cg_paged_attention_workspace) attention_workspace;
+decltype(&cg_paged_attention) attention;
 
 // attribute names
 PyObject *s_cdf, *s_max_tensors_key, *s_max_tensors_value, *s_data_chunks, *s_num_heads, *s_head_size, *s_bytestream,
@@ -466,6 +471,243 @@ PyObject *encode_finish(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- calls on a paged cache -------------------------------------------------------------------------
+// Each looks whether its arguments are the usual case, everything of the right shape and type on the current GPU, and then does all of
+// the call.  For any other arguments, wrong ones included, it does nothing: cachegen_b200.paged says what is wrong, or does it.
+enum class Use { kRead, kWritten };
+
+// Rows or pages: a plain strided tensor of this type whose innermost axis is contiguous.
+bool rows_of(PyObject *o, at::ScalarType type, at::Device dev, int64_t dims, Use use, at::Tensor *t) {
+    if (!plain(o)) return false;
+    *t = THPVariable_Unpack(o);
+    if (!t->defined() || !t->unsafeGetTensorImpl()->has_storage() || t->layout() != at::kStrided || t->scalar_type() != type || t->device() != dev ||
+        t->dim() != dims || t->is_conj() || t->is_neg() || t->requires_grad() || (t->stride(dims - 1) != 1 && t->size(dims - 1) > 1))
+        return false;
+    for (int64_t k = 0; use == Use::kWritten && k < dims; ++k)
+        if (t->stride(k) == 0 && t->size(k) > 1) return false;
+    return true;
+}
+bool first_of(PyObject *o, at::Tensor *t, at::Device *dev) {
+    if (!plain(o)) return false;
+    *t = THPVariable_Unpack(o);
+    if (!t->defined() || !is_16bit(t->scalar_type()) || !t->is_cuda()) return false;
+    *dev = t->device();
+    return dev->index() == c10::cuda::current_device();
+}
+bool indices_of(PyObject *o, at::Device dev, bool wide_too, at::Tensor *t) {
+    if (!plain(o)) return false;
+    *t = THPVariable_Unpack(o);
+    return usable(*t, at::kInt, dev) || (wide_too && usable(*t, at::kLong, dev));
+}
+bool apart(const at::Tensor &a, const at::Tensor &b) {
+    const auto end = [](const at::Tensor &t) {
+        int64_t n = 1;
+        for (int64_t k = 0; k < t.dim(); ++k) n += (t.size(k) - 1) * t.stride(k);
+        return static_cast<const char *>(t.data_ptr()) + 2 * n;
+    };
+    return !a.numel() || !b.numel() || end(a) <= static_cast<const char *>(b.data_ptr()) || end(b) <= static_cast<const char *>(a.data_ptr());
+}
+bool same_or_apart(const at::Tensor &a, const at::Tensor &b) { return (a.data_ptr() == b.data_ptr() && a.strides() == b.strides()) || apart(a, b); }
+void strides_of(const at::Tensor &t, int64_t *to, int64_t outer) {  // of all axes but the innermost; a layer axis that is not there: 0
+    const int64_t dims = t.dim() - 1;
+    for (int64_t k = 0; k < outer; ++k) to[k] = k < outer - dims ? 0 : t.stride(k - (outer - dims));
+}
+at::Tensor like(const at::Tensor &t, at::IntArrayRef shape) { return make(shape, t.options()); }
+
+// (turns or None, rotary_dims, interleaved, head size, positions): with them or without them as the job needs it
+bool turning(cg_rows_job *job, PyObject *const *a, at::Device dev, int64_t layers, int64_t tokens, int64_t head, at::Tensor *positions) {
+    if (a[0] == Py_None) return a[4] == Py_None;
+    int64_t rot, of;
+    if (!plain(a[0]) || !small_int(a[1], &rot) || !small_int(a[3], &of) || of != head || !indices_of(a[4], dev, true, positions)) return false;
+    const at::Tensor &turns = THPVariable_Unpack(a[0]);
+    if (!usable(turns, at::kLong, dev) || turns.numel() != rot / 2) return false;
+    if (positions->dim() == 2 && layers >= 0) {
+        if (positions->size(0) != layers || positions->size(1) != tokens) return false;
+        job->pos_layer = layers > 1 ? tokens : 0;
+    } else if (positions->dim() != 1 || positions->size(0) != tokens) {
+        return false;
+    }
+    job->positions = positions->data_ptr();
+    job->wide_positions = positions->scalar_type() == at::kLong;
+    job->turns = static_cast<const uint64_t *>(turns.data_ptr());
+    job->rotary_dims = static_cast<int32_t>(rot);
+    job->interleaved = a[2] == Py_True;
+    return true;
+}
+bool fits(std::initializer_list<int64_t> sizes) {
+    for (const int64_t n : sizes)
+        if (n > INT32_MAX) return false;
+    return true;
+}
+template <class Job> int run(int (*entry)(const Job *, void *), const Job &job, at::Device dev) {
+    void *stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    const WithoutGil released;
+    return entry(&job, stream);
+}
+
+// rotary(x, out or None, inverse, turns, rotary_dims, interleaved, head size, positions) -> out, an error code, or None
+PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor x, out, positions;
+    at::Device dev(at::kCPU);
+    if (n != 8 || !first_of(a[0], &x, &dev) || x.dim() < 3 || x.dim() > 4 || a[3] == Py_None) Py_RETURN_NONE;
+    if (!rows_of(a[0], x.scalar_type(), dev, x.dim(), Use::kRead, &x)) Py_RETURN_NONE;
+    const int64_t d = x.dim(), layers = d == 4 ? x.size(0) : 1, T = x.size(d - 3), H = x.size(d - 2), D = x.size(d - 1);
+    cg_rows_job job{};
+    if (!fits({layers, T, H, D}) || !turning(&job, a + 3, dev, d == 4 ? layers : -1, T, D, &positions)) Py_RETURN_NONE;
+    if (a[1] == Py_None) out = like(x, x.sizes());
+    else if (!rows_of(a[1], x.scalar_type(), dev, d, Use::kWritten, &out) || out.sizes() != x.sizes() || !same_or_apart(x, out)) Py_RETURN_NONE;
+    job.k = x.data_ptr();
+    job.k_out = out.data_ptr();
+    strides_of(x, job.k_strides, 3);
+    strides_of(out, job.k_out_strides, 3);
+    job.dtype = code(x.scalar_type());
+    job.nlayers = static_cast<int32_t>(layers), job.ntokens = static_cast<int32_t>(T), job.heads = static_cast<int32_t>(H);
+    job.head_size = static_cast<int32_t>(D), job.inverse = a[2] == Py_True;
+    const int rc = run(rotary_rows, job, dev);
+    return rc ? PyLong_FromLong(rc) : a[1] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[1]);
+    END_HANDLE_TH_ERRORS
+}
+
+// What append and gather have in common: k, v, k_pages, v_pages, slots, status, turns, rotary_dims, interleaved, head size, positions
+bool pages_job(PyObject *const *a, const at::Tensor &k, const at::Tensor &v, bool append, at::Device dev, cg_rows_job *job, at::Tensor *held) {
+    const int64_t d = k.dim(), layers = d == 4 ? k.size(0) : 1, T = k.size(d - 3), H = k.size(d - 2), D = k.size(d - 1);
+    at::Tensor &kp = held[0], &vp = held[1], &slots = held[2], &status = held[3];
+    const Use pages = append ? Use::kWritten : Use::kRead;
+    if (!rows_of(a[2], k.scalar_type(), dev, d + 1, pages, &kp) || !rows_of(a[3], k.scalar_type(), dev, d + 1, pages, &vp)) return false;
+    const int64_t P = kp.size(d - 3), S = kp.size(d - 2);
+    if (kp.sizes() != vp.sizes() || (d == 4 && kp.size(0) != layers) || kp.size(d - 1) != H || kp.size(d) != D || S == 0) return false;
+    if (!indices_of(a[4], dev, true, &slots) || slots.dim() != 1 || slots.size(0) != T) return false;
+    if (!indices_of(a[5], dev, false, &status) || status.numel() != 1) return false;
+    if (!fits({layers, T, H, D, S}) || !turning(job, a + 6, dev, -1, T, D, held + 4)) return false;
+    if (!apart(k, kp) || !apart(k, vp) || !apart(v, kp) || !apart(v, vp)) return false;
+    job->k = k.data_ptr(), job->v = v.data_ptr(), job->pages_k = kp.data_ptr(), job->pages_v = vp.data_ptr();
+    strides_of(k, job->k_strides, 3);
+    strides_of(v, job->v_strides, 3);
+    strides_of(kp, job->pages_k_strides, 4);
+    strides_of(vp, job->pages_v_strides, 4);
+    job->slots = slots.data_ptr(), job->wide_slots = slots.scalar_type() == at::kLong;
+    job->status = static_cast<int32_t *>(status.data_ptr());
+    job->num_pages = P, job->page_size = static_cast<int32_t>(S);
+    job->dtype = code(k.scalar_type());
+    job->nlayers = static_cast<int32_t>(layers), job->ntokens = static_cast<int32_t>(T), job->heads = static_cast<int32_t>(H);
+    job->head_size = static_cast<int32_t>(D);
+    return true;
+}
+
+// append(k, v, k_pages, v_pages, slots, status, turns, rotary_dims, interleaved, head size, positions, q or None, q_out or None)
+// -> q_out or True, an error code, or None
+PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor k, v, q, q_out, held[5];
+    at::Device dev(at::kCPU);
+    cg_rows_job job{};
+    if (n != 13 || !first_of(a[0], &k, &dev) || k.dim() < 3 || k.dim() > 4 || !rows_of(a[0], k.scalar_type(), dev, k.dim(), Use::kRead, &k) ||
+        !rows_of(a[1], k.scalar_type(), dev, k.dim(), Use::kRead, &v) || v.sizes() != k.sizes() || !pages_job(a, k, v, true, dev, &job, held))
+        Py_RETURN_NONE;
+    const bool queries = a[11] != Py_None;
+    if (!queries && a[12] != Py_None) Py_RETURN_NONE;
+    if (queries) {
+        if (k.dim() != 3 || !rows_of(a[11], k.scalar_type(), dev, 3, Use::kRead, &q) || q.size(0) != k.size(0) || q.size(2) != k.size(2)) Py_RETURN_NONE;
+        if (a[12] == Py_None) q_out = like(q, q.sizes());
+        else if (!rows_of(a[12], k.scalar_type(), dev, 3, Use::kWritten, &q_out) || q_out.sizes() != q.sizes() || !same_or_apart(q, q_out)) Py_RETURN_NONE;
+        job.q = q.data_ptr(), job.q_out = q_out.data_ptr();
+        strides_of(q, job.q_strides, 3);
+        strides_of(q_out, job.q_out_strides, 3);
+        job.q_heads = static_cast<int32_t>(q.size(1));
+    }
+    const int rc = run(append_rows, job, dev);
+    if (rc) return PyLong_FromLong(rc);
+    return !queries ? Py_NewRef(Py_True) : a[12] == Py_None ? THPVariable_Wrap(q_out) : Py_NewRef(a[12]);
+    END_HANDLE_TH_ERRORS
+}
+
+// gather(k or None, v or None, k_pages, v_pages, slots, status, turns, rotary_dims, interleaved, head size, positions)
+// -> (k, v), an error code, or None
+PyObject *gather(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor k, v, pages, slots, held[5];
+    at::Device dev(at::kCPU);
+    if (n != 11 || !first_of(a[2], &pages, &dev) || pages.dim() < 4 || pages.dim() > 5 || !indices_of(a[4], dev, true, &slots) || slots.dim() != 1) Py_RETURN_NONE;
+    std::vector<int64_t> shape(pages.sizes().begin(), pages.sizes().end());
+    shape.erase(shape.end() - 4);
+    shape[shape.size() - 3] = slots.size(0);
+    for (at::Tensor *t : {&k, &v}) {
+        PyObject *const given = t == &k ? a[0] : a[1];
+        if (given == Py_None) *t = like(pages, shape);
+        else if (!rows_of(given, pages.scalar_type(), dev, pages.dim() - 1, Use::kWritten, t) || t->sizes() != at::IntArrayRef(shape)) Py_RETURN_NONE;
+    }
+    cg_rows_job job{};
+    if (!pages_job(a, k, v, false, dev, &job, held)) Py_RETURN_NONE;
+    const int rc = run(gather_rows, job, dev);
+    if (rc) return PyLong_FromLong(rc);
+    return Py_BuildValue("(NN)", a[0] == Py_None ? THPVariable_Wrap(k) : Py_NewRef(a[0]), a[1] == Py_None ? THPVariable_Wrap(v) : Py_NewRef(a[1]));
+    END_HANDLE_TH_ERRORS
+}
+
+// attend(q, k_pages, v_pages, table, kv_lens, q_starts or None, scale, causal, window, max_q, out or None, lse wanted, status)
+// -> out or (out, lse), an error code, or None
+PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor q, kp, vp, table, lens, starts, out, lse, status, workspace;
+    at::Device dev(at::kCPU);
+    int64_t window, max_q;
+    if (n != 13 || !first_of(a[0], &q, &dev) || !rows_of(a[0], q.scalar_type(), dev, 3, Use::kRead, &q) ||
+        !rows_of(a[1], q.scalar_type(), dev, 4, Use::kRead, &kp) || !rows_of(a[2], q.scalar_type(), dev, 4, Use::kRead, &vp) ||
+        !indices_of(a[3], dev, false, &table) || !indices_of(a[4], dev, false, &lens) || !indices_of(a[12], dev, false, &status) ||
+        !PyFloat_CheckExact(a[6]) || !small_int(a[8], &window) || !small_int(a[9], &max_q))
+        Py_RETURN_NONE;
+    const int64_t R = q.size(0), Q = q.size(1), D = q.size(2), P = kp.size(0), S = kp.size(1), H = kp.size(2), B = lens.numel();
+    if (kp.sizes() != vp.sizes() || kp.size(3) != D || D % 8 || D == 0 || D > 128 || S == 0 || H == 0 || Q == 0 || Q % H || lens.dim() != 1 ||
+        B > CG_MAX_REQUESTS || table.dim() != 2 || table.size(0) != B || status.numel() != 1 || window < 0 || max_q < 0 ||
+        !fits({R, Q, H, S, table.size(1), window, max_q}))
+        Py_RETURN_NONE;
+    if (a[5] == Py_None ? R != B : !indices_of(a[5], dev, false, &starts) || starts.dim() != 1 || starts.numel() != B + 1) Py_RETURN_NONE;
+    if (a[10] != Py_None && (!rows_of(a[10], q.scalar_type(), dev, 3, Use::kWritten, &out) || out.sizes() != q.sizes() || !apart(out, q) || !apart(out, kp) ||
+                             !apart(out, vp)))
+        Py_RETURN_NONE;
+    if (a[10] == Py_None) out = like(q, q.sizes());
+    for (const at::Tensor *t : {&q, &kp, &vp, &out}) {
+        if (reinterpret_cast<uintptr_t>(t->data_ptr()) % 16) Py_RETURN_NONE;
+        for (int64_t k = 0; k + 1 < t->dim(); ++k)
+            if (t->stride(k) % 8 && t->size(k) > 1) Py_RETURN_NONE;
+    }
+    cg_attention_job job{};
+    if (a[11] == Py_True) {
+        lse = make({R, Q}, at::TensorOptions().dtype(at::kFloat).device(dev));
+        job.lse = static_cast<float *>(lse.data_ptr());
+    }
+    job.q = q.data_ptr(), job.pages_k = kp.data_ptr(), job.pages_v = vp.data_ptr(), job.out = out.data_ptr();
+    job.table = static_cast<const int32_t *>(table.data_ptr()), job.kv_lens = static_cast<const int32_t *>(lens.data_ptr());
+    job.q_starts = starts.defined() ? static_cast<const int32_t *>(starts.data_ptr()) : nullptr;
+    job.status = static_cast<int32_t *>(status.data_ptr());
+    job.table_row = table.stride(0), job.num_pages = P;
+    const auto steps = [](const at::Tensor &t, int64_t *to) {
+        for (int64_t k = 0; k + 1 < t.dim(); ++k) to[k] = t.size(k) > 1 ? t.stride(k) : 0;
+    };
+    steps(q, job.q_strides);
+    steps(out, job.out_strides);
+    steps(kp, job.pages_k_strides);
+    steps(vp, job.pages_v_strides);
+    job.dtype = code(q.scalar_type());
+    job.nrequests = static_cast<int32_t>(B), job.nrows = static_cast<int32_t>(R), job.q_heads = static_cast<int32_t>(Q);
+    job.heads = static_cast<int32_t>(H), job.head_size = static_cast<int32_t>(D), job.page_size = static_cast<int32_t>(S);
+    job.table_width = static_cast<int32_t>(table.size(1)), job.causal = a[7] == Py_True;
+    job.window = static_cast<int32_t>(window), job.max_q = static_cast<int32_t>(max_q);
+    job.scale = static_cast<float>(PyFloat_AS_DOUBLE(a[6]));
+    const int64_t need = attention_workspace(&job);
+    if (need < 0) return PyLong_FromLongLong(need);
+    if (need) {
+        workspace = make({need}, at::TensorOptions().dtype(at::kByte).device(dev));
+        job.workspace = workspace.data_ptr(), job.workspace_bytes = need;
+    }
+    const int rc = run(attention, job, dev);
+    if (rc) return PyLong_FromLong(rc);
+    PyObject *const result = a[10] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[10]);
+    return a[11] == Py_True ? Py_BuildValue("(NN)", result, THPVariable_Wrap(lse)) : result;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address})
 PyObject *bind(PyObject *, PyObject *addresses) {
     HANDLE_TH_ERRORS
@@ -479,6 +721,11 @@ PyObject *bind(PyObject *, PyObject *addresses) {
     encode_kv_workspace = reinterpret_cast<decltype(encode_kv_workspace)>(address("cg_encode_kv_workspace"));
     encode_kv_wait = reinterpret_cast<decltype(encode_kv_wait)>(address("cg_encode_kv_wait"));
     encode_kv_gather = reinterpret_cast<decltype(encode_kv_gather)>(address("cg_encode_kv_gather"));
+    rotary_rows = reinterpret_cast<decltype(rotary_rows)>(address("cg_rotary"));
+    append_rows = reinterpret_cast<decltype(append_rows)>(address("cg_append_paged"));
+    gather_rows = reinterpret_cast<decltype(gather_rows)>(address("cg_gather_paged"));
+    attention_workspace = reinterpret_cast<decltype(attention_workspace)>(address("cg_paged_attention_workspace"));
+    attention = reinterpret_cast<decltype(attention)>(address("cg_paged_attention"));
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -487,6 +734,10 @@ PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
                          {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL, nullptr},
                          {"encode_start", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(encode_start)), METH_FASTCALL, nullptr},
                          {"encode_finish", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(encode_finish)), METH_FASTCALL, nullptr},
+                         {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
+                         {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
+                         {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gather)), METH_FASTCALL, nullptr},
+                         {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

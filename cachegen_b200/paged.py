@@ -150,6 +150,25 @@ def _turning(job, rotary, positions, device, shape, D):
     job.rotary_dims, job.interleaved = rotary.rotary_dims, rotary.interleaved
 
 
+def _status_of(t):
+    """The status word of a tensor's GPU, None for a tensor on none."""
+    return _status_word(t.device) if t.is_cuda else None
+
+
+def _turns_for(rotary, t):
+    """What the native calls take of a Rotary, for tensors on t's GPU."""
+    if rotary is None or not t.is_cuda:
+        return None, 0, False, 0
+    return rotary.turns(t.device), rotary.rotary_dims, rotary.interleaved, rotary.head_size
+
+
+def _finish(done, what):
+    """The result of a native call; an error code becomes the error."""
+    if type(done) is int:
+        _lib.check(done, what)
+    return done
+
+
 def _run(entry, job, device):
     with on_device(device):
         rc = getattr(_lib.lib(), entry)(ctypes.byref(job), _stream(device))
@@ -176,6 +195,10 @@ def apply_rotary(x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, out: 
     """x [tokens, heads, head_size] or [n, tokens, heads, head_size] with every token turned to its position (`inverse`: back from
     it), in `out` (which may be x) or a new tensor.  positions: int32 or int64 [tokens], or [n, tokens].
     Moving cached keys by d positions is a turn by d: positions of d everywhere."""
+    if rotary is not None:
+        done = _lib.calls().rotary(x, out, inverse, *_turns_for(rotary, x), positions)
+        if done is not None:
+            return _finish(done, "apply_rotary")
     _head(x, "x")
     T, H, D = x.shape[-3:]
     dev = x.device
@@ -241,6 +264,10 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     there are any, are turned to `positions` [tokens] on the way.  Returns the queries: q_out (which may be q) or a new
     tensor.  A token with slot -1 is padding: nothing of it is written, its row of q_out neither.  Each slot belongs to one token:
     of two that name the same, either may be found there, or pieces of both."""
+    done = _lib.calls().append(k, v, k_pages, v_pages, slots, _status_of(k), *_turns_for(rotary, k), positions, q, q_out)
+    if done is not None:
+        done = _finish(done, "append_paged")
+        return None if done is True else done
     _head(k, "k")
     job = _pages_job(k, v, k_pages, v_pages, slots, rotary, positions, True)
     for name, t in (("k", k), ("v", v)):
@@ -267,6 +294,9 @@ def gather_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tens
     """The keys and values of the slots (int32 or int64 [tokens]), as k and v [tokens, heads, head_size] (new tensors if not given);
     of all layers if the pages have a leading axis.  With `rotary` the keys are turned back from `positions` [tokens].  Rows of
     tokens with slot -1 are left as they are."""
+    done = _lib.calls().gather(k, v, k_pages, v_pages, slots, _status_of(k_pages), *_turns_for(rotary, k_pages), positions)
+    if done is not None:
+        return _finish(done, "gather_paged")
     _check(k_pages.is_cuda, "k_pages must be a CUDA tensor")
     _check(k_pages.dtype in _DTYPES, f"k_pages must be float16 or bfloat16, got {k_pages.dtype}")
     _check(k_pages.dim() in (4, 5), "k_pages must have shape [pages, page_size, heads, head_size], with a leading axis for several layers")
@@ -303,6 +333,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     Returns `out` (a new tensor if not given; rows of no request are left as they are), with return_lse also the float32
     logarithm of each row's sum of exponentials [rows, q_heads]."""
+    scale = 1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None else scale
+    done = _lib.calls().attend(q, k_pages, v_pages, page_table, kv_lens, q_starts, scale, causal, window, max_q, out, return_lse, _status_of(q))
+    if done is not None:
+        return _finish(done, "paged_attention")
     _check(q.is_cuda, "q must be a CUDA tensor")
     _check(q.dtype in _DTYPES, f"q must be float16 or bfloat16, got {q.dtype}")
     dev, dtype = q.device, q.dtype
@@ -347,7 +381,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     job.pages_k_strides[:], job.pages_v_strides[:] = _steps(k_pages), _steps(v_pages)
     job.dtype, job.nrequests, job.nrows, job.q_heads, job.heads, job.head_size = _DTYPES[dtype], B, R, Q, H, D
     job.page_size, job.table_width, job.causal, job.window, job.max_q = S, page_table.shape[1], bool(causal), min(window, 2 ** 31 - 1), max_q
-    job.scale = 1.0 / math.sqrt(D) if scale is None else scale
+    job.scale = scale
     with on_device(dev):
         need = _lib.lib().cg_paged_attention_workspace(ctypes.byref(job))
         _lib.check(min(need, 0), "paged_attention")
