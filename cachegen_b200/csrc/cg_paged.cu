@@ -82,6 +82,9 @@ __global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const __grid_co
     const int block_y = blockIdx.x / a.token_blocks, token0 = (blockIdx.x - block_y * a.token_blocks) * a.tokens_per_block;
     const int mine = threadIdx.y / a.head_lanes, token = token0 + mine;
     const int layer1 = min(a.nlayers, (block_y + 1) * a.layers_per_block);
+    bool active = token < a.ntokens;
+    int64_t slot = 0;
+    if (a.slots && active) slot = index_at(a.slots, token, a.wide_slots);  // on its way while cosines are worked out
     // cosines are shared by the block's layers unless every layer has positions of its own; then a block has one layer
     const int64_t pos0 = static_cast<int64_t>(block_y) * a.layers_per_block * a.pos_layer;
     for (int i = tid; i < a.tokens_per_block * half; i += nthreads) {
@@ -94,18 +97,16 @@ __global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const __grid_co
             turned[i] = make_float2(c, a.back ? -s : s);
         }
     }
-    if (half) __syncthreads();
-    if (token >= a.ntokens) return;
     int64_t page = 0;
     int in_page = 0;
-    if (a.slots) {
-        const int64_t slot = index_at(a.slots, token, a.wide_slots);
-        if (slot < 0 || slot >= a.num_slots) {
+    if (a.slots && active) {
+        if (slot < 0 || slot >= a.num_slots) {  // a token of padding, or one that the cache has no place for
             if (slot != -1 && a.status && threadIdx.x == 0) atomicOr(a.status, CG_S_BAD_PAGE);
-            return;  // a token of padding, or one that the cache has no place for
+            active = false;
+        } else {
+            page = slot / a.page_size;
+            in_page = static_cast<int>(slot - page * a.page_size);
         }
-        page = slot / a.page_size;
-        in_page = static_cast<int>(slot - page * a.page_size);
     }
     const int head_lane = threadIdx.y - mine * a.head_lanes;
     int layer = block_y * a.layers_per_block, h = head_lane;
@@ -123,12 +124,8 @@ __global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const __grid_co
         const bool turns = 16 * j < a.rot;
         const int lo = 2 * (turns && !INTERLEAVED ? 8 * j : 16 * j), hi = turns && !INTERLEAVED ? lo + a.rot : lo + 16;  // bytes
         float2 cs[8];
-        if (turns) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) cs[i] = cs_row[8 * j + i];
-        }
         constexpr int kFlight = 2;  // rows of a thread in flight
-        while (true) {
+        for (bool first = true;; first = false) {
             char *to[kFlight];
             uint4 x[kFlight], y[kFlight];
             bool turn[kFlight];
@@ -137,13 +134,20 @@ __global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const __grid_co
                 int which, head;
                 find(which, head);
                 to[u] = nullptr;
-                if (layer < layer1) {
+                if (active && layer < layer1) {
                     const MoveRows &r = a.rows[which];
                     const char *from = row_of(r.src, r.src_paged, layer, token, page, in_page, head);
                     x[u] = *reinterpret_cast<const uint4 *>(from + lo);
                     y[u] = *reinterpret_cast<const uint4 *>(from + hi);
                     to[u] = row_of(r.dst, r.dst_paged, layer, token, page, in_page, head);
                     turn[u] = turns && r.turned;
+                }
+            }
+            if (first && half) {  // the cosines are there, the first rows on their way
+                __syncthreads();
+                if (turns) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) cs[i] = cs_row[8 * j + i];
                 }
             }
 #pragma unroll
@@ -155,6 +159,8 @@ __global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const __grid_co
             }
         }
     } else {
+        if (half) __syncthreads();
+        if (!active) return;
         for (;; h += a.head_lanes) {
             int which, head;
             find(which, head);
@@ -191,17 +197,18 @@ int launch_move(MoveArgs &a, bool interleaved, cudaStream_t st) {
         if (r.heads) vec = vec && vectors(r.src) && vectors(r.dst);
     }
     const int pieces = vec ? a.head_size / 16 : 32, lanes = kMoveThreads / pieces;
-    // Few tokens: a block each, all lanes on its heads, for the shortest time.  Many: a thread goes through eight rows or so, so
-    // that its cosines and its slot are worked out once for them: four tokens a block, then layers.
+    // Few tokens: a block each, all lanes on its heads, for the shortest time.  Many: a thread goes through up to sixteen rows, so that
+    // its cosines and its slot are worked out once for them: four tokens a block, then layers, as long as the blocks fill
+    // every SM twice.
+    const int64_t blocks = static_cast<int64_t>(sm_count()) * 8;
     const int64_t rows = static_cast<int64_t>(a.ntokens) * a.heads * a.nlayers;
-    const int64_t enough = static_cast<int64_t>(sm_count()) * 16 * lanes;  // rows that keep every SM busy twice over
-    a.tokens_per_block = lanes >= 4 && rows / 4 >= enough ? 4 : 1;
+    a.tokens_per_block = lanes >= 4 && rows / (4 * lanes) >= blocks ? 4 : 1;
     a.head_lanes = lanes / a.tokens_per_block;
     if (a.head_lanes > a.heads) a.head_lanes = a.heads;  // (idle lanes would only wait)
     a.layers_per_block = 1;
     if (a.pos_layer == 0) {
-        const int64_t per_layer = (a.heads + a.head_lanes - 1) / a.head_lanes;
-        while (a.layers_per_block < a.nlayers && a.layers_per_block * per_layer < 16 && rows / (8 * a.layers_per_block) >= enough)
+        const int64_t per_layer = (a.heads + a.head_lanes - 1) / a.head_lanes, groups = (a.ntokens + a.tokens_per_block - 1) / a.tokens_per_block;
+        while (a.layers_per_block < a.nlayers && a.layers_per_block * per_layer < 16 && groups * (a.nlayers / (2 * a.layers_per_block)) >= blocks)
             a.layers_per_block *= 2;
     }
     const int64_t gx = (static_cast<int64_t>(a.ntokens) + a.tokens_per_block - 1) / a.tokens_per_block;
