@@ -1,9 +1,10 @@
 // Attention over a paged KV cache: the entry point, and the kernel for few query rows a key/value head (single tokens, drafts).
 //
 // With up to 16 rows a head every cached value is used for few products and the kernel's time is that of reading the cache
-// once.  So a block is there to keep loads in flight: each of its warps walks through 16 keys at a time of its own, with its own
-// ring of asynchronous copies and no barrier of the block, and the warps' sums are joined when the block's piece of the
-// tile ends.  Products are m16n8k16 on fragments in registers: tcgen05 takes 64 rows at least, its accumulator would have to come back from
+// once.  So a block is there to keep loads in flight: four warps walk through 16 keys at a time each, every one with a warp of its own
+// that copies keys and values to a ring for it, and no barrier of the block; the warps' sums are joined when the block's piece of
+// the tile ends, while the next piece's keys are on their way.  Copies are 16 bytes a lane, asynchronous: pages may have any size and
+// strides.  (A bulk copy a row is one instruction for 32 rows, but took 2,400 cycles to issue where these take 500.)  Products are m16n8k16 on fragments in registers: tcgen05 takes 64 rows at least, its accumulator would have to come back from
 // tensor memory for each 16 keys, and at 16 rows the products take less than a fifth of the time that the keys take to arrive.
 #include "cg_attend.cuh"
 
@@ -28,12 +29,14 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// 16 bytes, or zeros where there is nothing to read
-__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+// 16 bytes, or zeros where there is nothing to read; and an arrival at a barrier when the thread's copies so far are there
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void arrive_behind_copies(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void sync_weighing_warps() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <int DT> __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     return Half16<DT>::from_float(lo) | static_cast<uint32_t>(Half16<DT>::from_float(hi)) << 16;
@@ -44,31 +47,86 @@ template <int DT> __device__ __forceinline__ bool not_finite2(uint32_t w) {
     return (w & e) == e || ((w >> 16) & e) == e;
 }
 
-// Shared memory: kWarps rings of kStages stages of 16 keys, then 16 values; rows of 2 * DP bytes, 16-byte pieces in an order
-// (piece ^ row % 8) in which eight rows' pieces of a matrix lie in different banks.  Where the piece ends the same memory holds the warps' sums.
-template <int DP> constexpr int kRingBytes = kStages * 2 * kChunk * DP * 2;
-// Behind it: the warps' maxima and sums, and a word that says whether values that are not finite were met where rows see unlike keys.
+// Shared memory: kWarps rings of kStages stages of 16 keys, then 16 values; rows are 16 bytes longer than their 2 * DP, so that the
+// eight rows of a matrix lie in different banks.  Then room for a part of the warps' sums, their maxima and sums of weights, a word that
+// says whether values that are not finite were met where rows see unlike keys, one that says that a wait was given up, and the stages'
+// barriers.  Two blocks share an SM.
+template <int DP> constexpr int kRowBytes2 = 2 * DP + 16;
+template <int DP> constexpr int kStageBytes = 2 * kChunk * kRowBytes2<DP>;
+template <int DP> constexpr int kRingBytes = kStages * kStageBytes<DP>;
 constexpr int most_of(int x, int y) { return x > y ? x : y; }
-template <int DP> constexpr int kMlAt = most_of(kWarps * kRingBytes<DP>, most_of(kWarps * kRowsM * (DP + 4) * 4, (CG_MAX_REQUESTS + 1) * 8 + 8));
-template <int DP> constexpr int kAttendSmem = kMlAt<DP> + kWarps * kRowsM * 8 + 16;
+constexpr int kSumFloats = 16 * 36;  // of a warp: 16 rows of 32 values or 8 of 64, four more between rows
+template <int DP> constexpr int kSumsAt = most_of(kWarps * kRingBytes<DP>, (CG_MAX_REQUESTS + 1) * 8 + 8);
+template <int DP> constexpr int kMlAt = kSumsAt<DP> + kWarps * kSumFloats * 4;
+template <int DP> constexpr int kAttendSmem = kMlAt<DP> + kWarps * kRowsM * 8 + 16 + 16 * kWarps * kStages;
+static_assert(2 * (kAttendSmem<128> + 1024) <= 228 * 1024, "two blocks an SM");
 
 template <int DT, int DP>
-__global__ void __launch_bounds__(kWarps * 32, 2) attend_rows_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __grid_constant__ AttendArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     float2(*row_ml)[kRowsM] = reinterpret_cast<float2(*)[kRowsM]>(smem + kMlAt<DP>);  // [kWarps]
     volatile int &row_odd = *reinterpret_cast<volatile int *>(smem + kMlAt<DP> + kWarps * kRowsM * 8);
-    constexpr int kPieces = DP / 8, kSteps = DP / 16;  // 16-byte pieces of a row; 16-value steps
-    constexpr int kRowsAtOnce = 32 / kPieces;          // rows that a warp copies with one instruction
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int g = lane >> 2, q2 = 2 * (lane & 3);
+    constexpr int kSteps = DP / 16, kRow = kRowBytes2<DP>;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, (tid >> 5) % kWarps, 0);
+    const bool copies = tid >= kWarps * 32;
     const uint32_t ring = smem_addr(smem) + warp * kRingBytes<DP>;
+    volatile int *failed = &row_odd + 1;
+    const uint32_t full = smem_addr(smem) + kMlAt<DP> + kWarps * kRowsM * 8 + 16 + 16 * kStages * warp, empty = full + 8 * kStages;
 
     Run<kRowsM, kRowsBK, kRowsCost> run;
-    run.template init<kWarps * 32, false>(a, reinterpret_cast<int64_t *>(smem));
+    run.template init<kWarps * 64, false>(a, reinterpret_cast<int64_t *>(smem));
     let_next_launch_start();
-    int4 join = make_int4(0, 0, 0, 0);
-    if (tid == 0) row_odd = 0;
+    if (tid == 0) row_odd = 0, *failed = 0;
+    if (!copies && lane == 0) {
+        for (int i = 0; i < kStages; ++i) bar_init(full + 8 * i, 32), bar_init(empty + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    uint32_t stage = 0, phase = 0;  // of the next chunk, of all pieces
+    bool ok = true;
     Piece p;
+    if (copies) {
+        // ================================================================ keys and values to the ring of warp `warp`
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");  // 128 threads of 56 and 128 of 200 registers: the 256 x 128 of the launch
+        constexpr int kPieces = DP / 8, kRowsAtOnce = 32 / kPieces;  // 16-byte pieces of a row; rows that a warp copies with one instruction
+        const int piece = lane % kPieces, in_head = 8 * piece < a.head_size ? 16 : 0;
+        const uint32_t place = ring + lane / kPieces * kRow + 16 * piece;
+        bool round = false;  // whether the stages have been used
+        while (ok && run.next(a, p)) {
+            const int nchunks = p.end - p.begin, key0 = p.begin * kRowsBK + warp * kChunk + (lane & 15);
+            const char *const keys = a.k + p.head * a.k_head + 16 * piece, *const values = a.v + p.head * a.v_head + 16 * piece;
+            const auto page_for = [&](int chunk) {  // lanes i and 16 + i: of key i
+                const int key = key0 + chunk * kRowsBK;
+                return chunk < nchunks && key >= p.tile.lo && key < p.tile.hi ? page_of(a, p.request, key / a.page_size) : -1;
+            };
+            int page = page_for(0);
+#pragma unroll 1
+            for (int chunk = 0; chunk < nchunks; ++chunk) {
+                const int in_page = (key0 + chunk * kRowsBK) % a.page_size;
+                // lanes below 16 have the keys' places, the others the values'
+                const int64_t at = lane < 16 ? page * a.k_page + in_page * a.k_token : page * a.v_page + in_page * a.v_token;
+                const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+                page = page_for(chunk + 1);
+                if (round && !(ok = warp_wait(empty + 8 * stage, phase ^ 1, failed, a.status))) break;
+                const uint32_t to = place + stage * kStageBytes<DP>;
+#pragma unroll
+                for (int i = 0; i < kChunk / kRowsAtOnce; ++i) {
+                    const int row = i * kRowsAtOnce + lane / kPieces;
+                    const int64_t k_at = __shfl_sync(0xffffffffu, at, row), v_at = __shfl_sync(0xffffffffu, at, 16 + row);
+                    const int bytes = there >> row & 1 ? in_head : 0;
+                    copy16(to + i * kRowsAtOnce * kRow, bytes ? keys + k_at : a.k, bytes);
+                    copy16(to + (kChunk + i * kRowsAtOnce) * kRow, bytes ? values + v_at : a.v, bytes);
+                }
+                arrive_behind_copies(full + 8 * stage);
+                if (++stage == kStages) stage = 0, phase ^= 1, round = true;
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        return;
+    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int g = lane >> 2, q2 = 2 * (lane & 3);
+    int4 join = make_int4(0, 0, 0, 0);
     while (run.next(a, p)) {
         const Lengths r = p.r;
         const int rows = min(kRowsM, r.n * a.group - p.t * kRowsM), row0 = p.t * kRowsM;
@@ -95,54 +153,24 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_rows_kernel(const __gri
         const int nchunks = p.end - p.begin;
         const int key0 = p.begin * kRowsBK + warp * kChunk;
 
-        // ---- copies: lane i (and i + 16) knows where key i of the chunk lies
-        const auto page_for = [&](int chunk) {
-            const int key = key0 + chunk * kRowsBK + (lane & 15);
-            return chunk < nchunks && key >= p.tile.lo && key < p.tile.hi ? page_of(a, p.request, key / a.page_size) : -1;
-        };
-        int page = page_for(0);
-        const auto fetch = [&](int chunk) {
-            if (chunk < nchunks) {
-                const int key = key0 + chunk * kRowsBK + (lane & 15), in_page = key % a.page_size;
-                const int64_t at_k = page * a.k_page + in_page * a.k_token + p.head * a.k_head;
-                const int64_t at_v = page * a.v_page + in_page * a.v_token + p.head * a.v_head;
-                const bool there = page >= 0;
-                const uint32_t to = ring + chunk % kStages * (2 * kChunk * DP * 2);
-                const int piece = lane % kPieces;
-#pragma unroll
-                for (int i = 0; i < kChunk / kRowsAtOnce; ++i) {
-                    const int row = i * kRowsAtOnce + lane / kPieces;
-                    const int64_t from_k = __shfl_sync(0xffffffffu, at_k, row), from_v = __shfl_sync(0xffffffffu, at_v, row);
-                    const bool copy = __shfl_sync(0xffffffffu, there, row) && 8 * piece < a.head_size;
-                    const uint32_t dst = to + row * (2 * DP) + ((piece ^ (row & 7)) << 4);
-                    copy16(dst, copy ? a.k + from_k + 16 * piece : a.k, copy);
-                    copy16(dst + kChunk * DP * 2, copy ? a.v + from_v + 16 * piece : a.v, copy);
-                }
-            }
-            copies_end_group();
-            page = page_for(chunk + 1);
-        };
-#pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) fetch(i);
-
         float o[kSteps * 2][4], m[2] = {kNegInf, kNegInf}, l[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kSteps * 2; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) o[i][k] = 0.0f;
         bool odd = false;
-        // this lane's row and piece of the four matrices of an ldmatrix
-        const int k_row = (lane & 7) + ((lane >> 4) << 3), k_piece = (lane >> 3) & 1;
-        const int v_row = lane & 15, v_piece = lane >> 4;
+        // this lane's row of the four matrices of an ldmatrix
+        const uint32_t k_row = ((lane & 7) + ((lane >> 4) << 3)) * kRow + (((lane >> 3) & 1) << 4), v_row = (kChunk + (lane & 15)) * kRow + ((lane >> 4) << 4);
+#pragma unroll 1
         for (int chunk = 0; chunk < nchunks; ++chunk) {
-            copies_wait<kStages - 2>();
-            __syncwarp();
-            const uint32_t k_at = ring + chunk % kStages * (2 * kChunk * DP * 2), v_at = k_at + kChunk * DP * 2;
+            ok = ok && warp_wait(full + 8 * stage, phase, failed, a.status);
+            if (!ok) break;
+            const uint32_t at = ring + stage * kStageBytes<DP>;
             float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
                 uint32_t b[4];
-                ldmatrix4(b, k_at + k_row * (2 * DP) + (((2 * k + k_piece) ^ (k_row & 7)) << 4));
+                ldmatrix4(b, at + k_row + 32 * k);
                 mma16816<DT>(s[0], qf[k], b[0], b[1]);
                 mma16816<DT>(s[1], qf[k], b[2], b[3]);
             }
@@ -151,10 +179,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_rows_kernel(const __gri
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int j = key + 8 * i + q2 + (k & 1);
-                    s[i][k] = all || (j >= lo[k >> 1] && j < hi[k >> 1]) ? s[i][k] * a.scale : kNegInf;
-                }
+                for (int k = 0; k < 4; ++k) s[i][k] *= a.scale;
+            if (!all) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int j = key + 8 * i + q2 + (k & 1);
+                        if (j < lo[k >> 1] || j >= hi[k >> 1]) s[i][k] = kNegInf;
+                    }
+            }
             float top[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -186,15 +220,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_rows_kernel(const __gri
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
                 uint32_t b[4];
-                ldmatrix4_trans(b, v_at + v_row * (2 * DP) + (((2 * k + v_piece) ^ (v_row & 7)) << 4));
+                ldmatrix4_trans(b, at + v_row + 32 * k);
                 if (!all) odd = odd || not_finite2<DT>(b[0]) || not_finite2<DT>(b[1]) || not_finite2<DT>(b[2]) || not_finite2<DT>(b[3]);
                 mma16816<DT>(o[2 * k], w, b[0], b[1]);
                 mma16816<DT>(o[2 * k + 1], w, b[2], b[3]);
             }
             __syncwarp();
-            fetch(chunk + kStages - 1);
+            if (lane == 0) bar_arrive(empty + 8 * stage);
+            if (++stage == kStages) stage = 0, phase ^= 1;
         }
-        copies_wait<0>();
         // ---- the warps' sums become one
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -203,64 +237,115 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attend_rows_kernel(const __gri
             if ((lane & 3) == 0) row_ml[warp][g + 8 * i] = make_float2(m[i], l[i]);
         }
         if (odd) row_odd = 1;
-        __syncthreads();
-        float *sums = reinterpret_cast<float *>(smem);  // [kWarps][kRowsM][DP + 4]
+        sync_weighing_warps();
         const bool slow = row_odd;
+        float keep[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float top = kNegInf;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) top = fmaxf(top, row_ml[k][g + 8 * i].x);
+            keep[i] = top == kNegInf ? 1.0f : exp2_approx(m[i] - top);
+        }
+        const int width = rows <= 8 ? 64 : 32;  // values of a row at a time
+        float *const sums = reinterpret_cast<float *>(smem + kSumsAt<DP>);  // [kWarps][rows][width + 4]
+        char *part = a.parts + (2 * blockIdx.x + (p.starts ? 1 : 0)) * part_bytes(kRowsM, DP);
         if (!slow) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float top = kNegInf;
+            for (int first = 0; first < DP; first += 32) {
+                if (first % width) continue;
+                if (first) sync_weighing_warps();
 #pragma unroll
-                for (int k = 0; k < kWarps; ++k) top = fmaxf(top, row_ml[k][g + 8 * i].x);
-                const float keep = top == kNegInf ? 1.0f : exp2_approx(m[i] - top);
-                float *to = sums + (warp * kRowsM + g + 8 * i) * (DP + 4) + q2;
+                for (int i = 0; i < 2; ++i) {
+                    if (i == 1 && width == 64) break;  // no more than eight rows
+                    float *to = sums + warp * kSumFloats + (g + 8 * i) * (width + 4) + q2;
 #pragma unroll
-                for (int k = 0; k < kSteps * 2; ++k) *reinterpret_cast<float2 *>(to + 8 * k) = make_float2(o[k][2 * i] * keep, o[k][2 * i + 1] * keep);
+                    for (int k = 0; k < 8; ++k) {
+                        if (first / 8 + k >= kSteps * 2 || 8 * k >= width) break;
+                        *reinterpret_cast<float2 *>(to + 8 * k) = make_float2(o[first / 8 + k][2 * i] * keep[i], o[first / 8 + k][2 * i + 1] * keep[i]);
+                    }
+                }
+                sync_weighing_warps();
+                for (int i = tid; i < rows * (width / 4); i += kWarps * 32) {
+                    const int row = i / (width / 4), col = 4 * (i % (width / 4));
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    float top = kNegInf, total = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < kWarps; ++k) {
+                        const float4 y = *reinterpret_cast<const float4 *>(sums + k * kSumFloats + row * (width + 4) + col);
+                        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+                        top = fmaxf(top, row_ml[k][row].x);
+                    }
+                    const float base = top == kNegInf ? 0.0f : top;
+#pragma unroll
+                    for (int k = 0; k < kWarps; ++k) total += exp2_approx(row_ml[k][row].x - base) * row_ml[k][row].y;
+                    if (p.whole) {
+                        store_joined<DT>(a, r, row0 + row, p.head, first + col, top, total, x);
+                    } else {
+                        *reinterpret_cast<float4 *>(part + (row * DP + first + col) * 4) = x;
+                        if (first + col == 0) reinterpret_cast<float2 *>(part + kRowsM * DP * 4)[row] = make_float2(top, total);
+                    }
+                }
             }
         } else {
             for (int row = warp; row < rows; row += kWarps) {
                 float x[DP / 32], top, total;
                 slow_row<DT, DP>(a, r, p.request, p.head, row0 + row, p.begin * kRowsBK, p.end * kRowsBK, x, top, total);
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) sums[row * (DP + 4) + lane + 32 * i] = x[i];
-                if (lane == 0) row_ml[0][row] = make_float2(top, total);
-            }
-        }
-        __syncthreads();
-        const int nparts = slow ? 1 : kWarps;
-        char *part = a.parts + (2 * blockIdx.x + (p.starts ? 1 : 0)) * part_bytes(kRowsM, DP);
-        for (int i = tid; i < rows * (DP / 4); i += kWarps * 32) {
-            const int row = i / (DP / 4), col = 4 * (i % (DP / 4));
-            float4 x = *reinterpret_cast<const float4 *>(sums + row * (DP + 4) + col);
-            float top = row_ml[0][row].x;
-            for (int k = 1; k < nparts; ++k) {
-                const float4 y = *reinterpret_cast<const float4 *>(sums + (k * kRowsM + row) * (DP + 4) + col);
-                x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-                top = fmaxf(top, row_ml[k][row].x);
-            }
-            const float base = top == kNegInf ? 0.0f : top;
-            float total = 0.0f;
-            for (int k = 0; k < nparts; ++k) total += exp2_approx(row_ml[k][row].x - base) * row_ml[k][row].y;
-            if (p.whole) {
-                const int at = row0 + row, token = at / a.group, head = p.head * a.group + at % a.group;
-                const bool sees = last_key(a, r, token) > first_key(a, r, token);
-                const float inv = 1.0f / total;
-                if (col < a.head_size) {
-                    const uint2 y = make_uint2(pack_pair<DT>(x.x * inv, x.y * inv), pack_pair<DT>(x.z * inv, x.w * inv));
-                    *reinterpret_cast<uint2 *>(a.out + (r.first + token) * a.out_token + head * a.out_head + 2 * col) = sees ? y : make_uint2(0u, 0u);
+                for (int i = 0; i < DP / 32; ++i) sums[warp * kSumFloats + lane + 32 * i] = x[i];
+                __syncwarp();
+                if (4 * lane < DP) {
+                    const float4 y = *reinterpret_cast<const float4 *>(sums + warp * kSumFloats + 4 * lane);
+                    if (p.whole) store_joined<DT>(a, r, row0 + row, p.head, 4 * lane, top, total, y);
+                    else *reinterpret_cast<float4 *>(part + (row * DP + 4 * lane) * 4) = y;
                 }
-                if (a.lse && col == 0)
-                    a.lse[static_cast<int64_t>(r.first + token) * a.q_heads + head] = sees ? (base + log2f(total)) * 0.693147180559945f : kNegInf;
-            } else {
-                *reinterpret_cast<float4 *>(part + i * 16) = x;
-                if (col == 0) reinterpret_cast<float2 *>(part + kRowsM * DP * 4)[row] = make_float2(top, total);
+                if (lane == 0 && !p.whole) reinterpret_cast<float2 *>(part + kRowsM * DP * 4)[row] = make_float2(top, total);
+                __syncwarp();
             }
         }
         if (p.sharers) join = make_int4(p.request, p.head, p.t, p.sharers);
-        if (tid == 0) row_odd = 0;  // (read by all in front of the barrier before)
-        __syncthreads();
+        if (slow) sync_weighing_warps();  // (all have read the word)
+        if (tid == 0) row_odd = 0;
+        sync_weighing_warps();
     }
     if (tid == 0 && a.joins) a.joins[blockIdx.x] = join;
+}
+
+// Joins what the CTAs of a divided tile have left.  Block i: the tile that begins in CTA i, if one does that is divided.  One long request
+// alone has few tiles, and each is divided among dozens of CTAs: the parts are spread over the block's threads.
+template <int DT, int DP>
+__global__ void __launch_bounds__(512) combine_rows_kernel(const __grid_constant__ AttendArgs a) {
+    __shared__ float4 sums[512];
+    __shared__ float2 tops[512];
+    wait_for_launch_before();
+    const int c = blockIdx.x, tid = threadIdx.x;
+    const int4 join = __ldcg(a.joins + c);
+    if (join.w == 0) return;
+    const Lengths r = lengths_of(a, join.x);
+    const int rows = min(kRowsM, r.n * a.group - join.z * kRowsM), items = rows * (DP / 4), lanes = 512 / items;
+    const int item = tid % items, part = tid / items, row = item / (DP / 4), col = 4 * (item % (DP / 4));
+    float top = kNegInf, total = 0.0f;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const auto add = [&](float2 ml, float4 x) {
+        const float now = fmaxf(top, ml.x), base = now == kNegInf ? 0.0f : now;
+        const float keep = exp2_approx(top - base), w = exp2_approx(ml.x - base);
+        total = total * keep + ml.y * w;
+        sum.x = sum.x * keep + x.x * w, sum.y = sum.y * keep + x.y * w, sum.z = sum.z * keep + x.z * w, sum.w = sum.w * keep + x.w * w;
+        top = now;
+    };
+    if (part < lanes) {
+#pragma unroll 4
+        for (int i = part; i < join.w; i += lanes) {
+            const char *p = a.parts + (2 * (c + i) + (i == 0)) * part_bytes(kRowsM, DP);
+            add(__ldcg(reinterpret_cast<const float2 *>(p + kRowsM * DP * 4) + row), __ldcg(reinterpret_cast<const float4 *>(p) + item));
+        }
+        sums[tid] = sum;
+        tops[tid] = make_float2(top, total);
+    }
+    __syncthreads();
+    if (part != 0) return;
+    for (int i = 1; i < lanes; ++i) add(tops[i * items + item], sums[i * items + item]);
+    store_joined<DT>(a, r, join.z * kRowsM + row, join.y, col, top, total, sum);
 }
 
 template <int DT, int DP>
@@ -268,9 +353,9 @@ int launch_attend_rows(const AttendArgs &a, int ctas, cudaStream_t st) {
     constexpr int smem = kAttendSmem<DP>;
     int rc = allow_smem(attend_rows_kernel<DT, DP>, smem);
     if (rc) return rc;
-    rc = launch(attend_rows_kernel<DT, DP>, dim3(ctas), kWarps * 32, smem, false, st, a);
+    rc = launch(attend_rows_kernel<DT, DP>, dim3(ctas), kWarps * 64, smem, false, st, a);
     if (rc || !a.joins) return rc;
-    return launch(combine_kernel<DT, kRowsM, DP, false>, dim3(ctas, kRowsM * (DP / 4) / 256), 256, 0, true, st, a);
+    return launch(combine_rows_kernel<DT, DP>, dim3(ctas), 512, 0, true, st, a);
 }
 
 // What a call launches, from what the host knows: the tensors' sizes.

@@ -136,8 +136,13 @@ template <int M, int BK, int COST> struct Run {
         const int c = blockIdx.x;
         at = to = 0;
         if (c < ctas) {
-            at = total * c / ctas;
-            to = total * (c + 1) / ctas;
+            if (total < (1 << 20) && ctas < (1 << 11)) {  // (a 64-bit division takes a hundred instructions)
+                at = static_cast<uint32_t>(total) * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);
+                to = static_cast<uint32_t>(total) * static_cast<uint32_t>(c + 1) / static_cast<uint32_t>(ctas);
+            } else {
+                at = total * c / ctas;
+                to = total * (c + 1) / ctas;
+            }
             int lo = 0, hi = a.nrequests - 1;  // the last request that begins at or before `at` and has rows
             while (lo < hi) {
                 const int mid = (lo + hi + 1) / 2;
@@ -147,10 +152,17 @@ template <int M, int BK, int COST> struct Run {
             b = lo;
             r = lengths_of(a, b);
             tiles = tiles_of<M>(a, r);
-            const int64_t per_head = (before[b + 1] - before[b]) / a.heads;
             int64_t rest = at - before[b];
-            h = static_cast<int>(rest / per_head);
-            rest -= h * per_head;
+            const int64_t of_request = before[b + 1] - before[b];
+            if (of_request < INT32_MAX) {
+                const uint32_t per_head = static_cast<uint32_t>(of_request) / static_cast<uint32_t>(a.heads);
+                h = static_cast<int>(static_cast<uint32_t>(rest) / per_head);
+                rest -= static_cast<int64_t>(h) * per_head;
+            } else {
+                const int64_t per_head = of_request / a.heads;
+                h = static_cast<int>(rest / per_head);
+                rest -= h * per_head;
+            }
             for (int first = 0;; first += 32) {  // 32 tiles at a time: how many end in front of `rest`
                 int s = first + lane < tiles ? tile_of<M, BK>(a, r, first + lane).units + COST : 0;
                 for (int d = 1; d < 32; d <<= 1) {
@@ -190,7 +202,9 @@ template <int M, int BK, int COST> struct Run {
             p.starts = begin == 0;
             p.whole = p.starts && end == p.tile.units;
             p.sharers = 0;
-            if (p.starts && !p.whole) p.sharers = static_cast<int>(((at + left) * ctas - 1) / total) - static_cast<int>(blockIdx.x) + 1;
+            if (p.starts && !p.whole)
+                p.sharers = (total < (1 << 20) ? static_cast<int>((static_cast<uint32_t>(at + left) * static_cast<uint32_t>(ctas) - 1) / static_cast<uint32_t>(total))
+                                               : static_cast<int>(((at + left) * ctas - 1) / total)) - static_cast<int>(blockIdx.x) + 1;
             at += take;
             skip = 0;
             ++t;
@@ -254,9 +268,65 @@ __device__ __forceinline__ void slow_row(const AttendArgs &a, const Lengths &r, 
     }
 }
 
-// Joins what the CTAs of a divided tile have left.  Block (i, j): rows j * ROWS .. of the tile that begins in CTA i.  COLUMNS: sums are stored
-// [DP / 4][M][4], as a kernel with a row a thread writes them side by side; else [M][DP].
-template <int DT, int M, int DP, bool COLUMNS>
+constexpr uint64_t kGiveUpNs = 10ull * 1000 * 1000 * 1000;  // a wait takes microseconds, or the length of a slow row
+// ---- barriers in shared memory --------------------------------------------------------------
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done;
+}
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+// Whether the phase ended.  If it does not within kGiveUpNs, or another wait of the block gave up, the block is told to end.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
+    uint64_t start = 0;
+#pragma unroll 1
+    for (uint32_t n = 1; !bar_try(bar, parity); ++n) {
+        if (n & 255) continue;
+        if (*failed) return false;
+        const uint64_t now = now_ns();
+        if (!start) start = now;
+        if (now - start > kGiveUpNs) {
+            *failed = 1;
+            if (status) atomicOr(status, CG_S_TIMEOUT);
+            return false;
+        }
+    }
+    return true;
+}
+// the same for a whole warp, with one result
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
+    return __all_sync(0xffffffffu, bar_wait(bar, parity, failed, status));
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, int bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// Values col .. col + 3 of row `at` of a request and key/value head, from a joined maximum, sum of weights and sums.
+template <int DT>
+__device__ __forceinline__ void store_joined(const AttendArgs &a, const Lengths &r, int at, int kv_head, int col, float top, float total, float4 sum) {
+    const int token = at / a.group, head = kv_head * a.group + at % a.group;
+    const bool sees = last_key(a, r, token) > first_key(a, r, token);
+    const float inv = 1.0f / total;
+    if (col < a.head_size) {
+        const uint16_t h[4] = {Half16<DT>::from_float(sum.x * inv), Half16<DT>::from_float(sum.y * inv), Half16<DT>::from_float(sum.z * inv),
+                               Half16<DT>::from_float(sum.w * inv)};
+        const uint2 y = make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
+        *reinterpret_cast<uint2 *>(a.out + (r.first + token) * a.out_token + head * a.out_head + 2 * col) = sees ? y : make_uint2(0u, 0u);
+    }
+    if (a.lse && col == 0)
+        a.lse[static_cast<int64_t>(r.first + token) * a.q_heads + head] =
+            sees ? ((top == kNegInf ? 0.0f : top) + log2f(total)) * 0.693147180559945f : kNegInf;
+}
+
+// Joins what the CTAs of a divided tile of many rows have left.  Block (i, j): rows j * kRows .. of the tile that begins in CTA i.  Sums are
+// stored [DP / 4][M][4], as a kernel with a row a thread writes them side by side.
+template <int DT, int M, int DP>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttendArgs a) {
     constexpr int kRows = 256 / (DP / 4);
     wait_for_launch_before();
@@ -264,12 +334,13 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
     const int4 join = __ldcg(a.joins + c);
     if (join.w == 0) return;
     const int tid = threadIdx.x;
-    const int row = blockIdx.y * kRows + (COLUMNS ? tid % kRows : tid / (DP / 4)), col = 4 * (COLUMNS ? tid / kRows : tid % (DP / 4));
+    const int row = blockIdx.y * kRows + tid % kRows, col = 4 * (tid / kRows);
     const Lengths r = lengths_of(a, join.x);
     const int64_t at = static_cast<int64_t>(join.z) * M + row;
     if (at >= static_cast<int64_t>(r.n) * a.group) return;
     const char *part = a.parts + (2 * c + 1) * part_bytes(M, DP);
     float top = kNegInf;
+#pragma unroll 4
     for (int i = 0; i < join.w; ++i) {
         const char *p = i ? a.parts + 2 * (c + i) * part_bytes(M, DP) : part;
         top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(p + M * DP * 4) + row).x);
@@ -281,21 +352,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
     for (int i = 0; i < join.w; ++i) {
         const char *p = i ? a.parts + 2 * (c + i) * part_bytes(M, DP) : part;
         const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + M * DP * 4) + row);
-        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p) + (COLUMNS ? col / 4 * M + row : row * (DP / 4) + col / 4));
+        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p) + col / 4 * M + row);
         const float w = exp2_approx(ml.x - base);
         total += w * ml.y;
         sum.x += w * x.x, sum.y += w * x.y, sum.z += w * x.z, sum.w += w * x.w;
     }
-    const int token = static_cast<int>(at / a.group), head = join.y * a.group + static_cast<int>(at % a.group);
-    const bool sees = last_key(a, r, token) > first_key(a, r, token);
-    const float inv = sees ? 1.0f / total : 0.0f;
-    if (col < a.head_size) {
-        uint16_t h[4] = {Half16<DT>::from_float(sees ? sum.x * inv : 0.0f), Half16<DT>::from_float(sees ? sum.y * inv : 0.0f),
-                         Half16<DT>::from_float(sees ? sum.z * inv : 0.0f), Half16<DT>::from_float(sees ? sum.w * inv : 0.0f)};
-        *reinterpret_cast<uint2 *>(a.out + (r.first + token) * a.out_token + head * a.out_head + 2 * col) = *reinterpret_cast<uint2 *>(h);
-    }
-    if (a.lse && col == 0)
-        a.lse[static_cast<int64_t>(r.first + token) * a.q_heads + head] = sees ? (base + log2f(total)) * 0.693147180559945f : kNegInf;
+    store_joined<DT>(a, r, static_cast<int>(at), join.y, col, top, total, sum);
 }
 
 // cg_attend_tiles.cu

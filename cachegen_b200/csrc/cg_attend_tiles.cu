@@ -24,42 +24,6 @@ namespace {
 
 constexpr int kTileThreads = 512;
 constexpr int kTileStages128 = 5;  // K or V tiles of 128 keys x 128 values
-constexpr uint64_t kGiveUpNs = 10ull * 1000 * 1000 * 1000;  // a wait takes microseconds, or the length of a slow row
-
-// ---- barriers in shared memory --------------------------------------------------------------
-__device__ __forceinline__ void bar_init(uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
-__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    return done;
-}
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-// Whether the phase ended.  If it does not within kGiveUpNs, or another wait of the block gave up, the block is told to end.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
-    uint64_t start = 0;
-#pragma unroll 1
-    for (uint32_t n = 1; !bar_try(bar, parity); ++n) {
-        if (n & 255) continue;
-        if (*failed) return false;
-        const uint64_t now = now_ns();
-        if (!start) start = now;
-        if (now - start > kGiveUpNs) {
-            *failed = 1;
-            if (status) atomicOr(status, CG_S_TIMEOUT);
-            return false;
-        }
-    }
-    return true;
-}
-// the same for a whole warp, with one result
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
-    return __all_sync(0xffffffffu, bar_wait(bar, parity, failed, status));
-}
 
 __device__ __forceinline__ bool elect_one() {
     uint32_t yes;
@@ -72,9 +36,6 @@ struct PageMaps {  // of keys and values [pages, heads, page_size, head_size]; r
     CUtensorMap k, v;
     int32_t rows;  // tokens of a box
 };
-__device__ __forceinline__ void bar_expect(uint32_t bar, int bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void tma_box(uint32_t to, const CUtensorMap *map, int value, int token, int head, int page, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map),
                  "r"(value), "r"(token), "r"(head), "r"(page), "r"(bar) : "memory");
@@ -671,7 +632,7 @@ template <int DT, int DP> int launch_tiles(const AttendArgs &a, int ctas, cudaSt
     if (rc) return rc;
     rc = launch(attend_tiles_kernel<DT, DP>, dim3(ctas), kTileThreads, smem, false, st, a, maps);
     if (rc || !a.joins) return rc;
-    return launch(combine_kernel<DT, kTileRows, DP, true>, dim3(ctas, kTileRows * (DP / 4) / 256), 256, 0, true, st, a);
+    return launch(combine_kernel<DT, kTileRows, DP>, dim3(ctas, kTileRows * (DP / 4) / 256), 256, 0, true, st, a);
 }
 
 }  // namespace
