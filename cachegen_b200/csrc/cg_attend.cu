@@ -126,27 +126,39 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
     }
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int g = lane >> 2, q2 = 2 * (lane & 3);
-    int4 join = make_int4(0, 0, 0, 0);
-    while (run.next(a, p)) {
-        const Lengths r = p.r;
-        const int rows = min(kRowsM, r.n * a.group - p.t * kRowsM), row0 = p.t * kRowsM;
-        // ---- this thread's two rows: the keys that they see, and the queries as fragments
-        int lo[2], hi[2];
-        uint32_t qf[kSteps][4];
+    Join join{};
+    uint32_t qf[kSteps][4];
+    const auto queries = [&](const Piece &x) {  // as fragments
+        const int rows = min(kRowsM, x.r.n * a.group - x.t * kRowsM);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int row = g + 8 * i, at = row0 + row, token = at / a.group;
-            const bool there = row < rows;
-            lo[i] = there ? first_key(a, r, token) : 0;
-            hi[i] = there ? last_key(a, r, token) : 0;
-            const char *q = a.q + (r.first + token) * a.q_token + (p.head * a.group + at % a.group) * a.q_head;
+            const int row = g + 8 * i, at = x.t * kRowsM + row, token = at / a.group;
+            const char *q = a.q + (x.r.first + token) * a.q_token + (x.head * a.group + at - token * a.group) * a.q_head + 2 * q2;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int d = 16 * s + 8 * k + q2;
-                    qf[s][i + 2 * k] = there && d < a.head_size ? __ldg(reinterpret_cast<const unsigned int *>(q + 2 * d)) : 0u;
-                }
+                for (int k = 0; k < 2; ++k) qf[s][i + 2 * k] = 0u;
+            if (row < rows) {
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        if (DP == a.head_size || 16 * s + 8 * k < a.head_size)
+                            qf[s][i + 2 * k] = __ldg(reinterpret_cast<const unsigned int *>(q + 2 * (16 * s + 8 * k)));
+            }
+        }
+    };
+    bool more = run.next(a, p);
+    if (more) queries(p);
+    while (more) {
+        const Lengths r = p.r;
+        const int rows = min(kRowsM, r.n * a.group - p.t * kRowsM), row0 = p.t * kRowsM;
+        int lo[2], hi[2];  // the keys that this thread's two rows see
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = g + 8 * i, token = (row0 + row) / a.group;
+            lo[i] = row < rows ? first_key(a, r, token) : 0;
+            hi[i] = row < rows ? last_key(a, r, token) : 0;
         }
         // chunks inside [all_lo, all_hi) are seen by all rows
         const int all_lo = first_key(a, r, (row0 + rows - 1) / a.group), all_hi = last_key(a, r, row0 / a.group);
@@ -229,6 +241,9 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
             if (lane == 0) bar_arrive(empty + 8 * stage);
             if (++stage == kStages) stage = 0, phase ^= 1;
         }
+        Piece next;
+        more = run.next(a, next);
+        if (more) queries(next);  // on their way while this piece ends
         // ---- the warps' sums become one
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -303,26 +318,28 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
                 __syncwarp();
             }
         }
-        if (p.sharers) join = make_int4(p.request, p.head, p.t, p.sharers);
+        if (p.sharers) join = join_for(p);
         if (slow) sync_weighing_warps();  // (all have read the word)
         if (tid == 0) row_odd = 0;
         sync_weighing_warps();
+        p = next;
     }
     if (tid == 0 && a.joins) a.joins[blockIdx.x] = join;
 }
 
+constexpr int kJoinThreads = 1024;
 // Joins what the CTAs of a divided tile have left.  Block i: the tile that begins in CTA i, if one does that is divided.  One long request
 // alone has few tiles, and each is divided among dozens of CTAs: the parts are spread over the block's threads.
 template <int DT, int DP>
-__global__ void __launch_bounds__(512) combine_rows_kernel(const __grid_constant__ AttendArgs a) {
-    __shared__ float4 sums[512];
-    __shared__ float2 tops[512];
+__global__ void __launch_bounds__(kJoinThreads) combine_rows_kernel(const __grid_constant__ AttendArgs a) {
+    __shared__ float4 sums[kJoinThreads];
+    __shared__ float2 tops[kJoinThreads];
     wait_for_launch_before();
     const int c = blockIdx.x, tid = threadIdx.x;
-    const int4 join = __ldcg(a.joins + c);
-    if (join.w == 0) return;
-    const Lengths r = lengths_of(a, join.x);
-    const int rows = min(kRowsM, r.n * a.group - join.z * kRowsM), items = rows * (DP / 4), lanes = 512 / items;
+    const Join join = join_of(a, c);
+    if (join.sharers == 0) return;
+    const Lengths r{join.first, join.n, join.kv};
+    const int rows = min(kRowsM, r.n * a.group - join.t * kRowsM), items = rows * (DP / 4), lanes = kJoinThreads / items;
     const int item = tid % items, part = tid / items, row = item / (DP / 4), col = 4 * (item % (DP / 4));
     float top = kNegInf, total = 0.0f;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -335,7 +352,7 @@ __global__ void __launch_bounds__(512) combine_rows_kernel(const __grid_constant
     };
     if (part < lanes) {
 #pragma unroll 4
-        for (int i = part; i < join.w; i += lanes) {
+        for (int i = part; i < join.sharers; i += lanes) {
             const char *p = a.parts + (2 * (c + i) + (i == 0)) * part_bytes(kRowsM, DP);
             add(__ldcg(reinterpret_cast<const float2 *>(p + kRowsM * DP * 4) + row), __ldcg(reinterpret_cast<const float4 *>(p) + item));
         }
@@ -345,7 +362,7 @@ __global__ void __launch_bounds__(512) combine_rows_kernel(const __grid_constant
     __syncthreads();
     if (part != 0) return;
     for (int i = 1; i < lanes; ++i) add(tops[i * items + item], sums[i * items + item]);
-    store_joined<DT>(a, r, join.z * kRowsM + row, join.y, col, top, total, sum);
+    store_joined<DT>(a, r, join.t * kRowsM + row, join.head, col, top, total, sum);
 }
 
 template <int DT, int DP>
@@ -355,7 +372,7 @@ int launch_attend_rows(const AttendArgs &a, int ctas, cudaStream_t st) {
     if (rc) return rc;
     rc = launch(attend_rows_kernel<DT, DP>, dim3(ctas), kWarps * 64, smem, false, st, a);
     if (rc || !a.joins) return rc;
-    return launch(combine_rows_kernel<DT, DP>, dim3(ctas), 512, 0, true, st, a);
+    return launch(combine_rows_kernel<DT, DP>, dim3(ctas), kJoinThreads, 0, true, st, a);
 }
 
 // What a call launches, from what the host knows: the tensors' sizes.
@@ -383,7 +400,7 @@ int plan_of(const cg_attention_job &j, Plan &p) {
     const int64_t tiles = (static_cast<int64_t>(j.nrows) * group / M + j.nrequests) * j.heads;  // at most
     const int64_t slots = static_cast<int64_t>(sm_count()) * (p.tiles ? 1 : 2);
     p.ctas = static_cast<int>(per_tile > slots || tiles * per_tile > slots ? slots : tiles * per_tile);
-    p.bytes = per_tile > 1 ? p.ctas * (2 * part_bytes(M, p.dp) + static_cast<int64_t>(sizeof(int4))) : 0;
+    p.bytes = per_tile > 1 ? p.ctas * (2 * part_bytes(M, p.dp) + static_cast<int64_t>(sizeof(Join))) : 0;
     return CG_OK;
 }
 
@@ -419,7 +436,7 @@ extern "C" int cg_paged_attention(const cg_attention_job *job, void *stream) {
     a.table = j.table, a.kv_lens = j.kv_lens, a.q_starts = j.q_starts, a.status = j.status;
     if (p.bytes) {
         a.parts = static_cast<char *>(j.workspace);
-        a.joins = reinterpret_cast<int4 *>(a.parts + p.bytes - p.ctas * static_cast<int64_t>(sizeof(int4)));
+        a.joins = reinterpret_cast<Join *>(a.parts + p.bytes - p.ctas * static_cast<int64_t>(sizeof(Join)));
     }
     a.q_token = 2 * j.q_strides[0], a.q_head = 2 * j.q_strides[1], a.out_token = 2 * j.out_strides[0], a.out_head = 2 * j.out_strides[1];
     a.k_page = 2 * j.pages_k_strides[0], a.k_token = 2 * j.pages_k_strides[1], a.k_head = 2 * j.pages_k_strides[2];

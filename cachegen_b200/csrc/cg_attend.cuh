@@ -12,13 +12,19 @@
 
 namespace cg {
 
+// The divided tile that begins in a CTA: what joins its parts needs to know of it.
+struct __align__(16) Join {
+    int32_t sharers;  // CTAs that have a part of it, 0: none begins here
+    int32_t first, n, kv, head, t, unused[2];
+};
+
 struct AttendArgs {
     const char *q, *k, *v;
     char *out;
     float *lse;
     const int32_t *table, *kv_lens, *q_starts;
     char *parts;    // [ctas][2] rows of sums, see part_bytes
-    int4 *joins;    // [ctas]: request, head, tile of the divided tile that begins in this CTA, CTAs that share it (0: none)
+    Join *joins;    // [ctas]
     int32_t *status;
     int64_t q_token, q_head, out_token, out_head, k_page, k_token, k_head, v_page, v_token, v_head;  // bytes
     int64_t table_row, num_pages;
@@ -97,6 +103,29 @@ template <int M, int BK, int COST> struct Run {
     template <int THREADS, bool MANY_TILES>
     __device__ __forceinline__ void init(const AttendArgs &a, int64_t *before) {
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+        if (!MANY_TILES && a.nrequests <= 32) {  // every warp by itself, a request a lane: no memory, no barriers
+            Lengths x{0, 0, 0};
+            int64_t units = 0;
+            if (lane < a.nrequests) {
+                x = lengths_of(a, lane, blockIdx.x == 0 && warp == 0);
+                const int n = tiles_of<M>(a, x);
+                for (int k = 0; k < n; ++k) units += tile_of<M, BK>(a, x, k).units + COST;
+            }
+            int64_t end = units * a.heads;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, end, d);
+                if (lane >= d) end += o;
+            }
+            total = __shfl_sync(0xffffffffu, end, 31);
+            share();
+            if (at < to) {
+                b = __popc(__ballot_sync(0xffffffffu, end <= at));  // requests that end at or in front of `at`
+                const int64_t begin = __shfl_sync(0xffffffffu, end - units * a.heads, b);
+                r = Lengths{__shfl_sync(0xffffffffu, x.first, b), __shfl_sync(0xffffffffu, x.n, b), __shfl_sync(0xffffffffu, x.kv, b)};
+                find(a, at - begin, __shfl_sync(0xffffffffu, units, b));
+            }
+            return;
+        }
         if (MANY_TILES) {
             for (int i = warp; i < a.nrequests; i += THREADS / 32) {
                 const Lengths x = lengths_of(a, i, blockIdx.x == 0 && lane == 0);
@@ -132,17 +161,8 @@ template <int M, int BK, int COST> struct Run {
         }
         __syncthreads();
         total = before[a.nrequests];
-        ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
-        const int c = blockIdx.x;
-        at = to = 0;
-        if (c < ctas) {
-            if (total < (1 << 20) && ctas < (1 << 11)) {  // (a 64-bit division takes a hundred instructions)
-                at = static_cast<uint32_t>(total) * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);
-                to = static_cast<uint32_t>(total) * static_cast<uint32_t>(c + 1) / static_cast<uint32_t>(ctas);
-            } else {
-                at = total * c / ctas;
-                to = total * (c + 1) / ctas;
-            }
+        share();
+        if (at < to) {
             int lo = 0, hi = a.nrequests - 1;  // the last request that begins at or before `at` and has rows
             while (lo < hi) {
                 const int mid = (lo + hi + 1) / 2;
@@ -151,33 +171,48 @@ template <int M, int BK, int COST> struct Run {
             }
             b = lo;
             r = lengths_of(a, b);
-            tiles = tiles_of<M>(a, r);
-            int64_t rest = at - before[b];
             const int64_t of_request = before[b + 1] - before[b];
-            if (of_request < INT32_MAX) {
-                const uint32_t per_head = static_cast<uint32_t>(of_request) / static_cast<uint32_t>(a.heads);
-                h = static_cast<int>(static_cast<uint32_t>(rest) / per_head);
-                rest -= static_cast<int64_t>(h) * per_head;
-            } else {
-                const int64_t per_head = of_request / a.heads;
-                h = static_cast<int>(rest / per_head);
-                rest -= h * per_head;
-            }
-            for (int first = 0;; first += 32) {  // 32 tiles at a time: how many end in front of `rest`
-                int s = first + lane < tiles ? tile_of<M, BK>(a, r, first + lane).units + COST : 0;
-                for (int d = 1; d < 32; d <<= 1) {
-                    const int o = __shfl_up_sync(0xffffffffu, s, d);
-                    if (lane >= d) s += o;
-                }
-                const int n = __popc(__ballot_sync(0xffffffffu, s <= rest && first + lane < tiles));
-                const int gone = __shfl_sync(0xffffffffu, s, n ? n - 1 : 0);
-                t = first + n;
-                if (n) rest -= gone;
-                if (n < 32) break;
-            }
-            skip = static_cast<int>(rest);
+            find(a, at - before[b], of_request < INT32_MAX ? static_cast<uint32_t>(of_request) / static_cast<uint32_t>(a.heads) : of_request / a.heads);
         }
         __syncthreads();  // the numbers' memory is free again
+    }
+
+    // This CTA's run: [at, to) of `total`.
+    __device__ __forceinline__ void share() {
+        const int c = blockIdx.x;
+        ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+        at = to = 0;
+        if (c >= ctas) return;
+        if (small()) {
+            at = static_cast<uint32_t>(total) * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);
+            to = static_cast<uint32_t>(total) * static_cast<uint32_t>(c + 1) / static_cast<uint32_t>(ctas);
+        } else {
+            at = total * c / ctas;
+            to = total * (c + 1) / ctas;
+        }
+    }
+    // whether products of a place and the number of CTAs are numbers of 32 bits (a 64-bit division takes a hundred instructions)
+    __device__ __forceinline__ bool small() const { return total < (1 << 20) && ctas < (1 << 11); }
+
+    // Head, tile and blocks in it of place `rest` of request b, whose lengths are in r; by a warp.
+    __device__ __forceinline__ void find(const AttendArgs &a, int64_t rest, int64_t per_head) {
+        const int lane = threadIdx.x & 31;
+        tiles = tiles_of<M>(a, r);
+        h = static_cast<int>(rest < INT32_MAX && per_head < INT32_MAX ? static_cast<uint32_t>(rest) / static_cast<uint32_t>(per_head) : rest / per_head);
+        rest -= h * per_head;
+        for (int first = 0;; first += 32) {  // 32 tiles at a time: how many end at or in front of `rest`
+            int s = first + lane < tiles ? tile_of<M, BK>(a, r, first + lane).units + COST : 0;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, s, d);
+                if (lane >= d) s += o;
+            }
+            const int n = __popc(__ballot_sync(0xffffffffu, s <= rest && first + lane < tiles));
+            const int gone = __shfl_sync(0xffffffffu, s, n ? n - 1 : 0);
+            t = first + n;
+            if (n) rest -= gone;
+            if (n < 32) break;
+        }
+        skip = static_cast<int>(rest);
     }
 
     __device__ __forceinline__ bool next(const AttendArgs &a, Piece &p) {
@@ -202,9 +237,11 @@ template <int M, int BK, int COST> struct Run {
             p.starts = begin == 0;
             p.whole = p.starts && end == p.tile.units;
             p.sharers = 0;
-            if (p.starts && !p.whole)
-                p.sharers = (total < (1 << 20) ? static_cast<int>((static_cast<uint32_t>(at + left) * static_cast<uint32_t>(ctas) - 1) / static_cast<uint32_t>(total))
-                                               : static_cast<int>(((at + left) * ctas - 1) / total)) - static_cast<int>(blockIdx.x) + 1;
+            if (p.starts && !p.whole) {
+                const int last = small() ? static_cast<int>((static_cast<uint32_t>(at + left) * static_cast<uint32_t>(ctas) - 1) / static_cast<uint32_t>(total))
+                                         : static_cast<int>(((at + left) * ctas - 1) / total);
+                p.sharers = last - static_cast<int>(blockIdx.x) + 1;
+            }
             at += take;
             skip = 0;
             ++t;
@@ -307,6 +344,14 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, int bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
+__device__ __forceinline__ Join join_of(const AttendArgs &a, int c) {
+    Join j;
+    const int4 *from = reinterpret_cast<const int4 *>(a.joins + c);
+    reinterpret_cast<int4 *>(&j)[0] = __ldcg(from), reinterpret_cast<int4 *>(&j)[1] = __ldcg(from + 1);
+    return j;
+}
+__device__ __forceinline__ Join join_for(const Piece &p) { return Join{p.sharers, p.r.first, p.r.n, p.r.kv, p.head, p.t, {0, 0}}; }
+
 // Values col .. col + 3 of row `at` of a request and key/value head, from a joined maximum, sum of weights and sums.
 template <int DT>
 __device__ __forceinline__ void store_joined(const AttendArgs &a, const Lengths &r, int at, int kv_head, int col, float top, float total, float4 sum) {
@@ -331,17 +376,17 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
     constexpr int kRows = 256 / (DP / 4);
     wait_for_launch_before();
     const int c = blockIdx.x;
-    const int4 join = __ldcg(a.joins + c);
-    if (join.w == 0) return;
+    const Join join = join_of(a, c);
+    if (join.sharers == 0) return;
     const int tid = threadIdx.x;
     const int row = blockIdx.y * kRows + tid % kRows, col = 4 * (tid / kRows);
-    const Lengths r = lengths_of(a, join.x);
-    const int64_t at = static_cast<int64_t>(join.z) * M + row;
+    const Lengths r{join.first, join.n, join.kv};
+    const int64_t at = static_cast<int64_t>(join.t) * M + row;
     if (at >= static_cast<int64_t>(r.n) * a.group) return;
     const char *part = a.parts + (2 * c + 1) * part_bytes(M, DP);
     float top = kNegInf;
 #pragma unroll 4
-    for (int i = 0; i < join.w; ++i) {
+    for (int i = 0; i < join.sharers; ++i) {
         const char *p = i ? a.parts + 2 * (c + i) * part_bytes(M, DP) : part;
         top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(p + M * DP * 4) + row).x);
     }
@@ -349,7 +394,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
     float total = 0.0f;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (int i = 0; i < join.w; ++i) {
+    for (int i = 0; i < join.sharers; ++i) {
         const char *p = i ? a.parts + 2 * (c + i) * part_bytes(M, DP) : part;
         const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + M * DP * 4) + row);
         const float4 x = __ldcg(reinterpret_cast<const float4 *>(p) + col / 4 * M + row);
@@ -357,7 +402,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
         total += w * ml.y;
         sum.x += w * x.x, sum.y += w * x.y, sum.z += w * x.z, sum.w += w * x.w;
     }
-    store_joined<DT>(a, r, static_cast<int>(at), join.y, col, top, total, sum);
+    store_joined<DT>(a, r, static_cast<int>(at), join.head, col, top, total, sum);
 }
 
 // cg_attend_tiles.cu

@@ -571,12 +571,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             }
         }
         if (warp == 13) {
-            int4 join = make_int4(0, 0, 0, 0);
+            Join join{};
             Piece x;
             bool more = true;
             for (int i = 0; more; ++i) {
                 more = run.next(a, x);
-                if (more && x.sharers) join = make_int4(x.request, x.head, x.t, x.sharers);
+                if (more && x.sharers) join = join_for(x);
                 if (i >= 2 && !warp_wait(bar(kPieceEmpty + (i & 1)), (i / 2 - 1) & 1, failed, a.status)) break;
                 if (lane == 0) {
                     Parcel &to = parcels[i & 1];
