@@ -397,6 +397,23 @@ def _steps(t):
     return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
 
 
+def split_pages(pages: torch.Tensor, fmt: str) -> tuple:
+    """Keys and values of a cache of all layers, as the calls above take them: [layers, 2, pages, page_size, heads, head_size] ("vllm")
+    or [layers, 2, pages, heads, page_size, head_size] ("huggingface")."""
+    _check(pages.dim() == 6 and pages.shape[1] == 2, "pages must have shape [layers, 2, pages, ...] with six dimensions")
+    if fmt == "huggingface":
+        pages = pages.transpose(3, 4)
+    return pages[:, 0], pages[:, 1]
+
+
+def split_blob(kv: torch.Tensor, fmt: str) -> tuple:
+    """Keys and values [layers, tokens, heads, head_size] of a KV blob: [layers, 2, tokens, heads, head_size] ("vllm") or
+    [layers, 2, heads, tokens, head_size] ("huggingface")."""
+    if fmt == "huggingface":
+        kv = kv.transpose(2, 3)
+    return kv[:, 0], kv[:, 1]
+
+
 def check_status(device=None) -> None:
     """Synchronises and raises if a kernel met a slot, page or length that does not fit since the last check (the
     status word is that of cachegen_b200.torchac_cuda.check_status)."""

@@ -611,6 +611,53 @@ class CacheGenDeserializer(Deserializer):
         return decode_many(encoder_outputs, self._bins_on(_device_of(encoder_outputs[0])), self.fmt, self.out_dtype,
                            out=out, workspace=self._workspace, delta=self.delta, host_bins=self._host_bins)
 
+    def decode_paged(self, encoder_outputs: List[CacheGenGPUEncoderOutput], pages: torch.Tensor, slots: torch.Tensor, rotary=None,
+                     positions: torch.Tensor = None) -> None:
+        """Consecutive chunks of one KV cache into a paged cache of all layers: decode_many into a blob that lasts as long as the call,
+        then cachegen_b200.paged.append_paged.  pages: [L, 2, pages, page_size, H, D] ("vllm") or [L, 2, pages, H, page_size, D]
+        ("huggingface"), whose type is decoded to; slots: where each token goes, int32 or int64.  With `rotary` (paged.Rotary) the keys are turned
+        to `positions`: of chunks whose keys were stored without positions the tokens' places; of others how far they move."""
+        from .. import paged
+        if not encoder_outputs:
+            raise RuntimeError("nothing to decode")
+        for eo in encoder_outputs:
+            if _chunk_tokens(eo) > self.chunk_size:
+                raise RuntimeError(f"a blob holds more tokens than chunk_size = {self.chunk_size}")
+        k_pages, v_pages = self._paged_parts(pages, slots, sum(_chunk_tokens(eo) for eo in encoder_outputs), encoder_outputs[0])
+        with on_device(pages.device):
+            kv = decode_many(encoder_outputs, self._bins_on(pages.device), self.fmt, pages.dtype, workspace=self._workspace, delta=self.delta,
+                             host_bins=self._host_bins)
+            if kv.device != pages.device:
+                raise RuntimeError(f"the chunks are on {kv.device}, the pages on {pages.device}")
+            paged.append_paged(*paged.split_blob(kv, self.fmt), k_pages, v_pages, slots, rotary=rotary, positions=positions)
+
+    def from_bytes_paged(self, blobs: List[bytes], pages: torch.Tensor, slots: torch.Tensor, rotary=None,
+                         positions: torch.Tensor = None) -> None:
+        """from_bytes_many into a paged cache of all layers, as decode_paged.  The pages' type is this object's out_dtype."""
+        from .. import paged
+        if pages.dtype != self.out_dtype:
+            raise TypeError(f"the pages are {pages.dtype}, this deserializer decodes to {self.out_dtype}: see its out_dtype argument")
+        with on_device(pages.device):
+            kv = self.from_bytes_many(blobs)
+            if kv.device != pages.device:
+                raise RuntimeError(f"the chunks are on {kv.device}, the pages on {pages.device}")
+            k, v = paged.split_blob(kv, self.fmt)
+            k_pages, v_pages = self._paged_parts(pages, slots, k.shape[1], None)
+            paged.append_paged(k, v, k_pages, v_pages, slots, rotary=rotary, positions=positions)
+
+    def _paged_parts(self, pages, slots, ntokens, chunk):
+        """Keys and values of the pages, checked as far as they can be in front of a decode."""
+        from .. import paged
+        if not pages.is_cuda or pages.dtype not in _DTYPES:
+            raise RuntimeError("pages must be a float16 or bfloat16 CUDA tensor")
+        k_pages, v_pages = paged.split_pages(pages, self.fmt)
+        L, _, _, H, D = k_pages.shape
+        if L != self._bins.numel() // 2 or chunk is not None and (H, D) != (chunk.num_heads, chunk.head_size):
+            raise RuntimeError(f"the pages have {L} layers of {H} heads of {D} values, which are not the chunks'")
+        if tuple(slots.shape) != (ntokens,):
+            raise RuntimeError(f"slots has shape {tuple(slots.shape)}, the chunks have {ntokens} tokens")
+        return k_pages, v_pages
+
     def decode_many_host(self, encoder_outputs: List[CacheGenGPUEncoderOutput], out: torch.Tensor = None,
                          groups: int = None) -> torch.Tensor:
         """decode_many for chunks whose tensors sit in pinned host memory: copies and decodes overlap.

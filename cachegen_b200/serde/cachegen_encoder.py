@@ -597,6 +597,12 @@ def encode_flat(kv: torch.Tensor, key_bins: torch.Tensor, value_bins: torch.Tens
 _settings_of = operator.attrgetter(*[f.name for f in dataclasses.fields(CacheGenConfig)])
 
 
+def _on_pages(pages: torch.Tensor):
+    if not pages.is_cuda:
+        raise RuntimeError("pages must be a CUDA tensor")
+    return on_device(pages.device)
+
+
 class CacheGenSerializer(Serializer):
     """Reference: enc.py:303-348.  `cachegen_config` may be given instead of looking it up from
     metadata.model_name (quality levels other than the built-in ones).  wire_format: "pickle" (the
@@ -669,6 +675,30 @@ class CacheGenSerializer(Serializer):
         ntokens = tensor.shape[2]
         return encode_function(tensor.cuda(), self.cachegen_config, self._key_bins, self._value_bins, ntokens,
                                max_bins=self.table_max_bins, delta=self.delta, info=self._bins())
+
+    def _from_pages(self, pages: torch.Tensor, slots: torch.Tensor, rotary, positions) -> torch.Tensor:
+        """The slots' tokens of a paged cache of all layers as a blob in this object's format."""
+        from .. import paged
+        k_pages, v_pages = paged.split_pages(pages, self.fmt)
+        L, _, _, H, D = k_pages.shape
+        if slots.dim() != 1 or slots.shape[0] == 0:
+            raise RuntimeError("slots must have one dimension and name a token at least")
+        kv = torch.empty((L, 2, slots.shape[0], H, D), dtype=pages.dtype, device=pages.device)
+        paged.gather_paged(k_pages, v_pages, slots, k=kv[:, 0], v=kv[:, 1], rotary=rotary, positions=positions)
+        return kv.permute(0, 1, 3, 2, 4) if self.fmt == "huggingface" else kv
+
+    def encode_paged(self, pages: torch.Tensor, slots: torch.Tensor, rotary=None,
+                     positions: torch.Tensor = None) -> CacheGenGPUEncoderOutput:
+        """`encode` of tokens of a paged cache of all layers, [L, 2, pages, page_size, H, D] ("vllm") or [L, 2, pages, H, page_size, D]
+        ("huggingface"): those in `slots` (int32 or int64, each a slot of the cache), in that order.  With `rotary` (paged.Rotary) the keys
+        are turned back from `positions` first, so that the chunk can be used at other places."""
+        with _on_pages(pages):
+            return self.encode(self._from_pages(pages, slots, rotary, positions))
+
+    def to_bytes_paged(self, pages: torch.Tensor, slots: torch.Tensor, rotary=None, positions: torch.Tensor = None) -> bytes:
+        """`to_bytes` of tokens of a paged cache, as encode_paged."""
+        with _on_pages(pages):
+            return self.to_bytes(self._from_pages(pages, slots, rotary, positions))
 
     def encode_many(self, tensor: torch.Tensor, chunk_tokens: int = None, batch: int = 16, streams: int = 3) -> list:
         """A whole KV cache, one encoded chunk per `chunk_tokens` (default: the configured chunk size)
