@@ -369,40 +369,40 @@ __device__ __forceinline__ void store_joined(const AttendArgs &a, const Lengths 
             sees ? ((top == kNegInf ? 0.0f : top) + log2f(total)) * 0.693147180559945f : kNegInf;
 }
 
-// Joins what the CTAs of a divided tile of many rows have left.  Block (i, j): rows j * kRows .. of the tile that begins in CTA i.  Sums are
-// stored [DP / 4][M][4], as a kernel with a row a thread writes them side by side.
+// Joins what the CTAs of a divided tile of many rows have left.  Block (i, j): 64 rows of the tile that begins in CTA i, a row a thread,
+// eight 16-byte pieces of it, all on their way together.  Sums are stored [DP / 4][M][4], as a kernel with a row a thread writes
+// them side by side.
 template <int DT, int M, int DP>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttendArgs a) {
-    constexpr int kRows = 256 / (DP / 4);
+__global__ void __launch_bounds__(64 * (DP / 32)) combine_kernel(const __grid_constant__ AttendArgs a) {
     wait_for_launch_before();
-    const int c = blockIdx.x;
+    const int c = blockIdx.x, row = blockIdx.y * 64 + threadIdx.x % 64, piece0 = threadIdx.x / 64 * 8;
     const Join join = join_of(a, c);
     if (join.sharers == 0) return;
-    const int tid = threadIdx.x;
-    const int row = blockIdx.y * kRows + tid % kRows, col = 4 * (tid / kRows);
     const Lengths r{join.first, join.n, join.kv};
     const int64_t at = static_cast<int64_t>(join.t) * M + row;
     if (at >= static_cast<int64_t>(r.n) * a.group) return;
-    const char *part = a.parts + (2 * c + 1) * part_bytes(M, DP);
-    float top = kNegInf;
-#pragma unroll 4
+    float top = kNegInf, total = 0.0f;
+    float4 sum[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int i = 0; i < join.sharers; ++i) {
-        const char *p = i ? a.parts + 2 * (c + i) * part_bytes(M, DP) : part;
-        top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(p + M * DP * 4) + row).x);
-    }
-    const float base = top == kNegInf ? 0.0f : top;
-    float total = 0.0f;
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = 0; i < join.sharers; ++i) {
-        const char *p = i ? a.parts + 2 * (c + i) * part_bytes(M, DP) : part;
+        const char *p = a.parts + (2 * (c + i) + (i == 0)) * part_bytes(M, DP);
         const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + M * DP * 4) + row);
-        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p) + col / 4 * M + row);
-        const float w = exp2_approx(ml.x - base);
-        total += w * ml.y;
-        sum.x += w * x.x, sum.y += w * x.y, sum.z += w * x.z, sum.w += w * x.w;
+        float4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = __ldcg(reinterpret_cast<const float4 *>(p) + (piece0 + k) * M + row);
+        const float now = fmaxf(top, ml.x), base = now == kNegInf ? 0.0f : now;
+        const float keep = exp2_approx(top - base), w = exp2_approx(ml.x - base);
+        total = total * keep + ml.y * w;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            sum[k].x = sum[k].x * keep + x[k].x * w, sum[k].y = sum[k].y * keep + x[k].y * w;
+            sum[k].z = sum[k].z * keep + x[k].z * w, sum[k].w = sum[k].w * keep + x[k].w * w;
+        }
+        top = now;
     }
-    store_joined<DT>(a, r, static_cast<int>(at), join.head, col, top, total, sum);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) store_joined<DT>(a, r, static_cast<int>(at), join.head, 4 * (piece0 + k), top, total, sum[k]);
 }
 
 // cg_attend_tiles.cu

@@ -317,20 +317,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             char *part = a.parts + (2 * blockIdx.x + (p.starts ? 1 : 0)) * part_bytes(kTileRows, DP);
             float2 *part_ml = reinterpret_cast<float2 *>(part + kTileRows * DP * 4);
             const bool sees = hi > lo;
-            // A value that is not finite, of a key that some rows do not see, is in all rows' sums: those rows are done again, from memory.
-            uint32_t again = 0;
-            if (any_masked) {
-                bool odd = false;
-                uint32_t y[32];
-#pragma unroll 1
-                for (int c = 0; c < DP / 32; ++c) {
-                    tmem_load32(y, o_mine + 32 * c);
-                    tmem_load_wait(y);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) odd = odd || (y[i] & 0x7F800000u) == 0x7F800000u;
-                }
-                again = __ballot_sync(0xffffffffu, odd && there);
-            }
+            bool odd = false;
             const float inv = sees ? 1.0f / l : 0.0f;
             const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | a.out_token | a.out_head) & 31) == 0;
             char *to = a.out + (r.first + token) * a.out_token + head * a.out_head;
@@ -339,6 +326,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             for (int c = 0; c < DP / 32; ++c) {
                 tmem_load32(y, o_mine + 32 * c);
                 tmem_load_wait(y);
+                if (any_masked) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) odd = odd || (y[i] & 0x7F800000u) == 0x7F800000u;
+                }
                 if (there && p.whole) {
                     // 32 bytes at a time where they are aligned: a thread's row is its own, and halves of a sector take as long
 #pragma unroll
@@ -368,7 +359,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             if (there && p.whole && a.lse)
                 a.lse[static_cast<int64_t>(r.first + token) * a.q_heads + head] = sees ? (m + log2f(l)) * 0.693147180559945f : kNegInf;
             if (there && !p.whole) part_ml[row] = make_float2(m, l);
-            for (; again; again &= again - 1) {
+            // A value that is not finite, of a key that some rows do not see, is in all rows' sums: those rows are done again, from memory.
+            for (uint32_t again = __ballot_sync(0xffffffffu, odd && there); again; again &= again - 1) {
                 const int i = half * 128 + 32 * (warp & 3) + __ffs(again) - 1;
                 __syncwarp();  // (the row has been written once)
                 float x[DP / 32], top, total;
@@ -529,13 +521,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 }
 #pragma unroll 1
                 for (int j = 0; j < blocks; ++j) {
-                    v_stage = tile_there();
-                    if (!ok) break;
                     const bool more = j + 1 < blocks;
+                    v_stage = tile_there();
+                    if (ok && more) k_stage = tile_there();  // (ahead of the weights, which all that follows waits for)
+                    if (!ok) break;
+                    const uint32_t v = v_desc + v_stage * kTile;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         if (half == halves) break;
-                        const uint32_t v = v_desc + v_stage * kTile;
                         if (!(ok = warp_wait(bar(kPFull + 2 * half), p_phase >> half & 1, failed, a.status))) break;
                         fence_after();
                         if (issues) {
@@ -547,26 +540,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                         fence_after();
                         if (issues) {
 #pragma unroll
-                            for (int k = 4; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, j > 0 || k > 0);
-                            if (half == halves - 1) commit(empty(v_stage));
-                        }
-                        if (more && half == 0) k_stage = tile_there();
-                        if (!ok) break;
-                        if (issues) {
-                            if (more) {
-                                scores(half, k_stage);
-                                commit(bar(kSFull + half));
-                                if (half == halves - 1) {
-                                    commit(empty(k_stage));
-                                    if (j + 2 == blocks) commit(bar(kQEmpty));
-                                }
-                            } else {
-                                commit(bar(kOFull + half));
-                            }
+                            for (int k = 4; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, true);
+                            if (more) scores(half, k_stage);
+                            commit(bar(more ? kSFull + half : kOFull + half));
                         }
                         __syncwarp();
                     }
                     if (!ok) break;
+                    if (issues) {
+                        commit(empty(v_stage));
+                        if (more) commit(empty(k_stage));
+                        if (j + 2 == blocks) commit(bar(kQEmpty));
+                    }
+                    __syncwarp();
                 }
             }
         }
@@ -632,7 +618,7 @@ template <int DT, int DP> int launch_tiles(const AttendArgs &a, int ctas, cudaSt
     if (rc) return rc;
     rc = launch(attend_tiles_kernel<DT, DP>, dim3(ctas), kTileThreads, smem, false, st, a, maps);
     if (rc || !a.joins) return rc;
-    return launch(combine_kernel<DT, kTileRows, DP>, dim3(ctas, kTileRows * (DP / 4) / 256), 256, 0, true, st, a);
+    return launch(combine_kernel<DT, kTileRows, DP>, dim3(ctas, kTileRows / 64), 64 * (DP / 32), 0, true, st, a);
 }
 
 }  // namespace
