@@ -33,6 +33,7 @@ struct AttendArgs {
 };
 
 constexpr float kNegInf = -INFINITY;
+constexpr int64_t kMostKeys = 1 << 30;  // of a request: places of keys and of blocks behind them stay numbers of 32 bits
 
 // bytes of one CTA's share of a tile: float sums[M][DP], then float2 (maximum, sum of weights)[M]
 __host__ __device__ constexpr int64_t part_bytes(int M, int DP) { return static_cast<int64_t>(M) * (DP * 4 + 8); }
@@ -46,7 +47,7 @@ __device__ __forceinline__ Lengths lengths_of(const AttendArgs &a, int b, bool r
     r.first = b, last = b + 1;
     if (a.q_starts) r.first = __ldg(a.q_starts + b), last = __ldg(a.q_starts + b + 1);
     r.kv = __ldg(a.kv_lens + b);
-    const int64_t room = static_cast<int64_t>(a.table_width) * a.page_size;
+    const int64_t room = min(static_cast<int64_t>(a.table_width) * a.page_size, kMostKeys);
     const bool bad = r.first < 0 || last < r.first || last > a.nrows || r.kv < 0 || r.kv > room;
     if (bad) {
         r.first = min(max(r.first, 0), a.nrows);
@@ -222,7 +223,11 @@ template <int M, int BK, int COST> struct Run {
                 if (++h >= a.heads) {
                     h = 0;
                     do {
-                        r = lengths_of(a, ++b);
+                        if (++b >= a.nrequests) {  // (lengths that change under way)
+                            at = to;
+                            return false;
+                        }
+                        r = lengths_of(a, b);
                         tiles = tiles_of<M>(a, r);
                     } while (tiles == 0);
                 }

@@ -155,7 +155,7 @@ template <int DP> constexpr int kTileStages = kTileStages128 * 128 / DP;
 template <int DP> constexpr int kBarsAt = (2 + kTileStages<DP>)*kTileBytes<DP>;
 template <int DP> constexpr int kTilesSmem = kBarsAt<DP> + 512 + 1024;  // and what it takes to begin at a multiple of 1024
 enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 2, kOFull = kPFull + 4, kPieceFull = kOFull + 2, kPieceEmpty = kPieceFull + 2,
-       kKvFull = kPieceEmpty + 2 };  // two each of S, O and pieces; P: the first 64 keys' weights of a
+       kKvFull = kPieceEmpty + 2 };  // two each of S, O and pieces; P: the first 96 keys' weights of a
 // half, then the others'
 
 // A piece as the scheduling warp hands it to the others, 48 bytes.
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
 
     if (warp < 8) {
         // ================================================================ softmax: a row a thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         const int half = warp >> 2, in_half = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_mine = s_at(half) + lanes, o_mine = o_at(half) + lanes;
@@ -300,11 +300,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     uint32_t w[16];
                     weigh<DT>(x[c], scale, down, w, sum);
                     tmem_store16(s_mine + 16 * c, w);
-                    if (c & 1) {
+                    if (c >= 2) {  // the products begin with three quarters of the weights, while the last are worked out
                         tmem_store_wait();
                         fence_before();
                         __syncwarp();
-                        if (lane == 0) bar_arrive(bar(kPFull + 2 * half + c / 2));
+                        if (lane == 0) bar_arrive(bar(kPFull + 2 * half + c - 2));
                     }
                 }
                 const float2 s0 = parts_of(sum[0]), s1 = parts_of(sum[1]);
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         }
     } else if (warp < 12) {
         // ================================================================ copies
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         const int w = warp - 8, piece = lane % kPieces;
         constexpr int kLag = 2;  // tiles that are on their way when one more is begun; the ring has to be longer by two
         static_assert(kStages >= kLag + 2, "the products may need the tile behind the one that they free");
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         tell(ok ? t : told);
     } else {
         // ================================================================ products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 12) {
             // the whole warp goes through the same steps, so that operands stay in uniform registers; one thread issues
             constexpr uint32_t qk = product(DT, kTileKeys, false), pv = product(DT, DP, true);
@@ -533,14 +533,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                         fence_after();
                         if (issues) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, j > 0 || k > 0);
+                            for (int k = 0; k < 6; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, j > 0 || k > 0);
                         }
                         if (!(ok = warp_wait(bar(kPFull + 2 * half + 1), p_phase >> half & 1, failed, a.status))) break;
                         p_phase ^= 1 << half;
                         fence_after();
                         if (issues) {
 #pragma unroll
-                            for (int k = 4; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, true);
+                            for (int k = 6; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, true);
                             if (more) scores(half, k_stage);
                             commit(bar(more ? kSFull + half : kOFull + half));
                         }
@@ -575,7 +575,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         }
         __syncwarp();
     }
-    // every product has been waited for (its O read), or the block has given up on one
+    // every product has been waited for (its O read), or the block has given up on one: what is on its way then takes microseconds
+    if (*failed)
+        for (const uint64_t start = now_ns(); now_ns() - start < 1000000;) {}
     fence_before();
     __syncthreads();
     fence_after();

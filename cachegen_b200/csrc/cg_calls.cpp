@@ -578,7 +578,8 @@ bool pages_job(PyObject *const *a, const at::Tensor &k, const at::Tensor &v, boo
     const int64_t P = kp.size(d - 3), S = kp.size(d - 2);
     if (kp.sizes() != vp.sizes() || (d == 4 && kp.size(0) != layers) || kp.size(d - 1) != H || kp.size(d) != D || S == 0) return false;
     if (!indices_of(a[4], dev, true, &slots) || slots.dim() != 1 || slots.size(0) != T) return false;
-    if (!indices_of(a[5], dev, false, &status) || status.numel() != 1) return false;
+    if (append && T && kp.data_ptr() == vp.data_ptr()) return false;
+    if (a[5] != Py_None && (!indices_of(a[5], dev, false, &status) || status.numel() != 1)) return false;
     if (!fits({layers, T, H, D, S}) || !turning(job, a + 6, dev, -1, T, D, held + 4)) return false;
     if (!apart(k, kp) || !apart(k, vp) || !apart(v, kp) || !apart(v, vp)) return false;
     job->k = k.data_ptr(), job->v = v.data_ptr(), job->pages_k = kp.data_ptr(), job->pages_v = vp.data_ptr();
@@ -587,7 +588,7 @@ bool pages_job(PyObject *const *a, const at::Tensor &k, const at::Tensor &v, boo
     strides_of(kp, job->pages_k_strides, 4);
     strides_of(vp, job->pages_v_strides, 4);
     job->slots = slots.data_ptr(), job->wide_slots = slots.scalar_type() == at::kLong;
-    job->status = static_cast<int32_t *>(status.data_ptr());
+    job->status = status.defined() ? static_cast<int32_t *>(status.data_ptr()) : nullptr;
     job->num_pages = P, job->page_size = static_cast<int32_t>(S);
     job->dtype = code(k.scalar_type());
     job->nlayers = static_cast<int32_t>(layers), job->ntokens = static_cast<int32_t>(T), job->heads = static_cast<int32_t>(H);
@@ -654,12 +655,12 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
     int64_t window, max_q;
     if (n != 13 || !first_of(a[0], &q, &dev) || !rows_of(a[0], q.scalar_type(), dev, 3, Use::kRead, &q) ||
         !rows_of(a[1], q.scalar_type(), dev, 4, Use::kRead, &kp) || !rows_of(a[2], q.scalar_type(), dev, 4, Use::kRead, &vp) ||
-        !indices_of(a[3], dev, false, &table) || !indices_of(a[4], dev, false, &lens) || !indices_of(a[12], dev, false, &status) ||
+        !indices_of(a[3], dev, false, &table) || !indices_of(a[4], dev, false, &lens) || (a[12] != Py_None && !indices_of(a[12], dev, false, &status)) ||
         !PyFloat_CheckExact(a[6]) || !small_int(a[8], &window) || !small_int(a[9], &max_q))
         Py_RETURN_NONE;
     const int64_t R = q.size(0), Q = q.size(1), D = q.size(2), P = kp.size(0), S = kp.size(1), H = kp.size(2), B = lens.numel();
     if (kp.sizes() != vp.sizes() || kp.size(3) != D || D % 8 || D == 0 || D > 128 || S == 0 || H == 0 || Q == 0 || Q % H || lens.dim() != 1 ||
-        B > CG_MAX_REQUESTS || table.dim() != 2 || table.size(0) != B || status.numel() != 1 || window < 0 || max_q < 0 ||
+        B > CG_MAX_REQUESTS || table.dim() != 2 || table.size(0) != B || (status.defined() && status.numel() != 1) || window < 0 || max_q < 0 ||
         !fits({R, Q, H, S, table.size(1), window, max_q}))
         Py_RETURN_NONE;
     if (a[5] == Py_None ? R != B : !indices_of(a[5], dev, false, &starts) || starts.dim() != 1 || starts.numel() != B + 1) Py_RETURN_NONE;
@@ -680,7 +681,7 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
     job.q = q.data_ptr(), job.pages_k = kp.data_ptr(), job.pages_v = vp.data_ptr(), job.out = out.data_ptr();
     job.table = static_cast<const int32_t *>(table.data_ptr()), job.kv_lens = static_cast<const int32_t *>(lens.data_ptr());
     job.q_starts = starts.defined() ? static_cast<const int32_t *>(starts.data_ptr()) : nullptr;
-    job.status = static_cast<int32_t *>(status.data_ptr());
+    job.status = status.defined() ? static_cast<int32_t *>(status.data_ptr()) : nullptr;
     job.table_row = table.stride(0), job.num_pages = P;
     const auto steps = [](const at::Tensor &t, int64_t *to) {
         for (int64_t k = 0; k + 1 < t.dim(); ++k) to[k] = t.size(k) > 1 ? t.stride(k) : 0;

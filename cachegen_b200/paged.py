@@ -12,7 +12,8 @@ Pages are tensors [num_pages, page_size, heads, head_size] of float16 or bfloat1
 made for several layers.  Slot s is token s % page_size of page s // page_size.
 
 Calls enqueue on the current stream of the tensors' device, allocate what they return and a workspace from
-torch's allocator, and wait for nothing, so they can be captured in a CUDA graph.  They compute no gradients.  The kernels
+torch's allocator, and wait for nothing, so they can be captured in a CUDA graph (which needs its Rotary as long as it is replayed, and
+reports to check_status if there was a call in front of its capture).  They compute no gradients.  The kernels
 check slots, pages and lengths: what lies outside is left out and noted for check_status.
 CacheGenDeserializer.decode_paged and CacheGenSerializer.encode_paged connect pages with the codec.
 """
@@ -25,7 +26,7 @@ import torch
 
 from . import _lib
 from .serde.cachegen_basics import on_device
-from .torchac_cuda import _check, _status_word
+from .torchac_cuda import _check, _status, _status_word
 
 _DTYPES = {torch.float16: _lib.CG_F16, torch.bfloat16: _lib.CG_BF16}
 _INDEX = (torch.int32, torch.int64)
@@ -151,8 +152,15 @@ def _turning(job, rotary, positions, device, shape, D):
 
 
 def _status_of(t):
-    """The status word of a tensor's GPU, None for a tensor on none."""
-    return _status_word(t.device) if t.is_cuda else None
+    """The status word of a tensor's GPU; None for a tensor on none, and in a capture in front of which there was no call: the word
+    outlives the graph, so it must not come from the graph's memory."""
+    if not t.is_cuda or (torch.cuda.is_current_stream_capturing() and (t.device.type, t.device.index) not in _status):
+        return None
+    return _status_word(t.device)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 def _turns_for(rotary, t):
@@ -242,13 +250,14 @@ def _pages_job(k, v, k_pages, v_pages, slots, rotary, positions, written):
     P, S = k_pages.shape[-4:-2]
     _rows(k_pages, "k_pages", dev, dtype, rank + 1, lead + (P, S, H, D), written)
     _rows(v_pages, "v_pages", dev, dtype, rank + 1, lead + (P, S, H, D), written)
+    _check(not written or not T or k_pages.data_ptr() != v_pages.data_ptr(), "k_pages and v_pages must not be the same memory")
     _indices(slots, "slots", dev, (T,))
     job = _lib.RowsJob()
     _turning(job, rotary, positions, dev, (T,), D)
     job.k, job.v, job.pages_k, job.pages_v = k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
     job.k_strides[:], job.v_strides[:] = _dense(k), _dense(v)
     job.pages_k_strides[:], job.pages_v_strides[:] = _paged(k_pages), _paged(v_pages)
-    job.slots, job.wide_slots, job.status = slots.data_ptr(), slots.dtype == torch.int64, _status_word(dev).data_ptr()
+    job.slots, job.wide_slots, job.status = slots.data_ptr(), slots.dtype == torch.int64, _address(_status_of(k))
     job.num_pages, job.page_size = P, max(S, 1)
     if S == 0:
         job.num_pages = 0
@@ -374,7 +383,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     job = _lib.AttentionJob()
     job.q, job.pages_k, job.pages_v, job.out = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
     job.lse = lse.data_ptr() if return_lse else None
-    job.table, job.kv_lens, job.status = page_table.data_ptr(), kv_lens.data_ptr(), _status_word(dev).data_ptr()
+    job.table, job.kv_lens, job.status = page_table.data_ptr(), kv_lens.data_ptr(), _address(_status_of(q))
     job.q_starts = q_starts.data_ptr() if q_starts is not None else None
     job.table_row, job.num_pages = page_table.stride(0), P
     job.q_strides[:], job.out_strides[:] = _steps(q), _steps(out)

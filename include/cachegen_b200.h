@@ -497,7 +497,7 @@ int cg_host_stage_end(void *handle_host);
  * (cg_rotary only).  Products are 32-bit floats, each value rounded once.  Rows that are not rotated are copied bit for bit.
  *
  * cg_rotary: k to k_out, which is k itself or does not overlap it; inverse: turned back.
- * cg_append_paged: keys rotated and values to the slots of their tokens; q (nlayers 1, q_heads 0: none) rotated to q_out.
+ * cg_append_paged: keys rotated and values to the slots of their tokens (pages_k and pages_v do not share values); q (nlayers 1, q_heads 0: none) rotated to q_out.
  * cg_gather_paged: the slots' values to v, and the keys turned back to k (inverse is implied).
  * head_size <= 512, 2 * heads + q_heads <= 65,536.  ntokens or nlayers 0: nothing is done.
  */
@@ -533,7 +533,8 @@ int cg_gather_paged(const cg_rows_job *job_host, void *stream);
  * lse: float32 [nrows, q_heads] or NULL.  max_q: the most rows of a request, or 0; it only chooses between two kernels.
  *
  * A page outside the cache counts as zeros, lengths that do not fit the table or the rows are cut; both raise CG_S_BAD_PAGE.
- * head_size: a multiple of 8 up to 128; nrequests <= CG_MAX_REQUESTS.  workspace: cg_paged_attention_workspace(job) bytes of device memory
+ * head_size: a multiple of 8 up to 128; nrequests <= CG_MAX_REQUESTS; at most 2^30 keys a request.  The arrays of lengths and pages
+ * must not change while the call runs.  workspace: cg_paged_attention_workspace(job) bytes of device memory
  * (16-byte aligned; 0: none), which calls on one stream may share.  nrows or nrequests 0: nothing is done.
  */
 #define CG_MAX_REQUESTS 4096

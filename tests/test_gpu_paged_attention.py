@@ -264,3 +264,48 @@ def test_many_requests():
         w = torch.softmax(b.q[i].double() @ k.T * b.scale, -1)
         # weights of 16 bits and the result's rounding, as in paged_ref.attention
         assert bool(((out[i].double() - w @ v).abs() <= 2.0 ** -11 * ((w @ v).abs() + 1.1 * (w @ v.abs())) + 2.0 ** -15).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("page", [8, 16, 32, 96, 128])
+@pytest.mark.parametrize("head", [8, 40, 64, 72, 128])
+def test_chunks_of_every_box(head, page, dtype):
+    """Pages that are read a box of tokens at a time, heads that fill a box and that do not; lengths that end inside a box; with
+    heads outside and inside of tokens."""
+    for transposed in (False, True):
+        b = Batch([(40, 40), (65, 333), (30, 200)], 4, 2, head, page, dtype, transposed=transposed, seed=head + page)
+        b.check(*b.call())
+    b.check(*b.call(window=77), window=77)
+
+
+def test_a_hint_that_is_too_small_costs_time_only():
+    b = Batch([(300, 900), (1, 50)], 4, 2, 64, 16, torch.float16)
+    b.check(*b.call(max_q=1))
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_one_key_value_head_of_many_and_strides_of_one_page(n):
+    """Pages and heads that are views of a larger cache: every stride differs from the contiguous one."""
+    big = torch.full((7, 16, 6, 3 * 64), math.nan, dtype=torch.float16, device="cuda")
+    b = Batch([(n, 60)], 4, 2, 64, 16, torch.float16)
+    pages = b.table[0, :4].long()
+    k, v = big[::2, :, ::3, 64:128], big[::2, :, 1::3, 128:]  # every second page, every third head, the middle and last 64 values
+    k.copy_(b.k[pages]), v.copy_(b.v[pages])
+    b.k, b.v, b.table = k, v, torch.tensor([[0, 1, 2, 3]], dtype=torch.int32, device="cuda")
+    b.check(*b.call())
+
+
+def test_a_capture_in_front_of_any_call(monkeypatch):
+    """The status word is not made of a graph's memory."""
+    from cachegen_b200 import paged, torchac_cuda
+    b = Batch([(1, 70)], 4, 2, 64, 16, torch.float16)
+    b.call()
+    words = {}
+    monkeypatch.setattr(paged, "_status", words)
+    monkeypatch.setattr(torchac_cuda, "_status", words)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = b.call()
+    assert not words
+    graph.replay()
+    b.check(*out)

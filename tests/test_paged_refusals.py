@@ -152,6 +152,8 @@ def test_append_refuses_what_does_not_go_together():
                  dict(q=t["k"][:2]), dict(q=t["k"], q_out=t["k"][:, :, :32]), dict(rotary=r, positions=at.float())):
         with pytest.raises(RuntimeError):
             paged.append_paged(**t, **more)
+    with pytest.raises(RuntimeError, match="same memory"):
+        paged.append_paged(t["k"], t["v"], t["k_pages"], t["k_pages"], t["slots"])
     buffer = torch.zeros((4, 2, 64), dtype=torch.float16, device="cuda")
     with pytest.raises(RuntimeError, match="overlap"):
         paged.append_paged(**t, q=buffer[:3], q_out=buffer[1:])
