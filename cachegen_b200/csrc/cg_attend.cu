@@ -55,7 +55,7 @@ template <int DP> constexpr int kRowBytes2 = 2 * DP + 16;
 template <int DP> constexpr int kStageBytes = 2 * kChunk * kRowBytes2<DP>;
 template <int DP> constexpr int kRingBytes = kStages * kStageBytes<DP>;
 constexpr int most_of(int x, int y) { return x > y ? x : y; }
-constexpr int kSumFloats = 16 * 36;  // of a warp: 16 rows of 32 values or 8 of 64, four more between rows
+constexpr int kSumFloats = 16 * 36;  // of a warp: 16 rows of 32 values, 8 of 64 or 4 of 128, four more between rows
 template <int DP> constexpr int kSumsAt = most_of(kWarps * kRingBytes<DP>, (CG_MAX_REQUESTS + 1) * 8 + 8);
 template <int DP> constexpr int kMlAt = kSumsAt<DP> + kWarps * kSumFloats * 4;
 template <int DP> constexpr int kAttendSmem = kMlAt<DP> + kWarps * kRowsM * 8 + 16 + 16 * kWarps * kStages;
@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
         }
         // chunks inside [all_lo, all_hi) are seen by all rows
         const int all_lo = first_key(a, r, (row0 + rows - 1) / a.group), all_hi = last_key(a, r, row0 / a.group);
+        const bool mixed = (row0 + rows - 1) / a.group != row0 / a.group;  // whether rows see unlike keys (what none sees is zero)
         const int nchunks = p.end - p.begin;
         const int key0 = p.begin * kRowsBK + warp * kChunk;
 
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
             for (int k = 0; k < kSteps; ++k) {
                 uint32_t b[4];
                 ldmatrix4_trans(b, at + v_row + 32 * k);
-                if (!all) odd = odd || not_finite2<DT>(b[0]) || not_finite2<DT>(b[1]) || not_finite2<DT>(b[2]) || not_finite2<DT>(b[3]);
+                if (!all && mixed) odd = odd || not_finite2<DT>(b[0]) || not_finite2<DT>(b[1]) || not_finite2<DT>(b[2]) || not_finite2<DT>(b[3]);
                 mma16816<DT>(o[2 * k], w, b[0], b[1]);
                 mma16816<DT>(o[2 * k + 1], w, b[2], b[3]);
             }
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
             for (int k = 0; k < kWarps; ++k) top = fmaxf(top, row_ml[k][g + 8 * i].x);
             keep[i] = top == kNegInf ? 1.0f : exp2_approx(m[i] - top);
         }
-        const int width = rows <= 8 ? 64 : 32;  // values of a row at a time
+        const int width = rows <= 4 ? DP : rows <= 8 ? 64 : 32;  // values of a row at a time
         float *const sums = reinterpret_cast<float *>(smem + kSumsAt<DP>);  // [kWarps][rows][width + 4]
         char *part = a.parts + (2 * blockIdx.x + (p.starts ? 1 : 0)) * part_bytes(kRowsM, DP);
         if (!slow) {
@@ -272,10 +273,10 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
                 if (first) sync_weighing_warps();
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (i == 1 && width == 64) break;  // no more than eight rows
+                    if (g + 8 * i >= rows) break;
                     float *to = sums + warp * kSumFloats + (g + 8 * i) * (width + 4) + q2;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
+                    for (int k = 0; k < kSteps * 2; ++k) {
                         if (first / 8 + k >= kSteps * 2 || 8 * k >= width) break;
                         *reinterpret_cast<float2 *>(to + 8 * k) = make_float2(o[first / 8 + k][2 * i] * keep[i], o[first / 8 + k][2 * i + 1] * keep[i]);
                     }
