@@ -97,12 +97,12 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
             const char *const keys = a.k + p.head * a.k_head + 16 * piece, *const values = a.v + p.head * a.v_head + 16 * piece;
             const auto page_for = [&](int chunk) {  // lanes i and 16 + i: of key i
                 const int key = key0 + chunk * kRowsBK;
-                return chunk < nchunks && key >= p.tile.lo && key < p.tile.hi ? page_of(a, p.request, key / a.page_size) : -1;
+                return chunk < nchunks && key >= p.tile.lo && key < p.tile.hi ? page_of(a, p.request, page_index(a, key)) : -1;
             };
             int page = page_for(0);
 #pragma unroll 1
             for (int chunk = 0; chunk < nchunks; ++chunk) {
-                const int in_page = (key0 + chunk * kRowsBK) % a.page_size;
+                const int in_page = place_in_page(a, key0 + chunk * kRowsBK);
                 // lanes below 16 have the keys' places, the others the values'
                 const int64_t at = lane < 16 ? page * a.k_page + in_page * a.k_token : page * a.v_page + in_page * a.v_token;
                 const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
@@ -445,6 +445,7 @@ extern "C" int cg_paged_attention(const cg_attention_job *job, void *stream) {
     a.table_row = j.table_row, a.num_pages = j.num_pages;
     a.nrequests = j.nrequests, a.nrows = j.nrows, a.q_heads = j.q_heads, a.heads = j.heads, a.group = j.q_heads / j.heads;
     a.head_size = j.head_size, a.page_size = j.page_size, a.table_width = j.table_width, a.causal = j.causal, a.window = j.window;
+    a.page_shift = j.page_size & (j.page_size - 1) ? -1 : __builtin_ctz(static_cast<unsigned>(j.page_size));
     a.scale = j.scale * 1.44269504088896340736f;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (p.tiles) return launch_attend_tiles(a, j.dtype, p.ctas, st);

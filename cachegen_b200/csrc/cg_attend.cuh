@@ -28,7 +28,7 @@ struct AttendArgs {
     int32_t *status;
     int64_t q_token, q_head, out_token, out_head, k_page, k_token, k_head, v_page, v_token, v_head;  // bytes
     int64_t table_row, num_pages;
-    int32_t nrequests, nrows, q_heads, heads, group, head_size, page_size, table_width, causal, window;
+    int32_t nrequests, nrows, q_heads, heads, group, head_size, page_size, page_shift, table_width, causal, window;  // page_shift: -1 for no power of two
     float scale;    // of the scores, times log2(e)
 };
 
@@ -256,6 +256,10 @@ template <int M, int BK, int COST> struct Run {
     }
 };
 
+// the page of a request that a key is in, counted from its first, and the key's place in it
+__device__ __forceinline__ int page_index(const AttendArgs &a, int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size; }
+__device__ __forceinline__ int place_in_page(const AttendArgs &a, int key) { return a.page_shift >= 0 ? key & (a.page_size - 1) : key % a.page_size; }
+
 // Where a page of a request lies, or -1.
 __device__ __forceinline__ int page_of(const AttendArgs &a, int b, int index) {
     const int page = __ldg(a.table + b * a.table_row + index);
@@ -375,39 +379,48 @@ __device__ __forceinline__ void store_joined(const AttendArgs &a, const Lengths 
 }
 
 // Joins what the CTAs of a divided tile of many rows have left.  Block (i, j): 64 rows of the tile that begins in CTA i, a row a thread,
-// eight 16-byte pieces of it, all on their way together.  Sums are stored [DP / 4][M][4], as a kernel with a row a thread writes
+// four 16-byte pieces of it, of four CTAs on their way together: one request's rows over a long context are in dozens.  Sums are stored [DP / 4][M][4], as a kernel with a row a thread writes
 // them side by side.
 template <int DT, int M, int DP>
-__global__ void __launch_bounds__(64 * (DP / 32)) combine_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(64 * (DP / 16)) combine_kernel(const __grid_constant__ AttendArgs a) {
     wait_for_launch_before();
-    const int c = blockIdx.x, row = blockIdx.y * 64 + threadIdx.x % 64, piece0 = threadIdx.x / 64 * 8;
+    const int c = blockIdx.x, row = blockIdx.y * 64 + threadIdx.x % 64, piece0 = threadIdx.x / 64 * 4;
     const Join join = join_of(a, c);
     if (join.sharers == 0) return;
     const Lengths r{join.first, join.n, join.kv};
     const int64_t at = static_cast<int64_t>(join.t) * M + row;
     if (at >= static_cast<int64_t>(r.n) * a.group) return;
     float top = kNegInf, total = 0.0f;
-    float4 sum[8];
+    float4 sum[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i = 0; i < join.sharers; ++i) {
-        const char *p = a.parts + (2 * (c + i) + (i == 0)) * part_bytes(M, DP);
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + M * DP * 4) + row);
-        float4 x[8];
+    for (int k = 0; k < 4; ++k) sum[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < join.sharers; i += 4) {
+        float2 ml[4];
+        float4 x[4][4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = __ldcg(reinterpret_cast<const float4 *>(p) + (piece0 + k) * M + row);
-        const float now = fmaxf(top, ml.x), base = now == kNegInf ? 0.0f : now;
-        const float keep = exp2_approx(top - base), w = exp2_approx(ml.x - base);
-        total = total * keep + ml.y * w;
+        for (int n = 0; n < 4; ++n) {
+            ml[n] = make_float2(kNegInf, 0.0f);
+            const char *p = a.parts + (2 * (c + i + n) + (i + n == 0)) * part_bytes(M, DP);
+            if (i + n < join.sharers) ml[n] = __ldcg(reinterpret_cast<const float2 *>(p + M * DP * 4) + row);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            sum[k].x = sum[k].x * keep + x[k].x * w, sum[k].y = sum[k].y * keep + x[k].y * w;
-            sum[k].z = sum[k].z * keep + x[k].z * w, sum[k].w = sum[k].w * keep + x[k].w * w;
+            for (int k = 0; k < 4; ++k)
+                x[n][k] = i + n < join.sharers ? __ldcg(reinterpret_cast<const float4 *>(p) + (piece0 + k) * M + row) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        top = now;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const float now = fmaxf(top, ml[n].x), base = now == kNegInf ? 0.0f : now;
+            const float keep = exp2_approx(top - base), w = exp2_approx(ml[n].x - base);
+            total = total * keep + ml[n].y * w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                sum[k].x = sum[k].x * keep + x[n][k].x * w, sum[k].y = sum[k].y * keep + x[n][k].y * w;
+                sum[k].z = sum[k].z * keep + x[n][k].z * w, sum[k].w = sum[k].w * keep + x[n][k].w * w;
+            }
+            top = now;
+        }
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) store_joined<DT>(a, r, static_cast<int>(at), join.head, 4 * (piece0 + k), top, total, sum[k]);
+    for (int k = 0; k < 4; ++k) store_joined<DT>(a, r, static_cast<int>(at), join.head, 4 * (piece0 + k), top, total, sum[k]);
 }
 
 // cg_attend_tiles.cu

@@ -153,9 +153,9 @@ template <int DT> __device__ __forceinline__ void weigh(const uint32_t (&x)[32],
 template <int DP> constexpr int kTileBytes = 128 * DP * 2;
 template <int DP> constexpr int kTileStages = kTileStages128 * 128 / DP;
 template <int DP> constexpr int kBarsAt = (2 + kTileStages<DP>)*kTileBytes<DP>;
-template <int DP> constexpr int kTilesSmem = kBarsAt<DP> + 512 + 1024;  // and what it takes to begin at a multiple of 1024
+template <int DP> constexpr int kTilesSmem = kBarsAt<DP> + 512 + 1024 + 1024;  // and what it takes to begin at a multiple of 1024
 enum { kQFull, kQEmpty, kSFull, kPFull = kSFull + 2, kOFull = kPFull + 4, kPieceFull = kOFull + 2, kPieceEmpty = kPieceFull + 2,
-       kKvFull = kPieceEmpty + 2 };  // two each of S, O and pieces; P: the first 96 keys' weights of a
+       kJoinReady = kPieceEmpty + 2, kJoinDone, kKvFull };  // two each of S, O and pieces; P: the first 96 keys' weights of a
 // half, then the others'
 
 // A piece as the scheduling warp hands it to the others, 48 bytes.
@@ -182,6 +182,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
     volatile int *failed = words + 1;
 
     Run<kTileRows, kTileKeys, kTileCost> run;  // (of warp 13; all find their run together)
+    if (tid == 0 && maps.rows) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+    }
     run.template init<kTileThreads, true>(a, reinterpret_cast<int64_t *>(mem));
     let_next_launch_start();
     if (tid == 0) {
@@ -195,6 +199,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             bar_init(bar(kPieceFull + i), 1);
             bar_init(bar(kPieceEmpty + i), 13);  // warps that read it
         }
+        bar_init(bar(kJoinReady), 4);
+        bar_init(bar(kJoinDone), 4);
         for (int s = 0; s < kStages; ++s) bar_init(full(s), 4), bar_init(empty(s), 1);
         *failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -208,6 +214,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
     // columns: S (and P) of the halves, then O
     const auto s_at = [&](int half) { return tmem + 128 * half; };
     const auto o_at = [&](int half) { return tmem + 256 + 128 * half; };
+    float2 *join_ml = reinterpret_cast<float2 *>(mem + kBarsAt<DP> + 512);  // [128]: maxima and sums of the second half
     // the next piece: every warp reads it for itself
     Parcel p;
     int pieces = 0;
@@ -224,32 +231,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
 
     if (warp < 8) {
         // ================================================================ softmax: a row a thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int half = warp >> 2, in_half = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_mine = s_at(half) + lanes, o_mine = o_at(half) + lanes;
-        uint32_t s_phase = 0, o_phase = 0;
+        uint32_t s_phase = 0, o_phase = 0, join_phase = 0;
         bool ok = true;
         while (ok && next_piece()) {
             const Lengths r{p.first, p.n, p.kv};
             const int blocks = p.end - p.begin, row0 = p.t * kTileRows, rows = min(kTileRows, r.n * a.group - row0);
-            const int row = half * 128 + in_half;
-            if (half * 128 >= rows) continue;
+            const bool both = rows <= 128;  // both halves have the same rows, and every second block each
+            const int step = both ? 2 : 1, first = both ? half : 0, top_row = both ? 0 : half * 128, row = top_row + in_half;
+            if (first >= blocks) continue;
             const bool there = row < rows;
             const int token = there ? (row0 + row) / a.group : 0, head = p.head * a.group + (there ? (row0 + row) % a.group : 0);
             // (rows behind the last see everything: they ask for no masks)
             const int lo = there ? first_key(a, r, token) : 0, hi = there ? last_key(a, r, token) : INT32_MAX;
-            const int half_lo = first_key(a, r, (row0 + min(rows, half * 128 + 128) - 1) / a.group), half_hi = last_key(a, r, (row0 + half * 128) / a.group);
+            const int half_lo = first_key(a, r, (row0 + min(rows, top_row + 128) - 1) / a.group), half_hi = last_key(a, r, (row0 + top_row) / a.group);
+            const bool any_masked = p.begin * kTileKeys < half_lo || p.end * kTileKeys > half_hi;
             float m = kNegInf, l = 0.0f;
-            bool any_masked = false;
-            for (int j = 0; j < blocks; ++j) {
+            for (int j = first; j < blocks; j += step) {
                 const int key = (p.begin + j) * kTileKeys;
                 ok = warp_wait(bar(kSFull + half), s_phase, failed, a.status);
                 s_phase ^= 1;
                 if (!ok) break;
                 fence_after();
                 const bool masked = key < half_lo || key + kTileKeys > half_hi;  // for one of the half's rows
-                any_masked = any_masked || masked;
                 uint32_t x[4][32];
                 tmem_load32(x[0], s_mine);
                 tmem_load32(x[1], s_mine + 32);
@@ -279,7 +286,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     const float keep = raise ? (m == kNegInf ? 0.0f : exp2_approx(m - high)) : 1.0f;
                     if (raise) m = high;
                     l *= keep;
-                    if (j > 0) {  // the products of the block before are done: this block's scores came behind them
+                    if (j > first) {  // the products of the block before are done: this block's scores came behind them
 #pragma unroll 1
                         for (int c = 0; c < DP / 32; ++c) {
                             uint32_t y[32];
@@ -314,6 +321,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             o_phase ^= 1;
             if (!ok) break;
             fence_after();
+            if (both && blocks > 1) {  // the first half adds the second's sums to its own
+                if (half) {
+                    join_ml[in_half] = make_float2(m, l);
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(bar(kJoinReady));
+                    ok = warp_wait(bar(kJoinDone), join_phase, failed, a.status);
+                    join_phase ^= 1;
+                    continue;
+                }
+                ok = warp_wait(bar(kJoinReady), join_phase, failed, a.status);
+                join_phase ^= 1;
+                if (!ok) break;
+                fence_after();
+                const float2 ml = join_ml[in_half];
+                const float high = fmaxf(m, ml.x), base = high == kNegInf ? 0.0f : high;
+                const float mine = exp2_approx(m - base), other = exp2_approx(ml.x - base);
+                l = l * mine + ml.y * other;
+                m = high;
+#pragma unroll 1
+                for (int c = 0; c < DP / 32; ++c) {
+                    uint32_t y[32], z[32];
+                    tmem_load32(y, o_mine + 32 * c);
+                    tmem_load32(z, o_mine + 128 + 32 * c);
+                    tmem_load_wait(y);
+                    tmem_load_wait(z);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * mine + __uint_as_float(z[i]) * other);
+                    tmem_store32(o_mine + 32 * c, y);
+                }
+                tmem_store_wait();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar(kJoinDone));
+            }
             char *part = a.parts + (2 * blockIdx.x + (p.starts ? 1 : 0)) * part_bytes(kTileRows, DP);
             float2 *part_ml = reinterpret_cast<float2 *>(part + kTileRows * DP * 4);
             const bool sees = hi > lo;
@@ -361,7 +403,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             if (there && !p.whole) part_ml[row] = make_float2(m, l);
             // A value that is not finite, of a key that some rows do not see, is in all rows' sums: those rows are done again, from memory.
             for (uint32_t again = __ballot_sync(0xffffffffu, odd && there); again; again &= again - 1) {
-                const int i = half * 128 + 32 * (warp & 3) + __ffs(again) - 1;
+                const int i = top_row + 32 * (warp & 3) + __ffs(again) - 1;
                 __syncwarp();  // (the row has been written once)
                 float x[DP / 32], top, total;
                 slow_row<DT, DP>(a, r, p.request, p.head, row0 + i, p.begin * kTileKeys, p.end * kTileKeys, x, top, total);
@@ -382,21 +424,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         }
     } else if (warp < 12) {
         // ================================================================ copies
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         const int w = warp - 8, piece = lane % kPieces;
-        constexpr int kLag = 2;  // tiles that are on their way when one more is begun; the ring has to be longer by two
-        static_assert(kStages >= kLag + 2, "the products may need the tile behind the one that they free");
+        // A tile of copies is told of when kLag more have been begun.  Products may need the second tile behind the first that is not free yet,
+        // so that one has to be told of while the ring holds both and what is between: kLag more than these three.
+        constexpr int kLag = 2;
+        static_assert(kStages >= kLag + 3, "the products would wait for a tile that waits for them");
         const uint32_t at_piece = static_cast<uint32_t>(piece / 8) * 16384;
-        int t = 0, told = 0, q_count = 0;
-        uint32_t by_tma = 0;  // bit i: this warp's part of tile t - 1 - i came by TMA, whose barrier knows when it is there
+        const bool box_lane = maps.rows && lane % maps.rows == 0;  // the lane of a box's first token
+        const int box_bytes = 32 * DP * 2;
+        int stage = 0, untold = 0, q_phase = 1;  // of the next tile; tiles by copies, the last ones begun, that have not been told of
+        uint32_t phase = 1;                      // (a barrier's phase before its first is over)
         bool ok = true;
-        const auto tell = [&](int upto) {  // copies that have arrived
-            for (; told < upto; ++told) {
-                if (by_tma >> (t - 1 - told) & 1) continue;
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) bar_arrive(full(told % kStages));
-            }
+        const auto tell_first = [&]() {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            const int at = stage - untold;
+            if (lane == 0) bar_arrive(full(at < 0 ? at + kStages : at));
+            --untold;
+        };
+        const auto tell_all = [&]() {
+            if (!untold) return;
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            while (untold) tell_first();
         };
         // where this lane's pieces of a tile go: rows 2 i + lane / 16 (of DP 64: 4 i + lane / 8) of the warp's 32
         constexpr int kOrders = 8 / kRowsAtOnce;  // of a row's pieces, which repeat every 8 rows
@@ -425,46 +475,47 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             const int blocks = p.end - p.begin, row0 = p.t * kTileRows, rows = min(kTileRows, r.n * a.group - row0);
             const auto page_for = [&](int j) {
                 const int key = (p.begin + j) * kTileKeys + 32 * w + lane;
-                return j < blocks && key >= p.lo && key < p.hi ? page_of(a, p.request, key / a.page_size) : -1;
+                return j < blocks && key >= p.lo && key < p.hi ? page_of(a, p.request, page_index(a, key)) : -1;
             };
             int page = page_for(0);
-            // what the products of the piece before need and is still on its way
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            tell(t);
+            tell_all();  // what the products of the piece before need
 #pragma unroll 1
             for (int j = 0; ok && j < blocks; ++j) {
-                const int key = (p.begin + j) * kTileKeys + 32 * w + lane, in_page = key % a.page_size, here = page;
+                const int in_page = place_in_page(a, (p.begin + j) * kTileKeys + 32 * w + lane), here = page;
                 const bool boxes = maps.rows && __all_sync(0xffffffffu, here >= 0);
                 page = page_for(j + 1);
+                if (boxes) tell_all();
 #pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv) {
-                    if (t >= kStages && !(ok = warp_wait(empty(t % kStages), (t / kStages - 1) & 1, failed, a.status))) break;
-                    const uint32_t tile = tiles_at + t % kStages * kTileBytes<DP>;
-                    by_tma = by_tma << 1 | boxes;
+                    if (!(ok = warp_wait(empty(stage), phase, failed, a.status))) break;
+                    const uint32_t tile = tiles_at + stage * kTileBytes<DP>;
                     if (boxes) {
-                        if (lane == 0) bar_expect(full(t % kStages), 32 * DP * 2);
+                        if (lane == 0) bar_expect(full(stage), box_bytes);
                         __syncwarp();
-                        if (lane % maps.rows == 0) {  // the lane of a box's first token
+                        if (box_lane) {
 #pragma unroll
                             for (int panel = 0; panel < DP / 64; ++panel)
-                                tma_box(tile + panel * 16384 + (32 * w + lane) * 128, kv ? &maps.v : &maps.k, 64 * panel, in_page, p.head, here, full(t % kStages));
+                                tma_box(tile + panel * 16384 + (32 * w + lane) * 128, kv ? &maps.v : &maps.k, 64 * panel, in_page, p.head, here, full(stage));
                         }
                     } else {
                         const char *at = kv ? a.v + here * a.v_page + in_page * a.v_token + p.head * a.v_head
                                             : a.k + here * a.k_page + in_page * a.k_token + p.head * a.k_head;
                         copy_rows(tile, at, here >= 0);
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        ++untold;
                     }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-                    ++t;
-                    tell(t - kLag);
+                    if (++stage == kStages) stage = 0, phase ^= 1;
+                    if (untold > kLag) {
+                        asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+                        tell_first();
+                    }
                 }
                 if (!ok || j > 0) continue;
                 // queries, behind the first block's tiles, which are on their way meanwhile: once the last products with the ones before are done
-                if (q_count && !(ok = warp_wait(bar(kQEmpty), (q_count - 1) & 1, failed, a.status))) break;
-                ++q_count;
+                if (!(ok = warp_wait(bar(kQEmpty), q_phase, failed, a.status))) break;
+                q_phase ^= 1;
 #pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
+                for (int half = 0; half < (rows > 128 ? 2 : 1); ++half) {
                     const int row = half * 128 + 32 * w + lane;
                     const bool there = row < rows;
                     const int token = there ? (row0 + row) / a.group : 0, head = p.head * a.group + (there ? (row0 + row) % a.group : 0);
@@ -475,14 +526,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) bar_arrive(bar(kQFull));
-                tell(t);
+                while (untold) tell_first();
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        tell(ok ? t : told);
+        if (ok) tell_all();
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         // ================================================================ products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 12) {
             // the whole warp goes through the same steps, so that operands stay in uniform registers; one thread issues
             constexpr uint32_t qk = product(DT, kTileKeys, false), pv = product(DT, DP, true);
@@ -509,13 +560,53 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 uint32_t k_stage = tile_there(), v_stage = 0;
                 if (!ok) break;
                 fence_after();
+                if (halves == 1) {  // both halves on the same rows
+                    const auto begin = [&](int half, uint32_t at, bool last) {  // scores of one block
+                        if (!issues) return;
+#pragma unroll
+                        for (int i = 0; i < DP / 16; ++i)
+                            mma_ss(s_at(half), q_desc + (i / 4) * 1024 + (i % 4) * 2, k_desc + at * kTile + (i / 4) * 1024 + (i % 4) * 2, kOperandHigh, qk, i > 0);
+                        commit(bar(kSFull + half));
+                        commit(empty(at));
+                        if (last) commit(bar(kQEmpty));
+                    };
+                    begin(0, k_stage, blocks == 1);
+                    v_stage = tile_there();
+                    if (ok && blocks > 1) {
+                        k_stage = tile_there();
+                        if (ok) fence_after(), begin(1, k_stage, blocks == 2);
+                    }
+#pragma unroll 1
+                    for (int j = 0; ok && j < blocks; ++j) {
+                        const int half = j & 1;
+                        const bool more = j + 2 < blocks;
+                        uint32_t v_next = 0;
+                        if (j + 1 < blocks) v_next = tile_there();
+                        if (!ok || !(ok = warp_wait(bar(kPFull + 2 * half), p_phase >> half & 1, failed, a.status)) ||
+                            !(ok = warp_wait(bar(kPFull + 2 * half + 1), p_phase >> half & 1, failed, a.status)))
+                            break;
+                        p_phase ^= 1 << half;
+                        fence_after();
+                        if (issues) {
+#pragma unroll
+                            for (int k = 0; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v_desc + v_stage * kTile + k * 128, kOperandHigh, pv, j > 1 || k > 0);
+                            if (!more) commit(bar(kOFull + half));
+                            commit(empty(v_stage));
+                        }
+                        if (more) {  // (not waited for in front of the products: the copies may need the tile that those free)
+                            k_stage = tile_there();
+                            if (ok) fence_after(), begin(half, k_stage, j + 3 == blocks);
+                        }
+                        v_stage = v_next;
+                        __syncwarp();
+                    }
+                    continue;
+                }
                 if (issues) {
                     scores(0, k_stage);
                     commit(bar(kSFull));
-                    if (halves == 2) {
-                        scores(1, k_stage);
-                        commit(bar(kSFull + 1));
-                    }
+                    scores(1, k_stage);
+                    commit(bar(kSFull + 1));
                     commit(empty(k_stage));
                     if (blocks == 1) commit(bar(kQEmpty));
                 }
@@ -528,7 +619,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     const uint32_t v = v_desc + v_stage * kTile;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        if (half == halves) break;
                         if (!(ok = warp_wait(bar(kPFull + 2 * half), p_phase >> half & 1, failed, a.status))) break;
                         fence_after();
                         if (issues) {
@@ -620,7 +710,7 @@ template <int DT, int DP> int launch_tiles(const AttendArgs &a, int ctas, cudaSt
     if (rc) return rc;
     rc = launch(attend_tiles_kernel<DT, DP>, dim3(ctas), kTileThreads, smem, false, st, a, maps);
     if (rc || !a.joins) return rc;
-    return launch(combine_kernel<DT, kTileRows, DP>, dim3(ctas, kTileRows / 64), 64 * (DP / 32), 0, true, st, a);
+    return launch(combine_kernel<DT, kTileRows, DP>, dim3(ctas, kTileRows / 64), 64 * (DP / 16), 0, true, st, a);
 }
 
 }  // namespace

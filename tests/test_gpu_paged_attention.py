@@ -309,3 +309,31 @@ def test_a_capture_in_front_of_any_call(monkeypatch):
     assert not words
     graph.replay()
     b.check(*out)
+
+
+@pytest.mark.parametrize("page", [1, 5, 16, 24, 64])
+@pytest.mark.parametrize("head", [64, 128])
+def test_few_rows_over_many_keys(head, page):
+    """Between one row and 128 a key/value head: from one block of keys to dozens, whole and divided, of pages of every kind."""
+    b = Batch([(5, 1), (20, 100), (9, 129), (30, 300), (17, 1500), (32, 5000), (25, 700)], 8, 2, head, page, torch.bfloat16, seed=page)
+    b.check(*b.call())
+    b.check(*b.call(window=333), window=333)
+
+
+def test_few_rows_of_many_requests_at_once():
+    """More tiles than blocks of a GPU, so that one block has several, of few rows and of many."""
+    lens = [(3 + 5 * (i % 11), 40 + 97 * (i % 13)) for i in range(60)]
+    lens = [(n, max(n, kv)) for n, kv in lens]
+    b = Batch(lens, 16, 4, 64, 16, torch.float16)
+    b.check(*b.call())
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_values_of_hidden_keys_stay_out_of_few_rows_over_many_keys(value):
+    b = Batch([(30, 700)], 4, 2, 64, 16, torch.float16)
+    j = 690
+    b.v[b.table[0].long()[j // 16], j % 16, 1, 3] = value
+    out, _ = b.call()
+    want, _, tol = attention(b.q, b.k, b.v, b.table, b.lens, b.scale)
+    fine = want.isfinite()
+    assert torch.equal(out.isfinite(), fine) and int((~fine).sum()) == 10 * 2 and bool(((out.double() - want).abs() <= tol)[fine].all())
