@@ -376,11 +376,15 @@ int launch_attend_rows(const AttendArgs &a, int ctas, cudaStream_t st) {
     return launch(combine_rows_kernel<DT, DP>, dim3(ctas), kJoinThreads, 0, true, st, a);
 }
 
+// Tiles of at most so many units stay whole: what a second kernel takes to join parts, 4 to 5 us, is more than these units take.
+constexpr int kUndividedUnits = 4;
+
 // What a call launches, from what the host knows: the tensors' sizes.
 struct Plan {
     bool tiles;      // the kernel for many rows
     int ctas, dp;
-    int64_t bytes;   // of the workspace: 0 if no tile can be divided
+    bool undivided;  // no tile is divided among CTAs
+    int64_t bytes;   // of the workspace: 0 if no tile is divided
 };
 
 int plan_of(const cg_attention_job &j, Plan &p) {
@@ -401,7 +405,8 @@ int plan_of(const cg_attention_job &j, Plan &p) {
     const int64_t tiles = (static_cast<int64_t>(j.nrows) * group / M + j.nrequests) * j.heads;  // at most
     const int64_t slots = static_cast<int64_t>(sm_count()) * (p.tiles ? 1 : 2);
     p.ctas = static_cast<int>(per_tile > slots || tiles * per_tile > slots ? slots : tiles * per_tile);
-    p.bytes = per_tile > 1 ? p.ctas * (2 * part_bytes(M, p.dp) + static_cast<int64_t>(sizeof(Join))) : 0;
+    p.undivided = per_tile <= kUndividedUnits;
+    p.bytes = !p.undivided ? p.ctas * (2 * part_bytes(M, p.dp) + static_cast<int64_t>(sizeof(Join))) : 0;
     return CG_OK;
 }
 
@@ -445,6 +450,7 @@ extern "C" int cg_paged_attention(const cg_attention_job *job, void *stream) {
     a.table_row = j.table_row, a.num_pages = j.num_pages;
     a.nrequests = j.nrequests, a.nrows = j.nrows, a.q_heads = j.q_heads, a.heads = j.heads, a.group = j.q_heads / j.heads;
     a.head_size = j.head_size, a.page_size = j.page_size, a.table_width = j.table_width, a.causal = j.causal, a.window = j.window;
+    a.undivided = p.undivided;
     a.page_shift = j.page_size & (j.page_size - 1) ? -1 : __builtin_ctz(static_cast<unsigned>(j.page_size));
     a.scale = j.scale * 1.44269504088896340736f;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -4,7 +4,8 @@
 // r % group of the head's group, so that a key that is read serves all of them.  A tile's work is counted in units, blocks of BK keys
 // that one of its rows sees (one unit at least).  All units of a call stand in one line, (request, head, tile, block), and every
 // CTA takes an equal run of it: whatever the batch's lengths, the CTAs end together.  A tile that two CTAs or more share leaves
-// a maximum, a sum and a product a row from each of them in the workspace, and combine_kernel joins those.  Lengths stay on the
+// a maximum, a sum and a product a row from each of them in the workspace, and a second kernel joins those.  Where all tiles are short
+// (`undivided`) a CTA takes the tiles that begin in its run, whole.  Lengths stay on the
 // GPU, so that one captured graph serves all of them: each CTA works out its own run.
 #pragma once
 
@@ -28,7 +29,7 @@ struct AttendArgs {
     int32_t *status;
     int64_t q_token, q_head, out_token, out_head, k_page, k_token, k_head, v_page, v_token, v_head;  // bytes
     int64_t table_row, num_pages;
-    int32_t nrequests, nrows, q_heads, heads, group, head_size, page_size, page_shift, table_width, causal, window;  // page_shift: -1 for no power of two
+    int32_t nrequests, nrows, q_heads, heads, group, head_size, page_size, page_shift, table_width, causal, window, undivided;  // page_shift: -1 for no power of two
     float scale;    // of the scores, times log2(e)
 };
 
@@ -214,6 +215,11 @@ template <int M, int BK, int COST> struct Run {
             if (n < 32) break;
         }
         skip = static_cast<int>(rest);
+        if (a.undivided && skip) {  // the tile that begins in front of this run is another's
+            at += tile_of<M, BK>(a, r, t).units + COST - skip;
+            skip = 0;
+            ++t;
+        }
     }
 
     __device__ __forceinline__ bool next(const AttendArgs &a, Piece &p) {
@@ -233,7 +239,8 @@ template <int M, int BK, int COST> struct Run {
                 }
             }
             p.tile = tile_of<M, BK>(a, r, t);
-            const int length = p.tile.units + COST, left = length - skip, take = static_cast<int>(min(static_cast<int64_t>(left), to - at));
+            const int length = p.tile.units + COST, left = length - skip;
+            const int take = a.undivided ? left : static_cast<int>(min(static_cast<int64_t>(left), to - at));
             const int begin = max(0, skip - COST), end = max(0, skip + take - COST);
             p.r = r;
             p.request = b, p.head = h, p.t = t;
