@@ -4,8 +4,12 @@
 // once.  So a block is there to keep loads in flight: four warps walk through 16 keys at a time each, every one with a warp of its own
 // that copies keys and values to a ring for it, and no barrier of the block; the warps' sums are joined when the block's piece of
 // the tile ends, while the next piece's keys are on their way.  Copies are 16 bytes a lane, asynchronous: pages may have any size and
-// strides.  (A bulk copy a row is one instruction for 32 rows, but took 2,400 cycles to issue where these take 500.)  Products are m16n8k16 on fragments in registers: tcgen05 takes 64 rows at least, its accumulator would have to come back from
-// tensor memory for each 16 keys, and at 16 rows the products take less than a fifth of the time that the keys take to arrive.
+// strides.  (A bulk copy a row is one instruction for 32 rows, but took 2,400 cycles to issue where these take 500.)  Products are
+// m16n8k16 on fragments in registers: tcgen05 takes 64 rows at least, its accumulator would have to come back from tensor memory for each
+// 16 keys, and at 16 rows the products take less than a fifth of the time that the keys take to arrive.
+//
+// A step of 64 requests of up to 4,096 tokens (32 / 8 heads, 753 MB): 147 us, 5.1 TB/s; the blocks read at 6.0 while they run.  One request of
+// 32,768 tokens (134 MB): 36 us, of which 6 pass before keys flow and 6 while 18 blocks' parts of each head are joined.
 #include "cg_attend.cuh"
 
 namespace cg {
@@ -376,7 +380,9 @@ int launch_attend_rows(const AttendArgs &a, int ctas, cudaStream_t st) {
     return launch(combine_rows_kernel<DT, DP>, dim3(ctas), kJoinThreads, 0, true, st, a);
 }
 
-// Tiles of at most so many units stay whole: what a second kernel takes to join parts, 4 to 5 us, is more than these units take.
+// Tiles of at most so many units stay whole: what a second kernel takes to join parts, 4 to 5 us, is more than these units take.  (40 requests
+// of 250 tokens of 32 heads: 41 us, divided 44; 400 rows over 300 keys of two requests: 18 us, divided 23.  With eight units one request of
+// 400 tokens takes 13.7 us instead of 10.3.)
 constexpr int kUndividedUnits = 4;
 
 // What a call launches, from what the host knows: the tensors' sizes.
@@ -397,7 +403,10 @@ int plan_of(const cg_attention_job &j, Plan &p) {
     if (j.nrequests > CG_MAX_REQUESTS) return CG_E_CAPACITY;
     const int64_t group = j.q_heads / j.heads;
     const int most = !j.q_starts ? 1 : j.max_q > 0 ? j.max_q : j.nrows;
-    p.tiles = most * group > kRowsM && j.scale > 0.0f;  // (its maxima are those of unscaled scores)
+    // More rows than one tile of the kernel for few would read the keys several times: 16 requests of 4,000 tokens with 20 rows a head take 59 us
+    // with the kernel for many and 91 with that for few, with 16 rows 58 and 57, with 4 rows 59 and 54.  (Its maxima are those of
+    // unscaled scores: a scale that is not positive is the other kernel's.)
+    p.tiles = most * group > kRowsM && j.scale > 0.0f;
     p.dp = j.head_size > 64 ? 128 : 64;
     const int M = p.tiles ? kTileRows : kRowsM, BK = p.tiles ? kTileKeys : kRowsBK;
     const int64_t keys = static_cast<int64_t>(j.table_width) * j.page_size;

@@ -29,7 +29,9 @@ struct AttendArgs {
     int32_t *status;
     int64_t q_token, q_head, out_token, out_head, k_page, k_token, k_head, v_page, v_token, v_head;  // bytes
     int64_t table_row, num_pages;
-    int32_t nrequests, nrows, q_heads, heads, group, head_size, page_size, page_shift, table_width, causal, window, undivided;  // page_shift: -1 for no power of two
+    int32_t page_shift;  // log2(page_size), -1 if that is no power of two
+    int32_t nrequests, nrows, q_heads, heads, group, head_size, page_size, table_width, causal, window;
+    int32_t undivided;  // tiles are not divided among CTAs
     float scale;    // of the scores, times log2(e)
 };
 
@@ -386,8 +388,8 @@ __device__ __forceinline__ void store_joined(const AttendArgs &a, const Lengths 
 }
 
 // Joins what the CTAs of a divided tile of many rows have left.  Block (i, j): 64 rows of the tile that begins in CTA i, a row a thread,
-// four 16-byte pieces of it, of four CTAs on their way together: one request's rows over a long context are in dozens.  Sums are stored [DP / 4][M][4], as a kernel with a row a thread writes
-// them side by side.
+// four 16-byte pieces of it, of four CTAs on their way together: one request's rows over a long context are in dozens.  Sums are stored
+// [DP / 4][M][4], as a kernel with a row a thread writes them side by side.
 template <int DT, int M, int DP>
 __global__ void __launch_bounds__(64 * (DP / 16)) combine_kernel(const __grid_constant__ AttendArgs a) {
     wait_for_launch_before();

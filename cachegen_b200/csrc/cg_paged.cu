@@ -199,7 +199,8 @@ int launch_move(MoveArgs &a, bool interleaved, cudaStream_t st) {
     const int pieces = vec ? a.head_size / 16 : 32, lanes = kMoveThreads / pieces;
     // Few tokens: a block each, all lanes on its heads, for the shortest time.  Many: a thread goes through up to sixteen rows, so that
     // its cosines and its slot are worked out once for them: four tokens a block, then layers, as long as the blocks fill
-    // every SM twice.
+    // every SM twice.  (1,999 tokens of 32 + 32 heads: 22.9 us by fours, 26.4 one by one; 1,999 keys of 32 layers of 8 heads: 48 us
+    // with eight layers a block, 80 with one.)
     const int64_t blocks = static_cast<int64_t>(sm_count()) * 8;
     const int64_t rows = static_cast<int64_t>(a.ntokens) * a.heads * a.nlayers;
     a.tokens_per_block = lanes >= 4 && rows / (4 * lanes) >= blocks ? 4 : 1;
