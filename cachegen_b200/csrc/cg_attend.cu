@@ -411,6 +411,7 @@ int plan_of(const cg_attention_job &j, Plan &p) {
     const int M = p.tiles ? kTileRows : kRowsM, BK = p.tiles ? kTileKeys : kRowsBK;
     const int64_t keys = static_cast<int64_t>(j.table_width) * j.page_size;
     const int64_t per_tile = keys <= BK ? 1 : (keys + BK - 1) / BK;                              // units of a tile, at most
+    if ((static_cast<int64_t>(j.nrows) * group / M + 1) * (per_tile + kTileCost) > INT32_MAX) return CG_E_CAPACITY;  // a request's units a head
     const int64_t tiles = (static_cast<int64_t>(j.nrows) * group / M + j.nrequests) * j.heads;  // at most
     const int64_t slots = static_cast<int64_t>(sm_count()) * (p.tiles ? 1 : 2);
     p.ctas = static_cast<int>(per_tile > slots || tiles * per_tile > slots ? slots : tiles * per_tile);

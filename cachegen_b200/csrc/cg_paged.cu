@@ -204,6 +204,9 @@ int launch_move(MoveArgs &a, bool interleaved, cudaStream_t st) {
     const int64_t blocks = static_cast<int64_t>(sm_count()) * 8;
     const int64_t rows = static_cast<int64_t>(a.ntokens) * a.heads * a.nlayers;
     a.tokens_per_block = lanes >= 4 && rows / (4 * lanes) >= blocks ? 4 : 1;
+    // (a block of few heads has more tokens, so that it has threads)
+    const int room = lanes / a.heads < a.ntokens ? lanes / a.heads : a.ntokens;
+    if (a.tokens_per_block < room) a.tokens_per_block = room;
     a.head_lanes = lanes / a.tokens_per_block;
     if (a.head_lanes > a.heads) a.head_lanes = a.heads;  // (idle lanes would only wait)
     a.layers_per_block = 1;

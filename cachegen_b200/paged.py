@@ -204,7 +204,7 @@ def apply_rotary(x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, out: 
     it), in `out` (which may be x) or a new tensor.  positions: int32 or int64 [tokens], or [n, tokens].
     Moving cached keys by d positions is a turn by d: positions of d everywhere."""
     if rotary is not None:
-        done = _lib.calls().rotary(x, out, inverse, *_turns_for(rotary, x), positions)
+        done = _lib.calls().rotary(x, out, bool(inverse), *_turns_for(rotary, x), positions)
         if done is not None:
             return _finish(done, "apply_rotary")
     _head(x, "x")
@@ -342,7 +342,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     Returns `out` (a new tensor if not given; rows of no request are left as they are), with return_lse also the float32
     logarithm of each row's sum of exponentials [rows, q_heads]."""
-    scale = 1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None else scale
+    scale = 1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None else float(scale)
+    causal, return_lse = bool(causal), bool(return_lse)
     done = _lib.calls().attend(q, k_pages, v_pages, page_table, kv_lens, q_starts, scale, causal, window, max_q, out, return_lse, _status_of(q))
     if done is not None:
         return _finish(done, "paged_attention")
@@ -389,7 +390,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     job.q_strides[:], job.out_strides[:] = _steps(q), _steps(out)
     job.pages_k_strides[:], job.pages_v_strides[:] = _steps(k_pages), _steps(v_pages)
     job.dtype, job.nrequests, job.nrows, job.q_heads, job.heads, job.head_size = _DTYPES[dtype], B, R, Q, H, D
-    job.page_size, job.table_width, job.causal, job.window, job.max_q = S, page_table.shape[1], bool(causal), min(window, 2 ** 31 - 1), max_q
+    job.page_size, job.table_width, job.causal, job.window, job.max_q = S, page_table.shape[1], causal, min(window, 2 ** 31 - 1), max_q
     job.scale = scale
     with on_device(dev):
         need = _lib.lib().cg_paged_attention_workspace(ctypes.byref(job))

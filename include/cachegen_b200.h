@@ -533,7 +533,8 @@ int cg_gather_paged(const cg_rows_job *job_host, void *stream);
  * lse: float32 [nrows, q_heads] or NULL.  max_q: the most rows of a request, or 0; it only chooses between two kernels.
  *
  * A page outside the cache counts as zeros, lengths that do not fit the table or the rows are cut; both raise CG_S_BAD_PAGE.
- * head_size: a multiple of 8 up to 128; nrequests <= CG_MAX_REQUESTS; at most 2^30 keys a request.  The arrays of lengths and pages
+ * head_size: a multiple of 8 up to 128; nrequests <= CG_MAX_REQUESTS; at most 2^30 keys a request, and rows times keys
+ * (by the table's width) of a key/value head below 2^45.  The arrays of lengths and pages
  * must not change while the call runs.  workspace: cg_paged_attention_workspace(job) bytes of device memory
  * (16-byte aligned; 0: none), which calls on one stream may share.  nrows or nrequests 0: nothing is done.
  */

@@ -337,3 +337,15 @@ def test_values_of_hidden_keys_stay_out_of_few_rows_over_many_keys(value):
     want, _, tol = attention(b.q, b.k, b.v, b.table, b.lens, b.scale)
     fine = want.isfinite()
     assert torch.equal(out.isfinite(), fine) and int((~fine).sum()) == 10 * 2 and bool(((out.double() - want).abs() <= tol)[fine].all())
+
+
+def test_arguments_of_kindred_types():
+    """Numbers for truth values, whole numbers and arrays' elements for floats: the same call."""
+    import numpy as np
+    b = Batch([(20, 50), (3, 9)], 4, 2, 64, 16, torch.float16)
+    for causal in (True, False):
+        want = b.call(causal=causal, scale=1.0, window=16)
+        for kind in (int, np.bool_):
+            got = b.call(causal=kind(causal), scale=1, window=16)
+            assert all(torch.equal(x, y) for x, y in zip(want, got))
+        assert all(torch.equal(x, y) for x, y in zip(want, b.call(causal=causal, scale=np.float64(1.0), window=16)))

@@ -33,7 +33,7 @@ def same(a, b):
 SHAPES = [  # lead, tokens, heads, head, rotary dims
     ((), 1, 1, 128, 128), ((), 37, 8, 128, 128), ((), 5, 3, 64, 32), ((), 9, 2, 80, 80), ((), 4, 1, 96, 48), ((3,), 17, 4, 128, 64),
     ((), 3, 2, 2, 2), ((), 6, 5, 7, 4), ((2,), 3, 3, 72, 40), ((), 3000, 8, 128, 128), ((33,), 130, 8, 128, 128), ((), 2, 300, 16, 16),
-    ((), 2, 1, 512, 512), ((70000,), 1, 1, 16, 16)]
+    ((), 2, 1, 512, 512), ((70000,), 1, 1, 16, 16), ((), 5000, 1, 128, 64), ((2,), 77, 1, 16, 16), ((), 1000, 3, 256, 128)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -51,6 +51,7 @@ def test_rotary(lead, tokens, heads, head, rot, interleaved, dtype):
     again = x.clone()
     assert paged.apply_rotary(again, positions.int(), r, out=again) is again and same(again, got)  # in place
     back = paged.apply_rotary(x, positions, r, inverse=True)
+    assert same(back, paged.apply_rotary(x, positions, r, inverse=1))
     assert near(back, x, turned(x, positions, r.frequencies, rot, interleaved, inverse=True), rot, interleaved)
 
 

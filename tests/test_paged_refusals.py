@@ -61,7 +61,7 @@ def test_attention_jobs_are_refused():
     for given, code in (({"dtype": 2}, -7), ({"nrequests": -1}, -2), ({"nrows": -1}, -2), ({"heads": 0}, -2), ({"q_heads": 0}, -2), ({"q_heads": 7}, -2),
                         ({"head_size": 0}, -2), ({"head_size": 136}, -2), ({"head_size": 68}, -5), ({"page_size": 0}, -2), ({"table_width": -1}, -2),
                         ({"num_pages": -1}, -2), ({"num_pages": 1 << 31}, -2), ({"window": -1}, -2), ({"max_q": -1}, -2), ({"nrows": 1 << 29}, -2),
-                        ({"q_starts": None}, -2), ({"nrequests": 4097}, -6)):
+                        ({"q_starts": None}, -2), ({"nrequests": 4097}, -6), ({"nrows": 1 << 27, "table_width": 1 << 21}, -6)):
         assert L.cg_paged_attention(attention_job(**given), None) == code, given
         assert L.cg_paged_attention_workspace(attention_job(**given)) == code, given
     for given, code in (({"q": None}, -1), ({"out": None}, -1), ({"kv_lens": None}, -1), ({"table": None}, -1), ({"pages_k": None}, -1), ({"pages_v": None}, -1),
