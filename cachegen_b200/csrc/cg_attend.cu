@@ -136,8 +136,8 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
         const int rows = min(kRowsM, x.r.n * a.group - x.t * kRowsM);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int row = g + 8 * i, at = x.t * kRowsM + row, token = at / a.group;
-            const char *q = a.q + (x.r.first + token) * a.q_token + (x.head * a.group + at - token * a.group) * a.q_head + 2 * q2;
+            const int row = g + 8 * i, at = x.t * kRowsM + row, token = token_of<kRowsM>(a, at);
+            const char *q = a.q + (x.r.first + token) * a.q_token + (x.head * a.group + member_of(a, at, token)) * a.q_head + 2 * q2;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
 #pragma unroll
@@ -160,13 +160,14 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
         int lo[2], hi[2];  // the keys that this thread's two rows see
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int row = g + 8 * i, token = (row0 + row) / a.group;
+            const int row = g + 8 * i, token = token_of<kRowsM>(a, row0 + row);
             lo[i] = row < rows ? first_key(a, r, token) : 0;
             hi[i] = row < rows ? last_key(a, r, token) : 0;
         }
         // chunks inside [all_lo, all_hi) are seen by all rows
-        const int all_lo = first_key(a, r, (row0 + rows - 1) / a.group), all_hi = last_key(a, r, row0 / a.group);
-        const bool mixed = (row0 + rows - 1) / a.group != row0 / a.group;  // whether rows see unlike keys (what none sees is zero)
+        const int first_token = token_of<kRowsM>(a, row0), last_token = token_of<kRowsM>(a, row0 + rows - 1);
+        const int all_lo = first_key(a, r, last_token), all_hi = last_key(a, r, first_token);
+        const bool mixed = last_token != first_token;  // whether rows see unlike keys (what none sees is zero)
         const int nchunks = p.end - p.begin;
         const int key0 = p.begin * kRowsBK + warp * kChunk;
 
@@ -397,7 +398,7 @@ int plan_of(const cg_attention_job &j, Plan &p) {
     if (j.dtype != CG_F16 && j.dtype != CG_BF16) return CG_E_DTYPE;
     if (j.nrequests < 0 || j.nrows < 0 || j.heads <= 0 || j.q_heads <= 0 || j.q_heads % j.heads || j.head_size <= 0 || j.page_size <= 0 ||
         j.table_width < 0 || j.num_pages < 0 || j.num_pages > INT32_MAX || j.window < 0 || j.max_q < 0 || j.head_size > 128 ||
-        static_cast<int64_t>(j.nrows) * j.q_heads > INT32_MAX || (!j.q_starts && j.nrows != j.nrequests))
+        static_cast<int64_t>(j.nrows) * j.q_heads > INT32_MAX - 512 || (!j.q_starts && j.nrows != j.nrequests))
         return CG_E_SHAPE;
     if (j.head_size % 8) return CG_E_ALIGN;
     if (j.nrequests > CG_MAX_REQUESTS) return CG_E_CAPACITY;
@@ -461,7 +462,8 @@ extern "C" int cg_paged_attention(const cg_attention_job *job, void *stream) {
     a.nrequests = j.nrequests, a.nrows = j.nrows, a.q_heads = j.q_heads, a.heads = j.heads, a.group = j.q_heads / j.heads;
     a.head_size = j.head_size, a.page_size = j.page_size, a.table_width = j.table_width, a.causal = j.causal, a.window = j.window;
     a.undivided = p.undivided;
-    a.page_shift = j.page_size & (j.page_size - 1) ? -1 : __builtin_ctz(static_cast<unsigned>(j.page_size));
+    const auto log2_of = [](int n) { return n & (n - 1) ? -1 : __builtin_ctz(static_cast<unsigned>(n)); };
+    a.page_shift = log2_of(j.page_size), a.group_shift = log2_of(a.group);
     a.scale = j.scale * 1.44269504088896340736f;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (p.tiles) return launch_attend_tiles(a, j.dtype, p.ctas, st);

@@ -253,10 +253,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             const int step = both ? 2 : 1, first = both ? half : 0, top_row = both ? 0 : half * 128, row = top_row + in_half;
             if (first >= blocks) continue;
             const bool there = row < rows;
-            const int token = there ? (row0 + row) / a.group : 0, head = p.head * a.group + (there ? (row0 + row) % a.group : 0);
+            const int token = there ? token_of<kTileRows>(a, row0 + row) : 0, head = p.head * a.group + (there ? member_of(a, row0 + row, token) : 0);
             // (rows behind the last see everything: they ask for no masks)
             const int lo = there ? first_key(a, r, token) : 0, hi = there ? last_key(a, r, token) : INT32_MAX;
-            const int half_lo = first_key(a, r, (row0 + min(rows, top_row + 128) - 1) / a.group), half_hi = last_key(a, r, (row0 + top_row) / a.group);
+            const int half_lo = first_key(a, r, token_of<kTileRows>(a, row0 + min(rows, top_row + 128) - 1)), half_hi = last_key(a, r, token_of<kTileRows>(a, row0 + top_row));
             const bool any_masked = p.begin * kTileKeys < half_lo || p.end * kTileKeys > half_hi;
             float m = kNegInf, l = 0.0f;
             for (int j = first; j < blocks; j += step) {
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 __syncwarp();  // (the row has been written once)
                 float x[DP / 32], top, total;
                 slow_row<DT, DP>(a, r, p.request, p.head, row0 + i, p.begin * kTileKeys, p.end * kTileKeys, x, top, total);
-                const int tok = (row0 + i) / a.group, hd = p.head * a.group + (row0 + i) % a.group;
+                const int tok = token_of<kTileRows>(a, row0 + i), hd = p.head * a.group + member_of(a, row0 + i, tok);
                 const bool any = last_key(a, r, tok) > first_key(a, r, tok);
 #pragma unroll
                 for (int c = 0; c < DP / 32; ++c) {
@@ -442,9 +442,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         const uint32_t at_piece = static_cast<uint32_t>(piece / 8) * 16384;
         const bool box_lane = maps.rows && lane % maps.rows == 0;  // the lane of a box's first token
         const int box_bytes = 32 * DP * 2;
-        int stage = 0, untold = 0, q_phase = 1;  // of the next tile; tiles by copies, the last ones begun, that have not been told of
+        int stage = 0, untold = 0, q_phase = 0;  // of the next tile; tiles by copies, the last ones begun, that have not been told of
         uint32_t phase = 1;                      // (a barrier's phase before its first is over)
-        bool ok = true;
+        bool ok = true, first_piece = true;
         const auto tell_first = [&]() {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -486,7 +486,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 const int key = (p.begin + j) * kTileKeys + 32 * w + lane;
                 return j < blocks && key >= p.lo && key < p.hi ? page_of(a, p.request, page_index(a, key)) : -1;
             };
+            const auto copy_queries = [&]() {
+#pragma unroll 1
+                for (int half = 0; half < (rows > 128 ? 2 : 1); ++half) {
+                    const int row = half * 128 + 32 * w + lane;
+                    const bool there = row < rows;
+                    const int token = there ? token_of<kTileRows>(a, row0 + row) : 0, head = p.head * a.group + (there ? member_of(a, row0 + row, token) : 0);
+                    copy_rows(base + half * kTileBytes<DP>, a.q + (r.first + token) * a.q_token + head * a.q_head, there);
+                }
+            };
             int page = page_for(0);
+            if (first_piece) copy_queries();  // while the table is read
             tell_all();  // what the products of the piece before need
 #pragma unroll 1
             for (int j = 0; ok && j < blocks; ++j) {
@@ -520,16 +530,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     }
                 }
                 if (!ok || j > 0) continue;
-                // queries, behind the first block's tiles, which are on their way meanwhile: once the last products with the ones before are done
-                if (!(ok = warp_wait(bar(kQEmpty), q_phase, failed, a.status))) break;
-                q_phase ^= 1;
-#pragma unroll 1
-                for (int half = 0; half < (rows > 128 ? 2 : 1); ++half) {
-                    const int row = half * 128 + 32 * w + lane;
-                    const bool there = row < rows;
-                    const int token = there ? (row0 + row) / a.group : 0, head = p.head * a.group + (there ? (row0 + row) % a.group : 0);
-                    copy_rows(base + half * kTileBytes<DP>, a.q + (r.first + token) * a.q_token + head * a.q_head, there);
+                // the queries of all pieces but the first, behind the first block's tiles: once the last products with the ones before are done
+                if (!first_piece) {
+                    if (!(ok = warp_wait(bar(kQEmpty), q_phase, failed, a.status))) break;
+                    q_phase ^= 1;
+                    copy_queries();
                 }
+                first_piece = false;
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
