@@ -118,8 +118,8 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
                     const int row = i * kRowsAtOnce + lane / kPieces;
                     const int64_t k_at = __shfl_sync(0xffffffffu, at, row), v_at = __shfl_sync(0xffffffffu, at, 16 + row);
                     const int bytes = there >> row & 1 ? in_head : 0;
-                    copy16(to + i * kRowsAtOnce * kRow, bytes ? keys + k_at : a.k, bytes);
-                    copy16(to + (kChunk + i * kRowsAtOnce) * kRow, bytes ? values + v_at : a.v, bytes);
+                    copy16(to + i * kRowsAtOnce * kRow, bytes ? keys + k_at : a.q, bytes);
+                    copy16(to + (kChunk + i * kRowsAtOnce) * kRow, bytes ? values + v_at : a.q, bytes);
                 }
                 arrive_behind_copies(full + 8 * stage);
                 if (++stage == kStages) stage = 0, phase ^= 1, round = true;

@@ -624,11 +624,11 @@ class CacheGenDeserializer(Deserializer):
             if _chunk_tokens(eo) > self.chunk_size:
                 raise RuntimeError(f"a blob holds more tokens than chunk_size = {self.chunk_size}")
         k_pages, v_pages = self._paged_parts(pages, slots, sum(_chunk_tokens(eo) for eo in encoder_outputs), encoder_outputs[0])
+        if _on_gpu(encoder_outputs[0]) and _device_of(encoder_outputs[0]) != pages.device:
+            raise RuntimeError(f"the chunks are on {_device_of(encoder_outputs[0])}, the pages on {pages.device}")
         with on_device(pages.device):
             kv = decode_many(encoder_outputs, self._bins_on(pages.device), self.fmt, pages.dtype, workspace=self._workspace, delta=self.delta,
                              host_bins=self._host_bins)
-            if kv.device != pages.device:
-                raise RuntimeError(f"the chunks are on {kv.device}, the pages on {pages.device}")
             paged.append_paged(*paged.split_blob(kv, self.fmt), k_pages, v_pages, slots, rotary=rotary, positions=positions)
 
     def from_bytes_paged(self, blobs: List[bytes], pages: torch.Tensor, slots: torch.Tensor, rotary=None,
