@@ -435,10 +435,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         // ================================================================ copies
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         const int w = warp - 8, piece = lane % kPieces;
-        // A tile of copies is told of when kLag more have been begun.  Products may need the second tile behind the first that is not free yet,
-        // so that one has to be told of while the ring holds both and what is between: kLag more than these three.
+        // A tile of copies is told of when kLag more have been begun.  Products may need the tile behind the first that is not free yet: the
+        // ring has to hold both and kLag more.
         constexpr int kLag = 2;
-        static_assert(kStages >= kLag + 3, "the products would wait for a tile that waits for them");
+        static_assert(kStages >= kLag + 2, "the products would wait for a tile that waits for them");
         const uint32_t at_piece = static_cast<uint32_t>(piece / 8) * 16384;
         const bool box_lane = maps.rows && lane % maps.rows == 0;  // the lane of a box's first token
         const int box_bytes = 32 * DP * 2;
@@ -498,14 +498,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             int page = page_for(0);
             if (first_piece) copy_queries();  // while the table is read
             tell_all();  // what the products of the piece before need
+            // Tiles in the order in which products use them: keys and values of a block after the other; with both halves on the same rows the
+            // next block's keys in front of a block's values.
+            const int behind = rows <= 128 ? 1 : 0;
+            int in_page = 0, here = -1, in_page_before = 0, here_before = -1;
 #pragma unroll 1
-            for (int j = 0; ok && j < blocks; ++j) {
-                const int in_page = place_in_page(a, (p.begin + j) * kTileKeys + 32 * w + lane), here = page;
-                const bool boxes = maps.rows && __all_sync(0xffffffffu, here >= 0);
+            for (int j = 0; ok && j < blocks + behind; ++j) {
+                in_page_before = in_page, here_before = here;
+                in_page = place_in_page(a, (p.begin + j) * kTileKeys + 32 * w + lane), here = page;
                 page = page_for(j + 1);
-                if (boxes) tell_all();
 #pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv) {
+                    if (kv ? j < behind : j >= blocks) continue;
+                    const int at_page = kv && behind ? here_before : here, at_token = kv && behind ? in_page_before : in_page;
+                    const bool boxes = maps.rows && __all_sync(0xffffffffu, at_page >= 0);
+                    if (boxes) tell_all();
                     if (!(ok = warp_wait(empty(stage), phase, failed, a.status))) break;
                     const uint32_t tile = tiles_at + stage * kTileBytes<DP>;
                     if (boxes) {
@@ -514,12 +521,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                         if (box_lane) {
 #pragma unroll
                             for (int panel = 0; panel < DP / 64; ++panel)
-                                tma_box(tile + panel * 16384 + (32 * w + lane) * 128, kv ? &maps.v : &maps.k, 64 * panel, in_page, p.head, here, full(stage));
+                                tma_box(tile + panel * 16384 + (32 * w + lane) * 128, kv ? &maps.v : &maps.k, 64 * panel, at_token, p.head, at_page, full(stage));
                         }
                     } else {
-                        const char *at = kv ? a.v + here * a.v_page + in_page * a.v_token + p.head * a.v_head
-                                            : a.k + here * a.k_page + in_page * a.k_token + p.head * a.k_head;
-                        copy_rows(tile, at, here >= 0);
+                        const char *at = kv ? a.v + at_page * a.v_page + at_token * a.v_token + p.head * a.v_head
+                                            : a.k + at_page * a.k_page + at_token * a.k_token + p.head * a.k_head;
+                        copy_rows(tile, at, at_page >= 0);
                         asm volatile("cp.async.commit_group;" ::: "memory");
                         ++untold;
                     }
@@ -587,8 +594,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                         if (last) commit(bar(kQEmpty));
                     };
                     begin(0, k_stage, blocks == 1);
-                    v_stage = tile_there();
-                    if (ok && blocks > 1) {
+                    if (blocks > 1) {
                         k_stage = tile_there();
                         if (ok) fence_after(), begin(1, k_stage, blocks == 2);
                     }
@@ -596,8 +602,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     for (int j = 0; ok && j < blocks; ++j) {
                         const int half = j & 1;
                         const bool more = j + 2 < blocks;
-                        uint32_t v_next = 0;
-                        if (j + 1 < blocks) v_next = tile_there();
+                        v_stage = tile_there();
                         if (!ok || !(ok = warp_wait(bar(kPFull + 2 * half), p_phase >> half & 1, failed, a.status)) ||
                             !(ok = warp_wait(bar(kPFull + 2 * half + 1), p_phase >> half & 1, failed, a.status)))
                             break;
@@ -609,11 +614,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                             if (!more) commit(bar(kOFull + half));
                             commit(empty(v_stage));
                         }
-                        if (more) {  // (not waited for in front of the products: the copies may need the tile that those free)
+                        if (more) {
                             k_stage = tile_there();
                             if (ok) fence_after(), begin(half, k_stage, j + 3 == blocks);
                         }
-                        v_stage = v_next;
                         __syncwarp();
                     }
                     continue;
