@@ -197,3 +197,11 @@ def test_attention_refuses(change):
         given[name] = how(given[name])
     with pytest.raises(RuntimeError):
         paged.paged_attention(**given)
+
+
+def test_turns_are_rounded_to_nearest():
+    import random
+    from fractions import Fraction
+    rng = random.Random(1)
+    for w in [1.0, 0.5, 1e-7, 1e-300, -0.25, 7.0, 0.0] + [rng.uniform(-1, 1) * 10.0 ** rng.randint(-12, 3) for _ in range(300)]:
+        assert paged._turns(w) == round(Fraction(w) / paged._TWO_PI * 2 ** 64) % 2 ** 64
