@@ -256,7 +256,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             const int token = there ? token_of<kTileRows>(a, row0 + row) : 0, head = p.head * a.group + (there ? member_of(a, row0 + row, token) : 0);
             // (rows behind the last see everything: they ask for no masks)
             const int lo = there ? first_key(a, r, token) : 0, hi = there ? last_key(a, r, token) : INT32_MAX;
-            const int half_lo = first_key(a, r, token_of<kTileRows>(a, row0 + min(rows, top_row + 128) - 1)), half_hi = last_key(a, r, token_of<kTileRows>(a, row0 + top_row));
+            const int half_lo = first_key(a, r, token_of<kTileRows>(a, row0 + min(rows, top_row + 128) - 1));
+            const int half_hi = last_key(a, r, token_of<kTileRows>(a, row0 + top_row));
             const bool any_masked = p.begin * kTileKeys < half_lo || p.end * kTileKeys > half_hi;
             float m = kNegInf, l = 0.0f;
             for (int j = first; j < blocks; j += step) {
@@ -475,8 +476,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 const uint64_t from = __shfl_sync(0xffffffffu, where, src);
                 const bool copy = in_head && (rows_there >> src & 1);
                 const uint32_t dst = tile + place[i % kOrders] + i / kOrders * 1024;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(copy ? from + 16 * piece : reinterpret_cast<uint64_t>(a.q)), "r"(copy ? 16 : 0)
-                             : "memory");
+                const uint64_t where_from = copy ? from + 16 * piece : reinterpret_cast<uint64_t>(a.q);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(where_from), "r"(copy ? 16 : 0) : "memory");
             }
         };
         while (ok && next_piece()) {
@@ -610,7 +611,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                         fence_after();
                         if (issues) {
 #pragma unroll
-                            for (int k = 0; k < kTileKeys / 16; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v_desc + v_stage * kTile + k * 128, kOperandHigh, pv, j > 1 || k > 0);
+                            for (int k = 0; k < kTileKeys / 16; ++k)
+                                mma_ts(o_at(half), s_at(half) + 8 * k, v_desc + v_stage * kTile + k * 128, kOperandHigh, pv, j > 1 || k > 0);
                             if (!more) commit(bar(kOFull + half));
                             commit(empty(v_stage));
                         }
@@ -714,8 +716,9 @@ bool map_pages(const AttendArgs &a, int dtype, PageMaps &maps) {
             if (sizes[i + 1] == 1) strides[i] = 16;  // never used
             if (strides[i] == 0 || strides[i] % 16 || strides[i] >= 1ull << 40) return false;
         }
-        return encode(&map, dtype == CG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<char *>(at), sizes, strides, box, steps,
-                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+        const CUtensorMapDataType type = dtype == CG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        return encode(&map, type, 4, const_cast<char *>(at), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     };
     if (!one(maps.k, a.k, a.k_token, a.k_head, a.k_page) || !one(maps.v, a.v, a.v_token, a.v_head, a.v_page)) return false;
     maps.rows = rows;
