@@ -69,9 +69,11 @@ template <int M> __device__ __forceinline__ int token_of(const AttendArgs &a, in
 }
 __device__ __forceinline__ int member_of(const AttendArgs &a, int row, int token) { return row - token * a.group; }
 
-// keys [lo, hi) that token i of n sees
+// keys [lo, hi) that token i of n sees.  (A place may be as low as -2^31 and a window as wide as 2^31 - 1: their difference is only taken where
+// the window ends behind the first key.)
 __device__ __forceinline__ int first_key(const AttendArgs &a, const Lengths &r, int i) {
-    return a.window > 0 ? max(0, r.kv - r.n + i - a.window + 1) : 0;
+    const int place = r.kv - r.n + i;
+    return a.window > 0 && place >= a.window ? place - a.window + 1 : 0;
 }
 __device__ __forceinline__ int last_key(const AttendArgs &a, const Lengths &r, int i) {
     return a.causal ? min(r.kv, max(0, r.kv - r.n + i + 1)) : r.kv;
