@@ -53,8 +53,8 @@ template <int DT> __device__ __forceinline__ bool not_finite2(uint32_t w) {
 
 // Shared memory: kWarps rings of kStages stages of 16 keys, then 16 values; rows are 16 bytes longer than their 2 * DP, so that the
 // eight rows of a matrix lie in different banks.  Then room for a part of the warps' sums, their maxima and sums of weights, a word that
-// says whether values that are not finite were met where rows see unlike keys, one that says that a wait was given up, and the stages'
-// barriers.  Two blocks share an SM.
+// says whether values that are not finite were met where rows see unlike keys, one that says that a wait was given up, one for bar_wait's
+// clock, and the stages' barriers.  Two blocks share an SM.
 template <int DP> constexpr int kRowBytes2 = 2 * DP + 16;
 template <int DP> constexpr int kStageBytes = 2 * kChunk * kRowBytes2<DP>;
 template <int DP> constexpr int kRingBytes = kStages * kStageBytes<DP>;
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
     Run<kRowsM, kRowsBK, kRowsCost> run;
     run.template init<kWarps * 64, false>(a, reinterpret_cast<int64_t *>(smem));
     let_next_launch_start();
-    if (tid == 0) row_odd = 0, *failed = 0;
+    if (tid == 0) row_odd = 0, failed[0] = failed[1] = 0;
     if (!copies && lane == 0) {
         for (int i = 0; i < kStages; ++i) bar_init(full + 8 * i, 32), bar_init(empty + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
         } else {
             for (int row = warp; row < rows; row += kWarps) {
                 float x[DP / 32], top, total;
-                slow_row<DT, DP>(a, r, p.request, p.head, row0 + row, p.begin * kRowsBK, p.end * kRowsBK, x, top, total);
+                slow_row<DT, DP>(a, r, p.request, p.head, row0 + row, p.begin * kRowsBK, p.end * kRowsBK, failed, x, top, total);
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i) sums[warp * kSumFloats + lane + 32 * i] = x[i];
                 __syncwarp();

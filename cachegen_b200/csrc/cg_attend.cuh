@@ -293,46 +293,121 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// One row over keys [k0, k1) by a warp, straight from memory: for tiles in which a key that some rows do not see has values that
-// are not finite, since a weight of zero does not keep those out of a product.  sums[i] is value lane + 32 i of the head.
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+// times in about milliseconds, as bar_wait compares them
+__device__ __forceinline__ uint32_t beat_of(uint64_t ns) { return static_cast<uint32_t>(ns >> 20); }
+__device__ __forceinline__ void beat(volatile int *failed) { failed[1] = static_cast<int>(beat_of(now_ns())); }
+
+// One row over keys [k0, k1) by a warp, straight from memory: for rows that do not see a key of their tile whose values are not finite,
+// since a weight of zero does not keep those out of a product.  32 keys at a time: a lane has a key's score, then each lane its values of all
+// keys.  sums[i] is value lane + 32 i of the head.
 template <int DT, int DP>
-__device__ __forceinline__ void slow_row(const AttendArgs &a, const Lengths &r, int b, int head, int row, int k0, int k1,
+__device__ __forceinline__ void slow_row(const AttendArgs &a, const Lengths &r, int b, int head, int row, int k0, int k1, volatile int *failed,
                                       float (&sums)[DP / 32], float &top, float &total) {
     const int lane = threadIdx.x & 31, token = row / a.group;
     const char *q = a.q + (r.first + token) * a.q_token + (head * a.group + member_of(a, row, token)) * a.q_head;
-    float x[DP / 32];
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-        const int d = lane + 32 * i;
-        x[i] = d < a.head_size ? Half16<DT>::to_float(reinterpret_cast<const uint16_t *>(q)[d]) : 0.0f;
-        sums[i] = 0.0f;
-    }
+    for (int i = 0; i < DP / 32; ++i) sums[i] = 0.0f;
     top = kNegInf, total = 0.0f;
     k0 = max(k0, first_key(a, r, token)), k1 = min(k1, last_key(a, r, token));
-    for (int j = k0; j < k1; ++j) {
-        const int page = page_of(a, b, page_index(a, j)), in_page = place_in_page(a, j);
+#pragma unroll 1
+    for (int j0 = k0; j0 < k1; j0 += 32) {
+        const int j = j0 + lane, page = j < k1 ? page_of(a, b, page_index(a, j)) : -1, in_page = place_in_page(a, j);
         const char *k = a.k + page * a.k_page + in_page * a.k_token + head * a.k_head;
-        const char *v = a.v + page * a.v_page + in_page * a.v_token + head * a.v_head;
-        float s = 0.0f, y[DP / 32];
+        const uint64_t v = reinterpret_cast<uint64_t>(a.v + page * a.v_page + in_page * a.v_token + head * a.v_head);
+        float s = 0.0f;
+        if (page >= 0) {
+#pragma unroll 2
+            for (int d = 0; d < a.head_size; d += 8) {
+                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(q + 2 * d)), y = __ldg(reinterpret_cast<const uint4 *>(k + 2 * d));
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-            const int d = lane + 32 * i;
-            const bool there = d < a.head_size && page >= 0;
-            s += there ? x[i] * Half16<DT>::to_float(reinterpret_cast<const uint16_t *>(k)[d]) : 0.0f;
-            y[i] = there ? Half16<DT>::to_float(reinterpret_cast<const uint16_t *>(v)[d]) : 0.0f;
+                for (int i = 0; i < 4; ++i)
+                    s += Half16<DT>::to_float(static_cast<uint16_t>(xs[i])) * Half16<DT>::to_float(static_cast<uint16_t>(ys[i])) +
+                         Half16<DT>::to_float(static_cast<uint16_t>(xs[i] >> 16)) * Half16<DT>::to_float(static_cast<uint16_t>(ys[i] >> 16));
+            }
         }
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        s *= a.scale;
-        const float now = fmaxf(top, s), base = now == kNegInf ? 0.0f : now;
+        s = j < k1 ? s * a.scale : kNegInf;
+        float now = fmaxf(top, s);
+        for (int d = 16; d; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+        const float base = now == kNegInf ? 0.0f : now;
         const float keep = exp2_approx(top - base), w = exp2_approx(s - base);
         total = total * keep + w;
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) sums[i] = sums[i] * keep + w * y[i];
+        for (int i = 0; i < DP / 32; ++i) sums[i] *= keep;
+        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+#pragma unroll 4
+        for (int n = 0; n < 32; ++n) {
+            const uint64_t from = __shfl_sync(0xffffffffu, v, n);
+            const float weight = __shfl_sync(0xffffffffu, w, n);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+                if ((there >> n & 1) && lane + 32 * i < a.head_size)
+                    sums[i] += weight * Half16<DT>::to_float(__ldg(reinterpret_cast<const uint16_t *>(from) + lane + 32 * i));
+        }
         top = now;
+        if (lane == 0) beat(failed);  // (others of the block wait for this row)
     }
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
 }
 
-constexpr uint64_t kGiveUpNs = 10ull * 1000 * 1000 * 1000;  // a wait takes microseconds, or the length of a slow row
+// Which of a warp's `rows` (a bit a lane; a lane's row sees [lo, hi)) have to be done again, because a key that they do not see has values in
+// [k0, k1) or [k2, k3) that are not finite.  Where a row sees a value of the same column that is no number, its result is that in any
+// case: a cache full of them costs one look at the blocks that not all rows see.  (A call, so that the kernel's loops stay close together: 8,192
+// tokens of 32 heads 590 us, with this in line 600.)
+template <int DT, int DP>
+__device__ __noinline__ uint32_t rows_again(const AttendArgs &a, int b, int head, uint32_t rows, int lo, int hi, int k0, int k1, int k2, int k3) {
+    constexpr int kMine = DP / 32;  // columns of a lane
+    constexpr uint32_t kExponent = DT == CG_F16 ? 0x7C00u : 0x7F80u, kAll = 0xffffffffu;
+    const int lane = threadIdx.x & 31, col = lane * kMine;
+    int bad0[kMine], bad1[kMine], nan0[kMine], nan1[kMine];  // the first and last keys
+#pragma unroll
+    for (int c = 0; c < kMine; ++c) bad0[c] = nan0[c] = INT32_MAX, bad1[c] = nan1[c] = -1;
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+        const int to = part ? k3 : k1;
+#pragma unroll 1
+        for (int j0 = part ? k2 : k0; j0 < to; j0 += 32) {
+            const int j = j0 + lane, page = j < to ? page_of(a, b, page_index(a, j)) : -1;
+            const uint64_t v = reinterpret_cast<uint64_t>(a.v + page * a.v_page + place_in_page(a, j) * a.v_token + head * a.v_head);
+            const uint32_t there = __ballot_sync(kAll, page >= 0);
+#pragma unroll 8
+            for (int n = 0; n < 32; ++n) {
+                const uint64_t from = __shfl_sync(kAll, v, n);
+                uint32_t x[kMine / 2] = {};
+                if ((there >> n & 1) && col < a.head_size) {
+#pragma unroll
+                    for (int c = 0; c < kMine / 2; ++c) x[c] = __ldg(reinterpret_cast<const unsigned int *>(from) + col / 2 + c);
+                }
+#pragma unroll
+                for (int c = 0; c < kMine; ++c) {
+                    const uint32_t u = x[c / 2] >> (16 * (c % 2)) & 0x7FFFu;
+                    if (u >= kExponent) bad0[c] = min(bad0[c], j0 + n), bad1[c] = j0 + n;
+                    if (u > kExponent) nan0[c] = min(nan0[c], j0 + n), nan1[c] = j0 + n;
+                }
+            }
+        }
+    }
+    uint32_t again = 0;
+    for (; rows; rows &= rows - 1) {
+        const int i = __ffs(rows) - 1, first = __shfl_sync(kAll, lo, i), behind = __shfl_sync(kAll, hi, i);
+        bool yes = false;
+#pragma unroll
+        for (int c = 0; c < kMine; ++c) {
+            const bool hidden = bad0[c] < first || bad1[c] >= behind;
+            const bool none = (nan0[c] >= first && nan0[c] < behind) || (nan1[c] >= first && nan1[c] < behind);
+            yes = yes || (hidden && !none);
+        }
+        if (__any_sync(kAll, yes)) again |= 1u << i;
+    }
+    return again;
+}
+
+constexpr uint64_t kGiveUpNs = 10ull * 1000 * 1000 * 1000;  // a wait takes microseconds
 // ---- barriers in shared memory --------------------------------------------------------------
 __device__ __forceinline__ void bar_init(uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
@@ -342,12 +417,9 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done;
 }
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-// Whether the phase ended.  If it does not within kGiveUpNs, or another wait of the block gave up, the block is told to end.
+// Whether the phase ended.  If it does not within kGiveUpNs, or another wait of the block gave up, the block is told to end.  Behind the word
+// that tells so stands the time (see beat) at which the block was last at work on something long, rows done again or a piece of many
+// keys: the wait goes on while that is recent.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
     uint64_t start = 0;
 #pragma unroll 1
@@ -357,6 +429,10 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
         const uint64_t now = now_ns();
         if (!start) start = now;
         if (now - start > kGiveUpNs) {
+            if (beat_of(now) - static_cast<uint32_t>(failed[1]) <= beat_of(kGiveUpNs)) {
+                start = now;
+                continue;
+            }
             *failed = 1;
             if (status) atomicOr(status, CG_S_TIMEOUT);
             return false;

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
     const auto full = [&](int s) { return bar(kKvFull + s); };
     const auto empty = [&](int s) { return bar(kKvFull + kStages + s); };
     static_assert(8 * (kKvFull + 2 * kStages) <= 320, "room for the barriers");
-    volatile int *words = reinterpret_cast<volatile int *>(mem + kBarsAt<DP> + 320);  // tensor memory, failed
+    volatile int *words = reinterpret_cast<volatile int *>(mem + kBarsAt<DP> + 320);  // tensor memory, failed, bar_wait's clock
     Parcel *parcels = reinterpret_cast<Parcel *>(mem + kBarsAt<DP> + 384);  // [2]
     volatile int *failed = words + 1;
 
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         bar_init(bar(kJoinReady), 4);
         bar_init(bar(kJoinDone), 4);
         for (int s = 0; s < kStages; ++s) bar_init(full(s), 4), bar_init(empty(s), 1);
-        *failed = 0;
+        failed[0] = failed[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) tmem_alloc(base + kBarsAt<DP> + 320, 512);
@@ -412,11 +412,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 a.lse[static_cast<int64_t>(r.first + token) * a.q_heads + head] = sees ? (m + log2f(l)) * 0.693147180559945f : kNegInf;
             if (there && !p.whole) part_ml[row] = make_float2(m, l);
             // A value that is not finite, of a key that some rows do not see, is in all rows' sums: those rows are done again, from memory.
-            for (uint32_t again = __ballot_sync(0xffffffffu, odd && there); again; again &= again - 1) {
+            // (Such keys lie in front of half_lo or from half_hi on; the blocks at these borders have keys that most rows see.)
+            uint32_t again = __ballot_sync(0xffffffffu, odd && there);
+            if (again) {
+                const int k0 = max(p.lo, p.begin * kTileKeys), k3 = min(p.hi, p.end * kTileKeys);
+                const int k1 = half_lo > k0 ? min(k3, (half_lo / kTileKeys + 1) * kTileKeys) : k0;
+                const int k2 = half_hi < k3 ? max(k1, max(half_hi - 1, 0) / kTileKeys * kTileKeys) : k3;
+                again = rows_again<DT, DP>(a, p.request, p.head, again, lo, hi, k0, k1, k2, k3);
+            }
+            for (; again; again &= again - 1) {
                 const int i = top_row + 32 * (warp & 3) + __ffs(again) - 1;
                 __syncwarp();  // (the row has been written once)
                 float x[DP / 32], top, total;
-                slow_row<DT, DP>(a, r, p.request, p.head, row0 + i, p.begin * kTileKeys, p.end * kTileKeys, x, top, total);
+                slow_row<DT, DP>(a, r, p.request, p.head, row0 + i, p.begin * kTileKeys, p.end * kTileKeys, failed, x, top, total);
                 const int tok = token_of<kTileRows>(a, row0 + i), hd = p.head * a.group + member_of(a, row0 + i, tok);
                 const bool any = last_key(a, r, tok) > first_key(a, r, tok);
 #pragma unroll
@@ -603,6 +611,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     for (int j = 0; ok && j < blocks; ++j) {
                         const int half = j & 1;
                         const bool more = j + 2 < blocks;
+                        if ((j & 1023) == 1023) beat(failed);  // (warp 13 waits for the length of a piece)
                         v_stage = tile_there();
                         if (!ok || !(ok = warp_wait(bar(kPFull + 2 * half), p_phase >> half & 1, failed, a.status)) ||
                             !(ok = warp_wait(bar(kPFull + 2 * half + 1), p_phase >> half & 1, failed, a.status)))
@@ -635,6 +644,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
 #pragma unroll 1
                 for (int j = 0; j < blocks; ++j) {
                     const bool more = j + 1 < blocks;
+                    if ((j & 1023) == 1023) beat(failed);
                     v_stage = tile_there();
                     if (ok && more) k_stage = tile_there();  // (ahead of the weights, which all that follows waits for)
                     if (!ok) break;

@@ -17,3 +17,81 @@ def test_windows_wider_than_any_context(lens, heads, window, causal):
     """More rows than keys, so that places are negative: such a window hides nothing."""
     b = Batch(lens, 4, heads, 64, 16, torch.float16)
     b.check(*b.call(window=window, causal=causal, max_q=max(n for n, _ in lens)), causal=causal)
+
+
+def put(b, request, key, head, column, value):
+    b.v[b.table[request].long()[key // 16], key % 16, head, column] = value
+
+
+def agrees(b, **how):
+    """Numbers within the tolerance, and infinities and values that are no numbers where the formula has them."""
+    out, _ = b.call(**how)
+    want, _, tol = attention(b.q, b.k, b.v, b.table, b.lens, b.scale, **how)
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isposinf(), want.isposinf()) and torch.equal(out.isneginf(), want.isneginf())
+    fine = want.isfinite()
+    assert bool(((out.double() - want).abs() <= tol)[fine].all())
+    return want
+
+
+def milliseconds(call):
+    """The least of five, by events, with the call captured, so that the host's part is not in it."""
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    times = []
+    for _ in range(5):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        graph.replay()
+        end.record()
+        end.synchronize()
+        times.append(start.elapsed_time(end))
+    return min(times)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+def test_a_value_that_is_not_finite_and_that_all_see_costs_nothing(dtype):
+    """An infinite value of a prompt's first token reaches every row by right: rows are not done again one by one, key by key, which takes
+    hundreds of times as long.  Neither are they where all values are no numbers.  (Bounds with room: three times, and 0.2 ms.)"""
+    b = Batch([(2000, 2000)], 8, 8, 128, 16, dtype)
+    usual = milliseconds(b.call)
+    put(b, 0, 0, 3, 100, math.inf)
+    want = agrees(b)
+    assert bool(want[:, 3, 100].isposinf().all()) and int(want.isinf().sum()) == 2000
+    assert milliseconds(b.call) <= 3 * usual + 0.2
+    b.v.fill_(math.nan)
+    out, lse = b.call()
+    assert bool(out.isnan().all()) and bool(lse.isfinite().all())
+    assert milliseconds(b.call) <= 3 * usual + 0.2
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("lens,q_heads,heads,head,how", [
+    ([(200, 9000)], 2, 2, 128, {}), ([(300, 4000), (40, 700)], 4, 2, 64, {}), ([(300, 1100)], 2, 2, 64, dict(window=150)),
+    ([(120, 1500)], 2, 1, 128, dict(window=300)), ([(150, 700)], 4, 4, 80, dict(window=64, causal=False)), ([(14, 600), (5, 5)], 2, 2, 128, dict(window=200)),
+    ([(260, 100)], 2, 2, 64, {})], ids=ids)
+def test_values_that_are_not_finite_anywhere(lens, q_heads, heads, head, how, dtype):
+    """Infinities and values that are no numbers at keys that all rows of a tile see, some or none; in tiles that are divided and in whole
+    ones, in blocks at the borders of what rows see."""
+    b = Batch(lens, q_heads, heads, head, 16, dtype, seed=5)
+    g = torch.Generator()
+    g.manual_seed(len(lens) + lens[0][0])
+    for request, (n, kv) in enumerate(lens):
+        places = [0, kv - 1, kv - 2] + torch.randint(0, kv, (4,), generator=g).tolist() + torch.randint(max(0, kv - n), kv, (6,), generator=g).tolist()
+        for i, key in enumerate(places):
+            column = int(torch.randint(0, head, (1,), generator=g))
+            put(b, request, key, i % heads, column, (math.inf, -math.inf, math.nan)[i % 3])
+    want = agrees(b, **how)
+    assert int((~want.isfinite()).sum()) > 0
+
+
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_new_values_that_are_all_not_finite(value):
+    """Every row is done again, or none, and each sees what it should."""
+    b = Batch([(140, 900), (300, 300)], 2, 2, 64, 16, torch.bfloat16)
+    for request, (n, kv) in enumerate([(140, 900), (300, 300)]):
+        j = torch.arange(kv - n, kv, device="cuda")
+        b.v[b.table[request].long()[j // 16], j % 16, 1] = value
+    want = agrees(b)
+    assert bool(want[:, 0].isfinite().all()) and not want[:, 1].isfinite().any()
