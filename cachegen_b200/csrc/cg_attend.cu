@@ -65,6 +65,11 @@ template <int DP> constexpr int kMlAt = kSumsAt<DP> + kWarps * kSumFloats * 4;
 template <int DP> constexpr int kAttendSmem = kMlAt<DP> + kWarps * kRowsM * 8 + 16 + 16 * kWarps * kStages;
 static_assert(2 * (kAttendSmem<128> + 1024) <= 228 * 1024, "two blocks an SM");
 
+// Weights are numbers up to 1, rounded to the cache's type for the second product.  Those of fp16 are 2^15 times that: its step stops
+// shrinking at 2^-14 and what is below 2^-25 is 0, where a million such weights beside a large one are 3 % of the result.  So they are off by half a
+// step down to 2^-29 of the largest; those below 2^-40 are 0, of n keys n 2^-40 together.  The sum of weights is as many times larger.
+template <int DT> constexpr float kLift = DT == CG_F16 ? 15.0f : 0.0f;
+
 template <int DT, int DP>
 __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __grid_constant__ AttendArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -224,7 +229,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
                     for (int k = 0; k < kSteps * 2; ++k) o[k][2 * i] *= keep, o[k][2 * i + 1] *= keep;
                 }
             }
-            const float base[2] = {m[0] == kNegInf ? 0.0f : m[0], m[1] == kNegInf ? 0.0f : m[1]};
+            const float base[2] = {m[0] == kNegInf ? 0.0f : m[0] - kLift<DT>, m[1] == kNegInf ? 0.0f : m[1] - kLift<DT>};
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -232,7 +237,6 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
                     s[i][k] = exp2_approx(s[i][k] - base[k >> 1]);
                     l[k >> 1] += s[i][k];
                 }
-            // weights are between 0 and 1 and rounded to the cache's type for the product: off by half a step each, without bias
             const uint32_t w[4] = {pack_pair<DT>(s[0][0], s[0][1]), pack_pair<DT>(s[0][2], s[0][3]),
                                    pack_pair<DT>(s[1][0], s[1][1]), pack_pair<DT>(s[1][2], s[1][3])};
 #pragma unroll
@@ -253,6 +257,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
         // ---- the warps' sums become one
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+            m[i] -= kLift<DT>;  // what the sums are relative to
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
             if ((lane & 3) == 0) row_ml[warp][g + 8 * i] = make_float2(m[i], l[i]);

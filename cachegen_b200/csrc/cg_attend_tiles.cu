@@ -145,7 +145,10 @@ template <int DT> __device__ __forceinline__ uint32_t round_pair(float lo, float
     else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
     return w;
 }
-// 32 scores to weights 2^(s * scale + down), rounded to 16 bits for the product: off by half a step each, without bias
+// 32 scores to weights 2^(s * scale + down), rounded to 16 bits for the product: off by half a step each.  Those of fp16 are 2^7 times what they
+// are of bf16, so up to 2^15 with a maximum that lags behind by 2^8: its step stops shrinking at 2^-14.  So half a step holds
+// down to 2^-21 of the largest; what is below 2^-32 is 0, of n keys n 2^-32 together.  The sum of weights is as many times larger.
+template <int DT> constexpr float kLift = DT == CG_F16 ? 7.0f : 0.0f;
 template <int DT> __device__ __forceinline__ void weigh(const uint32_t (&x)[32], uint64_t scale, uint64_t down, uint32_t (&w)[16], uint64_t (&sum)[2]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                         }
                     }
                 }
-                const float base = m == kNegInf ? 0.0f : -m;
+                const float base = m == kNegInf ? 0.0f : kLift<DT> - m;
                 const uint64_t scale = pair_of(a.scale, a.scale), down = pair_of(base, base);
                 uint64_t sum[2] = {0, 0};
                 // (weights take half the columns of the scores that they come from: these have been read)
@@ -327,6 +330,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 const float2 s0 = parts_of(sum[0]), s1 = parts_of(sum[1]);
                 l += (s0.x + s0.y) + (s1.x + s1.y);
             }
+            m -= kLift<DT>;  // what the sums are relative to
             ok = ok && warp_wait(bar(kOFull + half), o_phase, failed, a.status);
             o_phase ^= 1;
             if (!ok) break;

@@ -95,3 +95,43 @@ def test_new_values_that_are_all_not_finite(value):
         b.v[b.table[request].long()[j // 16], j % 16, 1] = value
     want = agrees(b)
     assert bool(want[:, 0].isfinite().all()) and not want[:, 1].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("n,requests", [(1, 600), (20, 160)])
+def test_many_small_weights_beside_a_large_one(n, requests, dtype):
+    """One key with a score of 17.375 and values 0 over a million with score 0 and values 1: each of these has 2^-25.07 of its weight, below half the
+    smallest fp16 number, and all together S = 3 %, so the result is S / (1 + S).  (Of more requests than there are blocks, so that blocks
+    have whole requests: parts without the large weight are relative to the small ones.)
+
+    Tolerance, as a share of the result: its rounding by half a step; that of a weight, by half a step in the rows' kernel; in the other, where
+    2^-18.07 is what fp16 has of it, by 2^-25, 0.8 %.  32-bit sums: up to 2^16 steps of 16 products, each off by 2^-23 of half the sum on average
+    (products may cut off): 0.4 %; and in the sum of weights a thread adds one at a time to the large one, for a quarter of a quarter of the
+    keys, and may lose all of these: S / 16, 0.2 %; exponents of 25 in 32 bits 2^-20.
+
+    With values of 1 at that key too the result is 1.  A 32-bit sum that has reached 1 may lose summands below 2^-24 of it whole, and these
+    are: the small weights that are summed with the large one, S / 4 of single rows (by one of four warps), S / 2 of chunks (by one of two groups)."""
+    from cachegen_b200 import paged
+    kv, D, page = 2 ** 20, 8, 64
+    k, v = torch.zeros((kv // page, page, 1, D), dtype=dtype, device="cuda"), torch.ones((kv // page, page, 1, D), dtype=dtype, device="cuda")
+    q = torch.zeros((n * requests, 1, D), dtype=dtype, device="cuda")
+    q[:, :, 0] = 1
+    table = torch.arange(kv // page, dtype=torch.int32, device="cuda").expand(requests, -1)
+    lens = torch.full((requests,), kv, dtype=torch.int32, device="cuda")
+    starts = torch.arange(0, n * requests + 1, n, dtype=torch.int32, device="cuda")
+    score = 17.375  # a bf16 number
+    half = torch.finfo(dtype).eps / 2
+    for main in (0, 500_000, kv - n):
+        k.zero_(), v.fill_(1)
+        k[main // page, main % page, 0, 0] = score
+        v[main // page, main % page] = 0
+        out, lse = paged.paged_attention(q, k, v, table, lens, starts, scale=1.0, max_q=n, return_lse=True)
+        small = torch.arange(kv - n, kv, device="cuda").double().repeat(requests)[:, None] * math.exp(-score)
+        want = (small / (1 + small))[..., None]
+        off = ((out.double() - want).abs() / want).max().item()
+        beside, _ = paged.paged_attention(q, k, torch.ones_like(v), table, lens, starts, scale=1.0, max_q=n, return_lse=True)
+        assert bool(((beside.double() - 1).abs() <= half + 0.001 + (small * (1 / 16 + (1 / 4 if n == 1 else 1 / 2)))[..., None]).all())
+        assert off <= 2 * half + 0.004 + 0.002 + (0.008 if n > 1 and dtype == torch.float16 else 0), off
+        # the sum of weights as above, and the logarithm's rounding, a step of 17 2^-19
+        assert bool(((lse.double() - score - torch.log1p(small)).abs() <= small / 16 + 2.0 ** -18).all())
+    paged.check_status()
