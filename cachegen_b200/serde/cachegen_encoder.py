@@ -680,9 +680,13 @@ class CacheGenSerializer(Serializer):
         """The slots' tokens of a paged cache of all layers as a blob in this object's format."""
         from .. import paged
         k_pages, v_pages = paged.split_pages(pages, self.fmt)
-        L, _, _, H, D = k_pages.shape
+        L, P, S, H, D = k_pages.shape
         if slots.dim() != 1 or slots.shape[0] == 0:
             raise RuntimeError("slots must have one dimension and name a token at least")
+        # a token without a slot would be stored as whatever the blob's memory had (the encode waits for the GPU too)
+        first, last = torch.stack(torch.aminmax(slots)).tolist()
+        if first < 0 or last >= P * S:
+            raise RuntimeError(f"slots must be between 0 and {P * S - 1}, there are some from {first} to {last}")
         kv = torch.empty((L, 2, slots.shape[0], H, D), dtype=pages.dtype, device=pages.device)
         paged.gather_paged(k_pages, v_pages, slots, k=kv[:, 0], v=kv[:, 1], rotary=rotary, positions=positions)
         return kv.permute(0, 1, 3, 2, 4) if self.fmt == "huggingface" else kv
@@ -691,7 +695,8 @@ class CacheGenSerializer(Serializer):
                      positions: torch.Tensor = None) -> CacheGenGPUEncoderOutput:
         """`encode` of tokens of a paged cache of all layers, [L, 2, pages, page_size, H, D] ("vllm") or [L, 2, pages, H, page_size, D]
         ("huggingface"): those in `slots` (int32 or int64, each a slot of the cache), in that order.  With `rotary` (paged.Rotary) the keys
-        are turned back from `positions` first, so that the chunk can be used at other places."""
+        are turned back from `positions` first, so that the chunk can be used at other places.  A slot that the cache does not have, padding
+        (-1) too, is an error."""
         with _on_pages(pages):
             return self.encode(self._from_pages(pages, slots, rotary, positions))
 
