@@ -499,13 +499,50 @@ bool indices_of(PyObject *o, at::Device dev, bool wide_too, at::Tensor *t) {
     *t = THPVariable_Unpack(o);
     return usable(*t, at::kInt, dev) || (wide_too && usable(*t, at::kLong, dev));
 }
+// Whether two tensors of 16-bit values share none, as cachegen_b200.paged's _are_apart: by ranges, or along the axes that they step along together.
+struct Axis {
+    int64_t step, size;
+};
+struct Axes {
+    Axis axis[5];
+    int n = 0;
+    int64_t span(int from) const {
+        int64_t values = 1;
+        for (int k = from; k < n; ++k) values += (axis[k].size - 1) * axis[k].step;
+        return values;
+    }
+};
+bool no_value_shared(int64_t gap, const Axes &a, int ia, const Axes &b, int ib) {
+    if (gap >= 2 * a.span(ia) || -gap >= 2 * b.span(ib)) return true;
+    const int64_t step = std::max(ia < a.n ? a.axis[ia].step : 0, ib < b.n ? b.axis[ib].step : 0);
+    if (step == 0) return false;
+    const bool in_a = ia < a.n && a.axis[ia].step == step, in_b = ib < b.n && b.axis[ib].step == step;
+    const int64_t na = in_a ? a.axis[ia].size : 1, nb = in_b ? b.axis[ib].size : 1;
+    const int64_t reach_a = 2 * a.span(ia + in_a), reach_b = 2 * b.span(ib + in_b), bytes = 2 * step;
+    const auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+    const int64_t first = std::max(floor_div(gap - reach_a, bytes) + 1, 1 - nb), last = std::min(-floor_div(-gap - reach_b, bytes) - 1, na - 1);
+    if (last - first >= 4) return false;
+    for (int64_t k = first; k <= last; ++k)
+        if (!no_value_shared(gap - k * bytes, a, ia + in_a, b, ib + in_b)) return false;
+    return true;
+}
+Axes axes_of(const at::Tensor &t) {
+    Axes x;
+    for (int64_t k = 0; k < t.dim(); ++k)
+        if (t.size(k) > 1) x.axis[x.n++] = Axis{t.stride(k), t.size(k)};
+    std::sort(x.axis, x.axis + x.n, [](const Axis &p, const Axis &q) { return p.step > q.step; });
+    return x;
+}
 bool apart(const at::Tensor &a, const at::Tensor &b) {
-    const auto end = [](const at::Tensor &t) {
-        int64_t n = 1;
-        for (int64_t k = 0; k < t.dim(); ++k) n += (t.size(k) - 1) * t.stride(k);
-        return static_cast<const char *>(t.data_ptr()) + 2 * n;
+    if (!a.numel() || !b.numel()) return true;
+    const auto reach = [](const at::Tensor &t) {
+        const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
+        int64_t values = 1;
+        for (size_t k = 0; k < sizes.size(); ++k) values += (sizes[k] - 1) * strides[k];
+        return 2 * values;
     };
-    return !a.numel() || !b.numel() || end(a) <= static_cast<const char *>(b.data_ptr()) || end(b) <= static_cast<const char *>(a.data_ptr());
+    const int64_t gap = static_cast<const char *>(b.const_data_ptr()) - static_cast<const char *>(a.const_data_ptr());
+    return gap >= reach(a) || -gap >= reach(b) || no_value_shared(gap, axes_of(a), 0, axes_of(b), 0);
 }
 bool same_or_apart(const at::Tensor &a, const at::Tensor &b) { return (a.data_ptr() == b.data_ptr() && a.strides() == b.strides()) || apart(a, b); }
 void strides_of(const at::Tensor &t, int64_t *to, int64_t outer) {  // of all axes but the innermost; a layer axis that is not there: 0
@@ -578,7 +615,7 @@ bool pages_job(PyObject *const *a, const at::Tensor &k, const at::Tensor &v, boo
     const int64_t P = kp.size(d - 3), S = kp.size(d - 2);
     if (kp.sizes() != vp.sizes() || (d == 4 && kp.size(0) != layers) || kp.size(d - 1) != H || kp.size(d) != D || S == 0) return false;
     if (!indices_of(a[4], dev, true, &slots) || slots.dim() != 1 || slots.size(0) != T) return false;
-    if (append && T && kp.data_ptr() == vp.data_ptr()) return false;
+    if (T && (append ? !apart(kp, vp) : !apart(k, v))) return false;
     if (a[5] != Py_None && (!indices_of(a[5], dev, false, &status) || status.numel() != 1)) return false;
     if (!fits({layers, T, H, D, S}) || !turning(job, a + 6, dev, -1, T, D, held + 4)) return false;
     if (!apart(k, kp) || !apart(k, vp) || !apart(v, kp) || !apart(v, vp)) return false;
@@ -611,7 +648,10 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (queries) {
         if (k.dim() != 3 || !rows_of(a[11], k.scalar_type(), dev, 3, Use::kRead, &q) || q.size(0) != k.size(0) || q.size(2) != k.size(2)) Py_RETURN_NONE;
         if (a[12] == Py_None) q_out = like(q, q.sizes());
-        else if (!rows_of(a[12], k.scalar_type(), dev, 3, Use::kWritten, &q_out) || q_out.sizes() != q.sizes() || !same_or_apart(q, q_out)) Py_RETURN_NONE;
+        else if (!rows_of(a[12], k.scalar_type(), dev, 3, Use::kWritten, &q_out) || q_out.sizes() != q.sizes() || !same_or_apart(q, q_out) ||
+                 !apart(q_out, k) || !apart(q_out, v) || !apart(q_out, held[0]) || !apart(q_out, held[1]))
+            Py_RETURN_NONE;
+        if (!apart(q, held[0]) || !apart(q, held[1])) Py_RETURN_NONE;
         job.q = q.data_ptr(), job.q_out = q_out.data_ptr();
         strides_of(q, job.q_strides, 3);
         strides_of(q_out, job.q_out_strides, 3);

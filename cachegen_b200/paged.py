@@ -198,11 +198,32 @@ def _same_or_apart(a, b, names):
 
 
 def _are_apart(a, b):
-    """Whether the ranges of memory from the first to the last value do not overlap."""
+    """Whether two tensors of 16-bit values share none: the ranges of memory from the first to the last value do not overlap, or, as
+    with the parts of one array, the axes that they step along together (from the widest step on) keep their values apart."""
     if not a.numel() or not b.numel():
         return True
-    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + 2 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))) for t in (a, b))
-    return a1 <= b0 or b1 <= a0
+    axes = [sorted(((s, n) for s, n in zip(t.stride(), t.shape) if n > 1), reverse=True) for t in (a, b)]
+    return _no_value_shared(b.data_ptr() - a.data_ptr(), *axes)
+
+
+def _no_value_shared(gap, a, b):
+    """The same for what begins `gap` bytes apart and has these (stride, size) axes, the widest strides first."""
+    if gap >= 2 * _span(a) or -gap >= 2 * _span(b):
+        return True
+    step = max(axes[0][0] for axes in (a, b) if axes) if a or b else 0
+    if step == 0:
+        return False
+    (na, rest_a), (nb, rest_b) = ((x[0][1], x[1:]) if x and x[0][0] == step else (1, x) for x in (a, b))
+    step, reach_a, reach_b = 2 * step, 2 * _span(rest_a), 2 * _span(rest_b)
+    # step i of a and step i - k of b begin gap - k * step apart: those k at which their rests' ranges meet (many only in odd layouts)
+    first = max((gap - reach_a) // step + 1, 1 - nb)
+    last = min(-((-gap - reach_b) // step) - 1, na - 1)
+    return last - first < 4 and all(_no_value_shared(gap - k * step, rest_a, rest_b) for k in range(first, last + 1))
+
+
+def _span(axes):
+    """Values from the first to the last."""
+    return 1 + sum((n - 1) * s for s, n in axes)
 
 
 def apply_rotary(x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, out: torch.Tensor = None,
@@ -257,7 +278,10 @@ def _pages_job(k, v, k_pages, v_pages, slots, rotary, positions, written):
     P, S = k_pages.shape[-4:-2]
     _rows(k_pages, "k_pages", dev, dtype, rank + 1, lead + (P, S, H, D), written)
     _rows(v_pages, "v_pages", dev, dtype, rank + 1, lead + (P, S, H, D), written)
-    _check(not written or not T or k_pages.data_ptr() != v_pages.data_ptr(), "k_pages and v_pages must not be the same memory")
+    written_k, written_v, names = (k_pages, v_pages, "k_pages and v_pages") if written else (k, v, "k and v")
+    _check(not T or written_k.data_ptr() != written_v.data_ptr(), f"{names} must not be the same memory")
+    if T:
+        _check(_are_apart(written_k, written_v), f"{names} must not overlap")
     _indices(slots, "slots", dev, (T,))
     job = _lib.RowsJob()
     _turning(job, rotary, positions, dev, (T,), D)
@@ -277,7 +301,7 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                  q_out: torch.Tensor = None) -> Optional[torch.Tensor]:
     """Writes k and v [tokens, heads, head_size] to the slots (int32 or int64 [tokens]) of their tokens; with a leading axis of
     layers, to the same slots of every layer's pages.  With `rotary` the keys, and the queries q [tokens, q_heads, head_size] if
-    there are any, are turned to `positions` [tokens] on the way.  Returns the queries: q_out (which may be q) or a new
+    there are any, are turned to `positions` [tokens] on the way.  Returns the queries: q_out (which may be q, nothing else) or a new
     tensor.  A token with slot -1 is padding: nothing of it is written, its row of q_out neither.  Each slot belongs to one token:
     of two that name the same, either may be found there, or pieces of both."""
     done = _lib.calls().append(k, v, k_pages, v_pages, slots, _status_of(k), *_turns_for(rotary, k), positions, q, q_out)
@@ -299,6 +323,10 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         else:
             _rows(q_out, "q_out", k.device, k.dtype, 3, q.shape, written=True)
             _same_or_apart(q, q_out, "q and q_out")
+            for name, t in (("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages)):
+                _apart(q_out, t, "q_out", name)
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            _apart(q, t, "q", name)
         job.q, job.q_out, job.q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
         job.q_strides[:], job.q_out_strides[:] = _dense(q), _dense(q_out)
     _run("cg_append_paged", job, k.device)

@@ -135,3 +135,34 @@ def test_many_small_weights_beside_a_large_one(n, requests, dtype):
         # the sum of weights as above, and the logarithm's rounding, a step of 17 2^-19
         assert bool(((lse.double() - score - torch.log1p(small)).abs() <= small / 16 + 2.0 ** -18).all())
     paged.check_status()
+
+
+def test_rows_beside_each_other_are_taken_and_overlapping_ones_refused(monkeypatch):
+    """Queries, keys and values of one array, rotated in place, by the native call too; what a block would write while another reads it is
+    refused by both paths."""
+    from cachegen_b200 import _lib, paged
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    qkv = torch.randn((9, 8, 64), generator=g, device="cuda").half()
+    pages = torch.zeros((3, 4, 2, 2, 64), dtype=torch.float16, device="cuda")
+    rotary, slots, at = paged.Rotary(64), torch.arange(9, device="cuda"), torch.arange(5, 14, device="cuda")
+    k_pages, v_pages = pages[:, :, 0], pages[:, :, 1]
+    want = [paged.apply_rotary(qkv[:, :4], at, rotary), paged.apply_rotary(qkv[:, 4:6], at, rotary), qkv[:, 6:].clone()]
+    taken, entry = [], _lib.native_calls().append
+    monkeypatch.setattr(_lib.native_calls(), "append", lambda *a: taken.append(entry(*a)) or taken[-1])
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    assert paged.append_paged(k, v, k_pages, v_pages, slots, rotary=rotary, positions=at, q=q, q_out=q) is q and taken[0] is q
+    assert torch.equal(q, want[0]) and torch.equal(pages.view(12, 2, 2, 64)[:9, 0], want[1]) and torch.equal(pages.view(12, 2, 2, 64)[:9, 1], want[2])
+    kv = torch.zeros((9, 2, 2, 64), dtype=torch.float16, device="cuda")
+    paged.gather_paged(k_pages, v_pages, slots, k=kv[:, 0], v=kv[:, 1])
+    assert torch.equal(kv, pages.view(12, 2, 2, 64)[:9])
+    some = k.contiguous()
+    for refused in (dict(q=some, q_out=k), dict(q=some, q_out=v), dict(q=some, q_out=qkv[:, 5:7]), dict(q=some, q_out=pages[0, 0, 0][None].expand(9, -1, -1)),
+                    dict(q=k_pages.reshape(12, 2, 64)[:9], q_out=pages.view(24, 2, 64)[:9]), dict(q=pages.view(24, 2, 64)[1:10])):
+        with pytest.raises(RuntimeError):
+            paged.append_paged(k, v, k_pages, v_pages, slots, **refused)
+    with pytest.raises(RuntimeError):
+        paged.append_paged(k, v, pages.view(24, 1, 2, 64)[:12], pages.view(24, 1, 2, 64)[6:18], slots)
+    with pytest.raises(RuntimeError):
+        paged.gather_paged(k_pages, v_pages, slots, k=some, v=some)
+    paged.check_status()

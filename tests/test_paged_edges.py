@@ -1,0 +1,105 @@
+"""What the Python path of the calls on a paged cache checks, on tensors that only say that they are on a GPU: nothing is launched."""
+import random
+
+import pytest
+import torch
+
+from cachegen_b200 import paged
+
+
+class OnGpu(torch.Tensor):
+    is_cuda = True
+
+
+def on_gpu(t):
+    return t.as_subclass(OnGpu)
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """The names of the calls that would have been launched."""
+    names = []
+    monkeypatch.setattr(paged, "_run", lambda entry, job, device: names.append(entry))
+    monkeypatch.setattr(paged, "_status_of", lambda t: None)
+    return names
+
+
+def values(t):
+    """Where a tensor's values lie."""
+    at = torch.full((1,), t.data_ptr() // 2)
+    for n, s in zip(t.shape, t.stride()):
+        at = (at[:, None] + torch.arange(n) * s).flatten()
+    return set(at.tolist())
+
+
+def test_tensors_that_share_a_value_are_never_taken_for_apart():
+    rng = random.Random(7)
+    buffer = torch.zeros(4000, dtype=torch.float16)
+    known = 0
+    for _ in range(4000):
+        views = []
+        # parts of one array, by slices and steps of its axes, and any strides at all
+        shape = [rng.randint(1, 5) for _ in range(rng.randint(2, 5))]
+        array = buffer[:torch.Size(shape).numel()].view(shape).permute(rng.sample(range(len(shape)), len(shape)))
+        for _ in range(2):
+            if rng.random() < 0.8:
+                v = array
+                for d in range(v.dim()):
+                    first = rng.randrange(v.shape[d])
+                    v = v.narrow(d, first, rng.randint(1, v.shape[d] - first))
+                    v = v[(slice(None),) * d + (slice(None, None, rng.randint(1, 2)),)]
+            else:
+                dims = rng.randint(1, 4)
+                v = buffer.as_strided([rng.randint(1, 4) for _ in range(dims)], [rng.randint(0, 40) for _ in range(dims)], rng.randint(0, 200))
+            views.append(v)
+        a, b = views
+        apart, shared = paged._are_apart(a, b), bool(values(a) & values(b))
+        assert paged._are_apart(b, a) == apart
+        assert not (apart and shared)
+        known += apart and not shared
+    assert known > 1000
+
+
+def test_parts_of_one_array_are_apart():
+    qkv = torch.zeros((9, 12, 64), dtype=torch.float16)  # tokens of queries, keys and values side by side
+    q, k, v = qkv[:, :8], qkv[:, 8:10], qkv[:, 10:]
+    flat = torch.zeros((9, 12 * 64), dtype=torch.float16)
+    other = torch.zeros((3, 2, 5, 4, 2, 64), dtype=torch.float16)  # layers, keys and values
+    for a, b in ((q, k), (k, v), (q, v), (flat[:, :512], flat[:, 512:640]), (flat[:1, :512], flat[1:2, :512]), (other[:, 0], other[:, 1]),
+                 (other[:, 0].transpose(2, 3), other[:, 1].transpose(2, 3)), (other[1, 0], other[1, 1]), (other[:, :, 0], other[:, :, 3]),
+                 (other[..., :32], other[..., 32:]), (other[..., 0, :], other[..., 1, :]), (qkv[::2], qkv[1::2]), (q, torch.zeros_like(q)), (q[:0], q)):
+        assert paged._are_apart(a, b) and paged._are_apart(b, a)
+        assert not a.numel() or not paged._are_apart(a, a)
+    for a, b in ((q, qkv[:, 7:9]), (qkv[1:], qkv[:-1]), (other[:, 0], other[:, :, 0]), (flat[:, :513], flat[:, 512:])):
+        assert not paged._are_apart(a, b) and not paged._are_apart(b, a)
+
+
+def rows(*shape):
+    return on_gpu(torch.zeros(shape, dtype=torch.float16))
+
+
+def test_append_and_gather_refuse_what_they_would_read_and_write_at_once(launched):
+    """Blocks write some tokens' rows while others read theirs."""
+    k, v, q = rows(6, 2, 64), rows(6, 2, 64), rows(6, 2, 64)
+    both = rows(2, 3, 4, 2, 64)
+    k_pages, v_pages, slots = both[0], both[1], on_gpu(torch.arange(6))
+    for q_out in (k, v, k_pages.view(12, 2, 64)[:6], v_pages.view(12, 2, 64)[6:]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            paged.append_paged(k, v, k_pages, v_pages, slots, q=q, q_out=q_out)
+    with pytest.raises(RuntimeError, match="overlap"):
+        paged.append_paged(k, v, k_pages, v_pages, slots, q=k_pages.view(12, 2, 64)[:6])
+    with pytest.raises(RuntimeError, match="overlap"):
+        paged.append_paged(k, v, both.view(6, 4, 2, 64)[:5], both.view(6, 4, 2, 64)[1:], slots)
+    seven = rows(7, 2, 64)
+    for k_to, v_to in ((k, k), (seven[:6], seven[1:])):
+        with pytest.raises(RuntimeError, match="overlap|same memory"):
+            paged.gather_paged(k_pages, v_pages, slots, k=k_to, v=v_to)
+    assert not launched
+    # the parts of one array go, in place too
+    qkv = rows(6, 8, 64)
+    pages = rows(3, 4, 2, 2, 64)
+    q = qkv[:, :4]
+    assert paged.append_paged(qkv[:, 4:6], qkv[:, 6:], pages[:, :, 0], pages[:, :, 1], slots, q=q, q_out=q) is q
+    kv = rows(6, 2, 2, 64)
+    paged.gather_paged(pages[:, :, 0], pages[:, :, 1], slots, k=kv[:, 0], v=kv[:, 1])
+    assert launched == ["cg_append_paged", "cg_gather_paged"]
