@@ -125,7 +125,7 @@ def _rows(t, name, device, dtype, rank, shape, written=False):
     _check(t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} must have an innermost stride of 1")
     if written:
         _check(all(s or n <= 1 for s, n in zip(t.stride(), t.shape)), f"{name} is written to and must not be expanded")
-    elif t.requires_grad and torch.is_grad_enabled():
+    if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient, which calls on a paged cache do not compute")
 
 

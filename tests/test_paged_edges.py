@@ -103,3 +103,24 @@ def test_append_and_gather_refuse_what_they_would_read_and_write_at_once(launche
     kv = rows(6, 2, 2, 64)
     paged.gather_paged(pages[:, :, 0], pages[:, :, 1], slots, k=kv[:, 0], v=kv[:, 1])
     assert launched == ["cg_append_paged", "cg_gather_paged"]
+
+
+def test_tensors_that_require_a_gradient_are_not_written_to(launched):
+    k, v, q, out = rows(6, 2, 64), rows(6, 2, 64), rows(6, 2, 64), rows(6, 2, 64)
+    k_pages, v_pages, slots = rows(3, 4, 2, 64), rows(3, 4, 2, 64), on_gpu(torch.arange(6))
+    table, lens = on_gpu(torch.zeros((6, 1), dtype=torch.int32)), on_gpu(torch.ones(6, dtype=torch.int32))
+    calls = {"k_pages": lambda: paged.append_paged(k, v, k_pages, v_pages, slots), "v_pages": lambda: paged.append_paged(k, v, k_pages, v_pages, slots),
+             "q_out": lambda: paged.append_paged(k, v, k_pages, v_pages, slots, q=q, q_out=out),
+             "k": lambda: paged.gather_paged(k_pages, v_pages, slots, k=k, v=v), "v": lambda: paged.gather_paged(k_pages, v_pages, slots, k=k, v=v),
+             "out": lambda: paged.paged_attention(q, k_pages, v_pages, table, lens, out=out)}
+    names = {"k_pages": k_pages, "v_pages": v_pages, "q_out": out, "k": k, "v": v, "out": out}
+    for name, call in calls.items():
+        names[name].requires_grad_()
+        with pytest.raises(RuntimeError, match=f"{name} requires a gradient"):
+            call()
+        names[name].requires_grad_(False)
+    assert not launched
+    k_pages.requires_grad_()
+    with torch.no_grad():
+        calls["k_pages"]()
+    assert launched == ["cg_append_paged"]
