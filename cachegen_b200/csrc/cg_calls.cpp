@@ -576,6 +576,10 @@ bool fits(std::initializer_list<int64_t> sizes) {
         if (n > INT32_MAX) return false;
     return true;
 }
+// Tells torch that a tensor was written to: a backward pass that kept it for later must not use what is in it now.
+void wrote(const at::Tensor &t) {
+    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // (those have no versions)
+}
 template <class Job> int run(int (*entry)(const Job *, void *), const Job &job, at::Device dev) {
     void *stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
     const WithoutGil released;
@@ -602,6 +606,7 @@ PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n) {
     job.nlayers = static_cast<int32_t>(layers), job.ntokens = static_cast<int32_t>(T), job.heads = static_cast<int32_t>(H);
     job.head_size = static_cast<int32_t>(D), job.inverse = a[2] == Py_True;
     const int rc = run(rotary_rows, job, dev);
+    if (!rc) wrote(out);
     return rc ? PyLong_FromLong(rc) : a[1] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[1]);
     END_HANDLE_TH_ERRORS
 }
@@ -659,6 +664,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     }
     const int rc = run(append_rows, job, dev);
     if (rc) return PyLong_FromLong(rc);
+    for (const at::Tensor *t : {&held[0], &held[1], &q_out}) wrote(*t);
     return !queries ? Py_NewRef(Py_True) : a[12] == Py_None ? THPVariable_Wrap(q_out) : Py_NewRef(a[12]);
     END_HANDLE_TH_ERRORS
 }
@@ -682,6 +688,7 @@ PyObject *gather(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!pages_job(a, k, v, false, dev, &job, held)) Py_RETURN_NONE;
     const int rc = run(gather_rows, job, dev);
     if (rc) return PyLong_FromLong(rc);
+    wrote(k), wrote(v);
     return Py_BuildValue("(NN)", a[0] == Py_None ? THPVariable_Wrap(k) : Py_NewRef(a[0]), a[1] == Py_None ? THPVariable_Wrap(v) : Py_NewRef(a[1]));
     END_HANDLE_TH_ERRORS
 }
@@ -744,6 +751,7 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
     }
     const int rc = run(attention, job, dev);
     if (rc) return PyLong_FromLong(rc);
+    wrote(out);
     PyObject *const result = a[10] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(a[10]);
     return a[11] == Py_True ? Py_BuildValue("(NN)", result, THPVariable_Wrap(lse)) : result;
     END_HANDLE_TH_ERRORS

@@ -190,6 +190,13 @@ def _run(entry, job, device):
     _lib.check(rc, entry)
 
 
+def _wrote(*tensors):
+    """Tells torch that tensors were written to: a backward pass that kept one for later must not use what is in it now."""
+    for t in tensors:
+        if t is not None and not t.is_inference():  # (those have no versions)
+            torch.autograd.graph.increment_version(t)
+
+
 def _same_or_apart(a, b, names):
     """Whether a call may read a while it writes b."""
     if a.data_ptr() == b.data_ptr() and a.stride() == b.stride():
@@ -253,6 +260,7 @@ def apply_rotary(x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, out: 
     job.dtype, job.nlayers, job.ntokens, job.heads, job.head_size = _DTYPES[x.dtype], lead, T, H, D
     job.inverse = bool(inverse)
     _run("cg_rotary", job, dev)
+    _wrote(out)
     return out
 
 
@@ -330,6 +338,7 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         job.q, job.q_out, job.q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
         job.q_strides[:], job.q_out_strides[:] = _dense(q), _dense(q_out)
     _run("cg_append_paged", job, k.device)
+    _wrote(k_pages, v_pages, q_out)
     return q_out
 
 
@@ -355,6 +364,7 @@ def gather_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tens
         for other, pages in (("k_pages", k_pages), ("v_pages", v_pages)):
             _apart(t, pages, name, other)
     _run("cg_gather_paged", job, k.device)
+    _wrote(k, v)
     return k, v
 
 
@@ -434,6 +444,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)  # of the graph's own memory in a capture
             job.workspace, job.workspace_bytes = workspace.data_ptr(), need
         _lib.check(_lib.lib().cg_paged_attention(ctypes.byref(job), _stream(dev)), "paged_attention")
+    _wrote(out)
     return (out, lse) if return_lse else out
 
 

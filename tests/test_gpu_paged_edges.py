@@ -166,3 +166,33 @@ def test_rows_beside_each_other_are_taken_and_overlapping_ones_refused(monkeypat
     with pytest.raises(RuntimeError):
         paged.gather_paged(k_pages, v_pages, slots, k=some, v=some)
     paged.check_status()
+
+
+def test_what_is_written_to_has_a_new_version(monkeypatch):
+    """Of the native calls and of the Python path: a backward pass that kept such a tensor refuses it."""
+    from cachegen_b200 import _lib, _plain_calls, paged
+    rotary, at = paged.Rotary(64), torch.arange(6, device="cuda")
+    table, lens = torch.zeros((6, 1), dtype=torch.int32, device="cuda"), torch.ones(6, dtype=torch.int32, device="cuda")
+
+    def rows(*shape):
+        return torch.zeros(shape, dtype=torch.float16, device="cuda")
+    calls = (lambda x, o: paged.apply_rotary(x, at, rotary, out=x), lambda x, o: paged.append_paged(o, o, x.view(6, 1, 2, 64), rows(6, 1, 2, 64), at),
+             lambda x, o: paged.append_paged(o, o, rows(6, 1, 2, 64), x.view(6, 1, 2, 64), at), lambda x, o: paged.append_paged(
+                 o, o, rows(6, 1, 2, 64), rows(6, 1, 2, 64), at, q=o, q_out=x),
+             lambda x, o: paged.gather_paged(rows(6, 1, 2, 64), rows(6, 1, 2, 64), at, k=x), lambda x, o: paged.gather_paged(
+                 rows(6, 1, 2, 64), rows(6, 1, 2, 64), at, v=x),
+             lambda x, o: paged.paged_attention(o, rows(1, 16, 2, 64), rows(1, 16, 2, 64), table, lens, out=x))
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(_lib, "_calls", _plain_calls)
+        for call in calls:
+            x, weight = rows(6, 2, 64), rows(6, 2, 64).requires_grad_()
+            y = (weight * x).sum()
+            call(x, rows(6, 2, 64))
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+            with torch.inference_mode():
+                call(rows(6, 2, 64), rows(6, 2, 64))
+                of_inference = rows(6, 2, 64)
+            call(of_inference, rows(6, 2, 64))
+    paged.check_status()

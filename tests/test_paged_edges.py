@@ -124,3 +124,24 @@ def test_tensors_that_require_a_gradient_are_not_written_to(launched):
     with torch.no_grad():
         calls["k_pages"]()
     assert launched == ["cg_append_paged"]
+
+
+def test_what_is_written_to_has_a_new_version(launched):
+    """A backward pass that kept such a tensor refuses it then."""
+    k, v, q, x = rows(6, 2, 64), rows(6, 2, 64), rows(6, 2, 64), rows(6, 2, 64)
+    k_pages, v_pages, slots = rows(3, 4, 2, 64), rows(3, 4, 2, 64), on_gpu(torch.arange(6))
+    tensors = (k, v, q, k_pages, v_pages)
+    versions = [t._version for t in tensors]
+    paged.append_paged(k, v, k_pages, v_pages, slots, q=q, q_out=q)
+    assert [t._version - w for t, w in zip(tensors, versions)] == [0, 0, 1, 1, 1]
+    paged.gather_paged(k_pages, v_pages, slots, k=k, v=v)
+    assert [t._version - w for t, w in zip(tensors, versions)] == [1, 1, 1, 1, 1]
+    weight = torch.ones((6, 2, 64), dtype=torch.float16, requires_grad=True)
+    y = (weight * x).sum()
+    paged.append_paged(k, v, k_pages, v_pages, slots, q=q, q_out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        pages = [rows(3, 4, 2, 64) for _ in range(2)]
+        paged.append_paged(k, v, *pages, slots)
+    paged.append_paged(k, v, *pages, slots)
