@@ -551,11 +551,13 @@ void strides_of(const at::Tensor &t, int64_t *to, int64_t outer) {  // of all ax
 }
 at::Tensor like(const at::Tensor &t, at::IntArrayRef shape) { return make(shape, t.options()); }
 
-// (turns or None, rotary_dims, interleaved, head size, positions): with them or without them as the job needs it
+// (turns or None, the stream that they were made on, rotary_dims, interleaved, head size, positions): with them or without them as the job needs it
 bool turning(cg_rows_job *job, PyObject *const *a, at::Device dev, int64_t layers, int64_t tokens, int64_t head, at::Tensor *positions) {
-    if (a[0] == Py_None) return a[4] == Py_None;
-    int64_t rot, of;
-    if (!plain(a[0]) || !small_int(a[1], &rot) || !small_int(a[3], &of) || of != head || !indices_of(a[4], dev, true, positions)) return false;
+    if (a[0] == Py_None) return a[5] == Py_None;
+    int64_t made_on, rot, of;
+    if (!plain(a[0]) || !small_int(a[1], &made_on) || !small_int(a[2], &rot) || !small_int(a[4], &of) || of != head ||
+        !indices_of(a[5], dev, true, positions))
+        return false;
     const at::Tensor &turns = THPVariable_Unpack(a[0]);
     if (!usable(turns, at::kLong, dev) || turns.numel() != rot / 2) return false;
     if (positions->dim() == 2 && layers >= 0) {
@@ -568,7 +570,11 @@ bool turning(cg_rows_job *job, PyObject *const *a, at::Device dev, int64_t layer
     job->wide_positions = positions->scalar_type() == at::kLong;
     job->turns = static_cast<const uint64_t *>(turns.data_ptr());
     job->rotary_dims = static_cast<int32_t>(rot);
-    job->interleaved = a[2] == Py_True;
+    job->interleaved = a[3] == Py_True;
+    // a Rotary may be dropped while the kernel reads its turns on another stream than theirs (a graph's is kept by its user)
+    const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(dev.index());
+    if (reinterpret_cast<int64_t>(stream.stream()) != made_on && c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None)
+        c10::cuda::CUDACachingAllocator::recordStream(turns.storage().data_ptr(), stream);
     return true;
 }
 bool fits(std::initializer_list<int64_t> sizes) {
@@ -586,12 +592,12 @@ template <class Job> int run(int (*entry)(const Job *, void *), const Job &job, 
     return entry(&job, stream);
 }
 
-// rotary(x, out or None, inverse, turns, rotary_dims, interleaved, head size, positions) -> out, an error code, or None
+// rotary(x, out or None, inverse, turns, their stream, rotary_dims, interleaved, head size, positions) -> out, an error code, or None
 PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     at::Tensor x, out, positions;
     at::Device dev(at::kCPU);
-    if (n != 8 || !first_of(a[0], &x, &dev) || x.dim() < 3 || x.dim() > 4 || a[3] == Py_None) Py_RETURN_NONE;
+    if (n != 9 || !first_of(a[0], &x, &dev) || x.dim() < 3 || x.dim() > 4 || a[3] == Py_None) Py_RETURN_NONE;
     if (!rows_of(a[0], x.scalar_type(), dev, x.dim(), Use::kRead, &x)) Py_RETURN_NONE;
     const int64_t d = x.dim(), layers = d == 4 ? x.size(0) : 1, T = x.size(d - 3), H = x.size(d - 2), D = x.size(d - 1);
     cg_rows_job job{};
@@ -611,7 +617,8 @@ PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// What append and gather have in common: k, v, k_pages, v_pages, slots, status, turns, rotary_dims, interleaved, head size, positions
+// What append and gather have in common: k, v, k_pages, v_pages, slots, status, turns, their stream, rotary_dims, interleaved, head size,
+// positions
 bool pages_job(PyObject *const *a, const at::Tensor &k, const at::Tensor &v, bool append, at::Device dev, cg_rows_job *job, at::Tensor *held) {
     const int64_t d = k.dim(), layers = d == 4 ? k.size(0) : 1, T = k.size(d - 3), H = k.size(d - 2), D = k.size(d - 1);
     at::Tensor &kp = held[0], &vp = held[1], &slots = held[2], &status = held[3];
@@ -638,22 +645,22 @@ bool pages_job(PyObject *const *a, const at::Tensor &k, const at::Tensor &v, boo
     return true;
 }
 
-// append(k, v, k_pages, v_pages, slots, status, turns, rotary_dims, interleaved, head size, positions, q or None, q_out or None)
+// append(k, v, k_pages, v_pages, slots, status, turns, their stream, rotary_dims, interleaved, head size, positions, q or None, q_out or None)
 // -> q_out or True, an error code, or None
 PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     at::Tensor k, v, q, q_out, held[5];
     at::Device dev(at::kCPU);
     cg_rows_job job{};
-    if (n != 13 || !first_of(a[0], &k, &dev) || k.dim() < 3 || k.dim() > 4 || !rows_of(a[0], k.scalar_type(), dev, k.dim(), Use::kRead, &k) ||
+    if (n != 14 || !first_of(a[0], &k, &dev) || k.dim() < 3 || k.dim() > 4 || !rows_of(a[0], k.scalar_type(), dev, k.dim(), Use::kRead, &k) ||
         !rows_of(a[1], k.scalar_type(), dev, k.dim(), Use::kRead, &v) || v.sizes() != k.sizes() || !pages_job(a, k, v, true, dev, &job, held))
         Py_RETURN_NONE;
-    const bool queries = a[11] != Py_None;
-    if (!queries && a[12] != Py_None) Py_RETURN_NONE;
+    const bool queries = a[12] != Py_None;
+    if (!queries && a[13] != Py_None) Py_RETURN_NONE;
     if (queries) {
-        if (k.dim() != 3 || !rows_of(a[11], k.scalar_type(), dev, 3, Use::kRead, &q) || q.size(0) != k.size(0) || q.size(2) != k.size(2)) Py_RETURN_NONE;
-        if (a[12] == Py_None) q_out = like(q, q.sizes());
-        else if (!rows_of(a[12], k.scalar_type(), dev, 3, Use::kWritten, &q_out) || q_out.sizes() != q.sizes() || !same_or_apart(q, q_out) ||
+        if (k.dim() != 3 || !rows_of(a[12], k.scalar_type(), dev, 3, Use::kRead, &q) || q.size(0) != k.size(0) || q.size(2) != k.size(2)) Py_RETURN_NONE;
+        if (a[13] == Py_None) q_out = like(q, q.sizes());
+        else if (!rows_of(a[13], k.scalar_type(), dev, 3, Use::kWritten, &q_out) || q_out.sizes() != q.sizes() || !same_or_apart(q, q_out) ||
                  !apart(q_out, k) || !apart(q_out, v) || !apart(q_out, held[0]) || !apart(q_out, held[1]))
             Py_RETURN_NONE;
         if (!apart(q, held[0]) || !apart(q, held[1])) Py_RETURN_NONE;
@@ -665,17 +672,17 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int rc = run(append_rows, job, dev);
     if (rc) return PyLong_FromLong(rc);
     for (const at::Tensor *t : {&held[0], &held[1], &q_out}) wrote(*t);
-    return !queries ? Py_NewRef(Py_True) : a[12] == Py_None ? THPVariable_Wrap(q_out) : Py_NewRef(a[12]);
+    return !queries ? Py_NewRef(Py_True) : a[13] == Py_None ? THPVariable_Wrap(q_out) : Py_NewRef(a[13]);
     END_HANDLE_TH_ERRORS
 }
 
-// gather(k or None, v or None, k_pages, v_pages, slots, status, turns, rotary_dims, interleaved, head size, positions)
+// gather(k or None, v or None, k_pages, v_pages, slots, status, turns, their stream, rotary_dims, interleaved, head size, positions)
 // -> (k, v), an error code, or None
 PyObject *gather(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     at::Tensor k, v, pages, slots, held[5];
     at::Device dev(at::kCPU);
-    if (n != 11 || !first_of(a[2], &pages, &dev) || pages.dim() < 4 || pages.dim() > 5 || !indices_of(a[4], dev, true, &slots) || slots.dim() != 1) Py_RETURN_NONE;
+    if (n != 12 || !first_of(a[2], &pages, &dev) || pages.dim() < 4 || pages.dim() > 5 || !indices_of(a[4], dev, true, &slots) || slots.dim() != 1) Py_RETURN_NONE;
     std::vector<int64_t> shape(pages.sizes().begin(), pages.sizes().end());
     shape.erase(shape.end() - 4);
     shape[shape.size() - 3] = slots.size(0);

@@ -66,7 +66,7 @@ class Rotary:
         self.frequencies = tuple(w)
         turns = [_turns(f) for f in w]
         self._turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64)
-        self._on = {}
+        self._on, self._made_on = {}, {}  # by device: the turns, and the stream whose memory they have
         if torch.cuda.is_available():
             self.turns(torch.device("cuda", torch.cuda.current_device()))
 
@@ -78,8 +78,12 @@ class Rotary:
                 raise RuntimeError("a Rotary is used on its device once before a capture there")
             with torch.inference_mode(False):
                 t = self._turns.to(device)  # from pageable memory: there for every stream when the call returns
+            self._made_on[device] = _stream(device)
             self._on[device] = t
         return t
+
+    def __getstate__(self):  # copies make their own
+        return {**self.__dict__, "_on": {}, "_made_on": {}}
 
 
 def _turns(radians: float) -> int:
@@ -154,7 +158,10 @@ def _turning(job, rotary, positions, device, shape, D):
     else:
         _indices(positions, "positions", device, shape[-1:])
     job.positions, job.wide_positions = positions.data_ptr(), positions.dtype == torch.int64
-    job.turns = rotary.turns(device).data_ptr()
+    turns = rotary.turns(device)
+    if not torch.cuda.is_current_stream_capturing():
+        turns.record_stream(torch.cuda.current_stream(device))  # a Rotary may be dropped while the kernel reads them
+    job.turns = turns.data_ptr()
     job.rotary_dims, job.interleaved = rotary.rotary_dims, rotary.interleaved
 
 
@@ -173,8 +180,9 @@ def _address(t):
 def _turns_for(rotary, t):
     """What the native calls take of a Rotary, for tensors on t's GPU."""
     if rotary is None or not t.is_cuda:
-        return None, 0, False, 0
-    return rotary.turns(t.device), rotary.rotary_dims, rotary.interleaved, rotary.head_size
+        return None, 0, 0, False, 0
+    turns = rotary.turns(t.device)
+    return turns, rotary._made_on[t.device], rotary.rotary_dims, rotary.interleaved, rotary.head_size
 
 
 def _finish(done, what):

@@ -196,3 +196,42 @@ def test_what_is_written_to_has_a_new_version(monkeypatch):
                 of_inference = rows(6, 2, 64)
             call(of_inference, rows(6, 2, 64))
     paged.check_status()
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_rotary_may_be_dropped_while_another_stream_uses_it(native, monkeypatch):
+    """Its memory is not handed out again before that stream is done.  (Nothing is written to what is handed out.)"""
+    from cachegen_b200 import _lib, _plain_calls, paged
+    if not native:
+        monkeypatch.setattr(_lib, "_calls", _plain_calls)
+    x, at = torch.ones((4, 2, 128), dtype=torch.float16, device="cuda"), torch.arange(4, device="cuda")
+    pages = torch.zeros((2, 1, 16, 2, 128), dtype=torch.float16, device="cuda")
+    calls = (lambda r: paged.apply_rotary(x, at, r), lambda r: paged.append_paged(x, x, pages[0], pages[1], at, rotary=r, positions=at),
+             lambda r: paged.gather_paged(pages[0], pages[1], at, rotary=r, positions=at))
+    side = torch.cuda.Stream()
+    for call in calls:
+        call(paged.Rotary(128))
+        torch.cuda.synchronize()
+        rotary = paged.Rotary(128)
+        address = rotary.turns(x.device).data_ptr()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(400_000_000)
+            call(rotary)
+        del rotary
+        handed_out = [torch.empty(64, dtype=torch.int64, device="cuda") for _ in range(100)]
+        assert not side.query()  # it waits still
+        assert address not in [t.data_ptr() for t in handed_out]
+        torch.cuda.synchronize()
+    paged.check_status()
+
+
+def test_a_rotary_can_be_copied():
+    import copy
+    import pickle
+    from cachegen_b200 import paged
+    x, at = torch.randn((4, 2, 64), device="cuda").half(), torch.arange(4, device="cuda")
+    r = paged.Rotary(64, rotary_dims=32, scaling=("linear", 2.0))
+    want = paged.apply_rotary(x, at, r)
+    for other in (copy.copy(r), copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
+        assert other.frequencies == r.frequencies and torch.equal(paged.apply_rotary(x, at, other), want)
+        assert other.turns(x.device) is not r.turns(x.device)
