@@ -173,6 +173,13 @@ def _status_of(t):
     return _status_word(t.device)
 
 
+def _set(job, **counts):
+    """Fields of a job that are 32-bit counts.  (ctypes cuts a larger number off without a word.)"""
+    for name, n in counts.items():
+        _check(n < 2 ** 31, f"{name}: {n} is more than a call takes")
+        setattr(job, name, n)
+
+
 def _address(t):
     return None if t is None else t.data_ptr()
 
@@ -265,8 +272,8 @@ def apply_rotary(x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, out: 
     _check(rotary is not None, "apply_rotary needs a Rotary")
     job.k, job.k_out = x.data_ptr(), out.data_ptr()
     job.k_strides[:], job.k_out_strides[:] = _dense(x), _dense(out)
-    job.dtype, job.nlayers, job.ntokens, job.heads, job.head_size = _DTYPES[x.dtype], lead, T, H, D
-    job.inverse = bool(inverse)
+    job.dtype, job.inverse = _DTYPES[x.dtype], bool(inverse)
+    _set(job, nlayers=lead, ntokens=T, heads=H, head_size=D)
     _run("cg_rotary", job, dev)
     _wrote(out)
     return out
@@ -305,10 +312,8 @@ def _pages_job(k, v, k_pages, v_pages, slots, rotary, positions, written):
     job.k_strides[:], job.v_strides[:] = _dense(k), _dense(v)
     job.pages_k_strides[:], job.pages_v_strides[:] = _paged(k_pages), _paged(v_pages)
     job.slots, job.wide_slots, job.status = slots.data_ptr(), slots.dtype == torch.int64, _address(_status_of(k))
-    job.num_pages, job.page_size = P, max(S, 1)
-    if S == 0:
-        job.num_pages = 0
-    job.dtype, job.nlayers, job.ntokens, job.heads, job.head_size = _DTYPES[dtype], lead[0] if lead else 1, T, H, D
+    job.dtype, job.num_pages = _DTYPES[dtype], P if S else 0
+    _set(job, nlayers=lead[0] if lead else 1, ntokens=T, heads=H, head_size=D, page_size=max(S, 1))
     return job
 
 
@@ -343,7 +348,8 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                 _apart(q_out, t, "q_out", name)
         for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
             _apart(q, t, "q", name)
-        job.q, job.q_out, job.q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+        job.q, job.q_out = q.data_ptr(), q_out.data_ptr()
+        _set(job, q_heads=q.shape[1])
         job.q_strides[:], job.q_out_strides[:] = _dense(q), _dense(q_out)
     _run("cg_append_paged", job, k.device)
     _wrote(k_pages, v_pages, q_out)
@@ -442,9 +448,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     job.table_row, job.num_pages = page_table.stride(0), P
     job.q_strides[:], job.out_strides[:] = _steps(q), _steps(out)
     job.pages_k_strides[:], job.pages_v_strides[:] = _steps(k_pages), _steps(v_pages)
-    job.dtype, job.nrequests, job.nrows, job.q_heads, job.heads, job.head_size = _DTYPES[dtype], B, R, Q, H, D
-    job.page_size, job.table_width, job.causal, job.window, job.max_q = S, page_table.shape[1], causal, min(window, 2 ** 31 - 1), max_q
-    job.scale = scale
+    job.dtype, job.causal, job.window, job.max_q, job.scale = _DTYPES[dtype], causal, min(window, 2 ** 31 - 1), min(max_q, 2 ** 31 - 1), scale
+    _set(job, nrequests=B, nrows=R, q_heads=Q, heads=H, head_size=D, page_size=S, table_width=page_table.shape[1])
     with on_device(dev):
         need = _lib.lib().cg_paged_attention_workspace(ctypes.byref(job))
         _lib.check(min(need, 0), "paged_attention")

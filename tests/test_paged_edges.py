@@ -4,7 +4,7 @@ import random
 import pytest
 import torch
 
-from cachegen_b200 import paged
+from cachegen_b200 import _lib, paged
 
 
 class OnGpu(torch.Tensor):
@@ -145,3 +145,19 @@ def test_what_is_written_to_has_a_new_version(launched):
         pages = [rows(3, 4, 2, 64) for _ in range(2)]
         paged.append_paged(k, v, *pages, slots)
     paged.append_paged(k, v, *pages, slots)
+
+
+def test_counts_beyond_32_bits_are_refused(launched, monkeypatch):
+    """They would be cut off: 2^32 + 4 tokens would be 4."""
+    T = 2 ** 32 + 4
+    k, slots = rows(1, 2, 64), on_gpu(torch.zeros(1, dtype=torch.int64))
+    k_pages, v_pages = (rows(3, 1, 2, 64).expand(3, T, 2, 64) for _ in range(2))  # pages of as many tokens, all the same memory
+    lens, table = on_gpu(torch.ones(1, dtype=torch.int32)), on_gpu(torch.zeros((1, 1), dtype=torch.int32))
+    monkeypatch.setattr(paged, "_turning", lambda *_: None)
+    monkeypatch.setattr(paged, "_turns_for", lambda *_: (None, 0, 0, False, 0))
+    x, at = (on_gpu(torch.empty(shape, dtype=dtype, device="meta")) for shape, dtype in (((T, 2, 64), torch.float16), ((T,), torch.int32)))
+    for call in (lambda: paged.gather_paged(k_pages, v_pages, slots, k=k, v=rows(1, 2, 64)), lambda: paged.paged_attention(k, k_pages, v_pages, table, lens),
+                 lambda: paged.apply_rotary(x, at, object())):
+        with pytest.raises(RuntimeError, match="more than a call takes"):
+            call()
+    assert not launched
