@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kMoveThreads = 256;
 constexpr int kMostHead = 512;
+constexpr int kMostCount = INT32_MAX - 512;  // of tokens and of layers: a block counts on to the end of its share, up to 256 behind the last
 
 // One of the up to three arrays of rows: queries, keys, values.  A side with `paged` set is addressed by slots.
 struct MoveSide {
@@ -244,8 +245,8 @@ int move(const cg_rows_job *job, Direction way, cudaStream_t st) {
     if (!job) return CG_E_NULL;
     const cg_rows_job &j = *job;
     if (j.dtype != CG_F16 && j.dtype != CG_BF16) return CG_E_DTYPE;
-    if (j.nlayers < 0 || j.ntokens < 0 || j.heads < 0 || j.q_heads < 0 || j.head_size <= 0 || j.head_size > kMostHead ||
-        static_cast<int64_t>(j.heads) * 2 + j.q_heads > 65536)
+    if (j.nlayers < 0 || j.nlayers > kMostCount || j.ntokens < 0 || j.ntokens > kMostCount || j.heads < 0 || j.q_heads < 0 ||
+        j.head_size <= 0 || j.head_size > kMostHead || static_cast<int64_t>(j.heads) * 2 + j.q_heads > 65536)
         return CG_E_SHAPE;
     if (j.rotary_dims < 0 || j.rotary_dims > j.head_size || j.rotary_dims % 2) return CG_E_SHAPE;
     if (j.nlayers == 0 || j.ntokens == 0) return CG_OK;

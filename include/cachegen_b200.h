@@ -500,7 +500,7 @@ int cg_host_stage_end(void *handle_host);
  * cg_append_paged: keys rotated and values to the slots of their tokens; q (nlayers 1, q_heads 0: none) rotated to q_out.  What is written
  * shares no value with anything else of the call, but for q_out with q.
  * cg_gather_paged: the slots' values to v, and the keys turned back to k (inverse is implied); k and v share no value.
- * head_size <= 512, 2 * heads + q_heads <= 65,536.  ntokens or nlayers 0: nothing is done.
+ * head_size <= 512, 2 * heads + q_heads <= 65,536, ntokens and nlayers <= 2^31 - 513.  ntokens or nlayers 0: nothing is done.
  */
 typedef struct cg_rows_job {
     const void *q;

@@ -161,3 +161,12 @@ def test_counts_beyond_32_bits_are_refused(launched, monkeypatch):
         with pytest.raises(RuntimeError, match="more than a call takes"):
             call()
     assert not launched
+
+
+def test_jobs_of_nearly_two_to_the_31_tokens_or_layers_are_refused():
+    """A block counts on to the end of its share of the tokens, behind the last."""
+    from test_paged_refusals import rows_job
+    L = _lib.lib()
+    for entry in (L.cg_rotary, L.cg_append_paged, L.cg_gather_paged):
+        for given in ({"ntokens": 2 ** 31 - 1}, {"ntokens": 2 ** 31 - 512}, {"nlayers": 2 ** 31 - 1}):
+            assert entry(rows_job(**given), None) == -2, given
