@@ -129,6 +129,7 @@ def _rows(t, name, device, dtype, rank, shape, written=False):
     _check(t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} must have an innermost stride of 1")
     if written:
         _check(all(s or n <= 1 for s, n in zip(t.stride(), t.shape)), f"{name} is written to and must not be expanded")
+    _check(not t.is_neg(), f"{name} is a view that negates its memory")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient, which calls on a paged cache do not compute")
 
@@ -138,6 +139,7 @@ def _indices(t, name, device, shape):
     _check(t.dtype in _INDEX, f"{name} must be int32 or int64")
     _check(tuple(t.shape) == shape, f"{name} has shape {tuple(t.shape)}, expected {shape}")
     _check(t.is_contiguous(), f"{name} must be contiguous")
+    _check(not t.is_neg(), f"{name} is a view that negates its memory")
 
 
 def _head(t, name):
@@ -426,6 +428,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             continue
         _check(t.is_cuda and t.device == dev, f"{name} must be on {dev}")
         _check(t.dtype == torch.int32, f"{name} must be int32")
+        _check(not t.is_neg(), f"{name} is a view that negates its memory")
         _check(t.dim() == len(shape) and all(w in (None, n) for w, n in zip(shape, t.shape)), f"{name} has shape {tuple(t.shape)}, expected {shape}")
         _check(t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} must have an innermost stride of 1")
     _check(q_starts is not None or R == B, f"without q_starts each of {B} requests has one row, q has {R}")

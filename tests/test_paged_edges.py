@@ -170,3 +170,18 @@ def test_jobs_of_nearly_two_to_the_31_tokens_or_layers_are_refused():
     for entry in (L.cg_rotary, L.cg_append_paged, L.cg_gather_paged):
         for given in ({"ntokens": 2 ** 31 - 1}, {"ntokens": 2 ** 31 - 512}, {"nlayers": 2 ** 31 - 1}):
             assert entry(rows_job(**given), None) == -2, given
+
+
+def test_views_that_negate_are_refused(launched):
+    """The kernels read the memory as it is."""
+    k, v, q = rows(6, 2, 64), rows(6, 2, 64), rows(6, 2, 64)
+    pages, slots = (rows(3, 4, 2, 64), rows(3, 4, 2, 64)), on_gpu(torch.arange(6))
+    table, lens = on_gpu(torch.zeros((6, 1), dtype=torch.int32)), on_gpu(torch.ones(6, dtype=torch.int32))
+    neg = torch._neg_view
+    for call in (lambda: paged.append_paged(neg(k), v, *pages, slots), lambda: paged.append_paged(k, v, *pages, neg(slots)),
+                 lambda: paged.append_paged(k, v, *pages, slots, q=neg(q)), lambda: paged.gather_paged(neg(pages[0]), pages[1], slots, k=k, v=v),
+                 lambda: paged.gather_paged(*pages, slots, k=neg(k), v=v), lambda: paged.paged_attention(neg(q), *pages, table, lens),
+                 lambda: paged.paged_attention(q, *pages, neg(table), lens), lambda: paged.paged_attention(q, *pages, table, neg(lens))):
+        with pytest.raises(RuntimeError, match="negates"):
+            call()
+    assert not launched
