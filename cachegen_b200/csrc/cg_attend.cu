@@ -8,8 +8,8 @@
 // m16n8k16 on fragments in registers: tcgen05 takes 64 rows at least, its accumulator would have to come back from tensor memory for each
 // 16 keys, and at 16 rows the products take less than a fifth of the time that the keys take to arrive.
 //
-// A step of 64 requests of up to 4,096 tokens (32 / 8 heads, 753 MB): 147 us, 5.1 TB/s; the blocks read at 6.0 while they run.  One request of
-// 32,768 tokens (134 MB): 36 us, of which 6 pass before keys flow and 6 while 18 blocks' parts of each head are joined.
+// A step of 64 requests of up to 4,096 tokens (32 / 8 heads, 753 MB): 150 us, 5.0 TB/s; the blocks read at 6.0 while they run.  One request of
+// 32,768 tokens (134 MB): 37 us, of which 6 pass before keys flow and 6 while 37 blocks' parts of each head are joined.
 #include "cg_attend.cuh"
 
 namespace cg {

@@ -12,14 +12,15 @@
 // A tile of at most 128 rows is worked on by both halves all the same: they take its blocks of keys in turn, and the first adds the second's
 // sums to its own at the end (49 rows over up to 27,300 keys of 18 requests: 113 us, by one half 133).
 //
-// A row's maximum is only raised when a score is more than 2^8 times beyond it in weight: weights up to 2^8 lose nothing as 16-bit or
-// 32-bit floats, and O, which has to be multiplied in tensor memory for every raise, is then left alone in nearly every block.
+// A row's maximum is only raised when a score is more than 2^8 times beyond it in weight: weights up to 2^8 (in fp16 2^15, see kLift) lose nothing as
+// 16-bit or 32-bit floats, and O, which has to be multiplied in tensor memory for every raise, is then left alone in nearly every block.
+// (Two halves of queries in turn, scores and weights in tensor memory, and a maximum that lags behind are published methods for such tensor cores.)
 //
 // Keys and values come by TMA, a box of up to 32 tokens of one page at a time, where pages allow it (8, 16 or a multiple of 32 tokens) and
 // all 32 are seen; else by 16-byte asynchronous copies: pages may have any size, a block's last keys may lie in the middle of one, and
 // what lies behind them has to arrive as zeros (a weight of zero does not keep NaN out of a product).
 //
-// 8,192 tokens of 32 heads: 585 us, 940 TFLOP/s with the power cap (1,050 in a cold run); 256 tokens over 16,384 keys, 64 / 8 heads: 147 us.
+// 8,192 tokens of 32 heads: 597 us, 921 TFLOP/s with the power cap (1,050 in a cold run); 256 tokens over 16,384 keys, 64 / 8 heads: 149 us.
 // A block of 128 keys takes 3,050 cycles for 256 rows: a half's weights take 1,750 and its products 1,180, and the halves take turns; the
 // products alone would take 2,048.  Loops stay loops and one thread issues the products: the roles' code shares the instruction
 // caches, and unrolled it took twice the time.
