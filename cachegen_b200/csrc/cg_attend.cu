@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
                 const int64_t at = lane < 16 ? page * a.k_page + in_page * a.k_token : page * a.v_page + in_page * a.v_token;
                 const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
                 page = page_for(chunk + 1);
-                if (round && !(ok = warp_wait(empty + 8 * stage, phase ^ 1, failed, a.status))) break;
+                if (round && !(ok = warp_wait(empty + 8 * stage, phase ^ 1, failed))) break;
                 const uint32_t to = place + stage * kStageBytes<DP>;
 #pragma unroll
                 for (int i = 0; i < kChunk / kRowsAtOnce; ++i) {
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
         const uint32_t k_row = ((lane & 7) + ((lane >> 4) << 3)) * kRow + (((lane >> 3) & 1) << 4), v_row = (kChunk + (lane & 15)) * kRow + ((lane >> 4) << 4);
 #pragma unroll 1
         for (int chunk = 0; chunk < nchunks; ++chunk) {
-            ok = ok && warp_wait(full + 8 * stage, phase, failed, a.status);
+            ok = ok && warp_wait(full + 8 * stage, phase, failed);
             if (!ok) break;
             const uint32_t at = ring + stage * kStageBytes<DP>;
             float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
                 float x[DP / 32], top, total;
                 slow_row<DT, DP>(a, r, p.request, p.head, row0 + row, p.begin * kRowsBK, p.end * kRowsBK, failed, x, top, total);
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) sums[warp * kSumFloats + lane + 32 * i] = x[i];
+                for (int i = 0; i < DP / 32; ++i) sums[warp * kSumFloats + lane * (DP / 32) + i] = x[i];
                 __syncwarp();
                 if (4 * lane < DP) {
                     const float4 y = *reinterpret_cast<const float4 *>(sums + warp * kSumFloats + 4 * lane);
@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(kWarps * 64, 2) attend_rows_kernel(const __gri
         p = next;
     }
     if (tid == 0 && a.joins) a.joins[blockIdx.x] = join;
+    if (tid == 0 && *failed && a.status) atomicOr(a.status, CG_S_TIMEOUT);
 }
 
 constexpr int kJoinThreads = 1024;

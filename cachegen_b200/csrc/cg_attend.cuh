@@ -302,14 +302,24 @@ __device__ __forceinline__ uint64_t now_ns() {
 __device__ __forceinline__ uint32_t beat_of(uint64_t ns) { return static_cast<uint32_t>(ns >> 20); }
 __device__ __forceinline__ void beat(volatile int *failed) { failed[1] = static_cast<int>(beat_of(now_ns())); }
 
+// A lane's values of a row of a head, DP / 32 side by side.
+template <int DP> __device__ __forceinline__ void load_mine(const AttendArgs &a, uint64_t row, bool there, uint32_t (&x)[DP / 64]) {
+    const int col = (threadIdx.x & 31) * (DP / 32);
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c) x[c] = there && col < a.head_size ? __ldg(reinterpret_cast<const unsigned int *>(row) + col / 2 + c) : 0u;
+}
+template <int DT> __device__ __forceinline__ float half_of(uint32_t pair, int upper) { return Half16<DT>::to_float(static_cast<uint16_t>(pair >> (16 * upper))); }
+
 // One row over keys [k0, k1) by a warp, straight from memory: for rows that do not see a key of their tile whose values are not finite,
-// since a weight of zero does not keep those out of a product.  32 keys at a time: a lane has a key's score, then each lane its values of all
-// keys.  sums[i] is value lane + 32 i of the head.
+// since a weight of zero does not keep those out of a product.  Eight keys on their way at a time.  sums[i] is value lane * (DP / 32) + i of the
+// head.
 template <int DT, int DP>
 __device__ __forceinline__ void slow_row(const AttendArgs &a, const Lengths &r, int b, int head, int row, int k0, int k1, volatile int *failed,
                                       float (&sums)[DP / 32], float &top, float &total) {
+    constexpr int kKeys = 8;
     const int lane = threadIdx.x & 31, token = row / a.group;
-    const char *q = a.q + (r.first + token) * a.q_token + (head * a.group + member_of(a, row, token)) * a.q_head;
+    uint32_t x[DP / 64];
+    load_mine<DP>(a, reinterpret_cast<uint64_t>(a.q + (r.first + token) * a.q_token + (head * a.group + member_of(a, row, token)) * a.q_head), true, x);
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) sums[i] = 0.0f;
     top = kNegInf, total = 0.0f;
@@ -317,53 +327,55 @@ __device__ __forceinline__ void slow_row(const AttendArgs &a, const Lengths &r, 
 #pragma unroll 1
     for (int j0 = k0; j0 < k1; j0 += 32) {
         const int j = j0 + lane, page = j < k1 ? page_of(a, b, page_index(a, j)) : -1, in_page = place_in_page(a, j);
-        const char *k = a.k + page * a.k_page + in_page * a.k_token + head * a.k_head;
+        const uint64_t k = reinterpret_cast<uint64_t>(a.k + page * a.k_page + in_page * a.k_token + head * a.k_head);
         const uint64_t v = reinterpret_cast<uint64_t>(a.v + page * a.v_page + in_page * a.v_token + head * a.v_head);
-        float s = 0.0f;
-        if (page >= 0) {
-#pragma unroll 2
-            for (int d = 0; d < a.head_size; d += 8) {
-                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(q + 2 * d)), y = __ldg(reinterpret_cast<const uint4 *>(k + 2 * d));
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s += Half16<DT>::to_float(static_cast<uint16_t>(xs[i])) * Half16<DT>::to_float(static_cast<uint16_t>(ys[i])) +
-                         Half16<DT>::to_float(static_cast<uint16_t>(xs[i] >> 16)) * Half16<DT>::to_float(static_cast<uint16_t>(ys[i] >> 16));
-            }
-        }
-        s = j < k1 ? s * a.scale : kNegInf;
-        float now = fmaxf(top, s);
-        for (int d = 16; d; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
-        const float base = now == kNegInf ? 0.0f : now;
-        const float keep = exp2_approx(top - base), w = exp2_approx(s - base);
-        total = total * keep + w;
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) sums[i] *= keep;
         const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-#pragma unroll 4
-        for (int n = 0; n < 32; ++n) {
-            const uint64_t from = __shfl_sync(0xffffffffu, v, n);
-            const float weight = __shfl_sync(0xffffffffu, w, n);
+#pragma unroll 1
+        for (int n = 0; n < 32 && j0 + n < k1; n += kKeys) {
+            uint32_t y[kKeys][DP / 64], z[kKeys][DP / 64];
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i)
-                if ((there >> n & 1) && lane + 32 * i < a.head_size)
-                    sums[i] += weight * Half16<DT>::to_float(__ldg(reinterpret_cast<const uint16_t *>(from) + lane + 32 * i));
+            for (int i = 0; i < kKeys; ++i) {
+                load_mine<DP>(a, __shfl_sync(0xffffffffu, k, n + i), there >> (n + i) & 1, y[i]);
+                load_mine<DP>(a, __shfl_sync(0xffffffffu, v, n + i), there >> (n + i) & 1, z[i]);
+            }
+            float s[kKeys], now = top;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+                s[i] = 0.0f;
+                if (there >> (n + i) & 1) {
+#pragma unroll
+                    for (int c = 0; c < DP / 32; ++c) s[i] += half_of<DT>(x[c / 2], c & 1) * half_of<DT>(y[i][c / 2], c & 1);
+                }
+                for (int d = 16; d; d >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
+                s[i] = j0 + n + i < k1 ? s[i] * a.scale : kNegInf;
+                now = fmaxf(now, s[i]);
+            }
+            const float base = now == kNegInf ? 0.0f : now, keep = exp2_approx(top - base);
+            total *= keep;
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) sums[c] *= keep;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+                const float w = exp2_approx(s[i] - base);
+                total += w;
+#pragma unroll
+                for (int c = 0; c < DP / 32; ++c) sums[c] += (there >> (n + i) & 1) ? w * half_of<DT>(z[i][c / 2], c & 1) : 0.0f;
+            }
+            top = now;
         }
-        top = now;
         if (lane == 0) beat(failed);  // (others of the block wait for this row)
     }
-    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
 }
 
 // Which of a warp's `rows` (a bit a lane; a lane's row sees [lo, hi)) have to be done again, because a key that they do not see has values in
 // [k0, k1) or [k2, k3) that are not finite.  Where a row sees a value of the same column that is no number, its result is that in any
-// case: a cache full of them costs one look at the blocks that not all rows see.  (A call, so that the kernel's loops stay close together: 8,192
-// tokens of 32 heads 590 us, with this in line 600.)
+// case: a cache full of them costs one look at the blocks that not all rows see.  (A call: in line, 8,192
+// tokens of 32 heads took as long or 10 us longer, as the kernel's code came to lie.)
 template <int DT, int DP>
 __device__ __noinline__ uint32_t rows_again(const AttendArgs &a, int b, int head, uint32_t rows, int lo, int hi, int k0, int k1, int k2, int k3) {
     constexpr int kMine = DP / 32;  // columns of a lane
     constexpr uint32_t kExponent = DT == CG_F16 ? 0x7C00u : 0x7F80u, kAll = 0xffffffffu;
-    const int lane = threadIdx.x & 31, col = lane * kMine;
+    const int lane = threadIdx.x & 31;
     int bad0[kMine], bad1[kMine], nan0[kMine], nan1[kMine];  // the first and last keys
 #pragma unroll
     for (int c = 0; c < kMine; ++c) bad0[c] = nan0[c] = INT32_MAX, bad1[c] = nan1[c] = -1;
@@ -377,12 +389,8 @@ __device__ __noinline__ uint32_t rows_again(const AttendArgs &a, int b, int head
             const uint32_t there = __ballot_sync(kAll, page >= 0);
 #pragma unroll 8
             for (int n = 0; n < 32; ++n) {
-                const uint64_t from = __shfl_sync(kAll, v, n);
-                uint32_t x[kMine / 2] = {};
-                if ((there >> n & 1) && col < a.head_size) {
-#pragma unroll
-                    for (int c = 0; c < kMine / 2; ++c) x[c] = __ldg(reinterpret_cast<const unsigned int *>(from) + col / 2 + c);
-                }
+                uint32_t x[kMine / 2];
+                load_mine<DP>(a, __shfl_sync(kAll, v, n), there >> n & 1, x);
 #pragma unroll
                 for (int c = 0; c < kMine; ++c) {
                     const uint32_t u = x[c / 2] >> (16 * (c % 2)) & 0x7FFFu;
@@ -417,10 +425,10 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done;
 }
-// Whether the phase ended.  If it does not within kGiveUpNs, or another wait of the block gave up, the block is told to end.  Behind the word
-// that tells so stands the time (see beat) at which the block was last at work on something long, rows done again or a piece of many
-// keys: the wait goes on while that is recent.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
+// Whether the phase ended.  If it does not within kGiveUpNs, or another wait of the block gave up, the block is told to end, and says so in the
+// status.  Behind the word that tells stands the time (see beat) at which the block was last at work on something long, rows done again or a
+// piece of many keys: the wait goes on while that is recent.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed) {
     uint64_t start = 0;
 #pragma unroll 1
     for (uint32_t n = 1; !bar_try(bar, parity); ++n) {
@@ -429,21 +437,14 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
         const uint64_t now = now_ns();
         if (!start) start = now;
         if (now - start > kGiveUpNs) {
-            if (beat_of(now) - static_cast<uint32_t>(failed[1]) <= beat_of(kGiveUpNs)) {
-                start = now;
-                continue;
-            }
-            *failed = 1;
-            if (status) atomicOr(status, CG_S_TIMEOUT);
-            return false;
+            if (beat_of(now) - static_cast<uint32_t>(failed[1]) > beat_of(kGiveUpNs)) *failed = 1;
+            start = now;
         }
     }
     return true;
 }
 // the same for a whole warp, with one result
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed, int32_t *status) {
-    return __all_sync(0xffffffffu, bar_wait(bar, parity, failed, status));
-}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed) { return __all_sync(0xffffffffu, bar_wait(bar, parity, failed)); }
 __device__ __forceinline__ void bar_expect(uint32_t bar, int bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }

@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
     Parcel p;
     int pieces = 0;
     const auto next_piece = [&]() {
-        if (!warp_wait(bar(kPieceFull + (pieces & 1)), pieces >> 1 & 1, failed, a.status)) return false;
+        if (!warp_wait(bar(kPieceFull + (pieces & 1)), pieces >> 1 & 1, failed)) return false;
         const int4 *from = reinterpret_cast<const int4 *>(parcels + (pieces & 1));
         int4 *to = reinterpret_cast<int4 *>(&p);
         to[0] = from[0], to[1] = from[1], to[2] = from[2];
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             float m = kNegInf, l = 0.0f;
             for (int j = first; j < blocks; j += step) {
                 const int key = (p.begin + j) * kTileKeys;
-                ok = warp_wait(bar(kSFull + half), s_phase, failed, a.status);
+                ok = warp_wait(bar(kSFull + half), s_phase, failed);
                 s_phase ^= 1;
                 if (!ok) break;
                 fence_after();
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 l += (s0.x + s0.y) + (s1.x + s1.y);
             }
             m -= kLift<DT>;  // what the sums are relative to
-            ok = ok && warp_wait(bar(kOFull + half), o_phase, failed, a.status);
+            ok = ok && warp_wait(bar(kOFull + half), o_phase, failed);
             o_phase ^= 1;
             if (!ok) break;
             fence_after();
@@ -342,11 +342,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     fence_before();
                     __syncwarp();
                     if (lane == 0) bar_arrive(bar(kJoinReady));
-                    ok = warp_wait(bar(kJoinDone), join_phase, failed, a.status);
+                    ok = warp_wait(bar(kJoinDone), join_phase, failed);
                     join_phase ^= 1;
                     continue;
                 }
-                ok = warp_wait(bar(kJoinReady), join_phase, failed, a.status);
+                ok = warp_wait(bar(kJoinReady), join_phase, failed);
                 join_phase ^= 1;
                 if (!ok) break;
                 fence_after();
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 const bool any = last_key(a, r, tok) > first_key(a, r, tok);
 #pragma unroll
                 for (int c = 0; c < DP / 32; ++c) {
-                    const int d = lane + 32 * c;
+                    const int d = lane * (DP / 32) + c;
                     if (!p.whole) reinterpret_cast<float *>(part)[(d / 4 * kTileRows + i) * 4 + d % 4] = x[c];
                     else if (d < a.head_size)
                         reinterpret_cast<uint16_t *>(a.out + (r.first + tok) * a.out_token + hd * a.out_head)[d] = any ? Half16<DT>::from_float(x[c] / total) : 0;
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     const int at_page = kv && behind ? here_before : here, at_token = kv && behind ? in_page_before : in_page;
                     const bool boxes = maps.rows && __all_sync(0xffffffffu, at_page >= 0);
                     if (boxes) tell_all();
-                    if (!(ok = warp_wait(empty(stage), phase, failed, a.status))) break;
+                    if (!(ok = warp_wait(empty(stage), phase, failed))) break;
                     const uint32_t tile = tiles_at + stage * kTileBytes<DP>;
                     if (boxes) {
                         if (lane == 0) bar_expect(full(stage), box_bytes);
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                 if (!ok || j > 0) continue;
                 // the queries of all pieces but the first, behind the first block's tiles: once the last products with the ones before are done
                 if (!first_piece) {
-                    if (!(ok = warp_wait(bar(kQEmpty), q_phase, failed, a.status))) break;
+                    if (!(ok = warp_wait(bar(kQEmpty), q_phase, failed))) break;
                     q_phase ^= 1;
                     copy_queries();
                 }
@@ -586,13 +586,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             };
             const auto tile_there = [&]() {  // its stage, when it is there
                 const uint32_t at = stage;
-                ok = warp_wait(full(at), phase, failed, a.status);
+                ok = warp_wait(full(at), phase, failed);
                 if (++stage == kStages) stage = 0, phase ^= 1;
                 return at;
             };
             while (ok && next_piece()) {
                 const int blocks = p.end - p.begin, rows = min(kTileRows, p.n * a.group - p.t * kTileRows), halves = rows > 128 ? 2 : 1;
-                if (!(ok = warp_wait(bar(kQFull), q_phase, failed, a.status))) break;
+                if (!(ok = warp_wait(bar(kQFull), q_phase, failed))) break;
                 q_phase ^= 1;
                 uint32_t k_stage = tile_there(), v_stage = 0;
                 if (!ok) break;
@@ -618,8 +618,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                         const bool more = j + 2 < blocks;
                         if ((j & 1023) == 1023) beat(failed);  // (warp 13 waits for the length of a piece)
                         v_stage = tile_there();
-                        if (!ok || !(ok = warp_wait(bar(kPFull + 2 * half), p_phase >> half & 1, failed, a.status)) ||
-                            !(ok = warp_wait(bar(kPFull + 2 * half + 1), p_phase >> half & 1, failed, a.status)))
+                        if (!ok || !(ok = warp_wait(bar(kPFull + 2 * half), p_phase >> half & 1, failed)) ||
+                            !(ok = warp_wait(bar(kPFull + 2 * half + 1), p_phase >> half & 1, failed)))
                             break;
                         p_phase ^= 1 << half;
                         fence_after();
@@ -656,13 +656,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
                     const uint32_t v = v_desc + v_stage * kTile;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        if (!(ok = warp_wait(bar(kPFull + 2 * half), p_phase >> half & 1, failed, a.status))) break;
+                        if (!(ok = warp_wait(bar(kPFull + 2 * half), p_phase >> half & 1, failed))) break;
                         fence_after();
                         if (issues) {
 #pragma unroll
                             for (int k = 0; k < 6; ++k) mma_ts(o_at(half), s_at(half) + 8 * k, v + k * 128, kOperandHigh, pv, j > 0 || k > 0);
                         }
-                        if (!(ok = warp_wait(bar(kPFull + 2 * half + 1), p_phase >> half & 1, failed, a.status))) break;
+                        if (!(ok = warp_wait(bar(kPFull + 2 * half + 1), p_phase >> half & 1, failed))) break;
                         p_phase ^= 1 << half;
                         fence_after();
                         if (issues) {
@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             for (int i = 0; more; ++i) {
                 more = run.next(a, x);
                 if (more && x.sharers) join = join_for(x);
-                if (i >= 2 && !warp_wait(bar(kPieceEmpty + (i & 1)), (i / 2 - 1) & 1, failed, a.status)) break;
+                if (i >= 2 && !warp_wait(bar(kPieceEmpty + (i & 1)), (i / 2 - 1) & 1, failed)) break;
                 if (lane == 0) {
                     Parcel &to = parcels[i & 1];
                     to = more ? Parcel{x.r.first, x.r.n, x.r.kv, x.request, x.head, x.t, x.begin, x.end, x.tile.lo, x.tile.hi, x.starts, x.whole} : Parcel{};
@@ -703,8 +703,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
         __syncwarp();
     }
     // every product has been waited for (its O read), or the block has given up on one: what is on its way then takes microseconds
-    if (*failed)
+    if (*failed) {
+        if (lane == 0 && a.status) atomicOr(a.status, CG_S_TIMEOUT);
         for (const uint64_t start = now_ns(); now_ns() - start < 1000000;) {}
+    }
     fence_before();
     __syncthreads();
     fence_after();
