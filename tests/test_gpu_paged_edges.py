@@ -235,3 +235,23 @@ def test_a_rotary_can_be_copied():
     for other in (copy.copy(r), copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
         assert other.frequencies == r.frequencies and torch.equal(paged.apply_rotary(x, at, other), want)
         assert other.turns(x.device) is not r.turns(x.device)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("n", [1, 20])
+def test_the_longest_request(n, dtype):
+    """2^30 keys, of two pages that are named again and again, one with values of 1 and one of 3.  Scores are 0: sums of 1 and 3 are exact in 32 bits
+    up to 2^24, a block's share has fewer, and joined they are powers of two or three quarters of one."""
+    from cachegen_b200 import paged
+    kv, page = 2 ** 30, 128
+    k, v = torch.zeros((2, page, 1, 8), dtype=dtype, device="cuda"), torch.ones((2, page, 1, 8), dtype=dtype, device="cuda")
+    v[1] = 3
+    table = torch.zeros((1, kv // page), dtype=torch.int32, device="cuda")
+    table[0, 1::2] = 1
+    q = torch.ones((n, 1, 8), dtype=dtype, device="cuda")
+    lens, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([kv], [0, n]))
+    for window in (0, 2 ** 29, 2 ** 30):
+        out, lse = paged.paged_attention(q, k, v, table, lens, starts, return_lse=True, window=window, max_q=n)
+        paged.check_status()
+        assert bool(((out.double() - 2).abs() <= 2 * torch.finfo(dtype).eps / 2 + 2.0 ** -10).all())
+        assert bool(((lse.double() - math.log(window or kv)).abs() <= 2.0 ** -18).all())  # (n keys more or less are nothing beside 2^29)
