@@ -20,7 +20,7 @@
 // all 32 are seen; else by 16-byte asynchronous copies: pages may have any size, a block's last keys may lie in the middle of one, and
 // what lies behind them has to arrive as zeros (a weight of zero does not keep NaN out of a product).
 //
-// 8,192 tokens of 32 heads: 597 us, 921 TFLOP/s with the power cap (1,050 in a cold run); 256 tokens over 16,384 keys, 64 / 8 heads: 149 us.
+// 8,192 tokens of 32 heads: 589 us, 933 TFLOP/s with the power cap (1,050 in a cold run); 256 tokens over 16,384 keys, 64 / 8 heads: 149 us.
 // A block of 128 keys takes 3,050 cycles for 256 rows: a half's weights take 1,750 and its products 1,180, and the halves take turns; the
 // products alone would take 2,048.  Loops stay loops and one thread issues the products: the roles' code shares the instruction
 // caches, and unrolled it took twice the time.
