@@ -15,8 +15,10 @@ CG_MAX_DECODE_JOBS = 40
 CG_MAX_ENCODE_LEVELS = 4
 CG_MAX_OFFSET_GROUPS = 96000
 CG_S_STREAM_OVERFLOW, CG_S_BAD_LENGTHS, CG_S_BAD_SYMBOL, CG_S_COUNT_OVERFLOW, CG_S_BAD_TABLE = 1, 2, 4, 8, 16
-CG_S_BAD_PAGE, CG_S_TIMEOUT = 32, 64
+CG_S_BAD_PAGE, CG_S_TIMEOUT, CG_S_NO_PAGE = 32, 64, 128
 CG_MAX_REQUESTS = 4096
+CG_LOGITS_F32 = 2
+CG_MAX_BEAMS, CG_MAX_CHOICES, CG_MAX_BEAM_CHOICES, CG_MAX_VOCAB = 256, 128, 8192, 1 << 24
 CG_TABLES_CDF, CG_TABLES_COUNTS, CG_TABLES_SPARSE = 0, 1, 2
 CG_LENGTHS_I32, CG_LENGTHS_U16 = 0, 1
 CG_E_CUDA = -8
@@ -101,6 +103,31 @@ class AttentionJob(ctypes.Structure):
         (ctypes.c_float, "scale", None)])
 
 
+class PagesJob(ctypes.Structure):
+    """cg_pages_job"""
+    _fields_ = _fields([
+        (ctypes.c_void_p, "table kv_lens refs which new_table new_lens moves places q_starts slots workspace status", None),
+        (ctypes.c_int64, "workspace_bytes table_row new_table_row num_pages", None),
+        (ctypes.c_int32, "nrows width page_size nnew wide release ntokens reserved", None)])
+
+
+class CopyJob(ctypes.Structure):
+    """cg_copy_job"""
+    _fields_ = _fields([
+        (ctypes.c_void_p, "pages_k pages_v src dst tokens status", None),
+        (ctypes.c_int64, "pages_k_strides pages_v_strides", 4),
+        (ctypes.c_int64, "num_pages", None),
+        (ctypes.c_int32, "nlayers ncopies page_size heads head_size wide", None)])
+
+
+class BeamJob(ctypes.Structure):
+    """cg_beam_job"""
+    _fields_ = _fields([
+        (ctypes.c_void_p, "logits scores out_scores tokens parents workspace", None),
+        (ctypes.c_int64, "workspace_bytes row_stride", None),
+        (ctypes.c_int32, "dtype nrequests beams vocab k reserved", None)])
+
+
 EXPORTS = [
     "cg_host_upload", "cg_host_stage", "cg_host_stage_ahead", "cg_host_stage_send", "cg_host_stage_end", "cg_host_download", "cg_decode_kv",
     "cg_stream_sizes", "cg_decode_packed", "cg_wait_word",
@@ -112,6 +139,8 @@ EXPORTS = [
     "cg_decode_offsets", "cg_decode_dequant", "cg_decode_dequant_static",
     "cg_quantize_cdf_delta", "cg_decode_dequant_delta",
     "cg_rotary", "cg_append_paged", "cg_gather_paged", "cg_paged_attention_workspace", "cg_paged_attention",
+    "cg_pages_workspace", "cg_copy_pages", "cg_fork_pages", "cg_free_pages", "cg_extend_pages", "cg_compact_pages",
+    "cg_beam_workspace", "cg_beam_select",
 ]
 CG_STATIC_OFFSET_ENTRIES = 131072
 
@@ -176,11 +205,19 @@ def lib():
         getattr(L, name).argtypes = [rows, p]
     L.cg_paged_attention_workspace.argtypes = [attention]
     L.cg_paged_attention.argtypes = [attention, p]
+    pages, copy, beams = ctypes.POINTER(PagesJob), ctypes.POINTER(CopyJob), ctypes.POINTER(BeamJob)
+    L.cg_pages_workspace.argtypes = [i64]
+    L.cg_copy_pages.argtypes = [copy, p]
+    L.cg_fork_pages.argtypes = L.cg_compact_pages.argtypes = [pages, copy, p]
+    L.cg_free_pages.argtypes = L.cg_extend_pages.argtypes = [pages, p]
+    L.cg_beam_workspace.argtypes = [beams]
+    L.cg_beam_select.argtypes = [beams, p]
     for name in EXPORTS:
         fn = getattr(L, name)
         if name not in ("cg_version", "cg_status_string", "cg_last_cuda_error"):
             fn.restype = i
-    L.cg_encode_kv_workspace.restype = L.cg_paged_attention_workspace.restype = i64
+    for name in ("cg_encode_kv_workspace", "cg_paged_attention_workspace", "cg_pages_workspace", "cg_beam_workspace"):
+        getattr(L, name).restype = i64
     _lib = L
     return L
 
@@ -259,4 +296,6 @@ def status_text(bits):
         names.append("a slot, page or length does not fit the paged cache")
     if bits & CG_S_TIMEOUT:
         names.append("a kernel gave up waiting; its output is not valid")
+    if bits & CG_S_NO_PAGE:
+        names.append("the paged cache had no free page left for a row")
     return "; ".join(names) if names else "ok"

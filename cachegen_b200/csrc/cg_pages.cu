@@ -1,0 +1,657 @@
+// Pages of a paged KV cache that several rows of a table may hold: forked, extended, given back, moved together and copied.
+//
+// refs[p] counts the rows that hold page p; 0: free.  All of it stays on the GPU: the calls read lengths, counts and tables there and
+// write them there, so that a step of a search needs no answer on the host and can be captured.  What is taken is always the free page of
+// the lowest number, for rows in their order, so results do not depend on the order in which blocks run: counts change by atomic
+// additions, whose sum has no order, and everything else is decided from prefix sums.
+//
+// Work on tables is bound by latency: some hundred kilobytes, and a chain of a few dependent reads.  Prefix sums over all pages and rows
+// are made by one cluster, whose blocks tell one another their totals through distributed shared memory: one launch, and no second
+// pass over a grid.  Copies are bound by memory: 16 bytes a thread, four in flight.
+#include "cg_common.cuh"
+
+namespace cg {
+namespace {
+
+constexpr int kClusterBlocks = 8, kClusterThreads = 512, kClusterWarps = kClusterThreads / 32;
+constexpr int kRowThreads = 256, kRowColumns = 1024;  // of a block that works on a row of a table
+constexpr int kCopyThreads = 256, kCopyVectors = 4;
+constexpr int64_t kMostPages = INT32_MAX - 8;  // a thread counts on by four
+
+struct Table {
+    const int32_t *entries, *lens;
+    int64_t row;  // entries from one row to the next
+    int32_t rows, width, page_size;
+    int32_t num_pages;
+    int32_t *status;
+};
+
+__device__ __forceinline__ void note(int32_t *status, int32_t what) {
+    if (status) atomicOr(status, what);
+}
+__device__ __forceinline__ int64_t index_at(const void *p, int64_t i, int wide) {
+    return wide ? __ldg(static_cast<const long long *>(p) + i) : __ldg(static_cast<const int *>(p) + i);
+}
+// Tokens of a row; a length that its table cannot hold is cut.
+__device__ __forceinline__ int32_t length_of(const Table &t, int row) {
+    const int64_t n = t.lens[row], most = static_cast<int64_t>(t.width) * t.page_size;
+    if (n >= 0 && n <= most) return static_cast<int32_t>(n);
+    note(t.status, CG_S_BAD_PAGE);
+    return n < 0 ? 0 : static_cast<int32_t>(most);
+}
+__device__ __forceinline__ int32_t pages_of(int64_t tokens, int32_t page_size) { return static_cast<int32_t>((tokens + page_size - 1) / page_size); }
+// A page that a row holds, or -1 for one that the cache does not have.
+__device__ __forceinline__ int32_t page_at(const Table &t, int row, int column) {
+    const int32_t p = t.entries[row * t.row + column];
+    if (p >= 0 && p < t.num_pages) return p;
+    note(t.status, CG_S_BAD_PAGE);
+    return -1;
+}
+
+// ---- sums over a cluster ----------------------------------------------------------------------------
+__device__ __forceinline__ int cluster_rank() {
+    int r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// Everything that the cluster's threads wrote, to whatever memory, is there for all of them afterwards.
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int64_t of_block(const int64_t *mine, int rank) {
+    uint32_t at;
+    int64_t v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+    return v;
+}
+// Sum over the threads of the block in front of this one; total: over all of them.  sums: room of the block's own for kClusterWarps + 1.
+template <class T> __device__ __forceinline__ T sum_before(T x, T *sums, T *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T upto = x;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const T y = __shfl_up_sync(~0u, upto, d);
+        if (lane >= d) upto += y;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    if (warp == 0) {
+        const T own = lane < kClusterWarps ? sums[lane] : 0;
+        T s = own;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const T y = __shfl_up_sync(~0u, s, d);
+            if (lane >= d) s += y;
+        }
+        if (lane < kClusterWarps) sums[lane] = s - own;
+        if (lane == kClusterWarps - 1) sums[kClusterWarps] = s;
+    }
+    __syncthreads();
+    *total = sums[kClusterWarps];
+    return sums[warp] + upto - x;
+}
+
+// A thread's run of pages, [first, last): runs of neighbouring threads and blocks follow one another.
+struct Run {
+    int32_t first, last;
+};
+__device__ __forceinline__ Run run_of(int32_t num_pages) {
+    const int64_t each = (static_cast<int64_t>(num_pages) + kClusterBlocks * kClusterThreads - 1) / (kClusterBlocks * kClusterThreads);
+    const int64_t run = (each + 3) / 4 * 4, first = (static_cast<int64_t>(cluster_rank()) * kClusterThreads + threadIdx.x) * run;
+    return Run{static_cast<int32_t>(first < num_pages ? first : num_pages), static_cast<int32_t>(first + run < num_pages ? first + run : num_pages)};
+}
+// f(page, its count) for every page of a run, in order
+template <class F>
+__device__ __forceinline__ void each_page(const int32_t *refs, const Run &run, bool vectors, F f) {
+    int32_t p = run.first;
+    if (vectors)
+        for (; p <= run.last - 4; p += 4) {
+            const int4 c = *reinterpret_cast<const int4 *>(refs + p);
+            f(p, c.x), f(p + 1, c.y), f(p + 2, c.z), f(p + 3, c.w);
+        }
+    for (; p < run.last; ++p) f(p, refs[p]);
+}
+
+// Room of a block for the sums above, and for what it tells the others.
+struct Sums {
+    int32_t pages[kClusterWarps + 1];
+    int64_t rows[kClusterWarps + 1], told[2];
+};
+
+// Writes the numbers of the first free pages to `list`, in order, as many as the cluster's threads want together (`wanted` is this
+// thread's), if there are so many.  Returns the sum of what the threads before this one want; free_pages: how many there are.
+// A barrier of the cluster stands between its reads of the counts and its end.
+__device__ __forceinline__ int64_t take_free(const int32_t *refs, int32_t num_pages, int64_t wanted, int32_t *list, Sums *s, int64_t *wanted_all,
+                                             int64_t *free_pages) {
+    const Run run = run_of(num_pages);
+    const bool vectors = reinterpret_cast<uintptr_t>(refs) % 16 == 0;
+    int32_t free = 0, block_free;
+    int64_t block_wanted;
+    each_page(refs, run, vectors, [&](int32_t, int32_t c) { free += c == 0; });
+    int64_t rank = sum_before(free, s->pages, &block_free), before = sum_before(wanted, s->rows, &block_wanted);
+    if (threadIdx.x == 0) s->told[0] = block_free, s->told[1] = block_wanted;
+    cluster_barrier();
+    *wanted_all = *free_pages = 0;
+    const int me = cluster_rank();
+    for (int r = 0; r < kClusterBlocks; ++r) {
+        const int64_t f = of_block(s->told, r), w = of_block(s->told + 1, r);
+        if (r < me) rank += f, before += w;
+        *free_pages += f, *wanted_all += w;
+    }
+    const int64_t most = *wanted_all;
+    if (free && rank < most)
+        each_page(refs, run, vectors, [&](int32_t p, int32_t c) {
+            if (c == 0 && rank < most) list[rank] = p;
+            rank += c == 0;
+        });
+    cluster_barrier();
+    return before;
+}
+
+// ---- fork ----------------------------------------------------------------------------------------------
+struct Writers {  // of a page that new rows would go on writing to
+    int32_t first, count;
+};
+struct ForkArgs {
+    Table old;
+    int32_t *table, *lens, *refs, *moves;  // of the new rows; moves [3][nnew]
+    const void *parents;
+    Writers *writers;  // [num_pages], of the pages that matter
+    int32_t *list;     // [nnew]
+    int32_t *copies;   // how many
+    int64_t row;
+    int32_t nnew, wide, release;
+};
+
+// A block per row and 1,024 columns: the new row's entries, and the counts' changes.  Where a new row holds what the old one of its
+// place held, as rows of one request do in the context that they share, nothing changes and no atomic is issued.
+__global__ void __launch_bounds__(kRowThreads) fork_tables_kernel(const __grid_constant__ ForkArgs a) {
+    let_next_launch_start();
+    const int parts = (a.old.width + kRowColumns - 1) / kRowColumns > 0 ? (a.old.width + kRowColumns - 1) / kRowColumns : 1;
+    const int row = blockIdx.x / parts, column0 = (blockIdx.x - row * parts) * kRowColumns;
+    int64_t parent = -1;
+    if (row < a.nnew) {
+        parent = index_at(a.parents, row, a.wide);
+        if (parent < -1 || parent >= a.old.rows) {
+            if (threadIdx.x == 0) note(a.old.status, CG_S_BAD_PAGE);
+            parent = -1;
+        }
+    }
+    const int32_t tokens = parent >= 0 ? length_of(a.old, static_cast<int>(parent)) : 0, need = pages_of(tokens, a.old.page_size);
+    const int32_t had = a.release && row < a.old.rows ? pages_of(length_of(a.old, row), a.old.page_size) : 0;
+    if (row < a.nnew && column0 == 0 && threadIdx.x == 0) a.lens[row] = tokens;
+    const int32_t last = tokens % a.old.page_size ? need - 1 : -1;  // the column of a page that is not full
+    for (int j = column0 + threadIdx.x; j < column0 + kRowColumns && j < a.old.width; j += kRowThreads) {
+        const int32_t now = j < need ? page_at(a.old, static_cast<int>(parent), j) : -1, before = j < had ? page_at(a.old, row, j) : -1;
+        if (row < a.nnew) a.table[row * a.row + j] = now;
+        if (now != before) {
+            if (now >= 0) atomicAdd(a.refs + now, 1);
+            if (before >= 0) atomicAdd(a.refs + before, -1);
+        }
+        if (j == last && now >= 0) a.writers[now] = Writers{INT32_MAX, 0};  // the same from every row that does it
+    }
+}
+
+// One cluster, a row a thread.  A page that is not full may be written to by one row only: the first of the new rows that hold it
+// keeps it, if no other row does (it is counted more often than by these), and each of the rest gets a copy.
+__global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kClusterThreads) fork_writers_kernel(const __grid_constant__ ForkArgs a) {
+    __shared__ Sums sums;
+    wait_for_launch_before();
+    const int32_t each = (a.nnew + kClusterBlocks - 1) / kClusterBlocks, row = cluster_rank() * each + threadIdx.x;
+    const bool here = threadIdx.x < each && row < a.nnew;
+    int32_t tokens = 0, page = -1, part = 0, column = 0;
+    if (here) {
+        tokens = a.lens[row];
+        part = tokens % a.old.page_size;
+        column = tokens / a.old.page_size;
+        if (part) page = a.table[row * a.row + column];
+        if (page >= 0) {
+            atomicMin(&a.writers[page].first, row);
+            atomicAdd(&a.writers[page].count, 1);
+        }
+    }
+    cluster_barrier();
+    bool copied = false;
+    if (page >= 0) copied = __ldcg(&a.writers[page].first) != row || __ldcg(&a.writers[page].count) != __ldcg(a.refs + page);
+    int64_t all, free;
+    const int64_t rank = take_free(a.refs, a.old.num_pages, copied, a.list, &sums, &all, &free);
+    if (copied) {
+        const bool found = rank < free;
+        const int32_t to = found ? __ldcg(a.list + rank) : -1;
+        atomicAdd(a.refs + page, -1);
+        a.table[row * a.row + column] = to;
+        if (found) {
+            a.refs[to] = 1;
+            a.moves[rank] = page;
+            a.moves[a.nnew + rank] = to;
+            a.moves[2 * a.nnew + rank] = part;
+        } else {  // the tokens of that page are lost
+            a.lens[row] = tokens - part;
+            note(a.old.status, CG_S_NO_PAGE);
+        }
+    }
+    const int32_t made = static_cast<int32_t>(all < free ? all : free);
+    for (int32_t r = made + cluster_rank() * kClusterThreads + threadIdx.x; r < a.nnew; r += kClusterBlocks * kClusterThreads)
+        a.moves[r] = a.moves[a.nnew + r] = a.moves[2 * a.nnew + r] = -1;
+    if (cluster_rank() == 0 && threadIdx.x == 0) *a.copies = made;
+}
+
+// ---- give back -----------------------------------------------------------------------------------------
+struct FreeArgs {
+    Table t;
+    int32_t *table, *lens, *refs;
+    const void *rows;  // or nullptr: all
+    int32_t nfree, wide;
+};
+// A block per row.  A row that is named twice is given back once: its length is taken by the first.
+__global__ void __launch_bounds__(kRowThreads) free_pages_kernel(const __grid_constant__ FreeArgs a) {
+    __shared__ int32_t taken;
+    const int64_t row = a.rows ? index_at(a.rows, blockIdx.x, a.wide) : blockIdx.x;
+    if (row < 0 || row >= a.t.rows) {
+        if (row != -1 && threadIdx.x == 0) note(a.t.status, CG_S_BAD_PAGE);
+        return;
+    }
+    if (threadIdx.x == 0) taken = atomicExch(a.lens + row, 0);
+    __syncthreads();
+    int64_t need = pages_of(taken < 0 ? 0 : taken, a.t.page_size);
+    if (taken < 0 || need > a.t.width) {
+        if (threadIdx.x == 0) note(a.t.status, CG_S_BAD_PAGE);
+        if (need > a.t.width) need = a.t.width;
+    }
+    for (int64_t j = threadIdx.x; j < need; j += kRowThreads) {
+        const int32_t p = page_at(a.t, static_cast<int>(row), static_cast<int>(j));
+        a.table[row * a.t.row + j] = -1;
+        if (p >= 0 && atomicAdd(a.refs + p, -1) <= 0) {  // nobody held it
+            atomicAdd(a.refs + p, 1);
+            note(a.t.status, CG_S_BAD_PAGE);
+        }
+    }
+}
+
+// ---- extend --------------------------------------------------------------------------------------------
+struct ExtendArgs {
+    Table t;
+    int32_t *table, *lens, *refs, *list;
+    const int32_t *starts;  // [rows + 1], or nullptr: a token a row
+    int64_t *slots;
+    int32_t ntokens;
+};
+struct Growth {  // of a row: its tokens and pages before, its new tokens (-1: they found no place) and where its pages stand in the list
+    int32_t tokens, fresh, start, asked;
+    int64_t rank;
+};
+__device__ __forceinline__ int32_t start_of(const ExtendArgs &a, int row) {
+    if (!a.starts) return row;
+    const int32_t s = a.starts[row];
+    if (s >= 0 && s <= a.ntokens) return s;
+    note(a.t.status, CG_S_BAD_PAGE);
+    return s < 0 ? 0 : a.ntokens;
+}
+// One cluster, a row a thread for the sums; then the threads of a block share its rows.
+__global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kClusterThreads) extend_pages_kernel(const __grid_constant__ ExtendArgs a) {
+    __shared__ Sums sums;
+    __shared__ Growth grown[CG_MAX_REQUESTS / kClusterBlocks];
+    wait_for_launch_before();
+    const int32_t S = a.t.page_size, each = (a.t.rows + kClusterBlocks - 1) / kClusterBlocks, row0 = cluster_rank() * each;
+    const int32_t row = row0 + threadIdx.x;
+    const bool here = threadIdx.x < each && row < a.t.rows;
+    Growth g{0, 0, 0, 0, 0};
+    int64_t wanted = 0;
+    if (here) {
+        g.start = start_of(a, row);
+        g.asked = start_of(a, row + 1) - g.start;
+        if (g.asked < 0) {
+            note(a.t.status, CG_S_BAD_PAGE);
+            g.asked = 0;
+        }
+        g.tokens = length_of(a.t, row);
+        g.fresh = g.asked;
+        const int64_t after = static_cast<int64_t>(g.tokens) + g.asked;
+        const int64_t pages = (after + S - 1) / S;
+        if (pages > a.t.width || after > INT32_MAX) {
+            note(a.t.status, CG_S_BAD_PAGE);
+            g.fresh = -1;
+        } else {
+            wanted = pages - pages_of(g.tokens, S);
+        }
+    }
+    int64_t all, free;
+    g.rank = take_free(a.refs, a.t.num_pages, wanted, a.list, &sums, &all, &free);
+    if (here) {
+        if (wanted > 0 && g.rank + wanted > free) {
+            note(a.t.status, CG_S_NO_PAGE);
+            g.fresh = -1;
+        }
+        if (g.fresh > 0) a.lens[row] = g.tokens + g.fresh;
+        grown[threadIdx.x] = g;
+    }
+    __syncthreads();
+    const int32_t mine = a.t.rows - row0 < each ? a.t.rows - row0 : each;  // rows of this block, none or less behind the last
+    int team = kClusterThreads;
+    while (team > 32 && team * mine > kClusterThreads) team /= 2;
+    for (int32_t r = threadIdx.x / team; r < mine; r += kClusterThreads / team) {
+        const Growth &x = grown[r];
+        const int32_t lane = threadIdx.x % team, before = pages_of(x.tokens, S);
+        int32_t *const entries = a.table + (row0 + r) * a.t.row;
+        if (x.fresh > 0) {
+            const int32_t pages = pages_of(static_cast<int64_t>(x.tokens) + x.fresh, S) - before;
+            for (int32_t j = lane; j < pages; j += team) {
+                const int32_t p = __ldcg(a.list + x.rank + j);
+                entries[before + j] = p;
+                a.refs[p] = 1;
+            }
+        }
+        for (int32_t i = lane; i < x.asked; i += team) {
+            int64_t slot = -1;
+            if (x.fresh > 0) {
+                const int64_t place = static_cast<int64_t>(x.tokens) + i;
+                const int32_t column = static_cast<int32_t>(place / S);
+                const int32_t p = column < before ? page_at(a.t, row0 + r, column) : __ldcg(a.list + x.rank + column - before);
+                if (p >= 0) slot = static_cast<int64_t>(p) * S + (place - static_cast<int64_t>(column) * S);
+            }
+            a.slots[x.start + i] = slot;
+        }
+    }
+    if (a.starts) {  // rows of no request
+        const int32_t first = start_of(a, 0), last = start_of(a, a.t.rows);
+        for (int32_t i = cluster_rank() * kClusterThreads + threadIdx.x; i < a.ntokens; i += kClusterBlocks * kClusterThreads)
+            if (i < first || i >= last) a.slots[i] = -1;
+    }
+}
+
+// ---- compact -------------------------------------------------------------------------------------------
+struct CompactArgs {
+    Table t;
+    int32_t *table, *refs, *places, *moves;  // moves [2][num_pages / 2]
+    int32_t *copies, *before_middle;
+};
+// One cluster.  With n pages held, those at n and behind go to the holes in front of n, the first to the first.
+__global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kClusterThreads) compact_places_kernel(const __grid_constant__ CompactArgs a) {
+    __shared__ Sums sums;
+    wait_for_launch_before();
+    const Run run = run_of(a.t.num_pages);
+    const bool vectors = reinterpret_cast<uintptr_t>(a.refs) % 16 == 0;
+    int32_t held = 0, block_held, n = 0;  // n: pages held
+    each_page(a.refs, run, vectors, [&](int32_t, int32_t c) { held += c != 0; });
+    int32_t before = sum_before(held, sums.pages, &block_held);
+    if (threadIdx.x == 0) sums.told[0] = block_held;
+    cluster_barrier();
+    const int me = cluster_rank();
+    for (int r = 0; r < kClusterBlocks; ++r) {
+        const int32_t h = static_cast<int32_t>(of_block(sums.told, r));
+        if (r < me) before += h;
+        n += h;
+    }
+    if (n >= run.first && n < run.last) {  // the thread whose pages n is one of
+        int32_t front = before;
+        for (int32_t p = run.first; p < n; ++p) front += a.refs[p] != 0;
+        *a.before_middle = front;
+    }
+    cluster_barrier();
+    const int32_t front = n < a.t.num_pages ? __ldcg(a.before_middle) : n, made = n - front;  // holes in front of n = held pages behind
+    const int32_t half = a.t.num_pages / 2;
+    each_page(a.refs, run, vectors, [&](int32_t p, int32_t c) {
+        if (c != 0 && p >= n) a.moves[before - front] = p;
+        if (c == 0 && p < n) a.moves[half + p - before] = p;
+        a.places[p] = c != 0 ? p : -1;
+        before += c != 0;
+    });
+    cluster_barrier();
+    for (int32_t r = cluster_rank() * kClusterThreads + threadIdx.x; r < half; r += kClusterBlocks * kClusterThreads) {
+        if (r < made) {
+            const int32_t from = __ldcg(a.moves + r), to = __ldcg(a.moves + half + r);
+            a.places[from] = to;
+            a.refs[to] = __ldcg(a.refs + from);
+            a.refs[from] = 0;
+        } else {
+            a.moves[r] = a.moves[half + r] = -1;
+        }
+    }
+    if (cluster_rank() == 0 && threadIdx.x == 0) *a.copies = made;
+}
+__global__ void __launch_bounds__(kRowThreads) compact_tables_kernel(const __grid_constant__ CompactArgs a) {
+    wait_for_launch_before();
+    const int parts = (a.t.width + kRowColumns - 1) / kRowColumns;
+    const int row = blockIdx.x / parts, column0 = (blockIdx.x - row * parts) * kRowColumns;
+    const int32_t need = pages_of(length_of(a.t, row), a.t.page_size);
+    for (int j = column0 + threadIdx.x; j < column0 + kRowColumns && j < need; j += kRowThreads) {
+        const int32_t p = page_at(a.t, row, j);
+        if (p < 0) continue;
+        const int32_t to = __ldcg(a.places + p);
+        if (to >= 0) a.table[row * a.t.row + j] = to;
+        else note(a.t.status, CG_S_BAD_PAGE);  // a page that nobody holds
+    }
+}
+
+// ---- copy ----------------------------------------------------------------------------------------------
+// A page as `outer` runs of `run` pieces (vectors or values) that follow one another in memory; outer index o stands for the page's
+// token o, its head o, or, where neither follows the other, for head o % heads of token o / heads.
+struct CopySide {
+    char *data;
+    int64_t layer, page, token, head;  // in elements
+    int32_t runs;                      // kWhole ..
+};
+enum Runs { kWhole, kTokens, kHeads, kNone };
+struct CopyArgs {
+    CopySide sides[2];
+    const void *src, *dst;
+    const int32_t *tokens, *count;  // or nullptr
+    int32_t *status;
+    int64_t units, num_pages;
+    int32_t ncopies, nlayers, page_size, heads, pieces;  // pieces of a head
+    int32_t parts, wide;
+};
+
+// A unit is a part of one page of one layer's keys or values: kCopyThreads x kCopyVectors pieces.
+template <class Piece>
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+    wait_for_launch_before();
+    const int32_t ncopies = a.count ? __ldcg(a.count) : a.ncopies, each = 2 * a.nlayers * a.parts;
+    const int64_t units = static_cast<int64_t>(ncopies) * each;
+    constexpr int kValues = sizeof(Piece) / 2;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int32_t copy = static_cast<int32_t>(u / each), in = static_cast<int32_t>(u - static_cast<int64_t>(copy) * each);
+        const int64_t from = a.wide ? __ldcg(static_cast<const long long *>(a.src) + copy) : __ldcg(static_cast<const int *>(a.src) + copy);
+        const int64_t to = a.wide ? __ldcg(static_cast<const long long *>(a.dst) + copy) : __ldcg(static_cast<const int *>(a.dst) + copy);
+        int32_t tokens = a.tokens ? __ldcg(a.tokens + copy) : a.page_size;
+        if (from < 0 || to < 0 || from >= a.num_pages || to >= a.num_pages || tokens < 0 || tokens > a.page_size) {
+            const bool padding = from == -1 || to == -1;
+            if (!padding && in == 0 && threadIdx.x == 0) note(a.status, CG_S_BAD_PAGE);
+            continue;
+        }
+        const int32_t which = in / a.parts, part = in - which * a.parts, layer = which >> 1;
+        const CopySide &s = a.sides[which & 1];
+        const int32_t pieces = tokens * a.heads * a.pieces, first = part * kCopyThreads * kCopyVectors;
+        if (first >= pieces || from == to) continue;
+        const int32_t run = s.runs == kWhole ? pieces : s.runs == kTokens ? a.heads * a.pieces : s.runs == kHeads ? tokens * a.pieces : a.pieces;
+        const char *const src = s.data + 2 * (layer * s.layer + from * s.page);
+        char *const dst = s.data + 2 * (layer * s.layer + to * s.page);
+        Piece x[kCopyVectors];
+        int64_t at[kCopyVectors];
+#pragma unroll
+        for (int v = 0; v < kCopyVectors; ++v) {
+            const int32_t e = first + v * kCopyThreads + threadIdx.x;
+            at[v] = -1;
+            if (e < pieces) {
+                if (s.runs == kWhole) {
+                    at[v] = static_cast<int64_t>(e) * kValues;
+                } else {
+                    const int32_t o = e / run, rest = e - o * run;
+                    const int64_t step = s.runs == kTokens ? o * s.token : s.runs == kHeads ? o * s.head : o / a.heads * s.token + o % a.heads * s.head;
+                    at[v] = step + static_cast<int64_t>(rest) * kValues;
+                }
+                x[v] = *reinterpret_cast<const Piece *>(src + 2 * at[v]);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < kCopyVectors; ++v)
+            if (at[v] >= 0) *reinterpret_cast<Piece *>(dst + 2 * at[v]) = x[v];
+    }
+}
+
+CopySide copy_side(void *data, const int64_t *s, int heads, int head_size) {
+    const bool heads_follow = s[3] == head_size || heads == 1, tokens_follow = s[2] == head_size;
+    const int runs = heads_follow && s[2] == static_cast<int64_t>(heads) * head_size ? kWhole : heads_follow ? kTokens : tokens_follow ? kHeads : kNone;
+    return CopySide{static_cast<char *>(data), s[0], s[1], s[2], s[3], runs};
+}
+bool vectors(const CopySide &s) {
+    return reinterpret_cast<uintptr_t>(s.data) % 16 == 0 && s.layer % 8 == 0 && s.page % 8 == 0 && s.token % 8 == 0 && s.head % 8 == 0;
+}
+
+// count: how many copies there are, on the GPU, or nullptr: ncopies; early: the launch in front writes what is read here and has
+// let this one start
+int copy_pages(const cg_copy_job &j, const int32_t *count, bool early, cudaStream_t st) {
+    if (j.ncopies == 0 || j.nlayers == 0 || j.page_size == 0) return CG_OK;
+    CopyArgs a{};
+    a.sides[0] = copy_side(j.pages_k, j.pages_k_strides, j.heads, j.head_size);
+    a.sides[1] = copy_side(j.pages_v, j.pages_v_strides, j.heads, j.head_size);
+    a.src = j.src, a.dst = j.dst, a.tokens = j.tokens, a.count = count, a.status = j.status;
+    a.num_pages = j.num_pages;
+    a.ncopies = j.ncopies, a.nlayers = j.nlayers, a.page_size = j.page_size, a.heads = j.heads, a.wide = j.wide;
+    const bool vec = j.head_size % 8 == 0 && vectors(a.sides[0]) && vectors(a.sides[1]);
+    a.pieces = vec ? j.head_size / 8 : j.head_size;
+    const int64_t pieces = static_cast<int64_t>(j.page_size) * j.heads * a.pieces;
+    a.parts = static_cast<int32_t>((pieces + kCopyThreads * kCopyVectors - 1) / (kCopyThreads * kCopyVectors));
+    const int64_t units = 2 * static_cast<int64_t>(j.nlayers) * a.parts * j.ncopies, most = static_cast<int64_t>(sm_count()) * 8;
+    const dim3 grid(static_cast<unsigned>(units < most ? units : most));
+    return vec ? launch(copy_pages_kernel<uint4>, grid, kCopyThreads, 0, early, st, a) : launch(copy_pages_kernel<uint16_t>, grid, kCopyThreads, 0, early, st, a);
+}
+
+int check_copy(const cg_copy_job &j) {
+    if (j.ncopies < 0 || j.nlayers < 0 || j.page_size <= 0 || j.heads <= 0 || j.head_size <= 0 || j.num_pages < 0 || j.num_pages > kMostPages) return CG_E_SHAPE;
+    // offsets inside a page, and units of one copy, are 32-bit numbers
+    if (static_cast<int64_t>(j.heads) * j.head_size > (1 << 28) || static_cast<int64_t>(j.page_size) * j.heads * j.head_size > (1 << 30) ||
+        static_cast<int64_t>(j.nlayers) * (static_cast<int64_t>(j.page_size) * j.heads * j.head_size / 1024 + 1) > (1 << 29))
+        return CG_E_CAPACITY;
+    return CG_OK;
+}
+
+// ---- entries -------------------------------------------------------------------------------------------
+struct Workspace {  // where its parts begin
+    int64_t writers, list, copies, total;
+};
+Workspace workspace_of(int64_t num_pages) {
+    Workspace w{};
+    w.writers = 64;  // two words of counts in front
+    w.list = w.writers + 8 * num_pages;
+    w.total = w.list + 4 * num_pages;
+    return w;
+}
+
+enum What { kFork, kFree, kExtend, kCompact };
+
+int check_pages(const cg_pages_job *job, What what) {
+    if (!job) return CG_E_NULL;
+    const cg_pages_job &j = *job;
+    if (j.nrows < 0 || j.width < 0 || j.page_size <= 0 || j.num_pages < 0 || j.num_pages > kMostPages || j.nnew < 0 || j.ntokens < 0) return CG_E_SHAPE;
+    if (j.nrows > CG_MAX_REQUESTS || ((what == kFork || (what == kFree && j.which)) && j.nnew > CG_MAX_REQUESTS)) return CG_E_CAPACITY;
+    if (static_cast<int64_t>(j.width) * j.page_size > INT32_MAX) return CG_E_SHAPE;
+    if ((j.nrows && ((j.width && !j.table) || !j.kv_lens)) || (j.num_pages && !j.refs)) return CG_E_NULL;
+    if (what == kFork && (!j.which || (j.width && !j.new_table) || !j.new_lens || !j.moves) && j.nnew) return CG_E_NULL;
+    if (what == kExtend && ((!j.slots && j.ntokens) || (!j.q_starts && j.ntokens != j.nrows))) return j.q_starts || !j.slots ? CG_E_NULL : CG_E_SHAPE;
+    if (what == kCompact && j.num_pages && (!j.places || (!j.moves && j.num_pages > 1))) return CG_E_NULL;
+    if (what != kFree) {
+        if (j.workspace_bytes < workspace_of(j.num_pages).total || !j.workspace) return CG_E_CAPACITY;
+        if (reinterpret_cast<uintptr_t>(j.workspace) % 16) return CG_E_ALIGN;
+    }
+    return CG_OK;
+}
+Table table_of(const cg_pages_job &j) {
+    return Table{j.table, j.kv_lens, j.table_row, j.nrows, j.width, j.page_size, static_cast<int32_t>(j.num_pages), j.status};
+}
+char *part_of(const cg_pages_job &j, int64_t at) { return static_cast<char *>(j.workspace) + at; }
+
+}  // namespace
+}  // namespace cg
+
+extern "C" int64_t cg_pages_workspace(int64_t num_pages) {
+    return num_pages < 0 || num_pages > cg::kMostPages ? CG_E_SHAPE : cg::workspace_of(num_pages).total;
+}
+
+extern "C" int cg_copy_pages(const cg_copy_job *job, void *stream) {
+    using namespace cg;
+    if (!job) return CG_E_NULL;
+    const cg_copy_job &j = *job;
+    if (const int rc = check_copy(j)) return rc;
+    if (j.ncopies == 0 || j.nlayers == 0) return CG_OK;
+    if (!j.pages_k || !j.pages_v || !j.src || !j.dst) return CG_E_NULL;
+    return copy_pages(j, nullptr, false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int cg_fork_pages(const cg_pages_job *job, const cg_copy_job *copy, void *stream) {
+    using namespace cg;
+    if (const int rc = check_pages(job, kFork)) return rc;
+    const cg_pages_job &j = *job;
+    if (copy) {
+        if (const int rc = check_copy(*copy)) return rc;
+        if (copy->nlayers && (!copy->pages_k || !copy->pages_v)) return CG_E_NULL;
+        if (copy->page_size != j.page_size || copy->num_pages != j.num_pages) return CG_E_SHAPE;
+    }
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const Workspace w = workspace_of(j.num_pages);
+    ForkArgs a{};
+    a.old = table_of(j);
+    a.table = j.new_table, a.lens = j.new_lens, a.refs = j.refs, a.moves = j.moves, a.parents = j.which;
+    a.writers = reinterpret_cast<Writers *>(part_of(j, w.writers)), a.list = reinterpret_cast<int32_t *>(part_of(j, w.list));
+    a.copies = reinterpret_cast<int32_t *>(part_of(j, 0));
+    a.row = j.new_table_row;
+    a.nnew = j.nnew, a.wide = j.wide, a.release = j.release;
+    const int rows = j.release && j.nrows > j.nnew ? j.nrows : j.nnew, parts = j.width > kRowColumns ? (j.width + kRowColumns - 1) / kRowColumns : 1;
+    if (rows == 0) return CG_OK;
+    if (static_cast<int64_t>(rows) * parts > INT32_MAX) return CG_E_SHAPE;
+    if (const int rc = launch(fork_tables_kernel, dim3(rows * parts), kRowThreads, 0, false, st, a)) return rc;
+    if (j.nnew == 0) return CG_OK;
+    if (const int rc = launch(fork_writers_kernel, dim3(kClusterBlocks), kClusterThreads, 0, true, st, a)) return rc;
+    if (!copy) return CG_OK;
+    cg_copy_job c = *copy;
+    c.src = j.moves, c.dst = j.moves + j.nnew, c.tokens = j.moves + 2 * static_cast<int64_t>(j.nnew);
+    c.wide = 0, c.ncopies = j.nnew, c.status = j.status;
+    return copy_pages(c, a.copies, false, st);
+}
+
+extern "C" int cg_free_pages(const cg_pages_job *job, void *stream) {
+    using namespace cg;
+    if (const int rc = check_pages(job, kFree)) return rc;
+    const cg_pages_job &j = *job;
+    FreeArgs a{table_of(j), j.table, j.kv_lens, j.refs, j.which, j.which ? j.nnew : j.nrows, j.wide};
+    if (a.nfree == 0) return CG_OK;
+    return launch(free_pages_kernel, dim3(a.nfree), kRowThreads, 0, false, static_cast<cudaStream_t>(stream), a);
+}
+
+extern "C" int cg_extend_pages(const cg_pages_job *job, void *stream) {
+    using namespace cg;
+    if (const int rc = check_pages(job, kExtend)) return rc;
+    const cg_pages_job &j = *job;
+    if (j.nrows == 0 && j.ntokens == 0) return CG_OK;
+    if (j.nrows == 0) return CG_E_SHAPE;  // tokens of nobody
+    const Workspace w = workspace_of(j.num_pages);
+    ExtendArgs a{table_of(j), j.table, j.kv_lens, j.refs, reinterpret_cast<int32_t *>(part_of(j, w.list)), j.q_starts, j.slots, j.ntokens};
+    return launch(extend_pages_kernel, dim3(kClusterBlocks), kClusterThreads, 0, false, static_cast<cudaStream_t>(stream), a);
+}
+
+extern "C" int cg_compact_pages(const cg_pages_job *job, const cg_copy_job *copy, void *stream) {
+    using namespace cg;
+    if (const int rc = check_pages(job, kCompact)) return rc;
+    const cg_pages_job &j = *job;
+    if (copy) {
+        if (const int rc = check_copy(*copy)) return rc;
+        if (copy->nlayers && (!copy->pages_k || !copy->pages_v)) return CG_E_NULL;
+        if (copy->page_size != j.page_size || copy->num_pages != j.num_pages) return CG_E_SHAPE;
+    }
+    if (j.num_pages == 0) return CG_OK;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int32_t *const words = reinterpret_cast<int32_t *>(part_of(j, 0));
+    CompactArgs a{table_of(j), j.table, j.refs, j.places, j.moves, words, words + 1};
+    if (const int rc = launch(compact_places_kernel, dim3(kClusterBlocks), kClusterThreads, 0, false, st, a)) return rc;
+    if (j.nrows && j.width) {
+        const int64_t blocks = static_cast<int64_t>(j.nrows) * ((j.width + kRowColumns - 1) / kRowColumns);
+        if (blocks > INT32_MAX) return CG_E_SHAPE;
+        if (const int rc = launch(compact_tables_kernel, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, false, st, a)) return rc;
+    }
+    if (!copy) return CG_OK;
+    cg_copy_job c = *copy;
+    c.src = j.moves, c.dst = j.moves + j.num_pages / 2, c.tokens = nullptr;
+    c.wide = 0, c.ncopies = static_cast<int32_t>(j.num_pages / 2), c.status = j.status;
+    return copy_pages(c, a.copies, false, st);
+}

@@ -5,11 +5,23 @@
     append_paged      keys and values of new tokens, or a blob of every layer, into pages, rotated on the way
     gather_paged      a range of a cache out of its pages, rotation undone on the way
     paged_attention   attention of the newest tokens of a batch of requests over their pages
-    check_status      raises if a kernel met a slot, page or length that does not fit
+    copy_pages        pages, or the first tokens of them, copied to other places of the cache
+    fork_pages        tables of new rows that go on from given ones: pages shared, the last ones copied where they have to be
+    extend_pages      room for new tokens: pages taken for them, and their slots
+    free_pages        pages given back
+    compact_pages     held pages moved to the front of the cache
+    beam_select       the best continuations of every request's beams
+    beam_step         these three together: a step of beam search, from logits to the slots of the chosen tokens
+    check_status      raises if a kernel met a slot, page or length that does not fit, or no free page
 
 Pages are tensors [num_pages, page_size, heads, head_size] of float16 or bfloat16, with any strides but an innermost one of 1
 (a cache that keeps a head's tokens together is passed as a transposed view); with a leading axis where a call is
 made for several layers.  Slot s is token s % page_size of page s // page_size.
+
+Rows of a page table may share pages.  refs (int32 [num_pages]) counts the rows that hold each page; 0: it is free.  A row of kv_len tokens
+holds the first ceil(kv_len / page_size) pages of its row of the table.  The calls that fork, extend, free and compact keep the counts,
+without a question to the GPU; a new cache's counts are zeros, and its tables' lengths too.  A page that is not full is held by one row wherever
+rows are to grow: fork_pages leaves it so.  Pages are taken from the lowest number on, for rows in their order.
 
 Calls enqueue on the current stream of the tensors' device, allocate what they return and a workspace from
 torch's allocator, and wait for nothing, so they can be captured in a CUDA graph (which needs its Rotary as long as it is replayed, and
@@ -29,6 +41,7 @@ from .serde.cachegen_basics import on_device
 from .torchac_cuda import _check, _status, _status_word
 
 _DTYPES = {torch.float16: _lib.CG_F16, torch.bfloat16: _lib.CG_BF16}
+_LOGITS = {**_DTYPES, torch.float32: _lib.CG_LOGITS_F32}
 _INDEX = (torch.int32, torch.int64)
 _TWO_PI = Fraction(628318530717958647692528676655900576839, 10 ** 38)
 
@@ -467,6 +480,276 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 def _steps(t):
     """Strides of the outer axes, with none for an axis of one."""
     return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
+
+
+def _whole(t, name, device, dtype, shape, written=False):
+    """Checks a tensor of numbers that a call on tables takes; None in shape: any size."""
+    _check(t.is_cuda and t.device == device, f"{name} must be on {device}")
+    _check(t.dtype == dtype, f"{name} must be {dtype}")
+    _check(t.dim() == len(shape) and all(w in (None, n) for w, n in zip(shape, t.shape)), f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    _check(t.is_contiguous() if len(shape) == 1 else t.stride(-1) == 1 or t.shape[-1] <= 1,
+           f"{name} must be contiguous" if len(shape) == 1 else f"{name} must have an innermost stride of 1")
+    if written:
+        _check(all(s or n <= 1 for s, n in zip(t.stride(), t.shape)), f"{name} is written to and must not be expanded")
+
+
+def _axes(t):
+    """(stride, size) of a tensor's axes in 16-bit values, the widest strides first."""
+    wide = t.element_size() // 2
+    axes = [(s * wide, n) for s, n in zip(t.stride(), t.shape) if n > 1] + ([(1, wide)] if wide > 1 else [])
+    return sorted(axes, reverse=True)
+
+
+def _all_apart(written, read):
+    """Checks that nothing that is written, as (name, tensor), shares memory with anything else."""
+    for i, (name, t) in enumerate(written):
+        for other, u in written[:i] + read:
+            if t.numel() and u.numel():
+                _check(_no_value_shared(u.data_ptr() - t.data_ptr(), _axes(t), _axes(u)), f"{name} must not overlap {other}")
+
+
+def _tables(page_table, kv_lens, refs, page_size, device, written):
+    """What the calls on tables have in common; `written`: whether the rows given are."""
+    _check(refs.is_cuda, "refs must be a CUDA tensor")
+    _whole(refs, "refs", device, torch.int32, (None,), True)
+    _check(kv_lens.dim() == 1, "kv_lens must have one dimension")
+    B = kv_lens.shape[0]
+    _whole(kv_lens, "kv_lens", device, torch.int32, (B,), written)
+    _whole(page_table, "page_table", device, torch.int32, (B, None), written)
+    _check(B <= _lib.CG_MAX_REQUESTS, f"at most {_lib.CG_MAX_REQUESTS} rows in a call")
+    _check(page_size > 0, "pages must hold a token at least")
+    W = page_table.shape[1]
+    _check(W * page_size < 2 ** 31, f"rows of {W} pages of {page_size} tokens are longer than a call takes")
+    job = _lib.PagesJob()
+    job.table, job.kv_lens, job.refs, job.status = page_table.data_ptr(), kv_lens.data_ptr(), refs.data_ptr(), _address(_status_of(refs))
+    job.table_row = page_table.stride(0)
+    _check(refs.shape[0] < 2 ** 31 - 8, f"refs: {refs.shape[0]} is more than a call takes")
+    job.num_pages = refs.shape[0]
+    _set(job, nrows=B, width=W, page_size=page_size)
+    return job
+
+
+def _workspace(job, device):
+    workspace = torch.empty(_lib.lib().cg_pages_workspace(job.num_pages), dtype=torch.uint8, device=device)  # of the graph's own memory in a capture
+    job.workspace, job.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    return workspace
+
+
+def _cache_of(k_pages, v_pages, refs, page_size):
+    """The page size, and the job of the copies in a cache, if one is given."""
+    if k_pages is None or v_pages is None:
+        _check(k_pages is None and v_pages is None, "k_pages and v_pages go together")
+        _check(page_size is not None, "without pages, page_size is needed")
+        return page_size, None
+    job, P, S = _copy_job(k_pages, v_pages, refs.device)
+    _check(page_size is None or page_size == S, f"page_size is {page_size}, pages hold {S} tokens")
+    _check(P == refs.shape[0], f"refs counts {refs.shape[0]} pages, the cache has {P}")
+    return S, job
+
+
+def _copy_job(k_pages, v_pages, device):
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        _check(t.is_cuda, f"{name} must be a CUDA tensor")
+        _check(t.dtype in _DTYPES, f"{name} must be float16 or bfloat16, got {t.dtype}")
+        _check(t.dim() in (4, 5), f"{name} must have shape [pages, page_size, heads, head_size], with a leading axis for several layers")
+        _rows(t, name, device, k_pages.dtype, k_pages.dim(), k_pages.shape, True)
+    _apart(k_pages, v_pages, "k_pages", "v_pages")
+    P, S, H, D = k_pages.shape[-4:]
+    _check(S > 0 and H > 0 and D > 0, "pages must hold a value at least")
+    job = _lib.CopyJob()
+    job.pages_k, job.pages_v = k_pages.data_ptr(), v_pages.data_ptr()
+    job.pages_k_strides[:], job.pages_v_strides[:] = ([0] * (5 - t.dim()) + list(_steps(t)) for t in (k_pages, v_pages))
+    job.num_pages, job.status = P, _address(_status_of(k_pages))
+    _set(job, nlayers=k_pages.shape[0] if k_pages.dim() == 5 else 1, page_size=S, heads=H, head_size=D)
+    return job, P, S
+
+
+def _run_pages(entry, job, copy, device):
+    with on_device(device):
+        _lib.check(getattr(_lib.lib(), entry)(ctypes.byref(job), None if copy is None else ctypes.byref(copy), _stream(device)), entry)
+
+
+def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, tokens: torch.Tensor = None) -> None:
+    """Copies pages src[i] to pages dst[i] (int32 or int64 [n]; -1 in either: nothing) of keys and values [pages, page_size, heads, head_size],
+    of every layer if they have a leading axis; with `tokens` (int32 [n]) only the first tokens[i] tokens of each.  No page is written to
+    twice, or read as well: what such a page holds afterwards is not defined."""
+    _check(k_pages.is_cuda, "k_pages must be a CUDA tensor")
+    dev = k_pages.device
+    job, _, _ = _copy_job(k_pages, v_pages, dev)
+    _check(src.dim() == 1, "src must have one dimension")
+    _check(src.dtype in _INDEX, "src must be int32 or int64")
+    _whole(src, "src", dev, src.dtype, (None,))
+    _whole(dst, "dst", dev, src.dtype, tuple(src.shape))
+    if tokens is not None:
+        _whole(tokens, "tokens", dev, torch.int32, tuple(src.shape))
+    _all_apart([("k_pages", k_pages), ("v_pages", v_pages)], [(n, t) for n, t in (("src", src), ("dst", dst), ("tokens", tokens)) if t is not None])
+    job.src, job.dst, job.tokens, job.wide = src.data_ptr(), dst.data_ptr(), _address(tokens), src.dtype == torch.int64
+    _set(job, ncopies=src.shape[0])
+    _run("cg_copy_pages", job, dev)
+    _wrote(k_pages, v_pages)
+
+
+def fork_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, parents: torch.Tensor, refs: torch.Tensor, k_pages: torch.Tensor = None,
+               v_pages: torch.Tensor = None, page_size: int = None, release: bool = True, out: tuple = None) -> tuple:
+    """Rows that go on where others are: new row i holds what row parents[i] (int32 or int64 [new rows]; -1: nothing) of page_table
+    (int32 [rows, width]) with kv_lens (int32 [rows]) holds.  With `release` the new rows take the place of all the old ones, as the
+    beams of a step take the place of those before; without it the old rows stay, as a context stays of which several answers are made.
+
+    refs (int32 [num_pages]) is brought up to date.  Of the new rows that would go on in the same page, because it is not full, the first keeps it
+    if no other row holds it, and each of the rest gets a free page; what stands in it so far is copied in k_pages and v_pages
+    [pages, page_size, heads, head_size], of every layer if they have a leading axis.  For a cache in parts, leave them out, name the
+    page_size, and call copy_pages(k, v, *moves) for each part.  A row for which no page is free loses the tokens of its last page, and
+    check_status says so.
+
+    Returns the new table and lengths, in `out` or new tensors (entries behind a row's pages are -1), and moves (int32 [3, new rows]):
+    from, to and tokens of the copies, in the rows' order, -1 behind the last."""
+    S, copy = _cache_of(k_pages, v_pages, refs, page_size)
+    dev = refs.device
+    job = _tables(page_table, kv_lens, refs, S, dev, False)
+    _check(parents.dim() == 1 and parents.dtype in _INDEX, "parents must be int32 or int64 with one dimension")
+    _whole(parents, "parents", dev, parents.dtype, (None,))
+    N, W = parents.shape[0], page_table.shape[1]
+    _check(N <= _lib.CG_MAX_REQUESTS, f"at most {_lib.CG_MAX_REQUESTS} rows in a call")
+    if out is None:
+        table, lens = torch.empty((N, W), dtype=torch.int32, device=dev), torch.empty((N,), dtype=torch.int32, device=dev)
+    else:
+        table, lens = out
+        _whole(table, "out[0]", dev, torch.int32, (N, W), True)
+        _whole(lens, "out[1]", dev, torch.int32, (N,), True)
+    moves = torch.empty((3, N), dtype=torch.int32, device=dev)
+    caches = [] if copy is None else [("k_pages", k_pages), ("v_pages", v_pages)]
+    _all_apart([("refs", refs), ("out[0]", table), ("out[1]", lens)] + caches,
+               [("page_table", page_table), ("kv_lens", kv_lens), ("parents", parents)])
+    job.which, job.wide, job.release = parents.data_ptr(), parents.dtype == torch.int64, bool(release)
+    job.new_table, job.new_lens, job.moves, job.new_table_row = table.data_ptr(), lens.data_ptr(), moves.data_ptr(), table.stride(0)
+    _set(job, nnew=N)
+    workspace = _workspace(job, dev)  # noqa: F841  (kept until the launches are made)
+    _run_pages("cg_fork_pages", job, copy, dev)
+    _wrote(refs, table, lens, k_pages, v_pages)
+    return table, lens, moves
+
+
+def free_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, page_size: int, rows: torch.Tensor = None) -> None:
+    """Rows (int32 or int64 [n], -1: none; default: all) of page_table and kv_lens hold nothing any more: their lengths become 0, their pages'
+    entries -1, and the pages are free where no other row holds them."""
+    _check(refs.is_cuda, "refs must be a CUDA tensor")
+    dev = refs.device
+    job = _tables(page_table, kv_lens, refs, page_size, dev, True)
+    if rows is not None:
+        _check(rows.dim() == 1 and rows.dtype in _INDEX, "rows must be int32 or int64 with one dimension")
+        _whole(rows, "rows", dev, rows.dtype, (None,))
+        _check(rows.shape[0] <= _lib.CG_MAX_REQUESTS, f"at most {_lib.CG_MAX_REQUESTS} rows in a call")
+        if not rows.shape[0]:
+            return
+        job.which, job.wide = rows.data_ptr(), rows.dtype == torch.int64
+        _set(job, nnew=rows.shape[0])
+    _all_apart([("refs", refs), ("page_table", page_table), ("kv_lens", kv_lens)], [] if rows is None else [("rows", rows)])
+    _run("cg_free_pages", job, dev)
+    _wrote(refs, page_table, kv_lens)
+
+
+def extend_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, page_size: int, q_starts: torch.Tensor = None,
+                 tokens: int = None) -> torch.Tensor:
+    """Room for new tokens: row b of page_table and kv_lens gets q_starts[b + 1] - q_starts[b] more (int32 [rows + 1], as paged_attention takes
+    it; `tokens` is how many there are in all, or how many the caller has room for; None: a token a row), and the pages that they need beyond those it has.
+    page_table, kv_lens and refs are brought up to date.
+
+    Returns the tokens' slots (int64 [tokens]), as append_paged and decode_paged take them: -1 for tokens of no row, and for those of a row for which
+    no page is free or that its table has no room for; that row stays as it is, and check_status says so."""
+    _check(refs.is_cuda, "refs must be a CUDA tensor")
+    dev = refs.device
+    job = _tables(page_table, kv_lens, refs, page_size, dev, True)
+    B = kv_lens.shape[0]
+    if q_starts is None:
+        _check(tokens is None or tokens == B, f"without q_starts each of {B} rows gets one token, not {tokens} in all")
+        tokens = B
+    else:
+        _check(tokens is not None and tokens >= 0, "q_starts needs the number of tokens in all")
+        _check(B > 0 or tokens == 0, "tokens of no row")
+        _whole(q_starts, "q_starts", dev, torch.int32, (B + 1,))
+        job.q_starts = q_starts.data_ptr()
+    slots = torch.empty((tokens,), dtype=torch.int64, device=dev)
+    job.slots = slots.data_ptr()
+    _set(job, ntokens=tokens)
+    _all_apart([("refs", refs), ("page_table", page_table), ("kv_lens", kv_lens)], [] if q_starts is None else [("q_starts", q_starts)])
+    workspace = _workspace(job, dev)  # noqa: F841
+    _run("cg_extend_pages", job, dev)
+    _wrote(refs, page_table, kv_lens)
+    return slots
+
+
+def compact_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, k_pages: torch.Tensor = None, v_pages: torch.Tensor = None,
+                  page_size: int = None) -> tuple:
+    """Moves held pages to the front: with n of them, those at n and behind go to the free places in front of n, the first to the first, in
+    k_pages and v_pages (or, for a cache in parts, by copy_pages(k, v, *moves) for each) and in page_table and refs.
+
+    Returns places (int32 [num_pages]): where each page now is, -1 if it was free, for other tables that name them; and moves
+    (int32 [2, num_pages // 2]): from and to, -1 behind the last.  The pages of places n and behind are free afterwards."""
+    S, copy = _cache_of(k_pages, v_pages, refs, page_size)
+    dev = refs.device
+    job = _tables(page_table, kv_lens, refs, S, dev, True)
+    P = refs.shape[0]
+    places, moves = torch.empty((P,), dtype=torch.int32, device=dev), torch.empty((2, P // 2), dtype=torch.int32, device=dev)
+    job.places, job.moves = places.data_ptr(), moves.data_ptr()
+    caches = [] if copy is None else [("k_pages", k_pages), ("v_pages", v_pages)]
+    _all_apart([("refs", refs), ("page_table", page_table)] + caches, [("kv_lens", kv_lens)])
+    workspace = _workspace(job, dev)  # noqa: F841
+    _run_pages("cg_compact_pages", job, copy, dev)
+    _wrote(refs, page_table, k_pages, v_pages)
+    return places, moves
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int = None) -> tuple:
+    """The best continuations of a step of beam search.  logits [requests * beams, vocabulary], float16, bfloat16 or float32; scores (float32
+    [requests, beams]): the beams' scores so far.  A continuation's score is its beam's plus the logarithm of its token's share of the beam's
+    softmax; of all of a request's the k (default: as many as beams) best are chosen, in falling order, equal ones by beam, then by token.  (Those of one beam
+    are in the order of their logits, whatever the scores lose of it.)
+
+    Returns scores (float32), tokens and parents (int32), all [requests, k]; parents are rows of logits, as fork_pages takes them.  Scores are
+    compared in 64 bits and rounded once.  A beam whose score is not finite has no continuations, nor have logits of -infinity or NaN,
+    which weigh nothing; logits of +infinity share their row's weight.  Behind a request's last continuation stand -infinity, -1 and -1."""
+    _check(logits.is_cuda, "logits must be a CUDA tensor")
+    _check(logits.dtype in _LOGITS, f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
+    _check(scores.dim() == 2, "scores must have shape [requests, beams]")
+    B, K = scores.shape
+    dev = logits.device
+    _rows(logits, "logits", dev, logits.dtype, 2, (B * K, None))
+    V = logits.shape[1]
+    _check(scores.is_cuda and scores.device == dev, f"scores must be on {dev}")
+    _check(scores.dtype == torch.float32 and scores.is_contiguous(), "scores must be float32 and contiguous")
+    _check(not scores.is_neg(), "scores is a view that negates its memory")
+    _check(not (scores.requires_grad and torch.is_grad_enabled()), "scores requires a gradient, which calls on a paged cache do not compute")
+    k = K if k is None else k
+    _check(0 < K <= _lib.CG_MAX_BEAMS and 0 < k <= _lib.CG_MAX_CHOICES and K * k <= _lib.CG_MAX_BEAM_CHOICES,
+           f"{k} of {K} beams' continuations: a call takes up to {_lib.CG_MAX_BEAMS} beams, {_lib.CG_MAX_CHOICES} choices and a product of {_lib.CG_MAX_BEAM_CHOICES}")
+    _check(0 < V <= _lib.CG_MAX_VOCAB, f"a vocabulary has 1 to {_lib.CG_MAX_VOCAB} tokens, not {V}")
+    out = torch.empty((B, k), dtype=torch.float32, device=dev)
+    tokens, parents = (torch.empty((B, k), dtype=torch.int32, device=dev) for _ in range(2))
+    job = _lib.BeamJob()
+    job.logits, job.scores, job.out_scores, job.tokens, job.parents = (t.data_ptr() for t in (logits, scores, out, tokens, parents))
+    job.dtype, job.row_stride = _LOGITS[logits.dtype], logits.stride(0)
+    _set(job, nrequests=B, beams=K, vocab=V, k=k)
+    with on_device(dev):
+        need = _lib.lib().cg_beam_workspace(ctypes.byref(job))
+        _lib.check(min(need, 0), "beam_select")
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        job.workspace, job.workspace_bytes = workspace.data_ptr(), need
+        _lib.check(_lib.lib().cg_beam_select(ctypes.byref(job), _stream(dev)), "beam_select")
+    return out, tokens, parents
+
+
+def beam_step(logits: torch.Tensor, scores: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, k_pages: torch.Tensor,
+              v_pages: torch.Tensor, out: tuple = None) -> tuple:
+    """A step of beam search on a paged cache, from the logits of the beams' newest tokens to the slots of their next ones: the best continuations
+    (beam_select), the rows that they go on from (fork_pages), and room for a token of each (extend_pages).
+
+    Returns scores and tokens [requests, beams], and of the new rows, in their order, the table, the lengths (the new tokens included) and the
+    tokens' slots, as append_paged and paged_attention take them.  A beam without a continuation has token -1 and becomes a row that
+    holds its new token's place alone; its score is -infinity, so nothing goes on from it."""
+    scores, tokens, parents = beam_select(logits, scores)
+    table, lens, _ = fork_pages(page_table, kv_lens, parents.view(-1), refs, k_pages, v_pages, out=out)
+    slots = extend_pages(table, lens, refs, k_pages.shape[-3])
+    return scores, tokens, table, lens, slots
 
 
 def split_pages(pages: torch.Tensor, fmt: str) -> tuple:

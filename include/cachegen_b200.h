@@ -98,6 +98,7 @@ extern "C" {
 #define CG_S_BAD_TABLE 16     /* CG_TABLES_SPARSE offsets reach past the table set (read as zero counts) */
 #define CG_S_BAD_PAGE 32      /* a slot or page outside the cache, or lengths that its tables have no room for */
 #define CG_S_TIMEOUT 64       /* a kernel gave up waiting for its own copies or products; its output is not valid */
+#define CG_S_NO_PAGE 128      /* a paged cache had no free page left for a row */
 
 /*
  * Sizes in bytes of the buffers a caller allocates for the fused calls, for one chunk of
@@ -554,6 +555,91 @@ typedef struct cg_attention_job {
 } cg_attention_job;
 int64_t cg_paged_attention_workspace(const cg_attention_job *job_host); /* bytes, or CG_E_* */
 int cg_paged_attention(const cg_attention_job *job_host, void *stream);
+
+/*
+ * Pages that several rows of a table may hold.  refs: int32 [num_pages], how many rows hold each page; 0: it is free.  A row holds
+ * the first ceil(kv_len / page_size) entries of its row of the table (int32 [nrows, width], rows table_row apart); kv_lens: int32 [nrows].
+ * A page that is not full (a row's last) is held by that row alone wherever the row is to grow.  What is taken is the free page of
+ * the lowest number, for rows in their order.  Pages that the cache does not have, lengths that do not fit the table, rows that are not
+ * there: left out, with CG_S_BAD_PAGE; a free page that is not there: CG_S_NO_PAGE.
+ *
+ * cg_fork_pages: new row i holds what row which[i] holds (-1: nothing).  new_table [nnew, width], rows new_table_row apart (-1 behind a row's
+ * pages), new_lens [nnew].  release: the old rows hold nothing any more (their table and lengths are not written).  Of the new rows that
+ * go on in a page that is not full, the first keeps it if no other row holds it, each of the rest gets a free page (or, if there is none, loses
+ * that page's tokens); moves: int32 [3, nnew]: from, to and tokens of the pages to be copied for that, in the rows' order, -1 behind
+ * the last.  copy: what to copy them in (its src, dst, tokens, ncopies, wide and status are not read), or NULL.  The new rows' arrays
+ * share nothing with the old ones'.
+ * cg_free_pages: rows which[0 .. nnew) (-1: none; NULL: all rows) hold nothing any more: their lengths become 0, their entries -1.
+ * cg_extend_pages: row r gets q_starts[r + 1] - q_starts[r] more tokens (int32 [nrows + 1], rising; NULL: one, and ntokens is nrows), with pages for them;
+ * slots [ntokens]: where they belong, -1 for tokens of no row and of rows that find no place: those stay as they are.
+ * cg_compact_pages: with n pages held, the held pages at n and behind move to the free places in front of n, the first to the first;
+ * counts and the table follow.  places: int32 [num_pages]: where each page now is, -1 if it was free; moves: int32 [2, num_pages / 2]: from
+ * and to, -1 behind the last.  copy as above.
+ * workspace: cg_pages_workspace(num_pages) bytes, 16-byte aligned, which calls on one stream may share (none for cg_free_pages).
+ * nrows, nnew <= CG_MAX_REQUESTS, width * page_size < 2^31, num_pages <= 2^31 - 9.
+ */
+typedef struct cg_pages_job {
+    int32_t *table, *kv_lens, *refs;
+    const void *which; /* int64 (wide) or int32 */
+    int32_t *new_table, *new_lens, *moves, *places;
+    const int32_t *q_starts;
+    int64_t *slots;
+    void *workspace;
+    int32_t *status; /* may be NULL */
+    int64_t workspace_bytes, table_row, new_table_row, num_pages;
+    int32_t nrows, width, page_size, nnew, wide, release, ntokens, reserved;
+} cg_pages_job;
+
+/*
+ * Page src[i] (int64 if wide, else int32) to page dst[i] of every layer's keys and values, or the first tokens[i] tokens of it (int32; NULL: all);
+ * -1 in either: nothing.  No page is written to twice or read as well.  pages [nlayers, num_pages, page_size, heads, head_size] as above.
+ * page_size * heads * head_size <= 2^30.
+ */
+typedef struct cg_copy_job {
+    void *pages_k, *pages_v;
+    const void *src, *dst;
+    const int32_t *tokens;
+    int32_t *status; /* may be NULL */
+    int64_t pages_k_strides[4], pages_v_strides[4];
+    int64_t num_pages;
+    int32_t nlayers, ncopies, page_size, heads, head_size, wide;
+} cg_copy_job;
+int64_t cg_pages_workspace(int64_t num_pages); /* bytes, or CG_E_* */
+int cg_copy_pages(const cg_copy_job *job_host, void *stream);
+int cg_fork_pages(const cg_pages_job *job_host, const cg_copy_job *copy_host, void *stream);
+int cg_free_pages(const cg_pages_job *job_host, void *stream);
+int cg_extend_pages(const cg_pages_job *job_host, void *stream);
+int cg_compact_pages(const cg_pages_job *job_host, const cg_copy_job *copy_host, void *stream);
+
+/*
+ * The best continuations of the beams of nrequests requests: of all (beam, token) of a request the k with the largest
+ *     score[beam] + x[beam, token] - log sum_w exp x[beam, w],
+ * in falling order of these numbers, equal ones by beam, then token.
+ *
+ * logits: CG_F16, CG_BF16 or CG_LOGITS_F32, rows of vocab values row_stride apart, nrequests * beams of them, innermost stride 1.  scores: float32
+ * [nrequests, beams]; a beam whose score is not finite has no continuations, and its logits are not read.  Logits of -infinity and NaN are no
+ * continuations and weigh nothing; where there are logits of +infinity, these share their row's weight and the others are none.
+ * out_scores (float32), tokens, parents (int32): [nrequests, k], parents as rows of logits; where a request has fewer than k
+ * continuations, -infinity, -1, -1 behind them.  Continuations of one beam are compared by their logits, those of different beams in 64
+ * bits; numbers are rounded once.
+ * workspace: cg_beam_workspace(job) bytes (16-byte aligned), which calls on one stream may share.
+ */
+#define CG_LOGITS_F32 2
+#define CG_MAX_BEAMS 256
+#define CG_MAX_CHOICES 128
+#define CG_MAX_BEAM_CHOICES 8192 /* beams * k */
+#define CG_MAX_VOCAB (1 << 24)
+typedef struct cg_beam_job {
+    const void *logits;
+    const float *scores;
+    float *out_scores;
+    int32_t *tokens, *parents;
+    void *workspace;
+    int64_t workspace_bytes, row_stride;
+    int32_t dtype, nrequests, beams, vocab, k, reserved;
+} cg_beam_job;
+int64_t cg_beam_workspace(const cg_beam_job *job_host); /* bytes, or CG_E_* */
+int cg_beam_select(const cg_beam_job *job_host, void *stream);
 
 #ifdef __cplusplus
 }
