@@ -239,7 +239,9 @@ def native_calls():
                                      f"`python -m cachegen_b200.build --force` ({e})") from e
     module.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value
                  for n in ("cg_decode_kv", "cg_encode_kv", "cg_encode_kv_workspace", "cg_encode_kv_wait", "cg_encode_kv_gather",
-                           "cg_rotary", "cg_append_paged", "cg_gather_paged", "cg_paged_attention_workspace", "cg_paged_attention")})
+                           "cg_rotary", "cg_append_paged", "cg_gather_paged", "cg_paged_attention_workspace", "cg_paged_attention",
+                           "cg_pages_workspace", "cg_copy_pages", "cg_fork_pages", "cg_free_pages", "cg_extend_pages", "cg_compact_pages",
+                           "cg_beam_workspace", "cg_beam_select")})
     return module
 
 

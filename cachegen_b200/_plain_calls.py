@@ -20,6 +20,7 @@ def _left(*_):
 
 
 rotary = append = gather = attend = _left
+copy_pages = fork_pages = free_pages = extend_pages = compact_pages = beam_select = _left
 
 
 def encode_start(job_at, kv, bins, max_bins, tail_at, workspace, row_off, counts_bytes, on, launch):

@@ -25,6 +25,7 @@ constexpr int kHeld = 1024, kHeldSoft = kHeld / 2;         // candidates of a bl
 constexpr int kChooseBlocks = 8;                           // of a request's cluster
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTilesPerPart = 4;
+constexpr int kChooseWarps = 8, kMostChooseWarps = 16, kSorted = 512, kMostList = 4096;
 // Relative error of a row's sum in 32 bits, and so the absolute one of its logarithm.  A term exp(-u) is 2 to the power of a product: the
 // difference u is off by 2^-24 of itself, the constant by 2^-26, the product by 2^-24, in all 2^-22.8 u; u on average, weighted with the terms, is
 // below 17 for up to 2^24 tokens (n terms of one size u beside the largest weigh n u exp(-u) / (1 + n exp(-u))): 2.3e-6.  The power itself: 2^-22.
@@ -50,7 +51,7 @@ struct BeamArgs {
     Part *parts;             // [rows][nparts]
     Candidate *candidates;   // [rows][nparts][room]
     int64_t row_stride;
-    int32_t beams, vocab, k, nparts, part_vectors, room, sort_room;
+    int32_t beams, vocab, k, nparts, part_vectors, room, list_room, sort_room;
 };
 
 // A float's bits in an order in which they compare as numbers without a sign; 0 and -0 are the same.
@@ -224,12 +225,19 @@ __device__ __noinline__ float keep_first(Shared &s, int32_t n, int32_t k, More m
     return least ? from_ordered(least) : -CUDART_INF_F;
 }
 
-// A value that k threads' keys reach, to 16 bits; 0 if fewer threads have one (a key above that of -infinity).
-__device__ __forceinline__ uint32_t reached(uint32_t key, int32_t k) {
-    uint32_t least = 0;
-    if (key <= ordered(-CUDART_INF_F)) key = 0;
+// A value that k of the block's keys reach, to 16 bits; 0 if there are fewer of them (above that of -infinity).  key(i), i < N: a thread's.
+template <int N, class Key>
+__device__ __forceinline__ uint32_t reached(int32_t k, Key key) {
+    uint32_t mine[N], least = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        mine[i] = key(i);
+        if (mine[i] <= ordered(-CUDART_INF_F)) mine[i] = 0;
+    }
     for (int bit = 31; bit >= 16; --bit) {
-        const int32_t c = __syncthreads_count(key >= (least | 1u << bit));
+        int32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c += __syncthreads_count(mine[i] >= (least | 1u << bit));
         if (c >= k) {
             least |= 1u << bit;
             if (c == k) break;
@@ -295,7 +303,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const __grid_constant
         // in front of it reach
         const bool first = v0 == from;
         if (first) {
-            const uint32_t key = reached(ordered(tile), k);
+            const uint32_t key = reached<1>(k, [&](int) { return ordered(tile); });
             least = key ? from_ordered(key) : -CUDART_INF_F;
         }
         const auto above = [&](float y) { return first ? y >= least && y > -CUDART_INF_F : y > least; };
@@ -317,11 +325,15 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const __grid_constant
         if (__syncthreads_or(any)) {
             const int32_t found = s.nheld;
             if (found > kHeld) {  // what was held in front of this tile is whole
+                uint4 copy[kVectors];  // (what is handed on by address would never be in registers)
+#pragma unroll
+                for (int u = 0; u < kVectors; ++u) copy[u] = now[u];
+                const int32_t token0 = x.token(v0 + tid, 0);
                 least = keep_first(s, n, k, [&](auto f) {
 #pragma unroll
                     for (int u = 0; u < kVectors; ++u)
 #pragma unroll
-                        for (int e = 0; e < L::kPer; ++e) f(value_of<DT>(now[u], e), x.token(v0 + u * kRowThreads + tid, e));
+                        for (int e = 0; e < L::kPer; ++e) f(value_of<DT>(copy[u], e), token0 + u * kRowThreads * L::kPer + e);
                 });
             } else if (found > kHeldSoft) {
                 least = keep_first(s, found, k, [](auto) {});
@@ -331,12 +343,22 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const __grid_constant
         }
     }
     // raised by what is held, or cut to k
-    if (n > kRowThreads || n > a.room) {
-        least = keep_first(s, n, k, [](auto) {});
-        n = s.nheld;
-    } else if (n > k) {
-        const uint32_t key = reached(tid < n ? ordered(s.held[tid].x) : 0u, k);
+    if (n > k) {
+        const uint32_t key = reached<kHeldSoft / kRowThreads>(k, [&](int i) {
+            const int32_t at = i * kRowThreads + tid;
+            return at < n ? ordered(s.held[at].x) : 0u;
+        });
         if (key) least = fmaxf(least, from_ordered(key));
+        int32_t left = 0;
+#pragma unroll
+        for (int i = 0; i < kHeldSoft / kRowThreads; ++i) {
+            const int32_t at = i * kRowThreads + tid;
+            left += __syncthreads_count(at < n && s.held[at].x >= least);
+        }
+        if (left > a.room) {  // equal ones
+            least = keep_first(s, n, k, [](auto) {});
+            n = s.nheld;
+        }
     }
     // the block's sum
     const int lane = tid % 32, warp = tid / 32;
@@ -366,9 +388,11 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const __grid_constant
     for (int d = 16; d; d /= 2) mine += __shfl_xor_sync(~0u, mine, d);
     if (lane == 0) s.parts[warp] = mine;
     if (tid == 0) s.nheld = 0;
-    const Candidate c = tid < n ? s.held[tid] : Candidate{-CUDART_INF_F, 0};
     __syncthreads();
-    if (tid < n && c.x >= least) a.candidates[static_cast<int64_t>(blockIdx.x) * a.room + atomicAdd(&s.nheld, 1)] = c;
+    for (int32_t at = tid; at < n; at += kRowThreads) {
+        const Candidate c = s.held[at];
+        if (c.x >= least) a.candidates[static_cast<int64_t>(blockIdx.x) * a.room + atomicAdd(&s.nheld, 1)] = c;
+    }
     __syncthreads();
     if (tid == 0) {
         double sum_all = 0.0;
@@ -464,36 +488,57 @@ __device__ int32_t sort_row(const BeamArgs &a, int32_t row, float least, uint64_
     return kept;
 }
 
+// A continuation of a request: its score, and what decides between equal ones, the beam, the logit and the token in one number.
+struct Choice {
+    double total;
+    uint64_t rest;
+    __device__ __forceinline__ int32_t beam() const { return 255 - static_cast<int32_t>(rest >> 56); }
+    __device__ __forceinline__ int32_t token() const { return 0xFFFFFF - static_cast<int32_t>(rest & 0xFFFFFF); }
+    __device__ __forceinline__ float x() const { return from_ordered(static_cast<uint32_t>(rest >> 24)); }
+    __device__ __forceinline__ bool before(const Choice &o) const { return total > o.total || (total == o.total && rest > o.rest); }
+};
+__device__ __forceinline__ uint64_t rest_of(int32_t beam, float x, int32_t token) {
+    return static_cast<uint64_t>(255 - beam) << 56 | static_cast<uint64_t>(ordered(x)) << 24 | static_cast<uint64_t>(0xFFFFFF - token);
+}
+__device__ __forceinline__ uint64_t ordered_double(double x) {
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(__dadd_rn(x, 0.0)));
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+
 // How room in shared memory is divided; K beams, W warps
 struct ChooseRoom {
     double *base, *sums;      // [K]: score - log sum exp(x - top); a block's share of a sum
+    Choice *list, *sorted;    // [list_room], [kSorted]; in their place, where these are too small,
     uint64_t *best, *sorting; // [K][k], [W][sort_room]
     float *top;               // [K]
     int32_t *count;           // [K]
     uint32_t *near;           // [K]: whether the sum is wanted in 64 bits; near[K]: whether any is
+    static __host__ __device__ size_t lists(const BeamArgs &a, int warps) {
+        const size_t usual = sizeof(Choice) * (static_cast<size_t>(a.list_room) + kSorted);
+        const size_t other = sizeof(uint64_t) * (static_cast<size_t>(a.beams) * a.k + static_cast<size_t>(warps) * a.sort_room);
+        return (usual > other ? usual : other) + 15 & ~static_cast<size_t>(15);
+    }
+    static size_t bytes(const BeamArgs &a, int warps) { return lists(a, warps) + a.beams * (2 * sizeof(double) + 3 * sizeof(float)) + sizeof(float); }
     __device__ ChooseRoom(char *at, const BeamArgs &a, int warps) {
-        base = reinterpret_cast<double *>(at);
-        sums = base + a.beams;
-        best = reinterpret_cast<uint64_t *>(sums + a.beams);
+        list = reinterpret_cast<Choice *>(at);
+        sorted = list + a.list_room;
+        best = reinterpret_cast<uint64_t *>(at);
         sorting = best + static_cast<int64_t>(a.beams) * a.k;
-        top = reinterpret_cast<float *>(sorting + static_cast<int64_t>(warps) * a.sort_room);
+        base = reinterpret_cast<double *>(at + lists(a, warps));
+        sums = base + a.beams;
+        top = reinterpret_cast<float *>(sums + a.beams);
         count = reinterpret_cast<int32_t *>(top + a.beams);
         near = reinterpret_cast<uint32_t *>(count + a.beams);
     }
 };
-size_t choose_smem(const BeamArgs &a, int warps) {
-    return sizeof(double) * 2 * a.beams + sizeof(uint64_t) * (static_cast<size_t>(a.beams) * a.k + static_cast<size_t>(warps) * a.sort_room) +
-           sizeof(float) * (3 * static_cast<size_t>(a.beams) + 1);
-}
 
 // x against the row's largest, so that logits of any size leave the scores their digits; where that is infinite, those that are share the row.
-__device__ __forceinline__ double entering(uint64_t key, float top) {
-    const float x = from_ordered(static_cast<uint32_t>(key >> 32));
+__device__ __forceinline__ double entering(float x, float top) {
     if (top < CUDART_INF_F) return static_cast<double>(x) - top;
     return x == CUDART_INF_F ? 0.0 : -CUDART_INF;
 }
 
-// One warp: the best of the rows' heads, k times.  doubt: marks rows whose heads are too close for sums in 32 bits.
+// One warp: the best of the heads of the rows' sorted candidates, k times.  doubt: marks rows whose heads are too close for sums in 32 bits.
 __device__ bool take_best(const BeamArgs &a, const ChooseRoom &r, int32_t request, bool doubt) {
     const int lane = threadIdx.x % 32;
     const int32_t mine = (a.beams - lane + 31) / 32;  // rows lane, lane + 32, ...: their heads, a byte each
@@ -503,7 +548,7 @@ __device__ bool take_best(const BeamArgs &a, const ChooseRoom &r, int32_t reques
     int32_t *const tokens = a.tokens + static_cast<int64_t>(request) * a.k, *const parents = a.parents + static_cast<int64_t>(request) * a.k;
     const auto head_of = [&](int32_t j) {
         const int32_t row = lane + 32 * j, at = static_cast<int32_t>(heads >> 8 * j & 0xFF);
-        return at < r.count[row] ? r.base[row] + entering(r.best[row * a.k + at], r.top[row]) : -CUDART_INF;
+        return at < r.count[row] ? r.base[row] + entering(from_ordered(static_cast<uint32_t>(r.best[row * a.k + at] >> 32)), r.top[row]) : -CUDART_INF;
     };
     for (int32_t i = 0; i < a.k; ++i) {
         double best = -CUDART_INF;
@@ -546,16 +591,106 @@ __device__ bool take_best(const BeamArgs &a, const ChooseRoom &r, int32_t reques
     return doubtful;
 }
 
+// The block puts n continuations in order: each counts those in front of it.
+__device__ __forceinline__ void sort_list(const Choice *list, Choice *sorted, int32_t n) {
+    for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
+        const Choice mine = list[i];
+        int32_t place = 0;
+        for (int32_t j = 0; j < n; ++j) place += list[j].before(mine);
+        sorted[place] = mine;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void write_sorted(const BeamArgs &a, const Choice *sorted, int32_t request, int32_t n) {
+    for (int32_t i = threadIdx.x; i < a.k; i += blockDim.x) {
+        const int64_t at = static_cast<int64_t>(request) * a.k + i;
+        const bool there = i < n;
+        const Choice c = sorted[there ? i : 0];
+        a.out[at] = there ? static_cast<float>(c.total) : -CUDART_INF_F;
+        a.tokens[at] = there ? c.token() : -1;
+        a.parents[at] = there ? request * a.beams + c.beam() : -1;
+    }
+}
+// The continuations that may be among the best, in *list; returns how many there are, more than `kSorted` if that is no use.  A bound that k of
+// one row reach drops most of them while they are read, the k-th largest of what is left (by the upper half of its bits) nearly all of the others; both with
+// room for what 32-bit sums are off.  *sorted is as large as kSorted.
+__device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const ChooseRoom &r, int32_t request, int32_t *counts, Choice **list, Choice **sorted) {
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+    double bound = -CUDART_INF;
+    for (int32_t i = lane; i < a.beams; i += 32) bound = fmax(bound, r.sums[i]);
+#pragma unroll
+    for (int d = 16; d; d /= 2) bound = fmax(bound, __shfl_xor_sync(~0u, bound, d));
+    bound -= 2.0 * kRowError;
+    const int32_t pairs = a.beams * a.nparts;
+    const int64_t first = static_cast<int64_t>(request) * pairs;
+    for (int32_t p0 = warp; p0 < pairs; p0 += 32 * warps) {
+        const int32_t mine = p0 + lane * warps;
+        int32_t count = 0;
+        if (mine < pairs) {
+            const Part *const part = a.parts + first + mine;
+            const int32_t beam = mine / a.nparts;
+            const float top = __ldcg(&part->top);
+            count = __ldcg(&part->count);
+            if (!(r.base[beam] + entering(top, r.top[beam]) >= bound)) count = 0;
+        }
+        for (uint32_t left = __ballot_sync(~0u, count > 0); left; left &= left - 1) {
+            const int from = __ffs(left) - 1, pair = p0 + from * warps, beam = pair / a.nparts;
+            const int32_t n = __shfl_sync(~0u, count, from);
+            const float2 *const candidates = reinterpret_cast<const float2 *>(a.candidates + (first + pair) * a.room);
+            for (int32_t i = lane; i < n; i += 32) {
+                const float2 c = __ldcg(candidates + i);
+                const double total = r.base[beam] + entering(c.x, r.top[beam]);
+                if (total >= bound && total > -CUDART_INF) {
+                    const int32_t at = atomicAdd(&counts[0], 1);
+                    if (at < a.list_room) r.list[at] = Choice{total, rest_of(beam, c.x, __float_as_int(c.y))};
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int32_t n = counts[0];
+    if (n > a.list_room) return INT32_MAX;
+    if (n <= 2 * a.k + 32) return n;
+    uint32_t least = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t want = least | 1u << bit;
+        int32_t c = 0;
+        for (int32_t i = threadIdx.x; i < n; i += blockDim.x) c += ordered_double(r.list[i].total) >> 32 >= want;
+        c = __reduce_add_sync(~0u, c);
+        int32_t *const sum = counts + 1 + bit % 3;  // one is filled, one is read, one is set back
+        if (lane == 0 && c) atomicAdd(sum, c);
+        __syncthreads();
+        if (*sum >= a.k) least = want;
+        if (threadIdx.x == 0) counts[1 + (bit + 1) % 3] = 0;
+    }
+    const uint64_t u = static_cast<uint64_t>(least) << 32;
+    bound = __longlong_as_double(static_cast<long long>(u >> 63 ? u & ~(1ull << 63) : ~u)) - 2.0 * kRowError;
+    if (threadIdx.x == 0) counts[0] = 0;
+    __syncthreads();
+    for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
+        if (r.list[i].total < bound) continue;
+        const int32_t at = atomicAdd(&counts[0], 1);
+        if (at < kSorted) r.sorted[at] = r.list[i];
+    }
+    __syncthreads();
+    *list = r.sorted, *sorted = r.list;
+    return counts[0];
+}
+
 // A cluster a request.  Its first block chooses; the others wait to be asked for sums in 64 bits.
 template <int DT>
-__global__ void __cluster_dims__(kChooseBlocks, 1, 1) choose_kernel(const __grid_constant__ BeamArgs a) {
+__global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostChooseWarps * 32) choose_kernel(const __grid_constant__ BeamArgs a) {
     extern __shared__ __align__(16) char room[];
-    __shared__ double warps_sums[32];
+    __shared__ double warps_sums[16];
+    __shared__ int32_t counts[4];
     const int rank = choose_rank(), lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const int32_t request = blockIdx.x / kChooseBlocks;
     const ChooseRoom r(room, a, warps);
+    Choice *list = r.list, *sorted = r.sorted;
+    int32_t n = 0;
     if (rank == 0) {
         for (int32_t i = threadIdx.x; i <= a.beams; i += blockDim.x) r.near[i] = 0;
+        if (threadIdx.x < 4) counts[threadIdx.x] = 0;
         wait_for_launch_before();
         for (int32_t i = warp; i < a.beams; i += warps) {
             const int32_t row = request * a.beams + i;
@@ -572,15 +707,38 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) choose_kernel(const __grid
             }
 #pragma unroll
             for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-            const int32_t n = top > -CUDART_INF_F ? sort_row(a, row, least, r.sorting + warp * a.sort_room, r.best + i * a.k) : 0;
             if (lane == 0) {
+                const bool any = top > -CUDART_INF_F;
+                const double base = any ? static_cast<double>(__ldg(a.scores + row)) - log(sum) : -CUDART_INF;
                 r.top[i] = top;
-                r.count[i] = n;
-                r.base[i] = static_cast<double>(__ldg(a.scores + row)) - log(sum);
+                r.base[i] = base;
+                r.sums[i] = any && least > -CUDART_INF_F ? base + entering(least, top) : -CUDART_INF;
             }
         }
         __syncthreads();
-        if (warp == 0 && take_best(a, r, request, true) && lane == 0) r.near[a.beams] = 1;
+        n = gather_choices(a, r, request, counts, &list, &sorted);
+        if (n <= kSorted) {
+            sort_list(list, sorted, n);
+            for (int32_t i = threadIdx.x; i + 1 < n; i += blockDim.x) {
+                const Choice &p = sorted[i], &q = sorted[i + 1];
+                if (p.total - q.total <= 2.0 * kRowError && p.beam() != q.beam() && (i < a.k || sorted[a.k - 1].total - p.total <= 2.0 * kRowError))
+                    r.near[p.beam()] = r.near[q.beam()] = r.near[a.beams] = 1;
+            }
+            __syncthreads();
+            if (!r.near[a.beams]) write_sorted(a, sorted, request, n);
+        } else {  // many equal ones: row by row
+            for (int32_t i = warp; i < a.beams; i += warps) {
+                const int32_t row = request * a.beams + i;
+                float least = -CUDART_INF_F;
+                for (int32_t p = lane; p < a.nparts; p += 32) least = fmaxf(least, __ldcg(&a.parts[static_cast<int64_t>(row) * a.nparts + p].least));
+#pragma unroll
+                for (int d = 16; d; d /= 2) least = fmaxf(least, __shfl_xor_sync(~0u, least, d));
+                const int32_t found = r.top[i] > -CUDART_INF_F ? sort_row(a, row, least, r.sorting + warp * a.sort_room, r.best + i * a.k) : 0;
+                if (lane == 0) r.count[i] = found;
+            }
+            __syncthreads();
+            if (warp == 0 && take_best(a, r, request, true) && lane == 0) r.near[a.beams] = 1;
+        }
     }
     cluster_barrier();
     const bool again = word_of_block(r.near + a.beams, 0);
@@ -609,15 +767,25 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) choose_kernel(const __grid
             }
         }
         cluster_barrier();
-        if (rank == 0 && warp == 0) {
-            for (int32_t i = lane; i < a.beams; i += 32) {
+        if (rank == 0) {
+            for (int32_t i = threadIdx.x; i < a.beams; i += blockDim.x) {
                 if (!r.near[i] || r.top[i] == CUDART_INF_F) continue;
                 double sum = 0.0;
                 for (int b = 0; b < kChooseBlocks; ++b) sum += double_of_block(r.sums + i, b);
                 r.base[i] = static_cast<double>(__ldg(a.scores + static_cast<int64_t>(request) * a.beams + i)) - log(sum);
             }
-            __syncwarp();
-            take_best(a, r, request, false);
+            __syncthreads();
+            if (n > kSorted) {
+                if (warp == 0) take_best(a, r, request, false);
+            } else {
+                for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
+                    Choice &c = list[i];
+                    c.total = r.base[c.beam()] + entering(c.x(), r.top[c.beam()]);
+                }
+                __syncthreads();
+                sort_list(list, sorted, n);
+                write_sorted(a, sorted, request, n);
+            }
         }
     }
     cluster_barrier();  // nobody reads another block's memory any more
@@ -641,7 +809,7 @@ Sizes sizes_of(const cg_beam_job &j, int sms) {
     if (parts < (tiles + kTilesPerPart - 1) / kTilesPerPart) parts = (tiles + kTilesPerPart - 1) / kTilesPerPart;
     z.part_vectors = static_cast<int32_t>((tiles + parts - 1) / parts * kTileVectors);
     z.nparts = static_cast<int32_t>((vectors + z.part_vectors - 1) / z.part_vectors);
-    z.room = 4 * j.k < kRowThreads ? (4 * j.k > 64 ? 4 * j.k : 64) : kRowThreads;
+    z.room = 4 * j.k > 64 ? 4 * j.k : 64;
     z.parts_bytes = (rows * z.nparts * static_cast<int64_t>(sizeof(Part)) + 15) / 16 * 16;
     z.total = z.parts_bytes + rows * z.nparts * z.room * static_cast<int64_t>(sizeof(Candidate));
     return z;
@@ -661,9 +829,8 @@ template <int DT>
 int run(BeamArgs &a, int32_t nrequests, cudaStream_t st) {
     const int64_t blocks = static_cast<int64_t>(nrequests) * a.beams * a.nparts;
     if (blocks > INT32_MAX) return CG_E_CAPACITY;
-    int warps = 8;
-    while (warps < a.beams && warps < 32) warps *= 2;
-    const size_t smem = choose_smem(a, warps);
+    const int warps = a.beams > kChooseWarps ? kMostChooseWarps : kChooseWarps;
+    const size_t smem = ChooseRoom::bytes(a, warps);
     if (const int rc = allow_smem(choose_kernel<DT>, smem)) return rc;
     if (const int rc = launch(rows_kernel<DT>, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, false, st, a)) return rc;
     return launch(choose_kernel<DT>, dim3(static_cast<unsigned>(nrequests) * kChooseBlocks), warps * 32, smem, true, st, a);
@@ -688,9 +855,10 @@ extern "C" int cg_beam_select(const cg_beam_job *job, void *stream) {
     if (reinterpret_cast<uintptr_t>(j.workspace) % 16 || reinterpret_cast<uintptr_t>(j.logits) % (j.dtype == kLogitF32 ? 4 : 2)) return CG_E_ALIGN;
     int sort_room = 64;
     while (sort_room < 4 * j.k && sort_room < 512) sort_room *= 2;
+    const int list_room = 4 * j.beams * j.k < kSorted ? kSorted : 4 * j.beams * j.k < kMostList ? 4 * j.beams * j.k : kMostList;
     BeamArgs a{j.logits, j.scores, j.out_scores, j.tokens, j.parents, static_cast<Part *>(j.workspace),
                reinterpret_cast<Candidate *>(static_cast<char *>(j.workspace) + z.parts_bytes), j.row_stride,
-               j.beams, j.vocab, j.k, z.nparts, z.part_vectors, z.room, sort_room};
+               j.beams, j.vocab, j.k, z.nparts, z.part_vectors, z.room, list_room, sort_room};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (j.dtype == CG_F16) return run<CG_F16>(a, j.nrequests, st);
     if (j.dtype == CG_BF16) return run<CG_BF16>(a, j.nrequests, st);

@@ -36,6 +36,14 @@ decltype(&cg_append_paged) append_rows;
 decltype(&cg_gather_paged) gather_rows;
 decltype(&cg_paged_attention_workspace) attention_workspace;
 decltype(&cg_paged_attention) attention;
+decltype(&cg_pages_workspace) pages_workspace;
+decltype(&cg_copy_pages) copy_rows;
+decltype(&cg_fork_pages) fork_rows;
+decltype(&cg_free_pages) free_rows;
+decltype(&cg_extend_pages) extend_rows;
+decltype(&cg_compact_pages) compact_rows;
+decltype(&cg_beam_workspace) beam_workspace;
+decltype(&cg_beam_select) best_beams;
 
 // attribute names
 PyObject *s_cdf, *s_max_tensors_key, *s_max_tensors_value, *s_data_chunks, *s_num_heads, *s_head_size, *s_bytestream,
@@ -764,6 +772,255 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- pages that rows share, and beams ----------------------------------------------------------------
+// Whether the memory from the first to the last value of two tensors is apart; where it is not, the general path looks closer.
+bool ranges_apart(const at::Tensor &a, const at::Tensor &b) {
+    if (!a.defined() || !b.defined() || !a.numel() || !b.numel()) return true;
+    const auto reach = [](const at::Tensor &t) {
+        int64_t values = 1;
+        for (int64_t k = 0; k < t.dim(); ++k) values += (t.size(k) - 1) * t.stride(k);
+        return values * static_cast<int64_t>(t.element_size());
+    };
+    const int64_t gap = static_cast<const char *>(b.const_data_ptr()) - static_cast<const char *>(a.const_data_ptr());
+    return gap >= reach(a) || -gap >= reach(b);
+}
+bool all_apart(std::initializer_list<const at::Tensor *> written, std::initializer_list<const at::Tensor *> read) {
+    for (auto a = written.begin(); a != written.end(); ++a) {
+        for (auto b = a + 1; b != written.end(); ++b)
+            if (!ranges_apart(**a, **b)) return false;
+        for (const at::Tensor *b : read)
+            if (!ranges_apart(**a, *b)) return false;
+    }
+    return true;
+}
+int32_t *ints(const at::Tensor &t) { return static_cast<int32_t *>(t.data_ptr()); }
+at::Tensor make_ints(at::IntArrayRef shape, at::Device dev) { return make(shape, at::TensorOptions().dtype(at::kInt).device(dev)); }
+
+// table, lens, refs, status: what calls on tables have in common.  *page_size is known.
+struct Tables {
+    at::Tensor table, lens, refs, status, workspace;
+    at::Device dev{at::kCPU};
+    int64_t rows = 0, width = 0, pages = 0;
+    bool read(PyObject *a_table, PyObject *a_lens, PyObject *a_refs, PyObject *a_status) {
+        if (!plain(a_refs)) return false;
+        refs = THPVariable_Unpack(a_refs);
+        if (!refs.defined() || !refs.is_cuda() || refs.device().index() != c10::cuda::current_device()) return false;
+        dev = refs.device();
+        if (!usable(refs, at::kInt, dev) || refs.dim() != 1 || !indices_of(a_lens, dev, false, &lens) || lens.dim() != 1 ||
+            !rows_of(a_table, at::kInt, dev, 2, Use::kWritten, &table) || (a_status != Py_None && (!indices_of(a_status, dev, false, &status) || status.numel() != 1)))
+            return false;
+        rows = lens.numel(), width = table.size(1), pages = refs.numel();
+        return table.size(0) == rows && rows <= CG_MAX_REQUESTS && pages < INT32_MAX - 8;
+    }
+    bool fill(cg_pages_job *job, int64_t page_size) const {
+        if (page_size <= 0 || page_size > INT32_MAX || width > INT32_MAX / page_size) return false;
+        job->table = ints(table), job->kv_lens = ints(lens), job->refs = ints(refs), job->status = status.defined() ? ints(status) : nullptr;
+        job->table_row = table.stride(0), job->num_pages = pages;
+        job->nrows = static_cast<int32_t>(rows), job->width = static_cast<int32_t>(width), job->page_size = static_cast<int32_t>(page_size);
+        return true;
+    }
+    void with_workspace(cg_pages_job *job) {
+        const int64_t need = pages_workspace(pages);
+        workspace = make({need}, at::TensorOptions().dtype(at::kByte).device(dev));
+        job->workspace = workspace.data_ptr(), job->workspace_bytes = need;
+    }
+};
+// A cache that copies are made in.
+struct CacheOf {
+    at::Tensor k, v;
+    cg_copy_job job{};
+    bool read(PyObject *a_k, PyObject *a_v, at::Device dev, const at::Tensor &status) {
+        at::Device on(at::kCPU);
+        if (!first_of(a_k, &k, &on) || on != dev || k.dim() < 4 || k.dim() > 5 || !rows_of(a_k, k.scalar_type(), dev, k.dim(), Use::kWritten, &k) ||
+            !rows_of(a_v, k.scalar_type(), dev, k.dim(), Use::kWritten, &v) || k.sizes() != v.sizes() || !apart(k, v))
+            return false;
+        const int64_t d = k.dim(), layers = d == 5 ? k.size(0) : 1;
+        if (!k.numel() || !fits({layers, k.size(d - 3), k.size(d - 2), k.size(d - 1)})) return false;
+        job.pages_k = k.data_ptr(), job.pages_v = v.data_ptr();
+        for (int64_t i = 0; i < 4; ++i) {
+            const int64_t axis = i + d - 5;
+            job.pages_k_strides[i] = axis >= 0 && k.size(axis) > 1 ? k.stride(axis) : 0;
+            job.pages_v_strides[i] = axis >= 0 && v.size(axis) > 1 ? v.stride(axis) : 0;
+        }
+        job.status = status.defined() ? ints(status) : nullptr;
+        job.num_pages = k.size(d - 4), job.nlayers = static_cast<int32_t>(layers), job.page_size = static_cast<int32_t>(k.size(d - 3));
+        job.heads = static_cast<int32_t>(k.size(d - 2)), job.head_size = static_cast<int32_t>(k.size(d - 1));
+        return true;
+    }
+};
+// The page size and the cache, from (k, v, page size), each of which may be None.
+bool cache_and_page(PyObject *const *a, const Tables &t, CacheOf *cache, bool *given, int64_t *page_size) {
+    *given = a[0] != Py_None;
+    if (!*given) return a[1] == Py_None && small_int(a[2], page_size);
+    if (!cache->read(a[0], a[1], t.dev, t.status) || cache->job.num_pages != t.pages) return false;
+    *page_size = cache->job.page_size;
+    int64_t said;
+    return a[2] == Py_None || (small_int(a[2], &said) && said == *page_size);
+}
+int run_pages(int (*entry)(const cg_pages_job *, const cg_copy_job *, void *), const cg_pages_job &job, const cg_copy_job *copy, at::Device dev) {
+    void *stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    const WithoutGil released;
+    return entry(&job, copy, stream);
+}
+
+// copy_pages(k, v, src, dst, tokens or None, status) -> True, an error code, or None
+PyObject *copy_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor first, src, dst, tokens, status;
+    at::Device dev(at::kCPU);
+    CacheOf cache;
+    if (n != 6 || !first_of(a[0], &first, &dev) || (a[5] != Py_None && (!indices_of(a[5], dev, false, &status) || status.numel() != 1)) ||
+        !cache.read(a[0], a[1], dev, status) || !indices_of(a[2], dev, true, &src) || src.dim() != 1 || !indices_of(a[3], dev, true, &dst) ||
+        dst.scalar_type() != src.scalar_type() || dst.sizes() != src.sizes() ||
+        (a[4] != Py_None && (!indices_of(a[4], dev, false, &tokens) || tokens.sizes() != src.sizes())) || !fits({src.numel()}) ||
+        !all_apart({&cache.k}, {&src, &dst, &tokens}) || !all_apart({&cache.v}, {&src, &dst, &tokens}))
+        Py_RETURN_NONE;
+    cg_copy_job &job = cache.job;
+    job.src = src.data_ptr(), job.dst = dst.data_ptr(), job.tokens = tokens.defined() ? ints(tokens) : nullptr;
+    job.wide = src.scalar_type() == at::kLong, job.ncopies = static_cast<int32_t>(src.numel());
+    const int rc = run(copy_rows, job, dev);
+    if (rc) return PyLong_FromLong(rc);
+    wrote(cache.k), wrote(cache.v);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// fork(table, lens, parents, refs, k or None, v or None, page size or None, release, out or None, status) -> (table, lens, moves), an error code, or None
+PyObject *fork_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Tables t;
+    CacheOf cache;
+    at::Tensor parents, table, lens;
+    bool given;
+    int64_t page_size;
+    cg_pages_job job{};
+    if (n != 10 || !t.read(a[0], a[1], a[3], a[9]) || !indices_of(a[2], t.dev, true, &parents) || parents.dim() != 1 || parents.numel() > CG_MAX_REQUESTS ||
+        !cache_and_page(a + 4, t, &cache, &given, &page_size) || !t.fill(&job, page_size))
+        Py_RETURN_NONE;
+    const int64_t N = parents.numel();
+    if (a[8] != Py_None) {
+        if (!PyTuple_CheckExact(a[8]) || PyTuple_GET_SIZE(a[8]) != 2 || !rows_of(PyTuple_GET_ITEM(a[8], 0), at::kInt, t.dev, 2, Use::kWritten, &table) ||
+            table.size(0) != N || table.size(1) != t.width || !indices_of(PyTuple_GET_ITEM(a[8], 1), t.dev, false, &lens) || lens.dim() != 1 || lens.numel() != N)
+            Py_RETURN_NONE;
+    }
+    if (!all_apart({&t.refs, &table, &lens, &cache.k}, {&t.table, &t.lens, &parents}) || !all_apart({&t.refs, &table, &lens, &cache.v}, {&t.table, &t.lens, &parents}))
+        Py_RETURN_NONE;
+    if (a[8] == Py_None) table = make_ints({N, t.width}, t.dev), lens = make_ints({N}, t.dev);
+    const at::Tensor moves = make_ints({3, N}, t.dev);
+    job.which = parents.data_ptr(), job.wide = parents.scalar_type() == at::kLong, job.release = a[7] == Py_True;
+    job.new_table = ints(table), job.new_lens = ints(lens), job.moves = ints(moves), job.new_table_row = table.stride(0), job.nnew = static_cast<int32_t>(N);
+    t.with_workspace(&job);
+    const int rc = run_pages(fork_rows, job, given ? &cache.job : nullptr, t.dev);
+    if (rc) return PyLong_FromLong(rc);
+    for (const at::Tensor *x : {&t.refs, &table, &lens, &cache.k, &cache.v}) wrote(*x);
+    if (a[8] == Py_None) return Py_BuildValue("(NNN)", THPVariable_Wrap(table), THPVariable_Wrap(lens), THPVariable_Wrap(moves));
+    return Py_BuildValue("(OON)", PyTuple_GET_ITEM(a[8], 0), PyTuple_GET_ITEM(a[8], 1), THPVariable_Wrap(moves));
+    END_HANDLE_TH_ERRORS
+}
+
+// free_pages(table, lens, refs, page size, rows or None, status) -> True, an error code, or None
+PyObject *free_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Tables t;
+    at::Tensor rows;
+    int64_t page_size;
+    cg_pages_job job{};
+    if (n != 6 || !t.read(a[0], a[1], a[2], a[5]) || !small_int(a[3], &page_size) || !t.fill(&job, page_size)) Py_RETURN_NONE;
+    if (a[4] != Py_None) {
+        if (!indices_of(a[4], t.dev, true, &rows) || rows.dim() != 1 || rows.numel() > CG_MAX_REQUESTS) Py_RETURN_NONE;
+        if (!rows.numel()) Py_RETURN_TRUE;
+        job.which = rows.data_ptr(), job.wide = rows.scalar_type() == at::kLong, job.nnew = static_cast<int32_t>(rows.numel());
+    }
+    if (!all_apart({&t.refs, &t.table, &t.lens}, {&rows})) Py_RETURN_NONE;
+    const int rc = run(free_rows, job, t.dev);
+    if (rc) return PyLong_FromLong(rc);
+    for (const at::Tensor *x : {&t.refs, &t.table, &t.lens}) wrote(*x);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// extend(table, lens, refs, page size, q_starts or None, tokens or None, status) -> slots, an error code, or None
+PyObject *extend_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Tables t;
+    at::Tensor starts;
+    int64_t page_size, tokens;
+    cg_pages_job job{};
+    if (n != 7 || !t.read(a[0], a[1], a[2], a[6]) || !small_int(a[3], &page_size) || !t.fill(&job, page_size)) Py_RETURN_NONE;
+    if (a[4] == Py_None) {
+        if (a[5] != Py_None && (!small_int(a[5], &tokens) || tokens != t.rows)) Py_RETURN_NONE;
+        tokens = t.rows;
+    } else {
+        if (!small_int(a[5], &tokens) || tokens < 0 || tokens > INT32_MAX || !t.rows || !indices_of(a[4], t.dev, false, &starts) || starts.dim() != 1 ||
+            starts.numel() != t.rows + 1)
+            Py_RETURN_NONE;
+        job.q_starts = ints(starts);
+    }
+    if (!all_apart({&t.refs, &t.table, &t.lens}, {&starts})) Py_RETURN_NONE;
+    const at::Tensor slots = make({tokens}, at::TensorOptions().dtype(at::kLong).device(t.dev));
+    job.slots = static_cast<int64_t *>(slots.data_ptr()), job.ntokens = static_cast<int32_t>(tokens);
+    t.with_workspace(&job);
+    const int rc = run(extend_rows, job, t.dev);
+    if (rc) return PyLong_FromLong(rc);
+    for (const at::Tensor *x : {&t.refs, &t.table, &t.lens}) wrote(*x);
+    return THPVariable_Wrap(slots);
+    END_HANDLE_TH_ERRORS
+}
+
+// compact(table, lens, refs, k or None, v or None, page size or None, status) -> (places, moves), an error code, or None
+PyObject *compact_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Tables t;
+    CacheOf cache;
+    bool given;
+    int64_t page_size;
+    cg_pages_job job{};
+    if (n != 7 || !t.read(a[0], a[1], a[2], a[6]) || !cache_and_page(a + 3, t, &cache, &given, &page_size) || !t.fill(&job, page_size) ||
+        !all_apart({&t.refs, &t.table, &cache.k}, {&t.lens}) || !all_apart({&t.refs, &t.table, &cache.v}, {&t.lens}))
+        Py_RETURN_NONE;
+    const at::Tensor places = make_ints({t.pages}, t.dev), moves = make_ints({2, t.pages / 2}, t.dev);
+    job.places = ints(places), job.moves = ints(moves);
+    t.with_workspace(&job);
+    const int rc = run_pages(compact_rows, job, given ? &cache.job : nullptr, t.dev);
+    if (rc) return PyLong_FromLong(rc);
+    for (const at::Tensor *x : {&t.refs, &t.table, &cache.k, &cache.v}) wrote(*x);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(places), THPVariable_Wrap(moves));
+    END_HANDLE_TH_ERRORS
+}
+
+// beam_select(logits, scores, k) -> (scores, tokens, parents), an error code, or None
+PyObject *beam_select(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor logits, scores;
+    int64_t k;
+    if (n != 3 || !plain(a[0]) || !plain(a[1]) || !small_int(a[2], &k)) Py_RETURN_NONE;
+    logits = THPVariable_Unpack(a[0]), scores = THPVariable_Unpack(a[1]);
+    if (!logits.defined() || !logits.is_cuda() || logits.device().index() != c10::cuda::current_device()) Py_RETURN_NONE;
+    const at::Device dev = logits.device();
+    const at::ScalarType type = logits.scalar_type();
+    if ((!is_16bit(type) && type != at::kFloat) || !rows_of(a[0], type, dev, 2, Use::kRead, &logits) || !usable(scores, at::kFloat, dev) || scores.requires_grad() ||
+        scores.dim() != 2)
+        Py_RETURN_NONE;
+    const int64_t B = scores.size(0), K = scores.size(1), V = logits.size(1);
+    if (logits.size(0) != B * K || K <= 0 || K > CG_MAX_BEAMS || k <= 0 || k > CG_MAX_CHOICES || K * k > CG_MAX_BEAM_CHOICES || V <= 0 || V > CG_MAX_VOCAB ||
+        B > INT32_MAX)
+        Py_RETURN_NONE;
+    const at::Tensor out = make({B, k}, scores.options()), tokens = make_ints({B, k}, dev), parents = make_ints({B, k}, dev);
+    cg_beam_job job{};
+    job.logits = logits.data_ptr(), job.scores = static_cast<const float *>(scores.data_ptr());
+    job.out_scores = static_cast<float *>(out.data_ptr()), job.tokens = ints(tokens), job.parents = ints(parents);
+    job.dtype = type == at::kFloat ? CG_LOGITS_F32 : code(type), job.row_stride = logits.stride(0);
+    job.nrequests = static_cast<int32_t>(B), job.beams = static_cast<int32_t>(K), job.vocab = static_cast<int32_t>(V), job.k = static_cast<int32_t>(k);
+    const int64_t need = beam_workspace(&job);
+    if (need < 0) return PyLong_FromLongLong(need);
+    const at::Tensor workspace = make({need}, at::TensorOptions().dtype(at::kByte).device(dev));
+    job.workspace = workspace.data_ptr(), job.workspace_bytes = need;
+    const int rc = run(best_beams, job, dev);
+    if (rc) return PyLong_FromLong(rc);
+    return Py_BuildValue("(NNN)", THPVariable_Wrap(out), THPVariable_Wrap(tokens), THPVariable_Wrap(parents));
+    END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address})
 PyObject *bind(PyObject *, PyObject *addresses) {
     HANDLE_TH_ERRORS
@@ -782,6 +1039,14 @@ PyObject *bind(PyObject *, PyObject *addresses) {
     gather_rows = reinterpret_cast<decltype(gather_rows)>(address("cg_gather_paged"));
     attention_workspace = reinterpret_cast<decltype(attention_workspace)>(address("cg_paged_attention_workspace"));
     attention = reinterpret_cast<decltype(attention)>(address("cg_paged_attention"));
+    pages_workspace = reinterpret_cast<decltype(pages_workspace)>(address("cg_pages_workspace"));
+    copy_rows = reinterpret_cast<decltype(copy_rows)>(address("cg_copy_pages"));
+    fork_rows = reinterpret_cast<decltype(fork_rows)>(address("cg_fork_pages"));
+    free_rows = reinterpret_cast<decltype(free_rows)>(address("cg_free_pages"));
+    extend_rows = reinterpret_cast<decltype(extend_rows)>(address("cg_extend_pages"));
+    compact_rows = reinterpret_cast<decltype(compact_rows)>(address("cg_compact_pages"));
+    beam_workspace = reinterpret_cast<decltype(beam_workspace)>(address("cg_beam_workspace"));
+    best_beams = reinterpret_cast<decltype(best_beams)>(address("cg_beam_select"));
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -794,6 +1059,12 @@ PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
                          {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
                          {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gather)), METH_FASTCALL, nullptr},
                          {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend)), METH_FASTCALL, nullptr},
+                         {"copy_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(copy_pages)), METH_FASTCALL, nullptr},
+                         {"fork_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fork_pages)), METH_FASTCALL, nullptr},
+                         {"free_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(free_pages)), METH_FASTCALL, nullptr},
+                         {"extend_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(extend_pages)), METH_FASTCALL, nullptr},
+                         {"compact_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(compact_pages)), METH_FASTCALL, nullptr},
+                         {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(beam_select)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

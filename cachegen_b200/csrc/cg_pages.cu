@@ -16,6 +16,7 @@ namespace {
 constexpr int kClusterBlocks = 8, kClusterThreads = 512, kClusterWarps = kClusterThreads / 32;
 constexpr int kRowThreads = 256, kRowColumns = 1024;  // of a block that works on a row of a table
 constexpr int kCopyThreads = 256, kCopyVectors = 4;
+constexpr int32_t kSlotsTogether = 2 * kClusterBlocks * kClusterThreads;
 constexpr int64_t kMostPages = INT32_MAX - 8;  // a thread counts on by four
 
 struct Table {
@@ -273,12 +274,13 @@ __global__ void __launch_bounds__(kRowThreads) free_pages_kernel(const __grid_co
 struct ExtendArgs {
     Table t;
     int32_t *table, *lens, *refs, *list;
+    int32_t *firsts;        // [rows]: where a row's new tokens begin, -1 if they found no place
     const int32_t *starts;  // [rows + 1], or nullptr: a token a row
     int64_t *slots;
     int32_t ntokens;
 };
-struct Growth {  // of a row: its tokens and pages before, its new tokens (-1: they found no place) and where its pages stand in the list
-    int32_t tokens, fresh, start, asked;
+struct Growth {  // of a row: its pages before, how many it gets, and where they stand in the list
+    int32_t before, pages;
     int64_t rank;
 };
 __device__ __forceinline__ int32_t start_of(const ExtendArgs &a, int row) {
@@ -288,32 +290,53 @@ __device__ __forceinline__ int32_t start_of(const ExtendArgs &a, int row) {
     note(a.t.status, CG_S_BAD_PAGE);
     return s < 0 ? 0 : a.ntokens;
 }
-// One cluster, a row a thread for the sums; then the threads of a block share its rows.
-__global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kClusterThreads) extend_pages_kernel(const __grid_constant__ ExtendArgs a) {
+// The slot of token i, whose row is found among the starts.
+__device__ __forceinline__ int64_t slot_of(const ExtendArgs &a, int32_t i) {
+    int32_t row = i, start = i;
+    if (a.starts) {
+        int32_t lo = 0, hi = a.t.rows;  // starts[lo] <= i < starts[hi], if any are
+        if (i < __ldg(a.starts) || i >= __ldg(a.starts + hi)) return -1;  // a token of no row
+        while (hi - lo > 1) {
+            const int32_t mid = (lo + hi) / 2;
+            if (__ldg(a.starts + mid) <= i) lo = mid;
+            else hi = mid;
+        }
+        row = lo;
+        start = max(0, __ldg(a.starts + row));
+    }
+    const int32_t first = __ldcg(a.firsts + row);
+    const int64_t place = static_cast<int64_t>(first) + i - start;
+    if (first < 0 || place < first || place >= __ldcg(a.lens + row)) return -1;
+    const int32_t column = static_cast<int32_t>(place / a.t.page_size), p = __ldcg(a.t.entries + row * a.t.row + column);
+    if (p >= 0 && p < a.t.num_pages) return static_cast<int64_t>(p) * a.t.page_size + (place - static_cast<int64_t>(column) * a.t.page_size);
+    note(a.t.status, CG_S_BAD_PAGE);
+    return -1;
+}
+// One cluster, a row a thread for the sums; then the threads of a block share its rows' new pages, and (`slots_too`) all of them the tokens.
+__global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kClusterThreads) extend_pages_kernel(const __grid_constant__ ExtendArgs a, int slots_too) {
     __shared__ Sums sums;
     __shared__ Growth grown[CG_MAX_REQUESTS / kClusterBlocks];
-    wait_for_launch_before();
+    let_next_launch_start();
     const int32_t S = a.t.page_size, each = (a.t.rows + kClusterBlocks - 1) / kClusterBlocks, row0 = cluster_rank() * each;
     const int32_t row = row0 + threadIdx.x;
     const bool here = threadIdx.x < each && row < a.t.rows;
-    Growth g{0, 0, 0, 0, 0};
+    int32_t tokens = 0, asked = 0;
     int64_t wanted = 0;
+    bool fits = true;
+    Growth g{0, 0, 0};
     if (here) {
-        g.start = start_of(a, row);
-        g.asked = start_of(a, row + 1) - g.start;
-        if (g.asked < 0) {
+        asked = start_of(a, row + 1) - start_of(a, row);
+        if (asked < 0) {
             note(a.t.status, CG_S_BAD_PAGE);
-            g.asked = 0;
+            asked = 0;
         }
-        g.tokens = length_of(a.t, row);
-        g.fresh = g.asked;
-        const int64_t after = static_cast<int64_t>(g.tokens) + g.asked;
-        const int64_t pages = (after + S - 1) / S;
-        if (pages > a.t.width || after > INT32_MAX) {
+        tokens = length_of(a.t, row);
+        g.before = pages_of(tokens, S);
+        const int64_t after = static_cast<int64_t>(tokens) + asked;
+        wanted = (after + S - 1) / S - g.before;
+        if (g.before + wanted > a.t.width) {
             note(a.t.status, CG_S_BAD_PAGE);
-            g.fresh = -1;
-        } else {
-            wanted = pages - pages_of(g.tokens, S);
+            fits = false, wanted = 0;
         }
     }
     int64_t all, free;
@@ -321,43 +344,33 @@ __global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kCluste
     if (here) {
         if (wanted > 0 && g.rank + wanted > free) {
             note(a.t.status, CG_S_NO_PAGE);
-            g.fresh = -1;
+            fits = false;
         }
-        if (g.fresh > 0) a.lens[row] = g.tokens + g.fresh;
+        if (fits && asked) a.lens[row] = tokens + asked;
+        g.pages = fits ? static_cast<int32_t>(wanted) : 0;
+        a.firsts[row] = fits ? tokens : -1;
         grown[threadIdx.x] = g;
     }
     __syncthreads();
     const int32_t mine = a.t.rows - row0 < each ? a.t.rows - row0 : each;  // rows of this block, none or less behind the last
     int team = kClusterThreads;
-    while (team > 32 && team * mine > kClusterThreads) team /= 2;
+    while (team > 1 && team * mine > kClusterThreads) team /= 2;
     for (int32_t r = threadIdx.x / team; r < mine; r += kClusterThreads / team) {
         const Growth &x = grown[r];
-        const int32_t lane = threadIdx.x % team, before = pages_of(x.tokens, S);
-        int32_t *const entries = a.table + (row0 + r) * a.t.row;
-        if (x.fresh > 0) {
-            const int32_t pages = pages_of(static_cast<int64_t>(x.tokens) + x.fresh, S) - before;
-            for (int32_t j = lane; j < pages; j += team) {
-                const int32_t p = __ldcg(a.list + x.rank + j);
-                entries[before + j] = p;
-                a.refs[p] = 1;
-            }
-        }
-        for (int32_t i = lane; i < x.asked; i += team) {
-            int64_t slot = -1;
-            if (x.fresh > 0) {
-                const int64_t place = static_cast<int64_t>(x.tokens) + i;
-                const int32_t column = static_cast<int32_t>(place / S);
-                const int32_t p = column < before ? page_at(a.t, row0 + r, column) : __ldcg(a.list + x.rank + column - before);
-                if (p >= 0) slot = static_cast<int64_t>(p) * S + (place - static_cast<int64_t>(column) * S);
-            }
-            a.slots[x.start + i] = slot;
+        for (int32_t j = threadIdx.x % team; j < x.pages; j += team) {
+            const int32_t p = __ldcg(a.list + x.rank + j);
+            a.table[(row0 + r) * a.t.row + x.before + j] = p;
+            a.refs[p] = 1;
         }
     }
-    if (a.starts) {  // rows of no request
-        const int32_t first = start_of(a, 0), last = start_of(a, a.t.rows);
-        for (int32_t i = cluster_rank() * kClusterThreads + threadIdx.x; i < a.ntokens; i += kClusterBlocks * kClusterThreads)
-            if (i < first || i >= last) a.slots[i] = -1;
-    }
+    if (!slots_too) return;
+    cluster_barrier();
+    for (int32_t i = cluster_rank() * kClusterThreads + threadIdx.x; i < a.ntokens; i += kClusterBlocks * kClusterThreads) a.slots[i] = slot_of(a, i);
+}
+__global__ void __launch_bounds__(kRowThreads) slots_kernel(const __grid_constant__ ExtendArgs a) {
+    wait_for_launch_before();
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x;
+    if (i < a.ntokens) a.slots[i] = slot_of(a, static_cast<int32_t>(i));
 }
 
 // ---- compact -------------------------------------------------------------------------------------------
@@ -443,18 +456,34 @@ struct CopyArgs {
     int32_t parts, wide;
 };
 
-// A unit is a part of one page of one layer's keys or values: kCopyThreads x kCopyVectors pieces.
+// A unit is a part of one page of one layer's keys or values: of what is copied of it, so that pages of which little is copied are shared out
+// as evenly as whole ones.  The next unit's numbers are on their way while one is copied.
+struct Copy {
+    int64_t from, to;
+    int32_t tokens;
+};
+__device__ __forceinline__ Copy copy_at(const CopyArgs &a, int32_t i) {
+    if (a.wide)
+        return Copy{__ldcg(static_cast<const long long *>(a.src) + i), __ldcg(static_cast<const long long *>(a.dst) + i), a.tokens ? __ldcg(a.tokens + i) : a.page_size};
+    return Copy{__ldcg(static_cast<const int *>(a.src) + i), __ldcg(static_cast<const int *>(a.dst) + i), a.tokens ? __ldcg(a.tokens + i) : a.page_size};
+}
 template <class Piece>
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
     wait_for_launch_before();
     const int32_t ncopies = a.count ? __ldcg(a.count) : a.ncopies, each = 2 * a.nlayers * a.parts;
     const int64_t units = static_cast<int64_t>(ncopies) * each;
     constexpr int kValues = sizeof(Piece) / 2;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int32_t copy = static_cast<int32_t>(u / each), in = static_cast<int32_t>(u - static_cast<int64_t>(copy) * each);
-        const int64_t from = a.wide ? __ldcg(static_cast<const long long *>(a.src) + copy) : __ldcg(static_cast<const int *>(a.src) + copy);
-        const int64_t to = a.wide ? __ldcg(static_cast<const long long *>(a.dst) + copy) : __ldcg(static_cast<const int *>(a.dst) + copy);
-        int32_t tokens = a.tokens ? __ldcg(a.tokens + copy) : a.page_size;
+    const int32_t step = static_cast<int32_t>(gridDim.x), over = step / each, rest = step - over * each;
+    int32_t which_next = static_cast<int32_t>(blockIdx.x) / each, in_next = static_cast<int32_t>(blockIdx.x) - which_next * each;
+    Copy next{};
+    if (blockIdx.x < units) next = copy_at(a, which_next);
+    for (int64_t u = blockIdx.x; u < units; u += step) {
+        const int32_t in = in_next;
+        const int64_t from = next.from, to = next.to;
+        const int32_t tokens = next.tokens;
+        which_next += over, in_next += rest;
+        if (in_next >= each) in_next -= each, ++which_next;
+        if (u + step < units) next = copy_at(a, which_next);
         if (from < 0 || to < 0 || from >= a.num_pages || to >= a.num_pages || tokens < 0 || tokens > a.page_size) {
             const bool padding = from == -1 || to == -1;
             if (!padding && in == 0 && threadIdx.x == 0) note(a.status, CG_S_BAD_PAGE);
@@ -462,8 +491,9 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
         }
         const int32_t which = in / a.parts, part = in - which * a.parts, layer = which >> 1;
         const CopySide &s = a.sides[which & 1];
-        const int32_t pieces = tokens * a.heads * a.pieces, first = part * kCopyThreads * kCopyVectors;
-        if (first >= pieces || from == to) continue;
+        const int32_t pieces = tokens * a.heads * a.pieces, share = ((pieces + a.parts - 1) / a.parts + 7) & ~7, first = part * share;
+        const int32_t last = first + share < pieces ? first + share : pieces;  // share <= kCopyThreads * kCopyVectors
+        if (first >= last || from == to) continue;
         const int32_t run = s.runs == kWhole ? pieces : s.runs == kTokens ? a.heads * a.pieces : s.runs == kHeads ? tokens * a.pieces : a.pieces;
         const char *const src = s.data + 2 * (layer * s.layer + from * s.page);
         char *const dst = s.data + 2 * (layer * s.layer + to * s.page);
@@ -473,7 +503,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
         for (int v = 0; v < kCopyVectors; ++v) {
             const int32_t e = first + v * kCopyThreads + threadIdx.x;
             at[v] = -1;
-            if (e < pieces) {
+            if (e < last) {
                 if (s.runs == kWhole) {
                     at[v] = static_cast<int64_t>(e) * kValues;
                 } else {
@@ -529,13 +559,14 @@ int check_copy(const cg_copy_job &j) {
 
 // ---- entries -------------------------------------------------------------------------------------------
 struct Workspace {  // where its parts begin
-    int64_t writers, list, copies, total;
+    int64_t writers, list, firsts, total;
 };
 Workspace workspace_of(int64_t num_pages) {
     Workspace w{};
     w.writers = 64;  // two words of counts in front
     w.list = w.writers + 8 * num_pages;
-    w.total = w.list + 4 * num_pages;
+    w.firsts = w.list + 4 * num_pages;
+    w.total = w.firsts + 4 * CG_MAX_REQUESTS;
     return w;
 }
 
@@ -626,8 +657,15 @@ extern "C" int cg_extend_pages(const cg_pages_job *job, void *stream) {
     if (j.nrows == 0 && j.ntokens == 0) return CG_OK;
     if (j.nrows == 0) return CG_E_SHAPE;  // tokens of nobody
     const Workspace w = workspace_of(j.num_pages);
-    ExtendArgs a{table_of(j), j.table, j.kv_lens, j.refs, reinterpret_cast<int32_t *>(part_of(j, w.list)), j.q_starts, j.slots, j.ntokens};
-    return launch(extend_pages_kernel, dim3(kClusterBlocks), kClusterThreads, 0, false, static_cast<cudaStream_t>(stream), a);
+    ExtendArgs a{table_of(j), j.table, j.kv_lens, j.refs, reinterpret_cast<int32_t *>(part_of(j, w.list)), reinterpret_cast<int32_t *>(part_of(j, w.firsts)),
+                 j.q_starts, j.slots, j.ntokens};
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Slots of a few tokens a row are the cluster's work too, those of prompts a grid's.
+    const bool together = j.ntokens <= kSlotsTogether;
+    if (const int rc = launch(extend_pages_kernel, dim3(kClusterBlocks), kClusterThreads, 0, false, st, a, together ? 1 : 0)) return rc;
+    if (together) return CG_OK;
+    const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(j.ntokens) + kRowThreads - 1) / kRowThreads);
+    return launch(slots_kernel, dim3(blocks), kRowThreads, 0, true, st, a);
 }
 
 extern "C" int cg_compact_pages(const cg_pages_job *job, const cg_copy_job *copy, void *stream) {

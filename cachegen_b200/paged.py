@@ -573,6 +573,10 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     """Copies pages src[i] to pages dst[i] (int32 or int64 [n]; -1 in either: nothing) of keys and values [pages, page_size, heads, head_size],
     of every layer if they have a leading axis; with `tokens` (int32 [n]) only the first tokens[i] tokens of each.  No page is written to
     twice, or read as well: what such a page holds afterwards is not defined."""
+    done = _lib.calls().copy_pages(k_pages, v_pages, src, dst, tokens, _status_of(k_pages))
+    if done is not None:
+        _finish(done, "copy_pages")
+        return
     _check(k_pages.is_cuda, "k_pages must be a CUDA tensor")
     dev = k_pages.device
     job, _, _ = _copy_job(k_pages, v_pages, dev)
@@ -603,6 +607,9 @@ def fork_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, parents: torch.T
 
     Returns the new table and lengths, in `out` or new tensors (entries behind a row's pages are -1), and moves (int32 [3, new rows]):
     from, to and tokens of the copies, in the rows' order, -1 behind the last."""
+    done = _lib.calls().fork_pages(page_table, kv_lens, parents, refs, k_pages, v_pages, page_size, bool(release), out, _status_of(refs))
+    if done is not None:
+        return _finish(done, "fork_pages")
     S, copy = _cache_of(k_pages, v_pages, refs, page_size)
     dev = refs.device
     job = _tables(page_table, kv_lens, refs, S, dev, False)
@@ -632,6 +639,10 @@ def fork_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, parents: torch.T
 def free_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, page_size: int, rows: torch.Tensor = None) -> None:
     """Rows (int32 or int64 [n], -1: none; default: all) of page_table and kv_lens hold nothing any more: their lengths become 0, their pages'
     entries -1, and the pages are free where no other row holds them."""
+    done = _lib.calls().free_pages(page_table, kv_lens, refs, page_size, rows, _status_of(refs))
+    if done is not None:
+        _finish(done, "free_pages")
+        return
     _check(refs.is_cuda, "refs must be a CUDA tensor")
     dev = refs.device
     job = _tables(page_table, kv_lens, refs, page_size, dev, True)
@@ -656,6 +667,9 @@ def extend_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Te
 
     Returns the tokens' slots (int64 [tokens]), as append_paged and decode_paged take them: -1 for tokens of no row, and for those of a row for which
     no page is free or that its table has no room for; that row stays as it is, and check_status says so."""
+    done = _lib.calls().extend_pages(page_table, kv_lens, refs, page_size, q_starts, tokens, _status_of(refs))
+    if done is not None:
+        return _finish(done, "extend_pages")
     _check(refs.is_cuda, "refs must be a CUDA tensor")
     dev = refs.device
     job = _tables(page_table, kv_lens, refs, page_size, dev, True)
@@ -685,6 +699,9 @@ def compact_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.T
 
     Returns places (int32 [num_pages]): where each page now is, -1 if it was free, for other tables that name them; and moves
     (int32 [2, num_pages // 2]): from and to, -1 behind the last.  The pages of places n and behind are free afterwards."""
+    done = _lib.calls().compact_pages(page_table, kv_lens, refs, k_pages, v_pages, page_size, _status_of(refs))
+    if done is not None:
+        return _finish(done, "compact_pages")
     S, copy = _cache_of(k_pages, v_pages, refs, page_size)
     dev = refs.device
     job = _tables(page_table, kv_lens, refs, S, dev, True)
@@ -708,6 +725,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int = None) -> tu
     Returns scores (float32), tokens and parents (int32), all [requests, k]; parents are rows of logits, as fork_pages takes them.  Scores are
     compared in 64 bits and rounded once.  A beam whose score is not finite has no continuations, nor have logits of -infinity or NaN,
     which weigh nothing; logits of +infinity share their row's weight.  Behind a request's last continuation stand -infinity, -1 and -1."""
+    k = scores.shape[-1] if k is None and scores.dim() else k
+    done = _lib.calls().beam_select(logits, scores, k)
+    if done is not None:
+        return _finish(done, "beam_select")
     _check(logits.is_cuda, "logits must be a CUDA tensor")
     _check(logits.dtype in _LOGITS, f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
     _check(scores.dim() == 2, "scores must have shape [requests, beams]")
@@ -719,7 +740,6 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int = None) -> tu
     _check(scores.dtype == torch.float32 and scores.is_contiguous(), "scores must be float32 and contiguous")
     _check(not scores.is_neg(), "scores is a view that negates its memory")
     _check(not (scores.requires_grad and torch.is_grad_enabled()), "scores requires a gradient, which calls on a paged cache do not compute")
-    k = K if k is None else k
     _check(0 < K <= _lib.CG_MAX_BEAMS and 0 < k <= _lib.CG_MAX_CHOICES and K * k <= _lib.CG_MAX_BEAM_CHOICES,
            f"{k} of {K} beams' continuations: a call takes up to {_lib.CG_MAX_BEAMS} beams, {_lib.CG_MAX_CHOICES} choices and a product of {_lib.CG_MAX_BEAM_CHOICES}")
     _check(0 < V <= _lib.CG_MAX_VOCAB, f"a vocabulary has 1 to {_lib.CG_MAX_VOCAB} tokens, not {V}")
