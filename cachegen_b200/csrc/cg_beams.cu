@@ -2,10 +2,10 @@
 //     score[beam] + x[beam, token] - log sum_w exp x[beam, w],
 // in falling order, equal ones by beam and token.
 //
-// rows_kernel reads the logits once.  Every thread keeps its largest value and the sum of exponentials against it, and a block keeps a
-// value that k of its logits reach: only what lies above that can be among the best, and is written down with its token.  A block's first
-// tile gives the value (the k-th largest of its threads' largest), what is written down raises it.  It is bound by memory, and by the
-// instructions of the sum: per logit one conversion, half a maximum, and halves of subtraction, product, exponential's own and addition.
+// rows_kernel reads the logits once.  Every thread keeps its largest value and a sum of exponentials.  k of a part's logits reach the k-th largest of its
+// threads' largest; what does not reach it cannot be among the best, and the rest, little more than k, is read again and written down with its
+// token.  It is bound by memory, and nearly by the exponentials' unit and the instructions of the sum: per logit a conversion, half a maximum, an
+// exponential, and half a multiplication-and-addition and an addition.
 //
 // choose_kernel joins the blocks' sums of a row, sorts what they wrote down, row by row (there the order is the logits' own), and takes the
 // best of the rows' heads k times.  Which of two rows' heads is better depends on both rows' sums, and those, in 32 bits, are known to
@@ -15,24 +15,27 @@
 
 #include <math_constants.h>
 
+#include <cstddef>
+
 namespace cg {
 namespace {
 
 constexpr int kLogitF32 = CG_LOGITS_F32;
-constexpr int kRowThreads = 256, kVectors = 4;             // of rows_kernel; 16-byte vectors of a thread in a tile
+constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32, kVectors = 4;  // of rows_kernel; 16-byte vectors of a thread in a tile
 constexpr int kTileVectors = kRowThreads * kVectors;
-constexpr int kHeld = 1024, kHeldSoft = kHeld / 2;         // candidates of a block, and from how many on it sorts out
+constexpr int kRowBlocks = 4;                              // on an SM
+constexpr int kTilesPerPart = 16, kTileRoom = 512;         // a part's tiles, and how many of its threads' tiles may have candidates
 constexpr int kChooseBlocks = 8;                           // of a request's cluster
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kTilesPerPart = 4;
 constexpr int kChooseWarps = 8, kMostChooseWarps = 16, kSorted = 512, kMostList = 4096;
-// Relative error of a row's sum in 32 bits, and so the absolute one of its logarithm.  A term exp(-u) is 2 to the power of a product: the
-// difference u is off by 2^-24 of itself, the constant by 2^-26, the product by 2^-24, in all 2^-22.8 u; u on average, weighted with the terms, is
-// below 17 for up to 2^24 tokens (n terms of one size u beside the largest weigh n u exp(-u) / (1 + n exp(-u))): 2.3e-6.  The power itself: 2^-22.
-// A thread's sum is made of 8 additions to each of four accumulators and three to join them a tile, and is carried from tile to tile: at most
-// (12 + kTilesPerPart) 2^-24; from there on sums are 64 bits wide.  Moved to a new maximum it takes another product and power, kTilesPerPart + 1
-// times at most with the block's: 2^-21.4 each.  In all below 2.3e-6 + 0.3e-6 + 1.0e-6 + 1.8e-6.
-constexpr double kRowError = 6e-6;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMostPlain = 32768.0f;                     // logits up to here are summed the quick way
+// Relative error of a row's sum in 32 bits, and so the absolute one of its logarithm.  A term is 2 to the power y = x log2(e) - c, c whole and at most 9 below
+// the thread's largest: with u = top - x, y is at most 1.45 u + 9 and off by 2^-24 of itself, so the term by 2^-24 (u + 6.3).  u on average, weighted with
+// the terms, is below 17 for up to 2^24 tokens (n terms of one size u beside the largest weigh n u exp(-u) / (1 + n exp(-u))): 1.4e-6.  log2(e) is off by
+// 2^-26 of itself, which for the largest term is known and taken out; for the others 1.4e-8 u: 0.3e-6.  The power itself: 2^-22.  A thread's sum is 8 additions to each of
+// four accumulators, two to join them and one a tile, the warp's 5 more: 31 2^-24 or 1.9e-6; from there on sums are 64 bits wide, and factors between them powers of
+// two.  In all below 1.4e-6 + 0.3e-6 + 0.3e-6 + 1.9e-6.
+constexpr double kRowError = 4e-6;
 
 struct Part {  // what a block found in its part of a row
     double sum;          // of exp(x - top)
@@ -51,7 +54,11 @@ struct BeamArgs {
     Part *parts;             // [rows][nparts]
     Candidate *candidates;   // [rows][nparts][room]
     int64_t row_stride;
-    int32_t beams, vocab, k, nparts, part_vectors, room, list_room, sort_room;
+    int32_t beams, vocab, k, room, list_room, sort_room;
+    // All rows' tiles stand in one line, every block takes block_tiles of them; its tiles of one row are `cuts` parts (most of one are empty).
+    int32_t row_tiles, block_tiles, cuts, line, nparts;  // nparts: room of a row
+    __device__ __forceinline__ int32_t first_block(int32_t row) const { return row * row_tiles / block_tiles; }
+    __device__ __forceinline__ int32_t parts_of(int32_t row) const { return (((row + 1) * row_tiles - 1) / block_tiles - first_block(row) + 1) * cuts; }
 };
 
 // A float's bits in an order in which they compare as numbers without a sign; 0 and -0 are the same.
@@ -80,11 +87,13 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
+// 2 to the power of a whole number that is not positive; 0 for what a float does not hold
+__device__ __forceinline__ float whole_power2(float n) { return n < -126.0f ? 0.0f : __int_as_float((127 + static_cast<int>(n)) << 23); }
 
 template <int DT> struct Logits;
 template <> struct Logits<CG_BF16> {
@@ -133,13 +142,15 @@ template <int DT> struct Row {
     __device__ __forceinline__ int32_t vectors() const { return (shift + vocab + L::kPer - 1) / L::kPer; }
     __device__ __forceinline__ int32_t token(int32_t v, int e) const { return v * L::kPer + e - shift; }
     __device__ __forceinline__ float at(int32_t token) const { return L::to_float(data[token]); }
-    __device__ __forceinline__ uint4 load(int32_t v) const {
-        const int32_t first = v * L::kPer - shift;
+    // whether vectors from .. to - 1 lie in the row as a whole
+    __device__ __forceinline__ bool whole(int32_t from, int32_t to) const { return from * L::kPer >= shift && to * L::kPer - shift <= vocab; }
+    __device__ __forceinline__ uint4 load_whole(int32_t v) const {
         uint4 x;
-        if (first >= 0 && first <= vocab - L::kPer) {
-            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(data + first));
-            return x;
-        }
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(data + (v * L::kPer - shift)));
+        return x;
+    }
+    __device__ __forceinline__ uint4 load(int32_t v) const { return whole(v, v + 1) ? load_whole(v) : load_part(data, vocab, v * L::kPer - shift); }
+    static __device__ __noinline__ uint4 load_part(const typename L::Value *data, int32_t vocab, int32_t first) {
         uint32_t w[4];  // the row's ends
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = L::kNone;
@@ -151,8 +162,7 @@ template <int DT> struct Row {
             if (L::kPer == 4) w[e & 3] = b;
             else w[e / 2] = e & 1 ? (w[e / 2] & 0xFFFFu) | b << 16 : (w[e / 2] & 0xFFFF0000u) | b;
         }
-        x = make_uint4(w[0], w[1], w[2], w[3]);
-        return x;
+        return make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
 template <int DT> __device__ __forceinline__ float value_of(const uint4 &x, int e) {
@@ -161,243 +171,261 @@ template <int DT> __device__ __forceinline__ float value_of(const uint4 &x, int 
 }
 
 struct Shared {
-    Candidate held[kHeld];
-    int32_t nheld, sums[2][kRowThreads / 32];
-    float tops[kRowThreads / 32];
-    double parts[kRowThreads / 32];
+    float most[kTilesPerPart][kRowThreads];  // of a thread's tiles the largest logit
+    uint16_t tiles[kTileRoom];               // tile * kRowThreads + thread of those that have candidates
+    int32_t ntiles, found;
+    float tops[kRowWarps], sums[kRowWarps], bases[kRowWarps];  // a warp's sum is sums * 2 ^ bases
+    alignas(8) int32_t digits[256];
+    int32_t digit, left;
 };
-// Sum over the block; `turn` alternates.
-__device__ __forceinline__ int32_t block_sum(Shared &s, int32_t x, int turn) {
-    const int32_t w = __reduce_add_sync(~0u, x);
-    if (threadIdx.x % 32 == 0) s.sums[turn & 1][threadIdx.x / 32] = w;
+
+// What k of the block's keys, one a thread, reach, and not many more than k; 0, if there are fewer of them above that of -infinity.  One warp goes through them bit by
+// bit, from the first bit on that is not the same in all of them, to the sixteenth.  A barrier stands in front of its end.
+__device__ __forceinline__ uint32_t reached(Shared &s, uint32_t key, int32_t k) {
+    s.digits[threadIdx.x] = static_cast<int32_t>(key > ordered(-CUDART_INF_F) ? key : 0);
     __syncthreads();
-    int32_t all = 0;
+    if (threadIdx.x < 32) {
+        uint32_t mine[kRowWarps], high = 0, low = ~0u;
 #pragma unroll
-    for (int i = 0; i < kRowThreads / 32; ++i) all += s.sums[turn & 1][i];
-    return all;
+        for (int i = 0; i < kRowWarps; ++i) {
+            mine[i] = static_cast<uint32_t>(s.digits[i * 32 + threadIdx.x]);
+            high = max(high, mine[i]), low = min(low, mine[i]);
+        }
+        high = __reduce_max_sync(~0u, high), low = __reduce_min_sync(~0u, low);
+        const int first = 31 - __clz(static_cast<int>((high ^ low) | 1u << 16));
+        uint32_t least = static_cast<uint32_t>(static_cast<uint64_t>(high) >> (first + 1) << (first + 1));
+        for (int bit = first; bit >= 16; --bit) {
+            int32_t c = 0;
+#pragma unroll
+            for (int i = 0; i < kRowWarps; ++i) c += mine[i] >= (least | 1u << bit);
+            c = __reduce_add_sync(~0u, c);
+            if (c < k) continue;
+            least |= 1u << bit;
+            if (c <= k + k / 4) break;
+        }
+        if (threadIdx.x == 0) s.left = static_cast<int32_t>(least);
+    }
+    __syncthreads();
+    return static_cast<uint32_t>(s.left);
 }
 
-// Keeps exactly the k first of `n` candidates and the elements that `more` goes through, by value and then by token (or all, if there are fewer
-// than k), bit by bit: what comes last is only met where values are equal by the hundred or rise along a row.  more(f) calls f(value, token).
-// Returns what k of them reach, or -infinity.
-template <class More>
-__device__ __noinline__ float keep_first(Shared &s, int32_t n, int32_t k, More more) {
-    Candidate mine[kHeld / kRowThreads];
-#pragma unroll
-    for (int i = 0; i < kHeld / kRowThreads; ++i) {
-        const int32_t at = i * kRowThreads + threadIdx.x;
-        mine[i] = at < n ? s.held[at] : Candidate{-CUDART_INF_F, 0};
+// The digit, of those counted from `first` on in steps of `step`, at which their sum reaches s.left, which becomes what is left for it.
+__device__ __forceinline__ int32_t digit_of(Shared &s, int first, int step) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int32_t left = s.left, d = first;
+        while (left > s.digits[d] && d + step >= 0 && d + step < 256) left -= s.digits[d], d += step;
+        s.digit = d, s.left = left;
     }
-    const auto each = [&](auto f) {
-#pragma unroll
-        for (int i = 0; i < kHeld / kRowThreads; ++i)
-            if (mine[i].x > -CUDART_INF_F) f(ordered(mine[i].x), mine[i].token);
-        more([&](float x, int32_t token) {
-            if (x > -CUDART_INF_F) f(ordered(x), token);
-        });
-    };
-    int turn = 0;
-    uint32_t least = 0;  // the largest that k of them reach; 0: there are fewer
-    for (int bit = 31; bit >= 0; --bit) {
-        int32_t c = 0;
-        each([&](uint32_t key, int32_t) { c += key >= (least | 1u << bit); });
-        if (block_sum(s, c, turn++) >= k) least |= 1u << bit;
-    }
-    int32_t above = 0;
-    each([&](uint32_t key, int32_t) { above += key > least; });
-    const int32_t wanted = k - block_sum(s, above, turn++);
-    uint32_t last = 0;  // the token up to which `wanted` of the equal ones lie
-    if (least) {
-        for (int bit = 30; bit >= 0; --bit) {
-            int32_t c = 0;
-            const uint32_t below = last | 1u << bit;
-            each([&](uint32_t key, int32_t token) { c += key == least && static_cast<uint32_t>(token) < below; });
-            if (block_sum(s, c, turn++) < wanted) last |= 1u << bit;
+    __syncthreads();
+    return s.digit;
+}
+// Writes exactly the k first of a part's logits, by value and then by token: read again digit by digit.  For parts where many are
+// equal; there are more than k.
+template <int DT>
+__device__ __noinline__ float write_first(Shared &s, const Row<DT> x, int32_t from, int32_t to, int32_t k, Candidate *out) {
+    using L = Logits<DT>;
+    const auto each = [&](auto f) {  // f(key, place in the part), for all but -infinity and NaN
+        for (int32_t v = from + threadIdx.x; v < to; v += kRowThreads) {
+            const uint4 w = x.load(v);
+            for (int e = 0; e < L::kPer; ++e) {
+                const float y = value_of<DT>(w, e);
+                if (y > -CUDART_INF_F) f(ordered(y), static_cast<uint32_t>((v - from) * L::kPer + e));
+            }
         }
+    };
+    const auto count = [&](auto digit) {  // digit(key, place): -1 for those that do not count
+        __syncthreads();
+        s.digits[threadIdx.x] = 0;
+        __syncthreads();
+        int32_t same = -1, times = 0;  // neighbours are often the same
+        each([&](uint32_t key, uint32_t place) {
+            const int32_t d = digit(key, place);
+            if (d != same) {
+                if (same >= 0) atomicAdd(&s.digits[same], times);
+                same = d, times = 0;
+            }
+            ++times;
+        });
+        if (same >= 0) atomicAdd(&s.digits[same], times);
+    };
+    static_assert(kRowThreads == 256, "a digit a thread");
+    __syncthreads();
+    if (threadIdx.x == 0) s.left = k, s.found = 0;
+    uint32_t least = 0, last = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        count([&](uint32_t key, uint32_t) { return shift < 24 && (key ^ least) >> (shift + 8) ? -1 : static_cast<int32_t>(key >> shift & 255); });
+        least |= static_cast<uint32_t>(digit_of(s, 255, -1)) << shift;
     }
-    __syncthreads();
-    if (threadIdx.x == 0) s.nheld = 0;
-    __syncthreads();
-    each([&](uint32_t key, int32_t token) {
-        if (key > least || (key == least && static_cast<uint32_t>(token) <= last)) s.held[atomicAdd(&s.nheld, 1)] = Candidate{from_ordered(key), token};
+    static_assert(kTilesPerPart * kTileVectors * 8 <= 1 << 24, "three digits");
+    for (int shift = 16; shift >= 0; shift -= 8) {
+        count([&](uint32_t key, uint32_t place) { return key != least || (place ^ last) >> (shift + 8) ? -1 : static_cast<int32_t>(place >> shift & 255); });
+        last |= static_cast<uint32_t>(digit_of(s, 0, 1)) << shift;
+    }
+    each([&](uint32_t key, uint32_t place) {
+        if (key > least || (key == least && place <= last)) out[atomicAdd(&s.found, 1)] = Candidate{from_ordered(key), x.token(from, 0) + static_cast<int32_t>(place)};
     });
     __syncthreads();
-    return least ? from_ordered(least) : -CUDART_INF_F;
+    return from_ordered(least);
 }
 
-// A value that k of the block's keys reach, to 16 bits; 0 if there are fewer of them (above that of -infinity).  key(i), i < N: a thread's.
-template <int N, class Key>
-__device__ __forceinline__ uint32_t reached(int32_t k, Key key) {
-    uint32_t mine[N], least = 0;
+__device__ __forceinline__ float of_warps(const Shared &s) {
+    float high = s.tops[0];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        mine[i] = key(i);
-        if (mine[i] <= ordered(-CUDART_INF_F)) mine[i] = 0;
-    }
-    for (int bit = 31; bit >= 16; --bit) {
-        int32_t c = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) c += __syncthreads_count(mine[i] >= (least | 1u << bit));
-        if (c >= k) {
-            least |= 1u << bit;
-            if (c == k) break;
+    for (int i = 1; i < kRowWarps; ++i) high = fmaxf(high, s.tops[i]);
+    return high;
+}
+// A part's sum where there are infinities or NaN: of ones for the infinite logits, or without the NaN.  For thread 0.
+template <int DT>
+__device__ __noinline__ double sum_again(Shared &s, const Row<DT> x, int32_t from, int32_t to) {
+    const float high = of_warps(s);
+    double mine = 0.0;
+    for (int32_t v = from + threadIdx.x; v < to; v += kRowThreads) {
+        const uint4 w = x.load(v);
+        for (int e = 0; e < Logits<DT>::kPer; ++e) {
+            const float y = value_of<DT>(w, e);
+            if (high == CUDART_INF_F) mine += y == CUDART_INF_F;
+            else if (y > -CUDART_INF_F) mine += power2(__fmul_rn(__fsub_rn(y, high), kLog2e));
         }
     }
-    return least;
+    double *const parts = reinterpret_cast<double *>(s.digits);  // (no longer in use)
+    static_assert(sizeof(s.digits) >= kRowWarps * sizeof(double) && offsetof(Shared, digits) % sizeof(double) == 0, "room for the warps' sums");
+#pragma unroll
+    for (int d = 16; d; d /= 2) mine += __shfl_xor_sync(~0u, mine, d);
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) parts[threadIdx.x / 32] = mine;
+    __syncthreads();
+    double whole = 0.0;
+    for (int i = 0; i < kRowWarps; ++i) whole += parts[i];
+    return whole;
+}
+
+// Vectors from .. to - 1 of a row, by the block.
+template <int DT>
+__device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, const Row<DT> &x, int32_t from, int32_t to, Part *out, Candidate *candidates) {
+    using L = Logits<DT>;
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    float top = -CUDART_INF_F, sum = 0.0f, base = 0.0f;
+    const uint64_t scale = pair_of(kLog2e, kLog2e);
+    int32_t tile = 0;
+#pragma unroll 1
+    for (int32_t v0 = from; v0 < to; v0 += kTileVectors, ++tile) {
+        uint4 now[kVectors];
+        if (v0 + kTileVectors <= to && x.whole(v0, v0 + kTileVectors)) {
+#pragma unroll
+            for (int u = 0; u < kVectors; ++u) now[u] = x.load_whole(v0 + u * kRowThreads + tid);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kVectors; ++u) {
+                const int32_t v = v0 + u * kRowThreads + tid;
+                now[u] = v < to ? x.load(v) : make_uint4(L::kNone, L::kNone, L::kNone, L::kNone);
+            }
+        }
+        float m = L::most(reinterpret_cast<const uint32_t *>(&now[0]));
+#pragma unroll
+        for (int u = 1; u < kVectors; ++u) m = fmaxf(m, L::most(reinterpret_cast<const uint32_t *>(&now[u])));
+        s.most[tile][tid] = m;
+        top = fmaxf(top, m);
+        const float want = __fmul_rn(m, kLog2e);
+        if ((want > base + 8.0f || sum == 0.0f) && want > -CUDART_INF_F) {
+            const float next = rintf(want);
+            sum = sum == 0.0f ? 0.0f : __fmul_rn(sum, whole_power2(base - next));
+            base = next;
+        }
+        const uint64_t minus = pair_of(-base, -base);
+        uint64_t acc[2] = {pair_of(0.0f, 0.0f), pair_of(0.0f, 0.0f)};
+#pragma unroll
+        for (int u = 0; u < kVectors; ++u) {
+#pragma unroll
+            for (int i = 0; i < L::kPer / 2; ++i) {
+                const float2 two = L::two(reinterpret_cast<const uint32_t *>(&now[u]), i);
+                const float2 y = of_pair(pair_fma(pair_of(two.x, two.y), scale, minus));
+                acc[i & 1] = pair_add(acc[i & 1], pair_of(power2(y.x), power2(y.y)));
+            }
+        }
+        const float2 both = of_pair(pair_add(acc[0], acc[1]));
+        sum = __fadd_rn(sum, __fadd_rn(both.x, both.y));
+    }
+    const bool odd = (sum != sum && top > -CUDART_INF_F) || top > kMostPlain;
+    const float high = from_ordered(__reduce_max_sync(~0u, ordered(top)));
+    const float warp_base = from_ordered(__reduce_max_sync(~0u, sum > 0.0f ? ordered(base) : 0x00800000u));
+    float warp_sum = sum > 0.0f ? __fmul_rn(sum, whole_power2(base - warp_base)) : 0.0f;
+#pragma unroll
+    for (int d = 16; d; d /= 2) warp_sum = __fadd_rn(warp_sum, __shfl_xor_sync(~0u, warp_sum, d));
+    if (lane == 0) s.tops[warp] = high, s.sums[warp] = warp_sum, s.bases[warp] = warp_base;
+    if (tid == 0) s.found = s.ntiles = 0;
+    // Candidates: what reaches the k-th largest of the threads' largest, or all if fewer than k threads have one.
+    const uint32_t least_key = reached(s, ordered(top), a.k);
+    float least = least_key ? from_ordered(least_key) : -CUDART_INF_F;
+    const auto fits = [&](float y) { return y >= least && y > -CUDART_INF_F; };
+    if (fits(top)) {
+        for (int t = 0; t < tile; ++t) {
+            if (!fits(s.most[t][tid])) continue;
+            const int32_t at = atomicAdd(&s.ntiles, 1);
+            if (at < kTileRoom) s.tiles[at] = static_cast<uint16_t>(t * kRowThreads + tid);
+        }
+    }
+    const float all_top = of_warps(s);
+    const bool again = __syncthreads_or(odd) || (all_top < -kMostPlain && all_top > -CUDART_INF_F);
+    // Those tiles are read again, from the L2 cache, a vector a thread.
+    const int32_t ntiles = s.ntiles;
+    if (ntiles <= kTileRoom) {
+        for (int32_t i = tid; i < kVectors * ntiles; i += kRowThreads) {
+            const int32_t at = s.tiles[i / kVectors], v = from + at / kRowThreads * kTileVectors + i % kVectors * kRowThreads + at % kRowThreads;
+            if (v >= to) continue;
+            const uint4 w = x.load(v);
+            if (!fits(L::most(reinterpret_cast<const uint32_t *>(&w)))) continue;
+#pragma unroll
+            for (int e = 0; e < L::kPer; ++e) {
+                const float y = value_of<DT>(w, e);
+                if (!fits(y)) continue;
+                const int32_t place = atomicAdd(&s.found, 1);
+                if (place < a.room) candidates[place] = Candidate{y, x.token(v, e)};
+            }
+        }
+    }
+    __syncthreads();
+    if (s.found > a.room || ntiles > kTileRoom) least = write_first<DT>(s, x, from, to, a.k, candidates);  // (the same for all threads)
+    double whole = 0.0;
+    if (again) whole = sum_again<DT>(s, x, from, to);
+    if (tid == 0) {
+        if (!again && all_top > -CUDART_INF_F) {
+            float all_base = -CUDART_INF_F;
+#pragma unroll
+            for (int i = 0; i < kRowWarps; ++i)
+                if (s.sums[i] > 0.0f) all_base = fmaxf(all_base, s.bases[i]);
+#pragma unroll
+            for (int i = 0; i < kRowWarps; ++i)
+                if (s.sums[i] > 0.0f) whole += static_cast<double>(s.sums[i]) * whole_power2(s.bases[i] - all_base);
+            whole *= exp2(all_base - static_cast<double>(kLog2e) * all_top);
+        }
+        *out = Part{whole, all_top, least, s.found, 0};
+    }
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(const __grid_constant__ BeamArgs a) {
-    using L = Logits<DT>;
+__global__ void __launch_bounds__(kRowThreads, kRowBlocks) rows_kernel(const __grid_constant__ BeamArgs a) {
     __shared__ Shared s;
-    const int32_t row = blockIdx.x / a.nparts, part = blockIdx.x - row * a.nparts, tid = threadIdx.x, k = a.k;
     let_next_launch_start();
-    Part *const out = a.parts + blockIdx.x;
-    const float score = __ldg(a.scores + row);
-    if (!(fabsf(score) < CUDART_INF_F)) {  // a beam that has not begun
-        if (tid == 0) *out = Part{0.0, -CUDART_INF_F, -CUDART_INF_F, 0, 0};
-        return;
-    }
-    const Row<DT> x(a, row);
-    const int32_t all = x.vectors(), from = min(all, part * a.part_vectors), to = min(all, from + a.part_vectors);
-    if (tid == 0) s.nheld = 0;
-    float top = -CUDART_INF_F, sum = 0.0f, least = -CUDART_INF_F;
-    int32_t n = 0;
-    const uint64_t scale = pair_of(kLog2e, kLog2e);
-    uint4 next[kVectors];
-    const auto fetch = [&](int32_t v0) {
-#pragma unroll
-        for (int u = 0; u < kVectors; ++u) {
-            const int32_t v = v0 + u * kRowThreads + tid;
-            next[u] = v < to ? x.load(v) : make_uint4(L::kNone, L::kNone, L::kNone, L::kNone);
+    int32_t at = static_cast<int32_t>(blockIdx.x) * a.block_tiles, row = at / a.row_tiles, cut = 0;
+    const int32_t end = min(a.line, at + a.block_tiles);
+    while (at < end) {
+        const int32_t first = row * a.row_tiles, row_end = min(end, first + a.row_tiles), to = min(row_end, at + kTilesPerPart);
+        const int64_t part = static_cast<int64_t>(row) * a.nparts + (static_cast<int32_t>(blockIdx.x) - a.first_block(row)) * a.cuts + cut;
+        const bool begun = fabsf(__ldg(a.scores + row)) < CUDART_INF_F;  // NaN has not
+        if (begun) {
+            const Row<DT> x(a, row);
+            do_part<DT>(a, s, x, (at - first) * kTileVectors, min(x.vectors(), (to - first) * kTileVectors), a.parts + part, a.candidates + part * a.room);
+        } else if (threadIdx.x == 0) {
+            a.parts[part] = Part{0.0, -CUDART_INF_F, -CUDART_INF_F, 0, 0};
         }
-    };
-    fetch(from);
-    for (int32_t v0 = from; v0 < to; v0 += kTileVectors) {
-        uint4 now[kVectors];
-        float most[kVectors];
-#pragma unroll
-        for (int u = 0; u < kVectors; ++u) now[u] = next[u];
-        if (v0 + kTileVectors < to) fetch(v0 + kTileVectors);
-#pragma unroll
-        for (int u = 0; u < kVectors; ++u) most[u] = L::most(reinterpret_cast<const uint32_t *>(&now[u]));
-        const float tile = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-        const float higher = fmaxf(top, tile);
-        if (higher > -CUDART_INF_F) {
-            const uint64_t minus = pair_of(-higher, -higher);
-            uint64_t acc[2] = {pair_of(__fmul_rn(sum, power2(__fmul_rn(__fsub_rn(top, higher), kLog2e))), 0.0f), pair_of(0.0f, 0.0f)};
-#pragma unroll
-            for (int u = 0; u < kVectors; ++u) {
-#pragma unroll
-                for (int i = 0; i < L::kPer / 2; ++i) {
-                    const float2 two = L::two(reinterpret_cast<const uint32_t *>(&now[u]), i);
-                    const float2 y = of_pair(pair_mul(pair_add(pair_of(two.x, two.y), minus), scale));
-                    acc[i & 1] = pair_add(acc[i & 1], pair_of(power2(y.x), power2(y.y)));
-                }
-            }
-            const float2 both = of_pair(pair_add(acc[0], acc[1]));
-            sum = __fadd_rn(both.x, both.y);
-            top = higher;
+        at = to, ++cut;
+        if (at == row_end) {
+            if (threadIdx.x == 0)
+                for (int32_t i = 1; cut + i <= a.cuts; ++i) a.parts[part + i] = Part{0.0, -CUDART_INF_F, -CUDART_INF_F, 0, 0};
+            ++row, cut = 0;
         }
-        // candidates: of the first tile what reaches the k-th largest of the threads' largest, of the others what lies above what k logits
-        // in front of it reach
-        const bool first = v0 == from;
-        if (first) {
-            const uint32_t key = reached<1>(k, [&](int) { return ordered(tile); });
-            least = key ? from_ordered(key) : -CUDART_INF_F;
-        }
-        const auto above = [&](float y) { return first ? y >= least && y > -CUDART_INF_F : y > least; };
-        const bool any = above(tile);
-        if (any) {
-#pragma unroll
-            for (int u = 0; u < kVectors; ++u) {
-                if (!above(most[u])) continue;
-#pragma unroll
-                for (int e = 0; e < L::kPer; ++e) {
-                    const float y = value_of<DT>(now[u], e);
-                    if (above(y)) {
-                        const int32_t at = atomicAdd(&s.nheld, 1);
-                        if (at < kHeld) s.held[at] = Candidate{y, x.token(v0 + u * kRowThreads + tid, e)};
-                    }
-                }
-            }
-        }
-        if (__syncthreads_or(any)) {
-            const int32_t found = s.nheld;
-            if (found > kHeld) {  // what was held in front of this tile is whole
-                uint4 copy[kVectors];  // (what is handed on by address would never be in registers)
-#pragma unroll
-                for (int u = 0; u < kVectors; ++u) copy[u] = now[u];
-                const int32_t token0 = x.token(v0 + tid, 0);
-                least = keep_first(s, n, k, [&](auto f) {
-#pragma unroll
-                    for (int u = 0; u < kVectors; ++u)
-#pragma unroll
-                        for (int e = 0; e < L::kPer; ++e) f(value_of<DT>(copy[u], e), token0 + u * kRowThreads * L::kPer + e);
-                });
-            } else if (found > kHeldSoft) {
-                least = keep_first(s, found, k, [](auto) {});
-            }
-            n = found > kHeldSoft ? s.nheld : found;
-            __syncthreads();
-        }
-    }
-    // raised by what is held, or cut to k
-    if (n > k) {
-        const uint32_t key = reached<kHeldSoft / kRowThreads>(k, [&](int i) {
-            const int32_t at = i * kRowThreads + tid;
-            return at < n ? ordered(s.held[at].x) : 0u;
-        });
-        if (key) least = fmaxf(least, from_ordered(key));
-        int32_t left = 0;
-#pragma unroll
-        for (int i = 0; i < kHeldSoft / kRowThreads; ++i) {
-            const int32_t at = i * kRowThreads + tid;
-            left += __syncthreads_count(at < n && s.held[at].x >= least);
-        }
-        if (left > a.room) {  // equal ones
-            least = keep_first(s, n, k, [](auto) {});
-            n = s.nheld;
-        }
-    }
-    // the block's sum
-    const int lane = tid % 32, warp = tid / 32;
-    float high = top;
-#pragma unroll
-    for (int d = 16; d; d /= 2) high = fmaxf(high, __shfl_xor_sync(~0u, high, d));
-    if (lane == 0) s.tops[warp] = high;
-    const bool odd = sum != sum || top == CUDART_INF_F;  // NaN or infinity among the logits
-    const bool again = __syncthreads_or(odd);
-#pragma unroll
-    for (int i = 0; i < kRowThreads / 32; ++i) high = fmaxf(high, s.tops[i]);
-    double mine = 0.0;
-    if (again) {
-        for (int32_t v = from + tid; v < to; v += kRowThreads) {
-            for (int e = 0; e < L::kPer; ++e) {
-                const int32_t t = x.token(v, e);
-                if (t < 0 || t >= a.vocab) continue;
-                const float y = x.at(t);
-                if (high == CUDART_INF_F) mine += y == CUDART_INF_F;
-                else if (y > -CUDART_INF_F) mine += power2(__fmul_rn(__fsub_rn(y, high), kLog2e));
-            }
-        }
-    } else if (high > -CUDART_INF_F) {
-        mine = __fmul_rn(sum, power2(__fmul_rn(__fsub_rn(top, high), kLog2e)));
-    }
-#pragma unroll
-    for (int d = 16; d; d /= 2) mine += __shfl_xor_sync(~0u, mine, d);
-    if (lane == 0) s.parts[warp] = mine;
-    if (tid == 0) s.nheld = 0;
-    __syncthreads();
-    for (int32_t at = tid; at < n; at += kRowThreads) {
-        const Candidate c = s.held[at];
-        if (c.x >= least) a.candidates[static_cast<int64_t>(blockIdx.x) * a.room + atomicAdd(&s.nheld, 1)] = c;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        double sum_all = 0.0;
-        for (int i = 0; i < kRowThreads / 32; ++i) sum_all += s.parts[i];
-        *out = Part{sum_all, high, least, s.nheld, 0};
+        if (at < end) __syncthreads();  // (what the block has in common is written to again)
     }
 }
 
@@ -435,7 +463,7 @@ __device__ int32_t sort_row(const BeamArgs &a, int32_t row, float least, uint64_
     const Part *const parts = a.parts + static_cast<int64_t>(row) * a.nparts;
     const Candidate *const candidates = a.candidates + static_cast<int64_t>(row) * a.nparts * a.room;
     const auto each = [&](auto f) {  // f(whether there is one, its key), by all lanes together
-        for (int32_t p = 0; p < a.nparts; ++p) {
+        for (int32_t p = 0; p < a.parts_of(row); ++p) {
             const int32_t count = __ldcg(&parts[p].count);
             for (int32_t i0 = 0; i0 < count; i0 += 32) {
                 Candidate c{-CUDART_INF_F, 0};
@@ -626,9 +654,9 @@ __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const Choos
     for (int32_t p0 = warp; p0 < pairs; p0 += 32 * warps) {
         const int32_t mine = p0 + lane * warps;
         int32_t count = 0;
-        if (mine < pairs) {
+        const int32_t beam = mine / a.nparts;
+        if (mine < pairs && mine - beam * a.nparts < a.parts_of(request * a.beams + beam)) {
             const Part *const part = a.parts + first + mine;
-            const int32_t beam = mine / a.nparts;
             const float top = __ldcg(&part->top);
             count = __ldcg(&part->count);
             if (!(r.base[beam] + entering(top, r.top[beam]) >= bound)) count = 0;
@@ -695,12 +723,13 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
         for (int32_t i = warp; i < a.beams; i += warps) {
             const int32_t row = request * a.beams + i;
             const Part *const parts = a.parts + static_cast<int64_t>(row) * a.nparts;
+            const int32_t nparts = a.parts_of(row);
             float top = -CUDART_INF_F, least = -CUDART_INF_F;
-            for (int32_t p = lane; p < a.nparts; p += 32) top = fmaxf(top, __ldcg(&parts[p].top)), least = fmaxf(least, __ldcg(&parts[p].least));
+            for (int32_t p = lane; p < nparts; p += 32) top = fmaxf(top, __ldcg(&parts[p].top)), least = fmaxf(least, __ldcg(&parts[p].least));
 #pragma unroll
             for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d)), least = fmaxf(least, __shfl_xor_sync(~0u, least, d));
             double sum = 0.0;
-            for (int32_t p = lane; p < a.nparts; p += 32) {
+            for (int32_t p = lane; p < nparts; p += 32) {
                 const float high = __ldcg(&parts[p].top);
                 if (high == top) sum += __ldcg(&parts[p].sum);
                 else if (high > -CUDART_INF_F && top < CUDART_INF_F) sum += __ldcg(&parts[p].sum) * exp(static_cast<double>(high) - top);
@@ -730,7 +759,7 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
             for (int32_t i = warp; i < a.beams; i += warps) {
                 const int32_t row = request * a.beams + i;
                 float least = -CUDART_INF_F;
-                for (int32_t p = lane; p < a.nparts; p += 32) least = fmaxf(least, __ldcg(&a.parts[static_cast<int64_t>(row) * a.nparts + p].least));
+                for (int32_t p = lane; p < a.parts_of(row); p += 32) least = fmaxf(least, __ldcg(&a.parts[static_cast<int64_t>(row) * a.nparts + p].least));
 #pragma unroll
                 for (int d = 16; d; d /= 2) least = fmaxf(least, __shfl_xor_sync(~0u, least, d));
                 const int32_t found = r.top[i] > -CUDART_INF_F ? sort_row(a, row, least, r.sorting + warp * a.sort_room, r.best + i * a.k) : 0;
@@ -792,23 +821,23 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
 }
 
 struct Sizes {
-    int32_t nparts, part_vectors, room;
+    int32_t row_tiles, block_tiles, cuts, line, nparts, room;
     int64_t parts_bytes, total;
 };
-int64_t row_vectors(const cg_beam_job &j) {
-    const int per = j.dtype == kLogitF32 ? 4 : 8;
-    return (static_cast<int64_t>(j.vocab) + 2 * (per - 1)) / per;  // the row may begin inside a vector
-}
-// Parts of a row: at most four tiles long, so that a part's end is not far and the bound on the sums' errors holds; shorter as long as
-// that fills the GPU, but not below a tile.
+// A line that is longer than numbers of 32 bits has a total of -1.
 Sizes sizes_of(const cg_beam_job &j, int sms) {
     Sizes z{};
-    const int64_t vectors = row_vectors(j), tiles = (vectors + kTileVectors - 1) / kTileVectors, rows = static_cast<int64_t>(j.nrequests) * j.beams;
-    int64_t parts = (8 * static_cast<int64_t>(sms) + rows - 1) / rows;
-    if (parts > tiles) parts = tiles;
-    if (parts < (tiles + kTilesPerPart - 1) / kTilesPerPart) parts = (tiles + kTilesPerPart - 1) / kTilesPerPart;
-    z.part_vectors = static_cast<int32_t>((tiles + parts - 1) / parts * kTileVectors);
-    z.nparts = static_cast<int32_t>((vectors + z.part_vectors - 1) / z.part_vectors);
+    const int per = j.dtype == kLogitF32 ? 4 : 8;
+    const int64_t vectors = (static_cast<int64_t>(j.vocab) + 2 * (per - 1)) / per;  // a row may begin inside a vector
+    const int64_t tiles = (vectors + kTileVectors - 1) / kTileVectors, rows = static_cast<int64_t>(j.nrequests) * j.beams, line = rows * tiles;
+    const int64_t blocks = static_cast<int64_t>(sms) * kRowBlocks, each = (line + blocks - 1) / blocks;
+    if (line > INT32_MAX / 2 || each > INT32_MAX / 2) {
+        z.total = -1;
+        return z;
+    }
+    z.row_tiles = static_cast<int32_t>(tiles), z.block_tiles = static_cast<int32_t>(each), z.line = static_cast<int32_t>(line);
+    z.cuts = static_cast<int32_t>(((each < tiles ? each : tiles) + kTilesPerPart - 1) / kTilesPerPart);
+    z.nparts = static_cast<int32_t>((tiles + each - 2) / each + 1) * z.cuts;
     z.room = 4 * j.k > 64 ? 4 * j.k : 64;
     z.parts_bytes = (rows * z.nparts * static_cast<int64_t>(sizeof(Part)) + 15) / 16 * 16;
     z.total = z.parts_bytes + rows * z.nparts * z.room * static_cast<int64_t>(sizeof(Candidate));
@@ -827,8 +856,7 @@ int check_job(const cg_beam_job *job) {
 
 template <int DT>
 int run(BeamArgs &a, int32_t nrequests, cudaStream_t st) {
-    const int64_t blocks = static_cast<int64_t>(nrequests) * a.beams * a.nparts;
-    if (blocks > INT32_MAX) return CG_E_CAPACITY;
+    const int64_t blocks = (static_cast<int64_t>(a.line) + a.block_tiles - 1) / a.block_tiles;
     const int warps = a.beams > kChooseWarps ? kMostChooseWarps : kChooseWarps;
     const size_t smem = ChooseRoom::bytes(a, warps);
     if (const int rc = allow_smem(choose_kernel<DT>, smem)) return rc;
@@ -841,7 +869,9 @@ int run(BeamArgs &a, int32_t nrequests, cudaStream_t st) {
 
 extern "C" int64_t cg_beam_workspace(const cg_beam_job *job) {
     if (const int rc = cg::check_job(job)) return rc;
-    return job->nrequests ? cg::sizes_of(*job, cg::sm_count()).total : 0;
+    if (job->nrequests == 0) return 0;
+    const int64_t total = cg::sizes_of(*job, cg::sm_count()).total;
+    return total < 0 ? CG_E_CAPACITY : total;
 }
 
 extern "C" int cg_beam_select(const cg_beam_job *job, void *stream) {
@@ -851,6 +881,7 @@ extern "C" int cg_beam_select(const cg_beam_job *job, void *stream) {
     if (j.nrequests == 0) return CG_OK;
     if (!j.logits || !j.scores || !j.out_scores || !j.tokens || !j.parents) return CG_E_NULL;
     const Sizes z = sizes_of(j, sm_count());
+    if (z.total < 0) return CG_E_CAPACITY;
     if (!j.workspace || j.workspace_bytes < z.total) return CG_E_CAPACITY;
     if (reinterpret_cast<uintptr_t>(j.workspace) % 16 || reinterpret_cast<uintptr_t>(j.logits) % (j.dtype == kLogitF32 ? 4 : 2)) return CG_E_ALIGN;
     int sort_room = 64;
@@ -858,7 +889,7 @@ extern "C" int cg_beam_select(const cg_beam_job *job, void *stream) {
     const int list_room = 4 * j.beams * j.k < kSorted ? kSorted : 4 * j.beams * j.k < kMostList ? 4 * j.beams * j.k : kMostList;
     BeamArgs a{j.logits, j.scores, j.out_scores, j.tokens, j.parents, static_cast<Part *>(j.workspace),
                reinterpret_cast<Candidate *>(static_cast<char *>(j.workspace) + z.parts_bytes), j.row_stride,
-               j.beams, j.vocab, j.k, z.nparts, z.part_vectors, z.room, list_room, sort_room};
+               j.beams, j.vocab, j.k, z.room, list_room, sort_room, z.row_tiles, z.block_tiles, z.cuts, z.line, z.nparts};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (j.dtype == CG_F16) return run<CG_F16>(a, j.nrequests, st);
     if (j.dtype == CG_BF16) return run<CG_BF16>(a, j.nrequests, st);
