@@ -26,7 +26,7 @@ constexpr int kTileVectors = kRowThreads * kVectors;
 constexpr int kRowBlocks = 4;                              // on an SM
 constexpr int kTilesPerPart = 16, kTileRoom = 512;         // a part's tiles, and how many of its threads' tiles may have candidates
 constexpr int kChooseBlocks = 8;                           // of a request's cluster
-constexpr int kChooseWarps = 8, kMostChooseWarps = 16, kSorted = 512, kMostList = 4096;
+constexpr int kChooseWarps = 8, kMostChooseWarps = 16, kSorted = 512, kSortedAtOnce = 256, kMostList = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMostPlain = 32768.0f;                     // logits up to here are summed the quick way
 // Relative error of a row's sum in 32 bits, and so the absolute one of its logarithm.  A term is 2 to the power y = x log2(e) - c, c whole and at most 9 below
@@ -34,13 +34,13 @@ constexpr float kMostPlain = 32768.0f;                     // logits up to here 
 // the terms, is below 17 for up to 2^24 tokens (n terms of one size u beside the largest weigh n u exp(-u) / (1 + n exp(-u))): 1.4e-6.  log2(e) is off by
 // 2^-26 of itself, which for the largest term is known and taken out; for the others 1.4e-8 u: 0.3e-6.  The power itself: 2^-22.  A thread's sum is 8 additions to each of
 // four accumulators, two to join them and one a tile, the warp's 5 more: 31 2^-24 or 1.9e-6; from there on sums are 64 bits wide, and factors between them powers of
-// two.  In all below 1.4e-6 + 0.3e-6 + 0.3e-6 + 1.9e-6.
-constexpr double kRowError = 4e-6;
+// two.  A row's parts are joined with powers of two and a logarithm of 32 bits: 2^-22 and 2^-23.  In all below 1.4e-6 + 0.3e-6 + 0.3e-6 + 1.9e-6 + 0.4e-6.
+constexpr double kRowError = 4.5e-6;
 
-struct Part {  // what a block found in its part of a row
-    double sum;          // of exp(x - top)
-    float top, least;    // the largest logit, and one that k logits of the part reach (-infinity if there are no k)
-    int32_t count, pad;  // candidates
+struct alignas(16) Part {  // what a block found in its part of a row
+    double sum;             // of exp(x - top)
+    float top, least;       // the largest logit, and one that k logits of the part reach (-infinity if there are no k)
+    int32_t count, pad[3];  // candidates
 };
 struct Candidate {
     float x;
@@ -61,6 +61,8 @@ struct BeamArgs {
     __device__ __forceinline__ int32_t parts_of(int32_t row) const { return (((row + 1) * row_tiles - 1) / block_tiles - first_block(row) + 1) * cuts; }
 };
 
+// whether a beam with this score has begun; NaN has not
+__device__ __forceinline__ bool begun(float score) { return fabsf(score) < CUDART_INF_F; }
 // A float's bits in an order in which they compare as numbers without a sign; 0 and -0 are the same.
 __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(__fadd_rn(x, 0.0f));
@@ -102,10 +104,12 @@ template <> struct Logits<CG_BF16> {
     static constexpr uint32_t kNone = 0xFF80FF80u;  // -infinity
     static __device__ __forceinline__ float to_float(uint16_t b) { return Half16<CG_BF16>::to_float(b); }
     static __device__ __forceinline__ float2 two(const uint32_t *w, int i) { return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u)); }
-    static __device__ __forceinline__ float most(const uint32_t *w) {
-        const auto at = [&](int i) { return *reinterpret_cast<const __nv_bfloat162 *>(w + i); };
-        const __nv_bfloat162 m = __hmax2(__hmax2(at(0), at(1)), __hmax2(at(2), at(3)));
-        return fmaxf(__low2float(m), __high2float(m));
+    template <int WORDS> static __device__ __forceinline__ float most(const uint32_t *w) {
+        __nv_bfloat162 m[2] = {*reinterpret_cast<const __nv_bfloat162 *>(w), *reinterpret_cast<const __nv_bfloat162 *>(w + 1)};
+#pragma unroll
+        for (int i = 2; i < WORDS; ++i) m[i & 1] = __hmax2(m[i & 1], *reinterpret_cast<const __nv_bfloat162 *>(w + i));
+        const __nv_bfloat162 both = __hmax2(m[0], m[1]);
+        return fmaxf(__low2float(both), __high2float(both));
     }
 };
 template <> struct Logits<CG_F16> {
@@ -114,10 +118,12 @@ template <> struct Logits<CG_F16> {
     static constexpr uint32_t kNone = 0xFC00FC00u;
     static __device__ __forceinline__ float to_float(uint16_t b) { return Half16<CG_F16>::to_float(b); }
     static __device__ __forceinline__ float2 two(const uint32_t *w, int i) { return __half22float2(*reinterpret_cast<const __half2 *>(w + i)); }
-    static __device__ __forceinline__ float most(const uint32_t *w) {
-        const auto at = [&](int i) { return *reinterpret_cast<const __half2 *>(w + i); };
-        const __half2 m = __hmax2(__hmax2(at(0), at(1)), __hmax2(at(2), at(3)));
-        return fmaxf(__low2float(m), __high2float(m));
+    template <int WORDS> static __device__ __forceinline__ float most(const uint32_t *w) {
+        __half2 m[2] = {*reinterpret_cast<const __half2 *>(w), *reinterpret_cast<const __half2 *>(w + 1)};
+#pragma unroll
+        for (int i = 2; i < WORDS; ++i) m[i & 1] = __hmax2(m[i & 1], *reinterpret_cast<const __half2 *>(w + i));
+        const __half2 both = __hmax2(m[0], m[1]);
+        return fmaxf(__low2float(both), __high2float(both));
     }
 };
 template <> struct Logits<kLogitF32> {
@@ -126,8 +132,11 @@ template <> struct Logits<kLogitF32> {
     static constexpr uint32_t kNone = 0xFF800000u;
     static __device__ __forceinline__ float to_float(uint32_t b) { return __uint_as_float(b); }
     static __device__ __forceinline__ float2 two(const uint32_t *w, int i) { return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])); }
-    static __device__ __forceinline__ float most(const uint32_t *w) {
-        return fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])), fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
+    template <int WORDS> static __device__ __forceinline__ float most(const uint32_t *w) {
+        float m[2] = {__uint_as_float(w[0]), __uint_as_float(w[1])};
+#pragma unroll
+        for (int i = 2; i < WORDS; ++i) m[i & 1] = fmaxf(m[i & 1], __uint_as_float(w[i]));
+        return fmaxf(m[0], m[1]);
     }
 };
 
@@ -300,30 +309,64 @@ __device__ __noinline__ double sum_again(Shared &s, const Row<DT> x, int32_t fro
     return whole;
 }
 
-// Vectors from .. to - 1 of a row, by the block.
+// A block's tiles in the line, each asked for while the one in front of it is worked on, across the ends of rows too.
+template <int DT> struct Line {
+    using L = Logits<DT>;
+    uint4 next[kVectors];
+    const uint4 *from;   // this thread's first vector of the tile that is asked for next
+    int32_t at, end, v0;  // that tile in the line, and its first vector in its row
+    int32_t row, shift;
+    bool there;
+
+    __device__ __forceinline__ void begin_row(const BeamArgs &a) {
+        there = begun(__ldg(a.scores + row));
+        const Row<DT> x(a, row);
+        shift = x.shift;
+        from = reinterpret_cast<const uint4 *>(x.data - x.shift) + (v0 + static_cast<int32_t>(threadIdx.x));
+    }
+    __device__ __forceinline__ Line(const BeamArgs &a, int32_t first, int32_t last) : at(first), end(last), row(first / a.row_tiles) {
+        v0 = (first - row * a.row_tiles) * kTileVectors;
+        begin_row(a);
+        ask(a);
+    }
+    __device__ __forceinline__ void ask(const BeamArgs &a) {
+        if (at >= end) return;
+        if (there) {
+            if (v0 * L::kPer >= shift && (v0 + kTileVectors) * L::kPer - shift <= a.vocab) {
+#pragma unroll
+                for (int u = 0; u < kVectors; ++u)
+                    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(next[u].x), "=r"(next[u].y), "=r"(next[u].z), "=r"(next[u].w)
+                                 : "l"(from + u * kRowThreads));
+            } else {  // the row's ends, and nothing behind them
+                const Row<DT> x(a, row);
+#pragma unroll
+                for (int u = 0; u < kVectors; ++u) next[u] = x.load(v0 + u * kRowThreads + static_cast<int32_t>(threadIdx.x));
+            }
+        }
+        ++at, v0 += kTileVectors, from += kTileVectors;
+        if (at < end && at == (row + 1) * a.row_tiles) {
+            ++row, v0 = 0;
+            begin_row(a);
+        }
+    }
+};
+
+// The next `tiles` tiles of the line, vectors from .. to - 1 of a row, by the block.
 template <int DT>
-__device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, const Row<DT> &x, int32_t from, int32_t to, Part *out, Candidate *candidates) {
+__device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, Line<DT> &line, const Row<DT> &x, int32_t from, int32_t to, int32_t tiles, Part *out,
+                                        Candidate *candidates) {
     using L = Logits<DT>;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     float top = -CUDART_INF_F, sum = 0.0f, base = 0.0f;
     const uint64_t scale = pair_of(kLog2e, kLog2e);
-    int32_t tile = 0;
 #pragma unroll 1
-    for (int32_t v0 = from; v0 < to; v0 += kTileVectors, ++tile) {
+    for (int32_t tile = 0; tile < tiles; ++tile) {
         uint4 now[kVectors];
-        if (v0 + kTileVectors <= to && x.whole(v0, v0 + kTileVectors)) {
 #pragma unroll
-            for (int u = 0; u < kVectors; ++u) now[u] = x.load_whole(v0 + u * kRowThreads + tid);
-        } else {
-#pragma unroll
-            for (int u = 0; u < kVectors; ++u) {
-                const int32_t v = v0 + u * kRowThreads + tid;
-                now[u] = v < to ? x.load(v) : make_uint4(L::kNone, L::kNone, L::kNone, L::kNone);
-            }
-        }
-        float m = L::most(reinterpret_cast<const uint32_t *>(&now[0]));
-#pragma unroll
-        for (int u = 1; u < kVectors; ++u) m = fmaxf(m, L::most(reinterpret_cast<const uint32_t *>(&now[u])));
+        for (int u = 0; u < kVectors; ++u) now[u] = line.next[u];
+        line.ask(a);
+        const float m = L::template most<4 * kVectors>(reinterpret_cast<const uint32_t *>(now));
         s.most[tile][tid] = m;
         top = fmaxf(top, m);
         const float want = __fmul_rn(m, kLog2e);
@@ -359,7 +402,7 @@ __device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, const Row<
     float least = least_key ? from_ordered(least_key) : -CUDART_INF_F;
     const auto fits = [&](float y) { return y >= least && y > -CUDART_INF_F; };
     if (fits(top)) {
-        for (int t = 0; t < tile; ++t) {
+        for (int t = 0; t < tiles; ++t) {
             if (!fits(s.most[t][tid])) continue;
             const int32_t at = atomicAdd(&s.ntiles, 1);
             if (at < kTileRoom) s.tiles[at] = static_cast<uint16_t>(t * kRowThreads + tid);
@@ -374,7 +417,7 @@ __device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, const Row<
             const int32_t at = s.tiles[i / kVectors], v = from + at / kRowThreads * kTileVectors + i % kVectors * kRowThreads + at % kRowThreads;
             if (v >= to) continue;
             const uint4 w = x.load(v);
-            if (!fits(L::most(reinterpret_cast<const uint32_t *>(&w)))) continue;
+            if (!fits(L::template most<4>(reinterpret_cast<const uint32_t *>(&w)))) continue;
 #pragma unroll
             for (int e = 0; e < L::kPer; ++e) {
                 const float y = value_of<DT>(w, e);
@@ -399,7 +442,7 @@ __device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, const Row<
                 if (s.sums[i] > 0.0f) whole += static_cast<double>(s.sums[i]) * whole_power2(s.bases[i] - all_base);
             whole *= exp2(all_base - static_cast<double>(kLog2e) * all_top);
         }
-        *out = Part{whole, all_top, least, s.found, 0};
+        *out = Part{whole, all_top, least, s.found, {}};
     }
 }
 
@@ -409,20 +452,22 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) rows_kernel(const __g
     let_next_launch_start();
     int32_t at = static_cast<int32_t>(blockIdx.x) * a.block_tiles, row = at / a.row_tiles, cut = 0;
     const int32_t end = min(a.line, at + a.block_tiles);
+    Line<DT> line(a, at, end);
     while (at < end) {
         const int32_t first = row * a.row_tiles, row_end = min(end, first + a.row_tiles), to = min(row_end, at + kTilesPerPart);
         const int64_t part = static_cast<int64_t>(row) * a.nparts + (static_cast<int32_t>(blockIdx.x) - a.first_block(row)) * a.cuts + cut;
-        const bool begun = fabsf(__ldg(a.scores + row)) < CUDART_INF_F;  // NaN has not
-        if (begun) {
+        if (begun(__ldg(a.scores + row))) {
             const Row<DT> x(a, row);
-            do_part<DT>(a, s, x, (at - first) * kTileVectors, min(x.vectors(), (to - first) * kTileVectors), a.parts + part, a.candidates + part * a.room);
-        } else if (threadIdx.x == 0) {
-            a.parts[part] = Part{0.0, -CUDART_INF_F, -CUDART_INF_F, 0, 0};
+            do_part<DT>(a, s, line, x, (at - first) * kTileVectors, min(x.vectors(), (to - first) * kTileVectors), to - at, a.parts + part,
+                        a.candidates + part * a.room);
+        } else {
+            for (int32_t i = at; i < to; ++i) line.ask(a);  // (nothing of these has been asked for)
+            if (threadIdx.x == 0) a.parts[part] = Part{0.0, -CUDART_INF_F, -CUDART_INF_F, 0, {}};
         }
         at = to, ++cut;
         if (at == row_end) {
             if (threadIdx.x == 0)
-                for (int32_t i = 1; cut + i <= a.cuts; ++i) a.parts[part + i] = Part{0.0, -CUDART_INF_F, -CUDART_INF_F, 0, 0};
+                for (int32_t i = 1; cut + i <= a.cuts; ++i) a.parts[part + i] = Part{0.0, -CUDART_INF_F, -CUDART_INF_F, 0, {}};
             ++row, cut = 0;
         }
         if (at < end) __syncthreads();  // (what the block has in common is written to again)
@@ -452,6 +497,18 @@ __device__ __forceinline__ double double_of_block(const double *mine, int rank) 
     double v;
     asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at_block(mine, rank)) : "memory");
     return v;
+}
+
+// 2^y for y <= 0, and log(x) for x > 0, to 2^-22 and 2^-23: 32-bit functions of what is left when whole powers of two are taken out.
+__device__ __forceinline__ double quick_power2(double y) {
+    if (!(y > -1000.0)) return 0.0;
+    const double n = rint(y);
+    return static_cast<double>(power2(static_cast<float>(y - n))) * __hiloint2double((1023 + static_cast<int>(n)) << 20, 0);
+}
+__device__ __forceinline__ double quick_log(double x) {
+    const int high = __double2hiint(x);
+    const float m = static_cast<float>(__hiloint2double((high & 0xFFFFF) | 1023 << 20, __double2loint(x)));
+    return ((high >> 20) - 1023) * 0.69314718055994531 + logf(m);
 }
 
 // Candidates as one number: by value, then the lower token first.
@@ -517,13 +574,14 @@ __device__ int32_t sort_row(const BeamArgs &a, int32_t row, float least, uint64_
 }
 
 // A continuation of a request: its score, and what decides between equal ones, the beam, the logit and the token in one number.
-struct Choice {
-    double total;
+struct alignas(16) Choice {
+    uint64_t key;  // the score, in an order in which numbers without a sign compare
     uint64_t rest;
+    __device__ __forceinline__ double total() const { return __longlong_as_double(static_cast<long long>(key >> 63 ? key & ~(1ull << 63) : ~key)); }
     __device__ __forceinline__ int32_t beam() const { return 255 - static_cast<int32_t>(rest >> 56); }
     __device__ __forceinline__ int32_t token() const { return 0xFFFFFF - static_cast<int32_t>(rest & 0xFFFFFF); }
     __device__ __forceinline__ float x() const { return from_ordered(static_cast<uint32_t>(rest >> 24)); }
-    __device__ __forceinline__ bool before(const Choice &o) const { return total > o.total || (total == o.total && rest > o.rest); }
+    __device__ __forceinline__ bool before(const Choice &o) const { return key > o.key || (key == o.key && rest > o.rest); }
 };
 __device__ __forceinline__ uint64_t rest_of(int32_t beam, float x, int32_t token) {
     return static_cast<uint64_t>(255 - beam) << 56 | static_cast<uint64_t>(ordered(x)) << 24 | static_cast<uint64_t>(0xFFFFFF - token);
@@ -541,12 +599,13 @@ struct ChooseRoom {
     float *top;               // [K]
     int32_t *count;           // [K]
     uint32_t *near;           // [K]: whether the sum is wanted in 64 bits; near[K]: whether any is
+    int32_t *places;          // [kSorted]
     static __host__ __device__ size_t lists(const BeamArgs &a, int warps) {
         const size_t usual = sizeof(Choice) * (static_cast<size_t>(a.list_room) + kSorted);
         const size_t other = sizeof(uint64_t) * (static_cast<size_t>(a.beams) * a.k + static_cast<size_t>(warps) * a.sort_room);
         return (usual > other ? usual : other) + 15 & ~static_cast<size_t>(15);
     }
-    static size_t bytes(const BeamArgs &a, int warps) { return lists(a, warps) + a.beams * (2 * sizeof(double) + 3 * sizeof(float)) + sizeof(float); }
+    static size_t bytes(const BeamArgs &a, int warps) { return lists(a, warps) + a.beams * (2 * sizeof(double) + 3 * sizeof(float)) + sizeof(float) * (1 + kSorted); }
     __device__ ChooseRoom(char *at, const BeamArgs &a, int warps) {
         list = reinterpret_cast<Choice *>(at);
         sorted = list + a.list_room;
@@ -557,6 +616,7 @@ struct ChooseRoom {
         top = reinterpret_cast<float *>(sums + a.beams);
         count = reinterpret_cast<int32_t *>(top + a.beams);
         near = reinterpret_cast<uint32_t *>(count + a.beams);
+        places = reinterpret_cast<int32_t *>(near + a.beams + 1);
     }
 };
 
@@ -619,13 +679,26 @@ __device__ bool take_best(const BeamArgs &a, const ChooseRoom &r, int32_t reques
     return doubtful;
 }
 
-// The block puts n continuations in order: each counts those in front of it.
-__device__ __forceinline__ void sort_list(const Choice *list, Choice *sorted, int32_t n) {
+// The block puts n continuations in order: it counts those in front of each, which several threads share.  places: [kSorted], zeros before and after.
+__device__ __forceinline__ void sort_list(const Choice *list, Choice *sorted, int32_t n, int32_t *places) {
+    if (n == 0) return;
+    int team = 1;
+    while (2 * team * n <= static_cast<int>(blockDim.x)) team *= 2;
+    const int32_t each = blockDim.x / team;
+    for (int32_t i0 = 0; i0 < n; i0 += each) {
+        const int32_t i = i0 + threadIdx.x % each, first = threadIdx.x / each;
+        if (i < n) {
+            const Choice mine = list[i];
+            int32_t place = 0;
+#pragma unroll 4
+            for (int32_t j = first; j < n; j += team) place += list[j].before(mine);
+            atomicAdd(&places[i], place);
+        }
+    }
+    __syncthreads();
     for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const Choice mine = list[i];
-        int32_t place = 0;
-        for (int32_t j = 0; j < n; ++j) place += list[j].before(mine);
-        sorted[place] = mine;
+        sorted[places[i]] = list[i];
+        places[i] = 0;
     }
     __syncthreads();
 }
@@ -634,56 +707,68 @@ __device__ __forceinline__ void write_sorted(const BeamArgs &a, const Choice *so
         const int64_t at = static_cast<int64_t>(request) * a.k + i;
         const bool there = i < n;
         const Choice c = sorted[there ? i : 0];
-        a.out[at] = there ? static_cast<float>(c.total) : -CUDART_INF_F;
+        a.out[at] = there ? static_cast<float>(c.total()) : -CUDART_INF_F;
         a.tokens[at] = there ? c.token() : -1;
         a.parents[at] = there ? request * a.beams + c.beam() : -1;
     }
 }
 // The continuations that may be among the best, in *list; returns how many there are, more than `kSorted` if that is no use.  A bound that k of
-// one row reach drops most of them while they are read, the k-th largest of what is left (by the upper half of its bits) nearly all of the others; both with
-// room for what 32-bit sums are off.  *sorted is as large as kSorted.
+// one row reach drops most of them while they are read; where that leaves many, the k-th largest of them (by the upper half of its bits) drops nearly all of the
+// others.  Both leave room for what 32-bit sums are off.  *sorted is as large as kSorted.
 __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const ChooseRoom &r, int32_t request, int32_t *counts, Choice **list, Choice **sorted) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     double bound = -CUDART_INF;
-    for (int32_t i = lane; i < a.beams; i += 32) bound = fmax(bound, r.sums[i]);
-#pragma unroll
-    for (int d = 16; d; d /= 2) bound = fmax(bound, __shfl_xor_sync(~0u, bound, d));
+    for (int32_t i = 0; i < a.beams; ++i) bound = fmax(bound, r.sums[i]);
     bound -= 2.0 * kRowError;
-    const int32_t pairs = a.beams * a.nparts;
+    const int32_t pairs = a.beams * a.nparts;  // of a beam and a part of its row
     const int64_t first = static_cast<int64_t>(request) * pairs;
     for (int32_t p0 = warp; p0 < pairs; p0 += 32 * warps) {
-        const int32_t mine = p0 + lane * warps;
+        // of each lane's pair the candidates that may do, and those of the lanes in front
+        const int32_t mine = p0 + lane * warps, my_beam = mine / a.nparts;
         int32_t count = 0;
-        const int32_t beam = mine / a.nparts;
-        if (mine < pairs && mine - beam * a.nparts < a.parts_of(request * a.beams + beam)) {
+        if (mine < pairs && mine - my_beam * a.nparts < a.parts_of(request * a.beams + my_beam)) {
             const Part *const part = a.parts + first + mine;
-            const float top = __ldcg(&part->top);
-            count = __ldcg(&part->count);
-            if (!(r.base[beam] + entering(top, r.top[beam]) >= bound)) count = 0;
+            const float top = part->top;
+            count = part->count;
+            if (!(r.base[my_beam] + entering(top, r.top[my_beam]) >= bound)) count = 0;
         }
-        for (uint32_t left = __ballot_sync(~0u, count > 0); left; left &= left - 1) {
-            const int from = __ffs(left) - 1, pair = p0 + from * warps, beam = pair / a.nparts;
-            const int32_t n = __shfl_sync(~0u, count, from);
-            const float2 *const candidates = reinterpret_cast<const float2 *>(a.candidates + (first + pair) * a.room);
-            for (int32_t i = lane; i < n; i += 32) {
-                const float2 c = __ldcg(candidates + i);
-                const double total = r.base[beam] + entering(c.x, r.top[beam]);
-                if (total >= bound && total > -CUDART_INF) {
-                    const int32_t at = atomicAdd(&counts[0], 1);
-                    if (at < a.list_room) r.list[at] = Choice{total, rest_of(beam, c.x, __float_as_int(c.y))};
-                }
-            }
+        int32_t upto = count;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int32_t y = __shfl_up_sync(~0u, upto, d);
+            if (lane >= d) upto += y;
+        }
+        const int32_t all = __shfl_sync(~0u, upto, 31);
+#pragma unroll 2
+        for (int32_t i0 = 0; i0 < all; i0 += 32) {
+            const int32_t i = i0 + lane;
+            int owner = 0;  // the first lane whose candidates end behind i
+#pragma unroll
+            for (int d = 16; d; d /= 2)
+                if (__shfl_sync(~0u, upto, owner + d - 1) <= i) owner += d;
+            const int32_t before = __shfl_sync(~0u, upto, owner) - __shfl_sync(~0u, count, owner), pair = p0 + owner * warps;
+            const bool here = i < all;
+            const int32_t beam = here ? pair / a.nparts : 0;
+            float2 c = make_float2(-CUDART_INF_F, 0.0f);
+            if (here) c = __ldcg(reinterpret_cast<const float2 *>(a.candidates + (first + pair) * a.room + (i - before)));
+            const double total = r.base[beam] + entering(c.x, r.top[beam]);
+            const bool kept = here && total >= bound && total > -CUDART_INF;
+            const uint32_t who = __ballot_sync(~0u, kept);
+            int32_t at = 0;
+            if (lane == 0 && who) at = atomicAdd(&counts[0], __popc(who));
+            at = __shfl_sync(~0u, at, 0) + __popc(who & ((1u << lane) - 1u));
+            if (kept && at < a.list_room) r.list[at] = Choice{ordered_double(total), rest_of(beam, c.x, __float_as_int(c.y))};
         }
     }
     __syncthreads();
     const int32_t n = counts[0];
     if (n > a.list_room) return INT32_MAX;
-    if (n <= 2 * a.k + 32) return n;
+    if (n <= kSortedAtOnce) return n;
     uint32_t least = 0;
     for (int bit = 31; bit >= 0; --bit) {
         const uint32_t want = least | 1u << bit;
         int32_t c = 0;
-        for (int32_t i = threadIdx.x; i < n; i += blockDim.x) c += ordered_double(r.list[i].total) >> 32 >= want;
+        for (int32_t i = threadIdx.x; i < n; i += blockDim.x) c += r.list[i].key >> 32 >= want;
         c = __reduce_add_sync(~0u, c);
         int32_t *const sum = counts + 1 + bit % 3;  // one is filled, one is read, one is set back
         if (lane == 0 && c) atomicAdd(sum, c);
@@ -691,12 +776,11 @@ __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const Choos
         if (*sum >= a.k) least = want;
         if (threadIdx.x == 0) counts[1 + (bit + 1) % 3] = 0;
     }
-    const uint64_t u = static_cast<uint64_t>(least) << 32;
-    bound = __longlong_as_double(static_cast<long long>(u >> 63 ? u & ~(1ull << 63) : ~u)) - 2.0 * kRowError;
+    bound = Choice{static_cast<uint64_t>(least) << 32, 0}.total() - 2.0 * kRowError;
     if (threadIdx.x == 0) counts[0] = 0;
     __syncthreads();
     for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
-        if (r.list[i].total < bound) continue;
+        if (r.list[i].total() < bound) continue;
         const int32_t at = atomicAdd(&counts[0], 1);
         if (at < kSorted) r.sorted[at] = r.list[i];
     }
@@ -709,7 +793,7 @@ __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const Choos
 template <int DT>
 __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostChooseWarps * 32) choose_kernel(const __grid_constant__ BeamArgs a) {
     extern __shared__ __align__(16) char room[];
-    __shared__ double warps_sums[16];
+    __shared__ double warps_sums[kMostChooseWarps];
     __shared__ int32_t counts[4];
     const int rank = choose_rank(), lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const int32_t request = blockIdx.x / kChooseBlocks;
@@ -718,6 +802,7 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
     int32_t n = 0;
     if (rank == 0) {
         for (int32_t i = threadIdx.x; i <= a.beams; i += blockDim.x) r.near[i] = 0;
+        for (int32_t i = threadIdx.x; i < kSorted; i += blockDim.x) r.places[i] = 0;
         if (threadIdx.x < 4) counts[threadIdx.x] = 0;
         wait_for_launch_before();
         for (int32_t i = warp; i < a.beams; i += warps) {
@@ -725,20 +810,19 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
             const Part *const parts = a.parts + static_cast<int64_t>(row) * a.nparts;
             const int32_t nparts = a.parts_of(row);
             float top = -CUDART_INF_F, least = -CUDART_INF_F;
-            for (int32_t p = lane; p < nparts; p += 32) top = fmaxf(top, __ldcg(&parts[p].top)), least = fmaxf(least, __ldcg(&parts[p].least));
-#pragma unroll
-            for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d)), least = fmaxf(least, __shfl_xor_sync(~0u, least, d));
+            for (int32_t p = lane; p < nparts; p += 32) top = fmaxf(top, parts[p].top), least = fmaxf(least, parts[p].least);
+            top = from_ordered(__reduce_max_sync(~0u, ordered(top))), least = from_ordered(__reduce_max_sync(~0u, ordered(least)));
             double sum = 0.0;
             for (int32_t p = lane; p < nparts; p += 32) {
-                const float high = __ldcg(&parts[p].top);
-                if (high == top) sum += __ldcg(&parts[p].sum);
-                else if (high > -CUDART_INF_F && top < CUDART_INF_F) sum += __ldcg(&parts[p].sum) * exp(static_cast<double>(high) - top);
+                const float high = parts[p].top;
+                if (high == top) sum += parts[p].sum;
+                else if (high > -CUDART_INF_F && top < CUDART_INF_F) sum += parts[p].sum * quick_power2((static_cast<double>(high) - top) * 1.4426950408889634);
             }
 #pragma unroll
             for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
             if (lane == 0) {
                 const bool any = top > -CUDART_INF_F;
-                const double base = any ? static_cast<double>(__ldg(a.scores + row)) - log(sum) : -CUDART_INF;
+                const double base = any ? static_cast<double>(__ldg(a.scores + row)) - quick_log(sum) : -CUDART_INF;
                 r.top[i] = top;
                 r.base[i] = base;
                 r.sums[i] = any && least > -CUDART_INF_F ? base + entering(least, top) : -CUDART_INF;
@@ -747,10 +831,10 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
         __syncthreads();
         n = gather_choices(a, r, request, counts, &list, &sorted);
         if (n <= kSorted) {
-            sort_list(list, sorted, n);
+            sort_list(list, sorted, n, r.places);
             for (int32_t i = threadIdx.x; i + 1 < n; i += blockDim.x) {
                 const Choice &p = sorted[i], &q = sorted[i + 1];
-                if (p.total - q.total <= 2.0 * kRowError && p.beam() != q.beam() && (i < a.k || sorted[a.k - 1].total - p.total <= 2.0 * kRowError))
+                if (p.total() - q.total() <= 2.0 * kRowError && p.beam() != q.beam() && (i < a.k || sorted[a.k - 1].total() - p.total() <= 2.0 * kRowError))
                     r.near[p.beam()] = r.near[q.beam()] = r.near[a.beams] = 1;
             }
             __syncthreads();
@@ -809,10 +893,10 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
             } else {
                 for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
                     Choice &c = list[i];
-                    c.total = r.base[c.beam()] + entering(c.x(), r.top[c.beam()]);
+                    c.key = ordered_double(r.base[c.beam()] + entering(c.x(), r.top[c.beam()]));
                 }
                 __syncthreads();
-                sort_list(list, sorted, n);
+                sort_list(list, sorted, n, r.places);
                 write_sorted(a, sorted, request, n);
             }
         }
