@@ -24,7 +24,7 @@ constexpr int kLogitF32 = CG_LOGITS_F32;
 constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32, kVectors = 4;  // of rows_kernel; 16-byte vectors of a thread in a tile
 constexpr int kTileVectors = kRowThreads * kVectors;
 constexpr int kRowBlocks = 4;                              // on an SM
-constexpr int kTilesPerPart = 16, kTileRoom = 512;         // a part's tiles, and how many of its threads' tiles may have candidates
+constexpr int kTilesPerPart = 16, kTileRoom = 64;          // a part's tiles, and how many of a warp's lanes' tiles may have candidates
 constexpr int kChooseBlocks = 8;                           // of a request's cluster
 constexpr int kChooseWarps = 8, kMostChooseWarps = 16, kSorted = 512, kSortedAtOnce = 256, kMostList = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -33,9 +33,9 @@ constexpr float kMostPlain = 32768.0f;                     // logits up to here 
 // the thread's largest: with u = top - x, y is at most 1.45 u + 9 and off by 2^-24 of itself, so the term by 2^-24 (u + 6.3).  u on average, weighted with
 // the terms, is below 17 for up to 2^24 tokens (n terms of one size u beside the largest weigh n u exp(-u) / (1 + n exp(-u))): 1.4e-6.  log2(e) is off by
 // 2^-26 of itself, which for the largest term is known and taken out; for the others 1.4e-8 u: 0.3e-6.  The power itself: 2^-22.  A thread's sum is 8 additions to each of
-// four accumulators, two to join them and one a tile, the warp's 5 more: 31 2^-24 or 1.9e-6; from there on sums are 64 bits wide, and factors between them powers of
-// two.  A row's parts are joined with powers of two and a logarithm of 32 bits: 2^-22 and 2^-23.  In all below 1.4e-6 + 0.3e-6 + 0.3e-6 + 1.9e-6 + 0.4e-6.
-constexpr double kRowError = 4.5e-6;
+// four accumulators, two to join them and one a tile, the warp's and the block's 8 more: 34 2^-24 or 2.1e-6, with factors that are whole powers of two.  Parts' sums are
+// taken to their largest, and joined, with two powers and a logarithm of 32 bits: 2^-21 and 2^-23.  In all below 1.4e-6 + 0.3e-6 + 0.3e-6 + 2.1e-6 + 0.6e-6.
+constexpr double kRowError = 5e-6;
 
 struct alignas(16) Part {  // what a block found in its part of a row
     double sum;             // of exp(x - top)
@@ -93,6 +93,17 @@ __device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c)
     uint64_t d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
+}
+// 2^y for y < 1000, and log(x) for x > 0, to 2^-22 and 2^-23: 32-bit functions of what is left when whole powers of two are taken out.
+__device__ __forceinline__ double quick_power2(double y) {
+    if (!(y > -1000.0)) return 0.0;
+    const double n = rint(y);
+    return static_cast<double>(power2(static_cast<float>(y - n))) * __hiloint2double((1023 + static_cast<int>(n)) << 20, 0);
+}
+__device__ __forceinline__ double quick_log(double x) {
+    const int high = __double2hiint(x);
+    const float m = static_cast<float>(__hiloint2double((high & 0xFFFFF) | 1023 << 20, __double2loint(x)));
+    return ((high >> 20) - 1023) * 0.69314718055994531 + logf(m);
 }
 // 2 to the power of a whole number that is not positive; 0 for what a float does not hold
 __device__ __forceinline__ float whole_power2(float n) { return n < -126.0f ? 0.0f : __int_as_float((127 + static_cast<int>(n)) << 23); }
@@ -180,42 +191,39 @@ template <int DT> __device__ __forceinline__ float value_of(const uint4 &x, int 
 }
 
 struct Shared {
-    float most[kTilesPerPart][kRowThreads];  // of a thread's tiles the largest logit
-    uint16_t tiles[kTileRoom];               // tile * kRowThreads + thread of those that have candidates
-    int32_t ntiles, found;
+    float most[kTilesPerPart][kRowThreads + 1];  // of a thread's tiles the largest logit
+    uint4 alone[kVectors][kRowThreads];       // a part's tile that is its only one
+    uint16_t tiles[kRowWarps][kTileRoom];     // tile * 32 + lane of those of a warp that have candidates
+    int32_t found;
     float tops[kRowWarps], sums[kRowWarps], bases[kRowWarps];  // a warp's sum is sums * 2 ^ bases
     alignas(8) int32_t digits[256];
     int32_t digit, left;
+    bool crowded, again;                      // more candidates than there is room for; a sum that the quick way does not give
 };
 
-// What k of the block's keys, one a thread, reach, and not many more than k; 0, if there are fewer of them above that of -infinity.  One warp goes through them bit by
-// bit, from the first bit on that is not the same in all of them, to the sixteenth.  A barrier stands in front of its end.
-__device__ __forceinline__ uint32_t reached(Shared &s, uint32_t key, int32_t k) {
-    s.digits[threadIdx.x] = static_cast<int32_t>(key > ordered(-CUDART_INF_F) ? key : 0);
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        uint32_t mine[kRowWarps], high = 0, low = ~0u;
+// What k of the block's keys (s.digits, 0 for none) reach, and not many more than k; 0, if there are fewer of them.  For one warp, which goes
+// through them bit by bit, from the first bit on that is not the same in all of them, to the sixteenth.
+__device__ __forceinline__ uint32_t reached(const Shared &s, int32_t k) {
+    uint32_t mine[kRowWarps], high = 0, low = ~0u;
 #pragma unroll
-        for (int i = 0; i < kRowWarps; ++i) {
-            mine[i] = static_cast<uint32_t>(s.digits[i * 32 + threadIdx.x]);
-            high = max(high, mine[i]), low = min(low, mine[i]);
-        }
-        high = __reduce_max_sync(~0u, high), low = __reduce_min_sync(~0u, low);
-        const int first = 31 - __clz(static_cast<int>((high ^ low) | 1u << 16));
-        uint32_t least = static_cast<uint32_t>(static_cast<uint64_t>(high) >> (first + 1) << (first + 1));
-        for (int bit = first; bit >= 16; --bit) {
-            int32_t c = 0;
-#pragma unroll
-            for (int i = 0; i < kRowWarps; ++i) c += mine[i] >= (least | 1u << bit);
-            c = __reduce_add_sync(~0u, c);
-            if (c < k) continue;
-            least |= 1u << bit;
-            if (c <= k + k / 4) break;
-        }
-        if (threadIdx.x == 0) s.left = static_cast<int32_t>(least);
+    for (int i = 0; i < kRowWarps; ++i) {
+        mine[i] = static_cast<uint32_t>(s.digits[i * 32 + threadIdx.x % 32]);
+        high = max(high, mine[i]), low = min(low, mine[i]);
     }
-    __syncthreads();
-    return static_cast<uint32_t>(s.left);
+    high = __reduce_max_sync(~0u, high), low = __reduce_min_sync(~0u, low);
+    const int first = 31 - __clz(static_cast<int>((high ^ low) | 1u << 16));
+    uint32_t least = static_cast<uint32_t>(static_cast<uint64_t>(high) >> (first + 1) << (first + 1));
+#pragma unroll 1
+    for (int bit = first; bit >= 16; --bit) {
+        int32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < kRowWarps; ++i) c += mine[i] >= (least | 1u << bit);
+        c = __reduce_add_sync(~0u, c);
+        if (c < k) continue;
+        least |= 1u << bit;
+        if (c <= k + k / 4) break;
+    }
+    return least;
 }
 
 // The digit, of those counted from `first` on in steps of `step`, at which their sum reaches s.left, which becomes what is left for it.
@@ -366,6 +374,10 @@ __device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, Line<DT> &
 #pragma unroll
         for (int u = 0; u < kVectors; ++u) now[u] = line.next[u];
         line.ask(a);
+        if (tiles == 1) {
+#pragma unroll
+            for (int u = 0; u < kVectors; ++u) s.alone[u][tid] = now[u];
+        }
         const float m = L::template most<4 * kVectors>(reinterpret_cast<const uint32_t *>(now));
         s.most[tile][tid] = m;
         top = fmaxf(top, m);
@@ -390,60 +402,72 @@ __device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, Line<DT> &
         sum = __fadd_rn(sum, __fadd_rn(both.x, both.y));
     }
     const bool odd = (sum != sum && top > -CUDART_INF_F) || top > kMostPlain;
-    const float high = from_ordered(__reduce_max_sync(~0u, ordered(top)));
+    const uint32_t key = ordered(top);
+    const float high = from_ordered(__reduce_max_sync(~0u, key));
     const float warp_base = from_ordered(__reduce_max_sync(~0u, sum > 0.0f ? ordered(base) : 0x00800000u));
     float warp_sum = sum > 0.0f ? __fmul_rn(sum, whole_power2(base - warp_base)) : 0.0f;
 #pragma unroll
     for (int d = 16; d; d /= 2) warp_sum = __fadd_rn(warp_sum, __shfl_xor_sync(~0u, warp_sum, d));
     if (lane == 0) s.tops[warp] = high, s.sums[warp] = warp_sum, s.bases[warp] = warp_base;
-    if (tid == 0) s.found = s.ntiles = 0;
-    // Candidates: what reaches the k-th largest of the threads' largest, or all if fewer than k threads have one.
-    const uint32_t least_key = reached(s, ordered(top), a.k);
-    float least = least_key ? from_ordered(least_key) : -CUDART_INF_F;
-    const auto fits = [&](float y) { return y >= least && y > -CUDART_INF_F; };
-    if (fits(top)) {
-        for (int t = 0; t < tiles; ++t) {
-            if (!fits(s.most[t][tid])) continue;
-            const int32_t at = atomicAdd(&s.ntiles, 1);
-            if (at < kTileRoom) s.tiles[at] = static_cast<uint16_t>(t * kRowThreads + tid);
-        }
+    s.digits[tid] = static_cast<int32_t>(top > -CUDART_INF_F ? key : 0);
+    if (tid == 0) s.found = 0, s.crowded = false;
+    const bool odd_ones = __syncthreads_or(odd);
+    // Candidates: what reaches the k-th largest of the threads' largest, or all if fewer than k threads have one.  One warp finds it, another joins the
+    // warps' sums meanwhile.
+    if (warp == 0) {
+        const uint32_t reach = reached(s, a.k);
+        if (lane == 0) s.left = static_cast<int32_t>(reach);
     }
-    const float all_top = of_warps(s);
-    const bool again = __syncthreads_or(odd) || (all_top < -kMostPlain && all_top > -CUDART_INF_F);
-    // Those tiles are read again, from the L2 cache, a vector a thread.
-    const int32_t ntiles = s.ntiles;
-    if (ntiles <= kTileRoom) {
-        for (int32_t i = tid; i < kVectors * ntiles; i += kRowThreads) {
-            const int32_t at = s.tiles[i / kVectors], v = from + at / kRowThreads * kTileVectors + i % kVectors * kRowThreads + at % kRowThreads;
-            if (v >= to) continue;
-            const uint4 w = x.load(v);
-            if (!fits(L::template most<4>(reinterpret_cast<const uint32_t *>(&w)))) continue;
+    if (warp == 1) {
+        const float top_here = lane < kRowWarps ? s.tops[lane] : -CUDART_INF_F, sum_here = lane < kRowWarps ? s.sums[lane] : 0.0f;
+        const float base_here = sum_here > 0.0f ? s.bases[lane % kRowWarps] : -CUDART_MAX_NORMAL_F;
+        const float all_top = from_ordered(__reduce_max_sync(~0u, ordered(top_here))), all_base = from_ordered(__reduce_max_sync(~0u, ordered(base_here)));
+        float whole = sum_here > 0.0f ? __fmul_rn(sum_here, whole_power2(base_here - all_base)) : 0.0f;
 #pragma unroll
-            for (int e = 0; e < L::kPer; ++e) {
-                const float y = value_of<DT>(w, e);
-                if (!fits(y)) continue;
-                const int32_t place = atomicAdd(&s.found, 1);
-                if (place < a.room) candidates[place] = Candidate{y, x.token(v, e)};
-            }
+        for (int d = kRowWarps / 2; d; d /= 2) whole = __fadd_rn(whole, __shfl_xor_sync(~0u, whole, d));
+        if (lane == 0) {
+            s.again = odd_ones || (all_top < -kMostPlain && all_top > -CUDART_INF_F);
+            out->top = all_top;
+            out->sum = whole > 0.0f ? whole * quick_power2(all_base - static_cast<double>(kLog2e) * all_top) : 0.0;
         }
     }
     __syncthreads();
-    if (s.found > a.room || ntiles > kTileRoom) least = write_first<DT>(s, x, from, to, a.k, candidates);  // (the same for all threads)
-    double whole = 0.0;
-    if (again) whole = sum_again<DT>(s, x, from, to);
-    if (tid == 0) {
-        if (!again && all_top > -CUDART_INF_F) {
-            float all_base = -CUDART_INF_F;
-#pragma unroll
-            for (int i = 0; i < kRowWarps; ++i)
-                if (s.sums[i] > 0.0f) all_base = fmaxf(all_base, s.bases[i]);
-#pragma unroll
-            for (int i = 0; i < kRowWarps; ++i)
-                if (s.sums[i] > 0.0f) whole += static_cast<double>(s.sums[i]) * whole_power2(s.bases[i] - all_base);
-            whole *= exp2(all_base - static_cast<double>(kLog2e) * all_top);
-        }
-        *out = Part{whole, all_top, least, s.found, {}};
+    const uint32_t least_key = static_cast<uint32_t>(s.left);
+    float least = least_key ? from_ordered(least_key) : -CUDART_INF_F;
+    const auto fits = [&](float y) { return y >= least && y > -CUDART_INF_F; };
+    // A warp's tiles that have some are read again, from the L2 cache, a vector a lane.
+    int32_t mine = 0;
+    for (uint32_t with = __ballot_sync(~0u, fits(top)); with; with &= with - 1) {  // a thread's tiles a lane each
+        const int thread = __ffs(static_cast<int>(with)) - 1;
+        const bool hit = lane < tiles && fits(s.most[lane % kTilesPerPart][warp * 32 + thread]);
+        const uint32_t who = __ballot_sync(~0u, hit);
+        const int32_t place = mine + __popc(who & ((1u << lane) - 1u));
+        if (hit && place < kTileRoom) s.tiles[warp][place] = static_cast<uint16_t>(lane * 32 + thread);
+        mine += __popc(who);
     }
+    if (mine > kTileRoom) s.crowded = true;
+    __syncwarp();
+    for (int32_t i = lane; i < kVectors * min(mine, kTileRoom); i += 32) {
+        const int32_t which = s.tiles[warp][i / kVectors], u = i % kVectors, thread = warp * 32 + which % 32;
+        const int32_t v = from + which / 32 * kTileVectors + u * kRowThreads + thread;
+        if (v >= to) continue;
+        const uint4 w = tiles == 1 ? s.alone[u][thread] : x.load(v);
+        if (!fits(L::template most<4>(reinterpret_cast<const uint32_t *>(&w)))) continue;
+#pragma unroll
+        for (int e = 0; e < L::kPer; ++e) {
+            const float y = value_of<DT>(w, e);
+            if (!fits(y)) continue;
+            const int32_t place = atomicAdd(&s.found, 1);
+            if (place < a.room) candidates[place] = Candidate{y, x.token(v, e)};
+        }
+    }
+    __syncthreads();
+    if (s.found > a.room || s.crowded) least = write_first<DT>(s, x, from, to, a.k, candidates);  // (the same for all threads)
+    if (s.again) {
+        const double whole = sum_again<DT>(s, x, from, to);
+        if (tid == 0) out->sum = whole;
+    }
+    if (tid == 0) out->least = least, out->count = s.found;
 }
 
 template <int DT>
@@ -497,18 +521,6 @@ __device__ __forceinline__ double double_of_block(const double *mine, int rank) 
     double v;
     asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at_block(mine, rank)) : "memory");
     return v;
-}
-
-// 2^y for y <= 0, and log(x) for x > 0, to 2^-22 and 2^-23: 32-bit functions of what is left when whole powers of two are taken out.
-__device__ __forceinline__ double quick_power2(double y) {
-    if (!(y > -1000.0)) return 0.0;
-    const double n = rint(y);
-    return static_cast<double>(power2(static_cast<float>(y - n))) * __hiloint2double((1023 + static_cast<int>(n)) << 20, 0);
-}
-__device__ __forceinline__ double quick_log(double x) {
-    const int high = __double2hiint(x);
-    const float m = static_cast<float>(__hiloint2double((high & 0xFFFFF) | 1023 << 20, __double2loint(x)));
-    return ((high >> 20) - 1023) * 0.69314718055994531 + logf(m);
 }
 
 // Candidates as one number: by value, then the lower token first.

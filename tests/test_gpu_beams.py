@@ -1,8 +1,8 @@
 """The best continuations of beams against the same by its definition in 64 bits.
 
 Tokens and parents are equal.  A score is off by the rounding to 32 bits, half a step or 2^-24 of itself, and by the error of a sum of exponentials in
-32 bits, which enters as a logarithm: below 4.5e-6 whatever the logits (a term exp(-u) is off by 2^-24 (u + 6.3) + 1.4e-8 u and 2^-22, u weighted with the terms is
-below 17 for 2^24 tokens, the 31 additions of a part's sum add 2^-24 each, and joining the parts 2^-22 and 2^-23)."""
+32 bits, which enters as a logarithm: below 5e-6 whatever the logits (a term exp(-u) is off by 2^-24 (u + 6.3) + 1.4e-8 u and 2^-22, u weighted with the terms is
+below 17 for 2^24 tokens, the 34 additions of a part's sum add 2^-24 each, and joining the parts 2^-21 and 2^-23)."""
 import numpy as np
 import pytest
 import torch
@@ -25,7 +25,7 @@ def check(logits, scores, k):
     g, w = got[0].cpu().numpy().astype(np.float64), want[0]
     there = np.isfinite(w)
     assert np.array_equal(g[~there], w[~there])
-    assert (np.abs(g[there] - w[there]) <= 4.5e-6 + 2.0 ** -24 * np.abs(w[there])).all()
+    assert (np.abs(g[there] - w[there]) <= 5e-6 + 2.0 ** -24 * np.abs(w[there])).all()
     return got
 
 
