@@ -24,7 +24,7 @@ constexpr int kLogitF32 = CG_LOGITS_F32;
 constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32, kVectors = 4;  // of rows_kernel; 16-byte vectors of a thread in a tile
 constexpr int kTileVectors = kRowThreads * kVectors;
 constexpr int kRowBlocks = 4;                              // on an SM
-constexpr int kTilesPerPart = 16, kTileRoom = 64;          // a part's tiles, and how many of a warp's lanes' tiles may have candidates
+constexpr int kTilesPerPart = 16, kTileRoom = 512;         // a part's tiles, and how many of its threads' tiles may have candidates
 constexpr int kChooseBlocks = 8;                           // of a request's cluster
 constexpr int kChooseWarps = 8, kMostChooseWarps = 16, kSorted = 512, kSortedAtOnce = 256, kMostList = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -191,39 +191,58 @@ template <int DT> __device__ __forceinline__ float value_of(const uint4 &x, int 
 }
 
 struct Shared {
-    float most[kTilesPerPart][kRowThreads + 1];  // of a thread's tiles the largest logit
+    float most[kTilesPerPart][kRowThreads];   // of a thread's tiles the largest logit
     uint4 alone[kVectors][kRowThreads];       // a part's tile that is its only one
-    uint16_t tiles[kRowWarps][kTileRoom];     // tile * 32 + lane of those of a warp that have candidates
-    int32_t found;
+    uint16_t tiles[kTileRoom];                // tile * kRowThreads + thread of those that have candidates
+    int32_t ntiles, found;
     float tops[kRowWarps], sums[kRowWarps], bases[kRowWarps];  // a warp's sum is sums * 2 ^ bases
     alignas(8) int32_t digits[256];
     int32_t digit, left;
-    bool crowded, again;                      // more candidates than there is room for; a sum that the quick way does not give
+    bool again;                               // a sum that the quick way does not give
 };
 
-// What k of the block's keys (s.digits, 0 for none) reach, and not many more than k; 0, if there are fewer of them.  For one warp, which goes
-// through them bit by bit, from the first bit on that is not the same in all of them, to the sixteenth.
-__device__ __forceinline__ uint32_t reached(const Shared &s, int32_t k) {
-    uint32_t mine[kRowWarps], high = 0, low = ~0u;
+// What k of the block's keys (s.digits, 0 for none) reach.  The first is for one warp: of the eight keys of a lane it looks at the largest two (k <= 16: the
+// largest) alone, and returns the k-th largest of these: a few more than k of all keys reach it.  (Bit by bit over all keys it took 3,500 to 5,000 cycles, so
+// 300 to 500.)  0: there are not so many.  The second is for all threads, and exact; the same for all.
+__device__ __forceinline__ uint32_t kth_of_lanes(const Shared &s, int32_t k) {
+    const int lane = threadIdx.x % 32;
+    uint32_t high = 0, second = 0;
 #pragma unroll
     for (int i = 0; i < kRowWarps; ++i) {
-        mine[i] = static_cast<uint32_t>(s.digits[i * 32 + threadIdx.x % 32]);
-        high = max(high, mine[i]), low = min(low, mine[i]);
+        const uint32_t x = static_cast<uint32_t>(s.digits[i * 32 + lane]);
+        second = max(second, min(high, x)), high = max(high, x);
     }
-    high = __reduce_max_sync(~0u, high), low = __reduce_min_sync(~0u, low);
-    const int first = 31 - __clz(static_cast<int>((high ^ low) | 1u << 16));
-    uint32_t least = static_cast<uint32_t>(static_cast<uint64_t>(high) >> (first + 1) << (first + 1));
-#pragma unroll 1
-    for (int bit = first; bit >= 16; --bit) {
-        int32_t c = 0;
-#pragma unroll
-        for (int i = 0; i < kRowWarps; ++i) c += mine[i] >= (least | 1u << bit);
-        c = __reduce_add_sync(~0u, c);
-        if (c < k) continue;
-        least |= 1u << bit;
-        if (c <= k + k / 4) break;
+    int32_t before = 0, before_second = 0;  // keys in front of this lane's, those of lower lanes first among equal ones
+    if (k <= 16) {
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t x = __shfl_sync(~0u, high, i);
+            before += x > high || (x == high && i < lane);
+        }
+        second = 0, before_second = INT32_MAX;
+    } else {
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t x = __shfl_sync(~0u, high, i), y = __shfl_sync(~0u, second, i);
+            before += (x > high || (x == high && i < lane)) + (y > high || (y == high && i < lane));
+            before_second += (x > second || (x == second && i <= lane)) + (y > second || (y == second && i < lane));
+        }
     }
-    return least;
+    const uint32_t mine = before == k - 1 ? high : before_second == k - 1 ? second : 0;
+    return __reduce_max_sync(~0u, mine);
+}
+constexpr int kMostOfLanes = 40;  // the largest k for the first: behind it lanes' third keys would be missed
+__device__ __noinline__ uint32_t kth_of_all(Shared &s, int32_t k) {
+    const uint32_t mine = static_cast<uint32_t>(s.digits[threadIdx.x]);
+    int32_t before = 0;
+#pragma unroll 4
+    for (int i = 0; i < kRowThreads; ++i) {
+        const uint32_t x = static_cast<uint32_t>(s.digits[i]);
+        before += x > mine || (x == mine && i < static_cast<int>(threadIdx.x));
+    }
+    if (before == k - 1) s.left = static_cast<int32_t>(mine);
+    __syncthreads();
+    return static_cast<uint32_t>(s.left);
 }
 
 // The digit, of those counted from `first` on in steps of `step`, at which their sum reaches s.left, which becomes what is left for it.
@@ -410,12 +429,12 @@ __device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, Line<DT> &
     for (int d = 16; d; d /= 2) warp_sum = __fadd_rn(warp_sum, __shfl_xor_sync(~0u, warp_sum, d));
     if (lane == 0) s.tops[warp] = high, s.sums[warp] = warp_sum, s.bases[warp] = warp_base;
     s.digits[tid] = static_cast<int32_t>(top > -CUDART_INF_F ? key : 0);
-    if (tid == 0) s.found = 0, s.crowded = false;
+    if (tid == 0) s.found = s.ntiles = 0;
     const bool odd_ones = __syncthreads_or(odd);
     // Candidates: what reaches the k-th largest of the threads' largest, or all if fewer than k threads have one.  One warp finds it, another joins the
     // warps' sums meanwhile.
     if (warp == 0) {
-        const uint32_t reach = reached(s, a.k);
+        const uint32_t reach = a.k <= kMostOfLanes ? kth_of_lanes(s, a.k) : 0;
         if (lane == 0) s.left = static_cast<int32_t>(reach);
     }
     if (warp == 1) {
@@ -432,24 +451,26 @@ __device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, Line<DT> &
         }
     }
     __syncthreads();
-    const uint32_t least_key = static_cast<uint32_t>(s.left);
+    uint32_t least_key = static_cast<uint32_t>(s.left);
+    if (!least_key) {  // (the same for all threads, which read it before it changes)
+        __syncthreads();
+        least_key = kth_of_all(s, a.k);
+    }
     float least = least_key ? from_ordered(least_key) : -CUDART_INF_F;
     const auto fits = [&](float y) { return y >= least && y > -CUDART_INF_F; };
-    // A warp's tiles that have some are read again, from the L2 cache, a vector a lane.
-    int32_t mine = 0;
-    for (uint32_t with = __ballot_sync(~0u, fits(top)); with; with &= with - 1) {  // a thread's tiles a lane each
-        const int thread = __ffs(static_cast<int>(with)) - 1;
-        const bool hit = lane < tiles && fits(s.most[lane % kTilesPerPart][warp * 32 + thread]);
-        const uint32_t who = __ballot_sync(~0u, hit);
-        const int32_t place = mine + __popc(who & ((1u << lane) - 1u));
-        if (hit && place < kTileRoom) s.tiles[warp][place] = static_cast<uint16_t>(lane * 32 + thread);
-        mine += __popc(who);
+    if (fits(top)) {
+#pragma unroll 4
+        for (int t = 0; t < tiles; ++t) {
+            if (!fits(s.most[t][tid])) continue;
+            const int32_t at = atomicAdd(&s.ntiles, 1);
+            if (at < kTileRoom) s.tiles[at] = static_cast<uint16_t>(t * kRowThreads + tid);
+        }
     }
-    if (mine > kTileRoom) s.crowded = true;
-    __syncwarp();
-    for (int32_t i = lane; i < kVectors * min(mine, kTileRoom); i += 32) {
-        const int32_t which = s.tiles[warp][i / kVectors], u = i % kVectors, thread = warp * 32 + which % 32;
-        const int32_t v = from + which / 32 * kTileVectors + u * kRowThreads + thread;
+    __syncthreads();
+    // Tiles that have some are read again, from the L2 cache, a vector a thread.
+    const int32_t ntiles = min(s.ntiles, kTileRoom);
+    for (int32_t i = tid; i < kVectors * ntiles; i += kRowThreads) {
+        const int32_t at = s.tiles[i / kVectors], u = i % kVectors, thread = at % kRowThreads, v = from + at / kRowThreads * kTileVectors + u * kRowThreads + thread;
         if (v >= to) continue;
         const uint4 w = tiles == 1 ? s.alone[u][thread] : x.load(v);
         if (!fits(L::template most<4>(reinterpret_cast<const uint32_t *>(&w)))) continue;
@@ -462,7 +483,7 @@ __device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, Line<DT> &
         }
     }
     __syncthreads();
-    if (s.found > a.room || s.crowded) least = write_first<DT>(s, x, from, to, a.k, candidates);  // (the same for all threads)
+    if (s.found > a.room || s.ntiles > kTileRoom) least = write_first<DT>(s, x, from, to, a.k, candidates);  // (the same for all threads)
     if (s.again) {
         const double whole = sum_again<DT>(s, x, from, to);
         if (tid == 0) out->sum = whole;
