@@ -26,7 +26,7 @@ constexpr int kTileVectors = kRowThreads * kVectors;
 constexpr int kRowBlocks = 4;                              // on an SM
 constexpr int kTilesPerPart = 16, kTileRoom = 512;         // a part's tiles, and how many of its threads' tiles may have candidates
 constexpr int kChooseBlocks = 8;                           // of a request's cluster
-constexpr int kChooseWarps = 8, kMostChooseWarps = 16, kSorted = 512, kSortedAtOnce = 256, kMostList = 4096;
+constexpr int kChooseWarps = 8, kMostChooseWarps = 16, kSorted = 512, kSortedAtOnce = 192, kBins = 256, kMostList = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMostPlain = 32768.0f;                     // logits up to here are summed the quick way
 // Relative error of a row's sum in 32 bits, and so the absolute one of its logarithm.  A term is 2 to the power y = x log2(e) - c, c whole and at most 9 below
@@ -746,8 +746,8 @@ __device__ __forceinline__ void write_sorted(const BeamArgs &a, const Choice *so
     }
 }
 // The continuations that may be among the best, in *list; returns how many there are, more than `kSorted` if that is no use.  A bound that k of
-// one row reach drops most of them while they are read; where that leaves many, the k-th largest of them (by the upper half of its bits) drops nearly all of the
-// others.  Both leave room for what 32-bit sums are off.  *sorted is as large as kSorted.
+// one row reach drops most of them while they are read; where that leaves many, they are counted in bins, and all behind the bin of the k-th and the next one are
+// dropped.  Both leave room for what 32-bit sums are off.  *sorted is as large as kSorted.
 __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const ChooseRoom &r, int32_t request, int32_t *counts, Choice **list, Choice **sorted) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     double bound = -CUDART_INF;
@@ -797,25 +797,47 @@ __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const Choos
     const int32_t n = counts[0];
     if (n > a.list_room) return INT32_MAX;
     if (n <= kSortedAtOnce) return n;
-    uint32_t least = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t want = least | 1u << bit;
-        int32_t c = 0;
-        for (int32_t i = threadIdx.x; i < n; i += blockDim.x) c += r.list[i].key >> 32 >= want;
-        c = __reduce_add_sync(~0u, c);
-        int32_t *const sum = counts + 1 + bit % 3;  // one is filled, one is read, one is set back
-        if (lane == 0 && c) atomicAdd(sum, c);
+    if (!(bound > -CUDART_INF)) {  // no row's part had k: from the least of the list on
+        uint32_t least = ~0u;
+        for (int32_t i = threadIdx.x; i < n; i += blockDim.x) least = min(least, static_cast<uint32_t>(r.list[i].key >> 32));
+        least = __reduce_min_sync(~0u, least);
+        if (lane == 0) atomicMin(reinterpret_cast<uint32_t *>(&counts[1]), least);
         __syncthreads();
-        if (*sum >= a.k) least = want;
-        if (threadIdx.x == 0) counts[1 + (bit + 1) % 3] = 0;
+        bound = Choice{static_cast<uint64_t>(static_cast<uint32_t>(counts[1])) << 32, 0}.total();
     }
-    bound = Choice{static_cast<uint64_t>(least) << 32, 0}.total() - 2.0 * kRowError;
+    double high = -CUDART_INF;  // the best of the rows' largest: there x - top is 0
+    for (int32_t i = 0; i < a.beams; ++i) high = fmax(high, r.base[i]);
+    const float width = static_cast<float>(high - bound) * (1.0f / kBins), a_bin = 1.0f / width;
+    if (!(width > 1e-4f && width < 1e30f)) return n;
+    static_assert(1e-4 > 16.0 * kRowError, "a bin is wider than what sums are off");
+    const auto bin = [&](const Choice &c) { return min(kBins - 1, static_cast<int32_t>(static_cast<float>(c.total() - bound) * a_bin)); };
+    for (int32_t i = threadIdx.x; i < n; i += blockDim.x) atomicAdd(&r.places[bin(r.list[i])], 1);
+    __syncthreads();
+    if (warp == 0) {  // the bin in which the k-th stands, counted from the last
+        constexpr int kEach = kBins / 32;
+        int32_t mine = 0;
+        for (int32_t i = 0; i < kEach; ++i) mine += r.places[kBins - 1 - lane * kEach - i];
+        int32_t upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int32_t y = __shfl_up_sync(~0u, upto, d);
+            if (lane >= d) upto += y;
+        }
+        if (upto >= a.k && upto - mine < a.k) {
+            int32_t left = a.k - (upto - mine), at = kBins - 1 - lane * kEach;
+            while (left > r.places[at]) left -= r.places[at--];  // (ends in this lane's share)
+            counts[1] = at;
+        }
+    }
     if (threadIdx.x == 0) counts[0] = 0;
     __syncthreads();
+    const int32_t first_bin = counts[1] - 1;  // one bin more than is counted, wider than what sums are off
+    for (int32_t i = threadIdx.x; i < kBins; i += blockDim.x) r.places[i] = 0;
     for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
-        if (r.list[i].total() < bound) continue;
+        const Choice c = r.list[i];
+        if (bin(c) < first_bin) continue;
         const int32_t at = atomicAdd(&counts[0], 1);
-        if (at < kSorted) r.sorted[at] = r.list[i];
+        if (at < kSorted) r.sorted[at] = c;
     }
     __syncthreads();
     *list = r.sorted, *sorted = r.list;
@@ -827,7 +849,7 @@ template <int DT>
 __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostChooseWarps * 32) choose_kernel(const __grid_constant__ BeamArgs a) {
     extern __shared__ __align__(16) char room[];
     __shared__ double warps_sums[kMostChooseWarps];
-    __shared__ int32_t counts[4];
+    __shared__ int32_t counts[2];
     const int rank = choose_rank(), lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const int32_t request = blockIdx.x / kChooseBlocks;
     const ChooseRoom r(room, a, warps);
@@ -836,7 +858,7 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
     if (rank == 0) {
         for (int32_t i = threadIdx.x; i <= a.beams; i += blockDim.x) r.near[i] = 0;
         for (int32_t i = threadIdx.x; i < kSorted; i += blockDim.x) r.places[i] = 0;
-        if (threadIdx.x < 4) counts[threadIdx.x] = 0;
+        if (threadIdx.x == 0) counts[0] = 0, counts[1] = -1;  // how many; a bin, or the upper half of a score's key
         wait_for_launch_before();
         for (int32_t i = warp; i < a.beams; i += warps) {
             const int32_t row = request * a.beams + i;
