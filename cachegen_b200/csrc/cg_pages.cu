@@ -16,8 +16,9 @@ namespace {
 constexpr int kClusterBlocks = 8, kClusterThreads = 512, kClusterWarps = kClusterThreads / 32;
 constexpr int kRowThreads = 256, kRowColumns = 1024;  // of a block that works on a row of a table
 constexpr int kCopyThreads = 256, kCopyVectors = 4;
+constexpr int64_t kAlonePages = 32768;  // up to here, and with a row a thread, one block does: 2,600 pages and 8 rows extended in 9 us by eight blocks
 constexpr int32_t kSlotsTogether = 2 * kClusterBlocks * kClusterThreads;
-constexpr int64_t kMostPages = INT32_MAX - 8;  // a thread counts on by four
+constexpr int64_t kMostPages = INT32_MAX - 512;  // a warp counts on behind its last page
 
 struct Table {
     const int32_t *entries, *lens;
@@ -50,104 +51,128 @@ __device__ __forceinline__ int32_t page_at(const Table &t, int row, int column) 
 }
 
 // ---- sums over a cluster ----------------------------------------------------------------------------
-__device__ __forceinline__ int cluster_rank() {
-    int r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+// BLOCKS of kClusterThreads threads, one or kClusterBlocks: a block alone needs no steps between blocks, of 2 us in all, and is enough for most caches.
+template <int BLOCKS> __device__ __forceinline__ int cluster_rank() {
+    int r = 0;
+    if (BLOCKS > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
 // Everything that the cluster's threads wrote, to whatever memory, is there for all of them afterwards.
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+template <int BLOCKS> __device__ __forceinline__ void cluster_barrier() {
+    if (BLOCKS > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else __syncthreads();
 }
-__device__ __forceinline__ int64_t of_block(const int64_t *mine, int rank) {
+template <int BLOCKS> __device__ __forceinline__ int64_t of_block(const int64_t *mine, int rank) {
+    if (BLOCKS == 1) return *mine;
     uint32_t at;
     int64_t v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(mine)), "r"(rank));
     asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
     return v;
 }
-// Sum over the threads of the block in front of this one; total: over all of them.  sums: room of the block's own for kClusterWarps + 1.
-template <class T> __device__ __forceinline__ T sum_before(T x, T *sums, T *total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    T upto = x;
+template <class T> __device__ __forceinline__ T sum_upto(T x) {  // over the warp's lanes up to this one
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-        const T y = __shfl_up_sync(~0u, upto, d);
-        if (lane >= d) upto += y;
+        const T y = __shfl_up_sync(~0u, x, d);
+        if (static_cast<int>(threadIdx.x & 31) >= d) x += y;
     }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    if (warp == 0) {
-        const T own = lane < kClusterWarps ? sums[lane] : 0;
-        T s = own;
+    return x;
+}
+// What a block's warps tell the other blocks.
+struct Told {
+    int64_t a[kClusterWarps], b[kClusterWarps];
+};
+struct Sums {  // in front of this warp, and of all warps
+    int64_t a, b, all_a, all_b;
+};
+// Sums over the cluster's warps of two numbers of each, in one step: a lane reads four warps' numbers.  A barrier of the cluster stands in it.
+template <int BLOCKS> __device__ __forceinline__ Sums over_warps(int64_t a, int64_t b, Told *told) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = cluster_rank<BLOCKS>() * kClusterWarps + warp;
+    if (lane == 0) told->a[warp] = a, told->b[warp] = b;
+    cluster_barrier<BLOCKS>();
+    constexpr int kEach = (BLOCKS * kClusterWarps + 31) / 32;
+    static_assert(kClusterWarps % kEach == 0, "a lane reads one block's");
+    int64_t x[kEach], y[kEach], sum_a = 0, sum_b = 0;
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const T y = __shfl_up_sync(~0u, s, d);
-            if (lane >= d) s += y;
-        }
-        if (lane < kClusterWarps) sums[lane] = s - own;
-        if (lane == kClusterWarps - 1) sums[kClusterWarps] = s;
+    for (int i = 0; i < kEach; ++i) {
+        const int w = lane * kEach + i;
+        const bool there = w < BLOCKS * kClusterWarps;
+        x[i] = there ? of_block<BLOCKS>(&told->a[w % kClusterWarps], w / kClusterWarps) : 0;
+        y[i] = there ? of_block<BLOCKS>(&told->b[w % kClusterWarps], w / kClusterWarps) : 0;
     }
-    __syncthreads();
-    *total = sums[kClusterWarps];
-    return sums[warp] + upto - x;
+    int64_t front_a = 0, front_b = 0;  // of this lane's warps those in front of mine
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        sum_a += x[i], sum_b += y[i];
+        if (lane * kEach + i < me) front_a += x[i], front_b += y[i];
+    }
+    Sums s;
+    const int64_t upto_a = sum_upto(front_a), upto_b = sum_upto(front_b), all_a = sum_upto(sum_a), all_b = sum_upto(sum_b);
+    s.a = __shfl_sync(~0u, upto_a, 31), s.b = __shfl_sync(~0u, upto_b, 31);
+    s.all_a = __shfl_sync(~0u, all_a, 31), s.all_b = __shfl_sync(~0u, all_b, 31);
+    return s;
 }
 
-// A thread's run of pages, [first, last): runs of neighbouring threads and blocks follow one another.
+// A warp's run of pages, [first, last), four neighbouring ones a lane at a time; runs of warps and blocks follow one another.
 struct Run {
     int32_t first, last;
 };
-__device__ __forceinline__ Run run_of(int32_t num_pages) {
-    const int64_t each = (static_cast<int64_t>(num_pages) + kClusterBlocks * kClusterThreads - 1) / (kClusterBlocks * kClusterThreads);
-    const int64_t run = (each + 3) / 4 * 4, first = (static_cast<int64_t>(cluster_rank()) * kClusterThreads + threadIdx.x) * run;
-    return Run{static_cast<int32_t>(first < num_pages ? first : num_pages), static_cast<int32_t>(first + run < num_pages ? first + run : num_pages)};
+template <int BLOCKS> __device__ __forceinline__ Run run_of(int32_t num_pages) {
+    constexpr int kAll = BLOCKS * kClusterWarps;
+    const int64_t run = ((static_cast<int64_t>(num_pages) + kAll - 1) / kAll + 127) / 128 * 128;
+    const int64_t first = (cluster_rank<BLOCKS>() * kClusterWarps + static_cast<int>(threadIdx.x >> 5)) * run, last = first + run;
+    return Run{static_cast<int32_t>(first < num_pages ? first : num_pages), static_cast<int32_t>(last < num_pages ? last : num_pages)};
 }
-// f(page, its count) for every page of a run, in order
-template <class F>
-__device__ __forceinline__ void each_page(const int32_t *refs, const Run &run, bool vectors, F f) {
-    int32_t p = run.first;
-    if (vectors)
-        for (; p <= run.last - 4; p += 4) {
-            const int4 c = *reinterpret_cast<const int4 *>(refs + p);
-            f(p, c.x), f(p + 1, c.y), f(p + 2, c.z), f(p + 3, c.w);
-        }
-    for (; p < run.last; ++p) f(p, refs[p]);
+// The counts of pages p .. p + 3; `behind` for those at `last` and behind.
+__device__ __forceinline__ int4 counts_at(const int32_t *refs, int32_t p, int32_t last, bool vectors, int32_t behind) {
+    if (vectors && p <= last - 4) return *reinterpret_cast<const int4 *>(refs + p);
+    int4 c = make_int4(behind, behind, behind, behind);
+    if (p < last) c.x = refs[p];
+    if (p < last - 1) c.y = refs[p + 1];
+    if (p < last - 2) c.z = refs[p + 2];
+    if (p < last - 3) c.w = refs[p + 3];
+    return c;
 }
-
-// Room of a block for the sums above, and for what it tells the others.
-struct Sums {
-    int32_t pages[kClusterWarps + 1];
-    int64_t rows[kClusterWarps + 1], told[2];
-};
+__device__ __forceinline__ int32_t zeros(const int4 &c) { return (c.x == 0) + (c.y == 0) + (c.z == 0) + (c.w == 0); }
+__device__ __forceinline__ int32_t free_in(const int32_t *refs, const Run &run, bool vectors) {
+    int32_t n = 0;
+#pragma unroll 4
+    for (int32_t p = run.first + 4 * static_cast<int32_t>(threadIdx.x & 31); p < run.last; p += 128) n += zeros(counts_at(refs, p, run.last, vectors, 1));
+    return __reduce_add_sync(~0u, n);
+}
 
 // Writes the numbers of the first free pages to `list`, in order, as many as the cluster's threads want together (`wanted` is this
 // thread's), if there are so many.  Returns the sum of what the threads before this one want; free_pages: how many there are.
-// A barrier of the cluster stands between its reads of the counts and its end.
-__device__ __forceinline__ int64_t take_free(const int32_t *refs, int32_t num_pages, int64_t wanted, int32_t *list, Sums *s, int64_t *wanted_all,
+// Barriers of the cluster stand between its reads of the counts and its end.
+template <int BLOCKS>
+__device__ __forceinline__ int64_t take_free(const int32_t *refs, int32_t num_pages, int64_t wanted, int32_t *list, Told *told, int64_t *wanted_all,
                                              int64_t *free_pages) {
-    const Run run = run_of(num_pages);
+    const Run run = run_of<BLOCKS>(num_pages);
     const bool vectors = reinterpret_cast<uintptr_t>(refs) % 16 == 0;
-    int32_t free = 0, block_free;
-    int64_t block_wanted;
-    each_page(refs, run, vectors, [&](int32_t, int32_t c) { free += c == 0; });
-    int64_t rank = sum_before(free, s->pages, &block_free), before = sum_before(wanted, s->rows, &block_wanted);
-    if (threadIdx.x == 0) s->told[0] = block_free, s->told[1] = block_wanted;
-    cluster_barrier();
-    *wanted_all = *free_pages = 0;
-    const int me = cluster_rank();
-    for (int r = 0; r < kClusterBlocks; ++r) {
-        const int64_t f = of_block(s->told, r), w = of_block(s->told + 1, r);
-        if (r < me) rank += f, before += w;
-        *free_pages += f, *wanted_all += w;
+    const int32_t free = free_in(refs, run, vectors);
+    const int64_t upto = sum_upto(wanted);
+    const Sums s = over_warps<BLOCKS>(free, __shfl_sync(~0u, upto, 31), told);
+    const int64_t most = s.all_b;
+    int64_t rank = s.a;
+    if (free && rank < most) {
+        for (int32_t p0 = run.first; p0 < run.last && rank < most; p0 += 128) {
+            const int32_t p = p0 + 4 * static_cast<int32_t>(threadIdx.x & 31);
+            const int4 c = counts_at(refs, p, run.last, vectors, 1);
+            const int32_t mine = zeros(c), before = sum_upto(mine);
+            int64_t at = rank + before - mine;
+            if (c.x == 0 && at < most) list[at] = p;
+            at += c.x == 0;
+            if (c.y == 0 && at < most) list[at] = p + 1;
+            at += c.y == 0;
+            if (c.z == 0 && at < most) list[at] = p + 2;
+            at += c.z == 0;
+            if (c.w == 0 && at < most) list[at] = p + 3;
+            rank += __shfl_sync(~0u, before, 31);
+        }
     }
-    const int64_t most = *wanted_all;
-    if (free && rank < most)
-        each_page(refs, run, vectors, [&](int32_t p, int32_t c) {
-            if (c == 0 && rank < most) list[rank] = p;
-            rank += c == 0;
-        });
-    cluster_barrier();
-    return before;
+    cluster_barrier<BLOCKS>();
+    *wanted_all = most, *free_pages = s.all_a;
+    return s.b + upto - wanted;
 }
 
 // ---- fork ----------------------------------------------------------------------------------------------
@@ -196,10 +221,12 @@ __global__ void __launch_bounds__(kRowThreads) fork_tables_kernel(const __grid_c
 
 // One cluster, a row a thread.  A page that is not full may be written to by one row only: the first of the new rows that hold it
 // keeps it, if no other row does (it is counted more often than by these), and each of the rest gets a copy.
-__global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kClusterThreads) fork_writers_kernel(const __grid_constant__ ForkArgs a) {
-    __shared__ Sums sums;
+template <int BLOCKS>
+__global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads) fork_writers_kernel(const __grid_constant__ ForkArgs a) {
+    __shared__ Told told;
+    let_next_launch_start();
     wait_for_launch_before();
-    const int32_t each = (a.nnew + kClusterBlocks - 1) / kClusterBlocks, row = cluster_rank() * each + threadIdx.x;
+    const int32_t each = (a.nnew + BLOCKS - 1) / BLOCKS, row = cluster_rank<BLOCKS>() * each + threadIdx.x;
     const bool here = threadIdx.x < each && row < a.nnew;
     int32_t tokens = 0, page = -1, part = 0, column = 0;
     if (here) {
@@ -212,11 +239,11 @@ __global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kCluste
             atomicAdd(&a.writers[page].count, 1);
         }
     }
-    cluster_barrier();
+    cluster_barrier<BLOCKS>();
     bool copied = false;
     if (page >= 0) copied = __ldcg(&a.writers[page].first) != row || __ldcg(&a.writers[page].count) != __ldcg(a.refs + page);
     int64_t all, free;
-    const int64_t rank = take_free(a.refs, a.old.num_pages, copied, a.list, &sums, &all, &free);
+    const int64_t rank = take_free<BLOCKS>(a.refs, a.old.num_pages, copied, a.list, &told, &all, &free);
     if (copied) {
         const bool found = rank < free;
         const int32_t to = found ? __ldcg(a.list + rank) : -1;
@@ -233,9 +260,9 @@ __global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kCluste
         }
     }
     const int32_t made = static_cast<int32_t>(all < free ? all : free);
-    for (int32_t r = made + cluster_rank() * kClusterThreads + threadIdx.x; r < a.nnew; r += kClusterBlocks * kClusterThreads)
+    for (int32_t r = made + cluster_rank<BLOCKS>() * kClusterThreads + threadIdx.x; r < a.nnew; r += BLOCKS * kClusterThreads)
         a.moves[r] = a.moves[a.nnew + r] = a.moves[2 * a.nnew + r] = -1;
-    if (cluster_rank() == 0 && threadIdx.x == 0) *a.copies = made;
+    if (cluster_rank<BLOCKS>() == 0 && threadIdx.x == 0) *a.copies = made;
 }
 
 // ---- give back -----------------------------------------------------------------------------------------
@@ -279,7 +306,7 @@ struct ExtendArgs {
     int64_t *slots;
     int32_t ntokens;
 };
-struct Growth {  // of a row: its pages before, how many it gets, and where they stand in the list
+struct Growth {  // of a row: its pages before, how many it gets, and where they stand in the list, or would
     int32_t before, pages;
     int64_t rank;
 };
@@ -313,11 +340,12 @@ __device__ __forceinline__ int64_t slot_of(const ExtendArgs &a, int32_t i) {
     return -1;
 }
 // One cluster, a row a thread for the sums; then the threads of a block share its rows' new pages, and (`slots_too`) all of them the tokens.
-__global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kClusterThreads) extend_pages_kernel(const __grid_constant__ ExtendArgs a, int slots_too) {
-    __shared__ Sums sums;
-    __shared__ Growth grown[CG_MAX_REQUESTS / kClusterBlocks];
+template <int BLOCKS>
+__global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads) extend_pages_kernel(const __grid_constant__ ExtendArgs a, int slots_too) {
+    __shared__ Told told;
+    __shared__ Growth grown[kClusterThreads];
     let_next_launch_start();
-    const int32_t S = a.t.page_size, each = (a.t.rows + kClusterBlocks - 1) / kClusterBlocks, row0 = cluster_rank() * each;
+    const int32_t S = a.t.page_size, each = (a.t.rows + BLOCKS - 1) / BLOCKS, row0 = cluster_rank<BLOCKS>() * each;
     const int32_t row = row0 + threadIdx.x;
     const bool here = threadIdx.x < each && row < a.t.rows;
     int32_t tokens = 0, asked = 0;
@@ -340,7 +368,7 @@ __global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kCluste
         }
     }
     int64_t all, free;
-    g.rank = take_free(a.refs, a.t.num_pages, wanted, a.list, &sums, &all, &free);
+    g.rank = take_free<BLOCKS>(a.refs, a.t.num_pages, wanted, a.list, &told, &all, &free);
     if (here) {
         if (wanted > 0 && g.rank + wanted > free) {
             note(a.t.status, CG_S_NO_PAGE);
@@ -352,20 +380,27 @@ __global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kCluste
         grown[threadIdx.x] = g;
     }
     __syncthreads();
+    // The block's rows' pages follow one another in the list: a page a thread, its row found among theirs.
     const int32_t mine = a.t.rows - row0 < each ? a.t.rows - row0 : each;  // rows of this block, none or less behind the last
-    int team = kClusterThreads;
-    while (team > 1 && team * mine > kClusterThreads) team /= 2;
-    for (int32_t r = threadIdx.x / team; r < mine; r += kClusterThreads / team) {
-        const Growth &x = grown[r];
-        for (int32_t j = threadIdx.x % team; j < x.pages; j += team) {
-            const int32_t p = __ldcg(a.list + x.rank + j);
-            a.table[(row0 + r) * a.t.row + x.before + j] = p;
+    if (mine > 0) {
+        const int64_t end = grown[mine - 1].rank + grown[mine - 1].pages;
+        for (int64_t r = grown[0].rank + threadIdx.x; r < end; r += kClusterThreads) {
+            int32_t lo = 0, hi = mine;  // ranks rise: the last row that begins at r or in front of it
+            while (hi - lo > 1) {
+                const int32_t mid = (lo + hi) / 2;
+                if (grown[mid].rank <= r) lo = mid;
+                else hi = mid;
+            }
+            const Growth &x = grown[lo];
+            if (r - x.rank >= x.pages) continue;  // of a row that found no place
+            const int32_t p = __ldcg(a.list + r);
+            a.table[(row0 + lo) * a.t.row + x.before + (r - x.rank)] = p;
             a.refs[p] = 1;
         }
     }
     if (!slots_too) return;
-    cluster_barrier();
-    for (int32_t i = cluster_rank() * kClusterThreads + threadIdx.x; i < a.ntokens; i += kClusterBlocks * kClusterThreads) a.slots[i] = slot_of(a, i);
+    cluster_barrier<BLOCKS>();
+    for (int32_t i = cluster_rank<BLOCKS>() * kClusterThreads + threadIdx.x; i < a.ntokens; i += BLOCKS * kClusterThreads) a.slots[i] = slot_of(a, i);
 }
 __global__ void __launch_bounds__(kRowThreads) slots_kernel(const __grid_constant__ ExtendArgs a) {
     wait_for_launch_before();
@@ -380,38 +415,44 @@ struct CompactArgs {
     int32_t *copies, *before_middle;
 };
 // One cluster.  With n pages held, those at n and behind go to the holes in front of n, the first to the first.
-__global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kClusterThreads) compact_places_kernel(const __grid_constant__ CompactArgs a) {
-    __shared__ Sums sums;
-    wait_for_launch_before();
-    const Run run = run_of(a.t.num_pages);
+template <int BLOCKS>
+__global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads) compact_places_kernel(const __grid_constant__ CompactArgs a) {
+    __shared__ Told told;
+    let_next_launch_start();
+    const Run run = run_of<BLOCKS>(a.t.num_pages);
     const bool vectors = reinterpret_cast<uintptr_t>(a.refs) % 16 == 0;
-    int32_t held = 0, block_held, n = 0;  // n: pages held
-    each_page(a.refs, run, vectors, [&](int32_t, int32_t c) { held += c != 0; });
-    int32_t before = sum_before(held, sums.pages, &block_held);
-    if (threadIdx.x == 0) sums.told[0] = block_held;
-    cluster_barrier();
-    const int me = cluster_rank();
-    for (int r = 0; r < kClusterBlocks; ++r) {
-        const int32_t h = static_cast<int32_t>(of_block(sums.told, r));
-        if (r < me) before += h;
-        n += h;
+    const int32_t lane = threadIdx.x & 31, free = free_in(a.refs, run, vectors);
+    const Sums sums = over_warps<BLOCKS>(free, run.last - run.first - free, &told);
+    const int32_t n = static_cast<int32_t>(sums.all_b);  // pages held
+    if (n >= run.first && n < run.last) {  // the warp whose pages n is one of: those held in front of it
+        int32_t front = 0;
+        for (int32_t p = run.first + lane; p < n; p += 32) front += a.refs[p] != 0;
+        front = __reduce_add_sync(~0u, front);
+        if (lane == 0) *a.before_middle = static_cast<int32_t>(sums.b) + front;
     }
-    if (n >= run.first && n < run.last) {  // the thread whose pages n is one of
-        int32_t front = before;
-        for (int32_t p = run.first; p < n; ++p) front += a.refs[p] != 0;
-        *a.before_middle = front;
-    }
-    cluster_barrier();
+    cluster_barrier<BLOCKS>();
     const int32_t front = n < a.t.num_pages ? __ldcg(a.before_middle) : n, made = n - front;  // holes in front of n = held pages behind
     const int32_t half = a.t.num_pages / 2;
-    each_page(a.refs, run, vectors, [&](int32_t p, int32_t c) {
-        if (c != 0 && p >= n) a.moves[before - front] = p;
-        if (c == 0 && p < n) a.moves[half + p - before] = p;
-        a.places[p] = c != 0 ? p : -1;
-        before += c != 0;
-    });
-    cluster_barrier();
-    for (int32_t r = cluster_rank() * kClusterThreads + threadIdx.x; r < half; r += kClusterBlocks * kClusterThreads) {
+    int32_t before = static_cast<int32_t>(sums.b);  // pages held in front of p0
+    for (int32_t p0 = run.first; p0 < run.last; p0 += 128) {
+        const int32_t p = p0 + 4 * lane;
+        const int4 c = counts_at(a.refs, p, run.last, vectors, 0);
+        const int32_t held = 4 - zeros(c), upto = sum_upto(held);
+        int32_t at = before + upto - held;
+        const int32_t count[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int32_t q = p + i;
+            if (p >= run.last - i) break;
+            if (count[i] != 0 && q >= n) a.moves[at - front] = q;
+            if (count[i] == 0 && q < n) a.moves[half + q - at] = q;
+            a.places[q] = count[i] != 0 ? q : -1;
+            at += count[i] != 0;
+        }
+        before += __shfl_sync(~0u, upto, 31);
+    }
+    cluster_barrier<BLOCKS>();
+    for (int32_t r = cluster_rank<BLOCKS>() * kClusterThreads + threadIdx.x; r < half; r += BLOCKS * kClusterThreads) {
         if (r < made) {
             const int32_t from = __ldcg(a.moves + r), to = __ldcg(a.moves + half + r);
             a.places[from] = to;
@@ -421,9 +462,10 @@ __global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kCluste
             a.moves[r] = a.moves[half + r] = -1;
         }
     }
-    if (cluster_rank() == 0 && threadIdx.x == 0) *a.copies = made;
+    if (cluster_rank<BLOCKS>() == 0 && threadIdx.x == 0) *a.copies = made;
 }
 __global__ void __launch_bounds__(kRowThreads) compact_tables_kernel(const __grid_constant__ CompactArgs a) {
+    let_next_launch_start();
     wait_for_launch_before();
     const int parts = (a.t.width + kRowColumns - 1) / kRowColumns;
     const int row = blockIdx.x / parts, column0 = (blockIdx.x - row * parts) * kRowColumns;
@@ -451,13 +493,13 @@ struct CopyArgs {
     const void *src, *dst;
     const int32_t *tokens, *count;  // or nullptr
     int32_t *status;
-    int64_t units, num_pages;
+    int64_t num_pages;
     int32_t ncopies, nlayers, page_size, heads, pieces;  // pieces of a head
-    int32_t parts, wide;
+    int32_t slices, wide;
 };
 
-// A unit is a part of one page of one layer's keys or values: of what is copied of it, so that pages of which little is copied are shared out
-// as evenly as whole ones.  The next unit's numbers are on their way while one is copied.
+// A unit is a slice of what is copied of one page of one layer's keys or values, so that pages of which little is copied are shared out as evenly as whole
+// ones; a block goes through it kCopyThreads x kCopyVectors pieces at a time.  The next unit's numbers are on their way while one is copied.
 struct Copy {
     int64_t from, to;
     int32_t tokens;
@@ -470,7 +512,7 @@ __device__ __forceinline__ Copy copy_at(const CopyArgs &a, int32_t i) {
 template <class Piece>
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
     wait_for_launch_before();
-    const int32_t ncopies = a.count ? __ldcg(a.count) : a.ncopies, each = 2 * a.nlayers * a.parts;
+    const int32_t ncopies = a.count ? __ldcg(a.count) : a.ncopies, each = 2 * a.nlayers * a.slices;
     const int64_t units = static_cast<int64_t>(ncopies) * each;
     constexpr int kValues = sizeof(Piece) / 2;
     const int32_t step = static_cast<int32_t>(gridDim.x), over = step / each, rest = step - over * each;
@@ -489,34 +531,36 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
             if (!padding && in == 0 && threadIdx.x == 0) note(a.status, CG_S_BAD_PAGE);
             continue;
         }
-        const int32_t which = in / a.parts, part = in - which * a.parts, layer = which >> 1;
+        const int32_t which = in / a.slices, slice = in - which * a.slices, layer = which >> 1;
         const CopySide &s = a.sides[which & 1];
-        const int32_t pieces = tokens * a.heads * a.pieces, share = ((pieces + a.parts - 1) / a.parts + 7) & ~7, first = part * share;
-        const int32_t last = first + share < pieces ? first + share : pieces;  // share <= kCopyThreads * kCopyVectors
+        const int32_t pieces = tokens * a.heads * a.pieces, share = ((pieces + a.slices - 1) / a.slices + 7) & ~7, first = slice * share;
+        const int32_t last = first + share < pieces ? first + share : pieces;
         if (first >= last || from == to) continue;
         const int32_t run = s.runs == kWhole ? pieces : s.runs == kTokens ? a.heads * a.pieces : s.runs == kHeads ? tokens * a.pieces : a.pieces;
         const char *const src = s.data + 2 * (layer * s.layer + from * s.page);
         char *const dst = s.data + 2 * (layer * s.layer + to * s.page);
-        Piece x[kCopyVectors];
-        int64_t at[kCopyVectors];
+        for (int32_t e0 = first + static_cast<int32_t>(threadIdx.x); e0 < last; e0 += kCopyThreads * kCopyVectors) {
+            Piece x[kCopyVectors];
+            int64_t at[kCopyVectors];
 #pragma unroll
-        for (int v = 0; v < kCopyVectors; ++v) {
-            const int32_t e = first + v * kCopyThreads + threadIdx.x;
-            at[v] = -1;
-            if (e < last) {
-                if (s.runs == kWhole) {
-                    at[v] = static_cast<int64_t>(e) * kValues;
-                } else {
-                    const int32_t o = e / run, rest = e - o * run;
-                    const int64_t step = s.runs == kTokens ? o * s.token : s.runs == kHeads ? o * s.head : o / a.heads * s.token + o % a.heads * s.head;
-                    at[v] = step + static_cast<int64_t>(rest) * kValues;
+            for (int v = 0; v < kCopyVectors; ++v) {
+                const int32_t e = e0 + v * kCopyThreads;
+                at[v] = -1;
+                if (e < last) {
+                    if (s.runs == kWhole) {
+                        at[v] = static_cast<int64_t>(e) * kValues;
+                    } else {
+                        const int32_t o = e / run, rest = e - o * run;
+                        const int64_t step = s.runs == kTokens ? o * s.token : s.runs == kHeads ? o * s.head : o / a.heads * s.token + o % a.heads * s.head;
+                        at[v] = step + static_cast<int64_t>(rest) * kValues;
+                    }
+                    x[v] = *reinterpret_cast<const Piece *>(src + 2 * at[v]);
                 }
-                x[v] = *reinterpret_cast<const Piece *>(src + 2 * at[v]);
             }
-        }
 #pragma unroll
-        for (int v = 0; v < kCopyVectors; ++v)
-            if (at[v] >= 0) *reinterpret_cast<Piece *>(dst + 2 * at[v]) = x[v];
+            for (int v = 0; v < kCopyVectors; ++v)
+                if (at[v] >= 0) *reinterpret_cast<Piece *>(dst + 2 * at[v]) = x[v];
+        }
     }
 }
 
@@ -542,8 +586,10 @@ int copy_pages(const cg_copy_job &j, const int32_t *count, bool early, cudaStrea
     const bool vec = j.head_size % 8 == 0 && vectors(a.sides[0]) && vectors(a.sides[1]);
     a.pieces = vec ? j.head_size / 8 : j.head_size;
     const int64_t pieces = static_cast<int64_t>(j.page_size) * j.heads * a.pieces;
-    a.parts = static_cast<int32_t>((pieces + kCopyThreads * kCopyVectors - 1) / (kCopyThreads * kCopyVectors));
-    const int64_t units = 2 * static_cast<int64_t>(j.nlayers) * a.parts * j.ncopies, most = static_cast<int64_t>(sm_count()) * 8;
+    // as many slices as give every block some units, none below what a block copies at a time
+    const int64_t parts = (pieces + kCopyThreads * kCopyVectors - 1) / (kCopyThreads * kCopyVectors), most = static_cast<int64_t>(sm_count()) * 8;
+    const int64_t pages = 2 * static_cast<int64_t>(j.nlayers) * j.ncopies, slices = (4 * most + pages - 1) / pages, units = pages * (slices < parts ? slices : parts);
+    a.slices = static_cast<int32_t>(slices < parts ? slices : parts);
     const dim3 grid(static_cast<unsigned>(units < most ? units : most));
     return vec ? launch(copy_pages_kernel<uint4>, grid, kCopyThreads, 0, early, st, a) : launch(copy_pages_kernel<uint16_t>, grid, kCopyThreads, 0, early, st, a);
 }
@@ -633,12 +679,15 @@ extern "C" int cg_fork_pages(const cg_pages_job *job, const cg_copy_job *copy, v
     if (static_cast<int64_t>(rows) * parts > INT32_MAX) return CG_E_SHAPE;
     if (const int rc = launch(fork_tables_kernel, dim3(rows * parts), kRowThreads, 0, false, st, a)) return rc;
     if (j.nnew == 0) return CG_OK;
-    if (const int rc = launch(fork_writers_kernel, dim3(kClusterBlocks), kClusterThreads, 0, true, st, a)) return rc;
+    const bool alone = j.num_pages <= kAlonePages && j.nnew <= kClusterThreads;
+    if (const int rc = alone ? launch(fork_writers_kernel<1>, dim3(1), kClusterThreads, 0, true, st, a)
+                             : launch(fork_writers_kernel<kClusterBlocks>, dim3(kClusterBlocks), kClusterThreads, 0, true, st, a))
+        return rc;
     if (!copy) return CG_OK;
     cg_copy_job c = *copy;
     c.src = j.moves, c.dst = j.moves + j.nnew, c.tokens = j.moves + 2 * static_cast<int64_t>(j.nnew);
     c.wide = 0, c.ncopies = j.nnew, c.status = j.status;
-    return copy_pages(c, a.copies, false, st);
+    return copy_pages(c, a.copies, true, st);
 }
 
 extern "C" int cg_free_pages(const cg_pages_job *job, void *stream) {
@@ -662,7 +711,9 @@ extern "C" int cg_extend_pages(const cg_pages_job *job, void *stream) {
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Slots of a few tokens a row are the cluster's work too, those of prompts a grid's.
     const bool together = j.ntokens <= kSlotsTogether;
-    if (const int rc = launch(extend_pages_kernel, dim3(kClusterBlocks), kClusterThreads, 0, false, st, a, together ? 1 : 0)) return rc;
+    const bool alone = j.num_pages <= kAlonePages && j.nrows <= kClusterThreads && j.ntokens <= 4 * kClusterThreads;
+    if (alone) return launch(extend_pages_kernel<1>, dim3(1), kClusterThreads, 0, false, st, a, 1);
+    if (const int rc = launch(extend_pages_kernel<kClusterBlocks>, dim3(kClusterBlocks), kClusterThreads, 0, false, st, a, together ? 1 : 0)) return rc;
     if (together) return CG_OK;
     const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(j.ntokens) + kRowThreads - 1) / kRowThreads);
     return launch(slots_kernel, dim3(blocks), kRowThreads, 0, true, st, a);
@@ -681,15 +732,17 @@ extern "C" int cg_compact_pages(const cg_pages_job *job, const cg_copy_job *copy
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int32_t *const words = reinterpret_cast<int32_t *>(part_of(j, 0));
     CompactArgs a{table_of(j), j.table, j.refs, j.places, j.moves, words, words + 1};
-    if (const int rc = launch(compact_places_kernel, dim3(kClusterBlocks), kClusterThreads, 0, false, st, a)) return rc;
+    if (const int rc = j.num_pages <= kAlonePages / 4 ? launch(compact_places_kernel<1>, dim3(1), kClusterThreads, 0, false, st, a)
+                                                      : launch(compact_places_kernel<kClusterBlocks>, dim3(kClusterBlocks), kClusterThreads, 0, false, st, a))
+        return rc;
     if (j.nrows && j.width) {
         const int64_t blocks = static_cast<int64_t>(j.nrows) * ((j.width + kRowColumns - 1) / kRowColumns);
         if (blocks > INT32_MAX) return CG_E_SHAPE;
-        if (const int rc = launch(compact_tables_kernel, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, false, st, a)) return rc;
+        if (const int rc = launch(compact_tables_kernel, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, true, st, a)) return rc;
     }
     if (!copy) return CG_OK;
     cg_copy_job c = *copy;
     c.src = j.moves, c.dst = j.moves + j.num_pages / 2, c.tokens = nullptr;
     c.wide = 0, c.ncopies = static_cast<int32_t>(j.num_pages / 2), c.status = j.status;
-    return copy_pages(c, a.copies, false, st);
+    return copy_pages(c, a.copies, true, st);
 }
