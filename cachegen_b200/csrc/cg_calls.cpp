@@ -810,7 +810,7 @@ struct Tables {
             !rows_of(a_table, at::kInt, dev, 2, Use::kWritten, &table) || (a_status != Py_None && (!indices_of(a_status, dev, false, &status) || status.numel() != 1)))
             return false;
         rows = lens.numel(), width = table.size(1), pages = refs.numel();
-        return table.size(0) == rows && rows <= CG_MAX_REQUESTS && pages <= INT32_MAX - 512;
+        return table.size(0) == rows && rows <= CG_MAX_REQUESTS && pages <= INT32_MAX - 1024;
     }
     bool fill(cg_pages_job *job, int64_t page_size) const {
         if (page_size <= 0 || page_size > INT32_MAX || width > INT32_MAX / page_size) return false;

@@ -18,7 +18,7 @@ constexpr int kRowThreads = 256, kRowColumns = 1024;  // of a block that works o
 constexpr int kCopyThreads = 256, kCopyVectors = 4;
 constexpr int64_t kAlonePages = 32768;  // up to here, and with a row a thread, one block does: 2,600 pages and 8 rows extended in 9 us by eight blocks
 constexpr int32_t kSlotsTogether = 2 * kClusterBlocks * kClusterThreads;
-constexpr int64_t kMostPages = INT32_MAX - 512;  // a warp counts on behind its last page
+constexpr int64_t kMostPages = INT32_MAX - 1024;  // a warp counts on behind its last page
 
 struct Table {
     const int32_t *entries, *lens;
@@ -113,31 +113,48 @@ template <int BLOCKS> __device__ __forceinline__ Sums over_warps(int64_t a, int6
     return s;
 }
 
-// A warp's run of pages, [first, last), four neighbouring ones a lane at a time; runs of warps and blocks follow one another.
+constexpr int32_t kRunStep = 512;
+// A warp's run of pages, [first, last); runs of warps and blocks follow one another.
 struct Run {
     int32_t first, last;
 };
 template <int BLOCKS> __device__ __forceinline__ Run run_of(int32_t num_pages) {
     constexpr int kAll = BLOCKS * kClusterWarps;
-    const int64_t run = ((static_cast<int64_t>(num_pages) + kAll - 1) / kAll + 127) / 128 * 128;
+    const int64_t run = ((static_cast<int64_t>(num_pages) + kAll - 1) / kAll + kRunStep - 1) / kRunStep * kRunStep;
     const int64_t first = (cluster_rank<BLOCKS>() * kClusterWarps + static_cast<int>(threadIdx.x >> 5)) * run, last = first + run;
     return Run{static_cast<int32_t>(first < num_pages ? first : num_pages), static_cast<int32_t>(last < num_pages ? last : num_pages)};
 }
-// The counts of pages p .. p + 3; `behind` for those at `last` and behind.
-__device__ __forceinline__ int4 counts_at(const int32_t *refs, int32_t p, int32_t last, bool vectors, int32_t behind) {
-    if (vectors && p <= last - 4) return *reinterpret_cast<const int4 *>(refs + p);
-    int4 c = make_int4(behind, behind, behind, behind);
-    if (p < last) c.x = refs[p];
-    if (p < last - 1) c.y = refs[p + 1];
-    if (p < last - 2) c.z = refs[p + 2];
-    if (p < last - 3) c.w = refs[p + 3];
-    return c;
+// The counts of a lane's sixteen of the run's pages p0 .. p0 + kRunStep - 1, four by four `apart` pages from one another; `behind` for those
+// behind the run.  Whole steps are loaded without a branch in between, all at once.
+__device__ __forceinline__ void counts_of(const int32_t *refs, int32_t p, int32_t apart, const Run &run, int32_t p0, bool vectors, int32_t behind, int4 (&c)[4]) {
+    if (vectors && p0 <= run.last - kRunStep) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = *reinterpret_cast<const int4 *>(refs + p + i * apart);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int32_t q = p + i * apart;
+        c[i].x = q < run.last ? refs[q] : behind;
+        c[i].y = q < run.last - 1 ? refs[q + 1] : behind;
+        c[i].z = q < run.last - 2 ? refs[q + 2] : behind;
+        c[i].w = q < run.last - 3 ? refs[q + 3] : behind;
+    }
 }
-__device__ __forceinline__ int32_t zeros(const int4 &c) { return (c.x == 0) + (c.y == 0) + (c.z == 0) + (c.w == 0); }
+__device__ __forceinline__ int32_t zeros(const int4 (&c)[4]) {
+    int32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += (c[i].x == 0) + (c[i].y == 0) + (c[i].z == 0) + (c[i].w == 0);
+    return n;
+}
 __device__ __forceinline__ int32_t free_in(const int32_t *refs, const Run &run, bool vectors) {
     int32_t n = 0;
-#pragma unroll 4
-    for (int32_t p = run.first + 4 * static_cast<int32_t>(threadIdx.x & 31); p < run.last; p += 128) n += zeros(counts_at(refs, p, run.last, vectors, 1));
+#pragma unroll 2
+    for (int32_t p0 = run.first; p0 < run.last; p0 += kRunStep) {
+        int4 c[4];
+        counts_of(refs, p0 + 4 * static_cast<int32_t>(threadIdx.x & 31), 128, run, p0, vectors, 1, c);
+        n += zeros(c);
+    }
     return __reduce_add_sync(~0u, n);
 }
 
@@ -155,18 +172,19 @@ __device__ __forceinline__ int64_t take_free(const int32_t *refs, int32_t num_pa
     const int64_t most = s.all_b;
     int64_t rank = s.a;
     if (free && rank < most) {
-        for (int32_t p0 = run.first; p0 < run.last && rank < most; p0 += 128) {
-            const int32_t p = p0 + 4 * static_cast<int32_t>(threadIdx.x & 31);
-            const int4 c = counts_at(refs, p, run.last, vectors, 1);
-            const int32_t mine = zeros(c), before = sum_upto(mine);
+        for (int32_t p0 = run.first; p0 < run.last && rank < most; p0 += kRunStep) {  // sixteen neighbouring pages a lane
+            const int32_t p = p0 + 16 * static_cast<int32_t>(threadIdx.x & 31);
+            int4 c[4];
+            counts_of(refs, p, 4, run, p0, vectors, 1, c);
+            const int32_t mine = zeros(c);
+            const int32_t before = sum_upto(mine);
             int64_t at = rank + before - mine;
-            if (c.x == 0 && at < most) list[at] = p;
-            at += c.x == 0;
-            if (c.y == 0 && at < most) list[at] = p + 1;
-            at += c.y == 0;
-            if (c.z == 0 && at < most) list[at] = p + 2;
-            at += c.z == 0;
-            if (c.w == 0 && at < most) list[at] = p + 3;
+            const auto put = [&](int32_t count, int32_t page) {
+                if (count == 0 && at < most) list[at] = page;
+                at += count == 0;
+            };
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put(c[i].x, p + 4 * i), put(c[i].y, p + 4 * i + 1), put(c[i].z, p + 4 * i + 2), put(c[i].w, p + 4 * i + 3);
             rank += __shfl_sync(~0u, before, 31);
         }
     }
@@ -434,21 +452,21 @@ __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads
     const int32_t front = n < a.t.num_pages ? __ldcg(a.before_middle) : n, made = n - front;  // holes in front of n = held pages behind
     const int32_t half = a.t.num_pages / 2;
     int32_t before = static_cast<int32_t>(sums.b);  // pages held in front of p0
-    for (int32_t p0 = run.first; p0 < run.last; p0 += 128) {
-        const int32_t p = p0 + 4 * lane;
-        const int4 c = counts_at(a.refs, p, run.last, vectors, 0);
-        const int32_t held = 4 - zeros(c), upto = sum_upto(held);
+    for (int32_t p0 = run.first; p0 < run.last; p0 += kRunStep) {
+        const int32_t p = p0 + 16 * lane;
+        int4 c[4];
+        counts_of(a.refs, p, 4, run, p0, vectors, 0, c);
+        const int32_t held = 16 - zeros(c), upto = sum_upto(held);
         int32_t at = before + upto - held;
-        const int32_t count[4] = {c.x, c.y, c.z, c.w};
+        const auto place = [&](int32_t count, int32_t q) {
+            if (q >= run.last) return;
+            if (count != 0 && q >= n) a.moves[at - front] = q;
+            if (count == 0 && q < n) a.moves[half + q - at] = q;
+            a.places[q] = count != 0 ? q : -1;
+            at += count != 0;
+        };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int32_t q = p + i;
-            if (p >= run.last - i) break;
-            if (count[i] != 0 && q >= n) a.moves[at - front] = q;
-            if (count[i] == 0 && q < n) a.moves[half + q - at] = q;
-            a.places[q] = count[i] != 0 ? q : -1;
-            at += count[i] != 0;
-        }
+        for (int i = 0; i < 4; ++i) place(c[i].x, p + 4 * i), place(c[i].y, p + 4 * i + 1), place(c[i].z, p + 4 * i + 2), place(c[i].w, p + 4 * i + 3);
         before += __shfl_sync(~0u, upto, 31);
     }
     cluster_barrier<BLOCKS>();

@@ -523,7 +523,7 @@ def _tables(page_table, kv_lens, refs, page_size, device, written):
     job = _lib.PagesJob()
     job.table, job.kv_lens, job.refs, job.status = page_table.data_ptr(), kv_lens.data_ptr(), refs.data_ptr(), _address(_status_of(refs))
     job.table_row = page_table.stride(0)
-    _check(refs.shape[0] <= 2 ** 31 - 513, f"refs: {refs.shape[0]} is more than a call takes")
+    _check(refs.shape[0] <= 2 ** 31 - 1025, f"refs: {refs.shape[0]} is more than a call takes")
     job.num_pages = refs.shape[0]
     _set(job, nrows=B, width=W, page_size=page_size)
     return job
