@@ -16,7 +16,7 @@ namespace {
 constexpr int kClusterBlocks = 8, kClusterThreads = 512, kClusterWarps = kClusterThreads / 32;
 constexpr int kRowThreads = 256, kRowColumns = 1024;  // of a block that works on a row of a table
 constexpr int kCopyThreads = 256, kCopyVectors = 4;
-constexpr int64_t kAlonePages = 32768;  // up to here, and with a row a thread, one block does: 2,600 pages and 8 rows extended in 9 us by eight blocks
+constexpr int64_t kAlonePages = 8192;  // up to here, and with a row a thread, one block does: 2,600 pages and 8 rows extended in 9 us by eight blocks
 constexpr int32_t kSlotsTogether = 2 * kClusterBlocks * kClusterThreads;
 constexpr int64_t kMostPages = INT32_MAX - 1024;  // a warp counts on behind its last page
 
@@ -78,62 +78,62 @@ template <class T> __device__ __forceinline__ T sum_upto(T x) {  // over the war
     }
     return x;
 }
-// What a block's warps tell the other blocks.
+// Room of a block for the sums: its warps' numbers, its own for the other blocks, and what the blocks in front and all of them have.
 struct Told {
-    int64_t a[kClusterWarps], b[kClusterWarps];
+    int64_t a[kClusterWarps], b[kClusterWarps], block[2], front[2], all[2];
 };
 struct Sums {  // in front of this warp, and of all warps
     int64_t a, b, all_a, all_b;
 };
-// Sums over the cluster's warps of two numbers of each, in one step: a lane reads four warps' numbers.  A barrier of the cluster stands in it.
+// Sums over the cluster's warps of two numbers of each.  One warp of a block asks the other blocks: with every warp asking for every number it took 10,000 cycles.
+// A barrier of the cluster stands in it.
 template <int BLOCKS> __device__ __forceinline__ Sums over_warps(int64_t a, int64_t b, Told *told) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = cluster_rank<BLOCKS>() * kClusterWarps + warp;
+    static_assert(kClusterWarps <= 32 && BLOCKS <= 32, "a lane each");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (lane == 0) told->a[warp] = a, told->b[warp] = b;
+    __syncthreads();
+    const int64_t x = lane < kClusterWarps ? told->a[lane] : 0, y = lane < kClusterWarps ? told->b[lane] : 0;
+    const int64_t upto_x = sum_upto(x), upto_y = sum_upto(y);
+    Sums s{__shfl_sync(~0u, upto_x - x, warp), __shfl_sync(~0u, upto_y - y, warp), __shfl_sync(~0u, upto_x, 31), __shfl_sync(~0u, upto_y, 31)};
+    if (BLOCKS == 1) return s;
+    if (threadIdx.x == 0) told->block[0] = s.all_a, told->block[1] = s.all_b;
     cluster_barrier<BLOCKS>();
-    constexpr int kEach = (BLOCKS * kClusterWarps + 31) / 32;
-    static_assert(kClusterWarps % kEach == 0, "a lane reads one block's");
-    int64_t x[kEach], y[kEach], sum_a = 0, sum_b = 0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int w = lane * kEach + i;
-        const bool there = w < BLOCKS * kClusterWarps;
-        x[i] = there ? of_block<BLOCKS>(&told->a[w % kClusterWarps], w / kClusterWarps) : 0;
-        y[i] = there ? of_block<BLOCKS>(&told->b[w % kClusterWarps], w / kClusterWarps) : 0;
+    if (warp == 0) {
+        const int64_t p = lane < BLOCKS ? of_block<BLOCKS>(&told->block[0], lane) : 0, q = lane < BLOCKS ? of_block<BLOCKS>(&told->block[1], lane) : 0;
+        const int64_t upto_p = sum_upto(p), upto_q = sum_upto(q);
+        if (lane == cluster_rank<BLOCKS>()) told->front[0] = upto_p - p, told->front[1] = upto_q - q;
+        if (lane == 31) told->all[0] = upto_p, told->all[1] = upto_q;
     }
-    int64_t front_a = 0, front_b = 0;  // of this lane's warps those in front of mine
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        sum_a += x[i], sum_b += y[i];
-        if (lane * kEach + i < me) front_a += x[i], front_b += y[i];
-    }
-    Sums s;
-    const int64_t upto_a = sum_upto(front_a), upto_b = sum_upto(front_b), all_a = sum_upto(sum_a), all_b = sum_upto(sum_b);
-    s.a = __shfl_sync(~0u, upto_a, 31), s.b = __shfl_sync(~0u, upto_b, 31);
-    s.all_a = __shfl_sync(~0u, all_a, 31), s.all_b = __shfl_sync(~0u, all_b, 31);
+    __syncthreads();
+    s.a += told->front[0], s.b += told->front[1];
+    s.all_a = told->all[0], s.all_b = told->all[1];
     return s;
 }
 
-constexpr int32_t kRunStep = 512;
+// Steps of a warp: for small caches of four pages a lane, so that more warps have some, else of sixteen.
+template <int BLOCKS> constexpr int32_t kQuads = BLOCKS > 1 ? 4 : 1;
+template <int BLOCKS> constexpr int32_t kRunStep = 128 * kQuads<BLOCKS>;
 // A warp's run of pages, [first, last); runs of warps and blocks follow one another.
 struct Run {
     int32_t first, last;
 };
 template <int BLOCKS> __device__ __forceinline__ Run run_of(int32_t num_pages) {
     constexpr int kAll = BLOCKS * kClusterWarps;
-    const int64_t run = ((static_cast<int64_t>(num_pages) + kAll - 1) / kAll + kRunStep - 1) / kRunStep * kRunStep;
+    const int64_t run = ((static_cast<int64_t>(num_pages) + kAll - 1) / kAll + kRunStep<BLOCKS> - 1) / kRunStep<BLOCKS> * kRunStep<BLOCKS>;
     const int64_t first = (cluster_rank<BLOCKS>() * kClusterWarps + static_cast<int>(threadIdx.x >> 5)) * run, last = first + run;
     return Run{static_cast<int32_t>(first < num_pages ? first : num_pages), static_cast<int32_t>(last < num_pages ? last : num_pages)};
 }
-// The counts of a lane's sixteen of the run's pages p0 .. p0 + kRunStep - 1, four by four `apart` pages from one another; `behind` for those
-// behind the run.  Whole steps are loaded without a branch in between, all at once.
-__device__ __forceinline__ void counts_of(const int32_t *refs, int32_t p, int32_t apart, const Run &run, int32_t p0, bool vectors, int32_t behind, int4 (&c)[4]) {
-    if (vectors && p0 <= run.last - kRunStep) {
+// The counts of a lane's pages of a step that begins at p0, four by four `apart` pages from one another; `behind` for those behind the run.  Whole steps are loaded
+// without a branch in between, all at once.
+template <int QUADS>
+__device__ __forceinline__ void counts_of(const int32_t *refs, int32_t p, int32_t apart, const Run &run, int32_t p0, bool vectors, int32_t behind, int4 (&c)[QUADS]) {
+    if (vectors && p0 <= run.last - 128 * QUADS) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = *reinterpret_cast<const int4 *>(refs + p + i * apart);
+        for (int i = 0; i < QUADS; ++i) c[i] = *reinterpret_cast<const int4 *>(refs + p + i * apart);
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < QUADS; ++i) {
         const int32_t q = p + i * apart;
         c[i].x = q < run.last ? refs[q] : behind;
         c[i].y = q < run.last - 1 ? refs[q + 1] : behind;
@@ -141,17 +141,17 @@ __device__ __forceinline__ void counts_of(const int32_t *refs, int32_t p, int32_
         c[i].w = q < run.last - 3 ? refs[q + 3] : behind;
     }
 }
-__device__ __forceinline__ int32_t zeros(const int4 (&c)[4]) {
+template <int QUADS> __device__ __forceinline__ int32_t zeros(const int4 (&c)[QUADS]) {
     int32_t n = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n += (c[i].x == 0) + (c[i].y == 0) + (c[i].z == 0) + (c[i].w == 0);
+    for (int i = 0; i < QUADS; ++i) n += (c[i].x == 0) + (c[i].y == 0) + (c[i].z == 0) + (c[i].w == 0);
     return n;
 }
-__device__ __forceinline__ int32_t free_in(const int32_t *refs, const Run &run, bool vectors) {
+template <int BLOCKS> __device__ __forceinline__ int32_t free_in(const int32_t *refs, const Run &run, bool vectors) {
     int32_t n = 0;
 #pragma unroll 2
-    for (int32_t p0 = run.first; p0 < run.last; p0 += kRunStep) {
-        int4 c[4];
+    for (int32_t p0 = run.first; p0 < run.last; p0 += kRunStep<BLOCKS>) {
+        int4 c[kQuads<BLOCKS>];
         counts_of(refs, p0 + 4 * static_cast<int32_t>(threadIdx.x & 31), 128, run, p0, vectors, 1, c);
         n += zeros(c);
     }
@@ -166,30 +166,30 @@ __device__ __forceinline__ int64_t take_free(const int32_t *refs, int32_t num_pa
                                              int64_t *free_pages) {
     const Run run = run_of<BLOCKS>(num_pages);
     const bool vectors = reinterpret_cast<uintptr_t>(refs) % 16 == 0;
-    const int32_t free = free_in(refs, run, vectors);
+    const int32_t free = free_in<BLOCKS>(refs, run, vectors);
     const int64_t upto = sum_upto(wanted);
     const Sums s = over_warps<BLOCKS>(free, __shfl_sync(~0u, upto, 31), told);
-    const int64_t most = s.all_b;
-    int64_t rank = s.a;
+    const int32_t most = static_cast<int32_t>(s.all_b < num_pages ? s.all_b : num_pages);
+    int32_t rank = static_cast<int32_t>(s.a);
     if (free && rank < most) {
-        for (int32_t p0 = run.first; p0 < run.last && rank < most; p0 += kRunStep) {  // sixteen neighbouring pages a lane
-            const int32_t p = p0 + 16 * static_cast<int32_t>(threadIdx.x & 31);
-            int4 c[4];
+        for (int32_t p0 = run.first; p0 < run.last && rank < most; p0 += kRunStep<BLOCKS>) {  // neighbouring pages a lane
+            const int32_t p = p0 + 4 * kQuads<BLOCKS> * static_cast<int32_t>(threadIdx.x & 31);
+            int4 c[kQuads<BLOCKS>];
             counts_of(refs, p, 4, run, p0, vectors, 1, c);
             const int32_t mine = zeros(c);
             const int32_t before = sum_upto(mine);
-            int64_t at = rank + before - mine;
+            int32_t at = rank + before - mine;
             const auto put = [&](int32_t count, int32_t page) {
                 if (count == 0 && at < most) list[at] = page;
                 at += count == 0;
             };
 #pragma unroll
-            for (int i = 0; i < 4; ++i) put(c[i].x, p + 4 * i), put(c[i].y, p + 4 * i + 1), put(c[i].z, p + 4 * i + 2), put(c[i].w, p + 4 * i + 3);
+            for (int i = 0; i < kQuads<BLOCKS>; ++i) put(c[i].x, p + 4 * i), put(c[i].y, p + 4 * i + 1), put(c[i].z, p + 4 * i + 2), put(c[i].w, p + 4 * i + 3);
             rank += __shfl_sync(~0u, before, 31);
         }
     }
     cluster_barrier<BLOCKS>();
-    *wanted_all = most, *free_pages = s.all_a;
+    *wanted_all = s.all_b, *free_pages = s.all_a;
     return s.b + upto - wanted;
 }
 
@@ -439,7 +439,7 @@ __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads
     let_next_launch_start();
     const Run run = run_of<BLOCKS>(a.t.num_pages);
     const bool vectors = reinterpret_cast<uintptr_t>(a.refs) % 16 == 0;
-    const int32_t lane = threadIdx.x & 31, free = free_in(a.refs, run, vectors);
+    const int32_t lane = threadIdx.x & 31, free = free_in<BLOCKS>(a.refs, run, vectors);
     const Sums sums = over_warps<BLOCKS>(free, run.last - run.first - free, &told);
     const int32_t n = static_cast<int32_t>(sums.all_b);  // pages held
     if (n >= run.first && n < run.last) {  // the warp whose pages n is one of: those held in front of it
@@ -452,11 +452,11 @@ __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads
     const int32_t front = n < a.t.num_pages ? __ldcg(a.before_middle) : n, made = n - front;  // holes in front of n = held pages behind
     const int32_t half = a.t.num_pages / 2;
     int32_t before = static_cast<int32_t>(sums.b);  // pages held in front of p0
-    for (int32_t p0 = run.first; p0 < run.last; p0 += kRunStep) {
-        const int32_t p = p0 + 16 * lane;
-        int4 c[4];
+    for (int32_t p0 = run.first; p0 < run.last; p0 += kRunStep<BLOCKS>) {
+        const int32_t p = p0 + 4 * kQuads<BLOCKS> * lane;
+        int4 c[kQuads<BLOCKS>];
         counts_of(a.refs, p, 4, run, p0, vectors, 0, c);
-        const int32_t held = 16 - zeros(c), upto = sum_upto(held);
+        const int32_t held = 4 * kQuads<BLOCKS> - zeros(c), upto = sum_upto(held);
         int32_t at = before + upto - held;
         const auto place = [&](int32_t count, int32_t q) {
             if (q >= run.last) return;
@@ -466,7 +466,7 @@ __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads
             at += count != 0;
         };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) place(c[i].x, p + 4 * i), place(c[i].y, p + 4 * i + 1), place(c[i].z, p + 4 * i + 2), place(c[i].w, p + 4 * i + 3);
+        for (int i = 0; i < kQuads<BLOCKS>; ++i) place(c[i].x, p + 4 * i), place(c[i].y, p + 4 * i + 1), place(c[i].z, p + 4 * i + 2), place(c[i].w, p + 4 * i + 3);
         before += __shfl_sync(~0u, upto, 31);
     }
     cluster_barrier<BLOCKS>();
@@ -750,7 +750,7 @@ extern "C" int cg_compact_pages(const cg_pages_job *job, const cg_copy_job *copy
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int32_t *const words = reinterpret_cast<int32_t *>(part_of(j, 0));
     CompactArgs a{table_of(j), j.table, j.refs, j.places, j.moves, words, words + 1};
-    if (const int rc = j.num_pages <= kAlonePages / 4 ? launch(compact_places_kernel<1>, dim3(1), kClusterThreads, 0, false, st, a)
+    if (const int rc = j.num_pages <= kAlonePages ? launch(compact_places_kernel<1>, dim3(1), kClusterThreads, 0, false, st, a)
                                                       : launch(compact_places_kernel<kClusterBlocks>, dim3(kClusterBlocks), kClusterThreads, 0, false, st, a))
         return rc;
     if (j.nrows && j.width) {
