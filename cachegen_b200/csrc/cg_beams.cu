@@ -196,7 +196,7 @@ struct Shared {
     uint16_t tiles[kTileRoom];                // tile * kRowThreads + thread of those that have candidates
     int32_t ntiles, found;
     float tops[kRowWarps], sums[kRowWarps], bases[kRowWarps];  // a warp's sum is sums * 2 ^ bases
-    alignas(8) int32_t digits[256];
+    alignas(8) int32_t digits[256];           // also of the threads the largest logits' keys
     int32_t digit, left;
     bool again;                               // a sum that the quick way does not give
 };
@@ -272,7 +272,7 @@ __device__ __noinline__ float write_first(Shared &s, const Row<DT> x, int32_t fr
     };
     const auto count = [&](auto digit) {  // digit(key, place): -1 for those that do not count
         __syncthreads();
-        s.digits[threadIdx.x] = 0;
+        for (int d = threadIdx.x; d < 256; d += kRowThreads) s.digits[d] = 0;
         __syncthreads();
         int32_t same = -1, times = 0;  // neighbours are often the same
         each([&](uint32_t key, uint32_t place) {
@@ -285,7 +285,6 @@ __device__ __noinline__ float write_first(Shared &s, const Row<DT> x, int32_t fr
         });
         if (same >= 0) atomicAdd(&s.digits[same], times);
     };
-    static_assert(kRowThreads == 256, "a digit a thread");
     __syncthreads();
     if (threadIdx.x == 0) s.left = k, s.found = 0;
     uint32_t least = 0, last = 0;
