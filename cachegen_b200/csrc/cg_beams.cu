@@ -606,14 +606,13 @@ __device__ int32_t sort_row(const BeamArgs &a, int32_t row, float least, uint64_
 }
 
 // A continuation of a request: its score, and what decides between equal ones, the beam, the logit and the token in one number.
-struct alignas(16) Choice {
+struct Choice {
     uint64_t key;  // the score, in an order in which numbers without a sign compare
     uint64_t rest;
     __device__ __forceinline__ double total() const { return __longlong_as_double(static_cast<long long>(key >> 63 ? key & ~(1ull << 63) : ~key)); }
     __device__ __forceinline__ int32_t beam() const { return 255 - static_cast<int32_t>(rest >> 56); }
     __device__ __forceinline__ int32_t token() const { return 0xFFFFFF - static_cast<int32_t>(rest & 0xFFFFFF); }
     __device__ __forceinline__ float x() const { return from_ordered(static_cast<uint32_t>(rest >> 24)); }
-    __device__ __forceinline__ bool before(const Choice &o) const { return key > o.key || (key == o.key && rest > o.rest); }
 };
 __device__ __forceinline__ uint64_t rest_of(int32_t beam, float x, int32_t token) {
     return static_cast<uint64_t>(255 - beam) << 56 | static_cast<uint64_t>(ordered(x)) << 24 | static_cast<uint64_t>(0xFFFFFF - token);
@@ -623,10 +622,17 @@ __device__ __forceinline__ uint64_t ordered_double(double x) {
     return u >> 63 ? ~u : u | 1ull << 63;
 }
 
+// A list of them, keys and rests apart: sorting reads the keys.
+struct Choices {
+    uint64_t *keys, *rests;
+    __device__ __forceinline__ Choice at(int32_t i) const { return Choice{keys[i], rests[i]}; }
+    __device__ __forceinline__ void put(int32_t i, const Choice &c) const { keys[i] = c.key, rests[i] = c.rest; }
+};
+
 // How room in shared memory is divided; K beams, W warps
 struct ChooseRoom {
     double *base, *sums;      // [K]: score - log sum exp(x - top); a block's share of a sum
-    Choice *list, *sorted;    // [list_room], [kSorted]; in their place, where these are too small,
+    Choices list, sorted;     // [list_room], [kSorted]; in their place, where these are too small,
     uint64_t *best, *sorting; // [K][k], [W][sort_room]
     float *top;               // [K]
     int32_t *count;           // [K]
@@ -639,8 +645,10 @@ struct ChooseRoom {
     }
     static size_t bytes(const BeamArgs &a, int warps) { return lists(a, warps) + a.beams * (2 * sizeof(double) + 3 * sizeof(float)) + sizeof(float) * (1 + kSorted); }
     __device__ ChooseRoom(char *at, const BeamArgs &a, int warps) {
-        list = reinterpret_cast<Choice *>(at);
-        sorted = list + a.list_room;
+        list.keys = reinterpret_cast<uint64_t *>(at);
+        list.rests = list.keys + a.list_room;
+        sorted.keys = list.rests + a.list_room;
+        sorted.rests = sorted.keys + kSorted;
         best = reinterpret_cast<uint64_t *>(at);
         sorting = best + static_cast<int64_t>(a.beams) * a.k;
         base = reinterpret_cast<double *>(at + lists(a, warps));
@@ -711,34 +719,45 @@ __device__ bool take_best(const BeamArgs &a, const ChooseRoom &r, int32_t reques
     return doubtful;
 }
 
-// The block puts n continuations in order: it counts those in front of each, which several threads share.  places: [kSorted], zeros before and after.
-__device__ __forceinline__ void sort_list(const Choice *list, Choice *sorted, int32_t n, int32_t *places) {
+// The block puts n continuations in order: it counts those in front of each, which several threads share, by their keys; rests are looked at where keys are the
+// same.  places: [kSorted], zeros before and after.
+__device__ __forceinline__ void sort_list(const Choices &list, const Choices &sorted, int32_t n, int32_t *places) {
     if (n == 0) return;
     int team = 1;
     while (2 * team * n <= static_cast<int>(blockDim.x)) team *= 2;
-    const int32_t each = blockDim.x / team;
+    const int32_t each = blockDim.x / team, share = ((n + team - 1) / team + 1) & ~1;
     for (int32_t i0 = 0; i0 < n; i0 += each) {
-        const int32_t i = i0 + threadIdx.x % each, first = threadIdx.x / each;
-        if (i < n) {
-            const Choice mine = list[i];
-            int32_t place = 0;
-#pragma unroll 4
-            for (int32_t j = first; j < n; j += team) place += list[j].before(mine);
-            atomicAdd(&places[i], place);
+        const int32_t i = i0 + threadIdx.x % each, first = threadIdx.x / each * share, last = min(n, first + share);
+        if (i < n && first < last) {
+            const uint64_t mine = list.keys[i];
+            int32_t place = 0, same = 0;
+            int32_t j = first;
+#pragma unroll 2
+            for (; j < last - 1; j += 2) {  // (first is even)
+                const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(list.keys + j);
+                place += (two.x > mine) + (two.y > mine);
+                same += (two.x == mine) + (two.y == mine);
+            }
+            if (j < last) place += list.keys[j] > mine, same += list.keys[j] == mine;
+            if (same > (i >= first && i < last)) {
+                const uint64_t rest = list.rests[i];
+                for (j = first; j < last; ++j) place += list.keys[j] == mine && list.rests[j] > rest;
+            }
+            if (place) atomicAdd(&places[i], place);
         }
     }
     __syncthreads();
     for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
-        sorted[places[i]] = list[i];
+        sorted.put(places[i], list.at(i));
         places[i] = 0;
     }
     __syncthreads();
 }
-__device__ __forceinline__ void write_sorted(const BeamArgs &a, const Choice *sorted, int32_t request, int32_t n) {
+__device__ __forceinline__ void write_sorted(const BeamArgs &a, const Choices &sorted, int32_t request, int32_t n) {
     for (int32_t i = threadIdx.x; i < a.k; i += blockDim.x) {
         const int64_t at = static_cast<int64_t>(request) * a.k + i;
         const bool there = i < n;
-        const Choice c = sorted[there ? i : 0];
+        const Choice c = sorted.at(there ? i : 0);
         a.out[at] = there ? static_cast<float>(c.total()) : -CUDART_INF_F;
         a.tokens[at] = there ? c.token() : -1;
         a.parents[at] = there ? request * a.beams + c.beam() : -1;
@@ -747,7 +766,7 @@ __device__ __forceinline__ void write_sorted(const BeamArgs &a, const Choice *so
 // The continuations that may be among the best, in *list; returns how many there are, more than `kSorted` if that is no use.  A bound that k of
 // one row reach drops most of them while they are read; where that leaves many, they are counted in bins, and all behind the bin of the k-th and the next one are
 // dropped.  Both leave room for what 32-bit sums are off.  *sorted is as large as kSorted.
-__device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const ChooseRoom &r, int32_t request, int32_t *counts, Choice **list, Choice **sorted) {
+__device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const ChooseRoom &r, int32_t request, int32_t *counts, Choices *list, Choices *sorted) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     double bound = -CUDART_INF;
     for (int32_t i = 0; i < a.beams; ++i) bound = fmax(bound, r.sums[i]);
@@ -771,7 +790,7 @@ __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const Choos
             if (lane >= d) upto += y;
         }
         const int32_t all = __shfl_sync(~0u, upto, 31);
-#pragma unroll 2
+#pragma unroll 1
         for (int32_t i0 = 0; i0 < all; i0 += 32) {
             const int32_t i = i0 + lane;
             int owner = 0;  // the first lane whose candidates end behind i
@@ -779,17 +798,13 @@ __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const Choos
             for (int d = 16; d; d /= 2)
                 if (__shfl_sync(~0u, upto, owner + d - 1) <= i) owner += d;
             const int32_t before = __shfl_sync(~0u, upto, owner) - __shfl_sync(~0u, count, owner), pair = p0 + owner * warps;
-            const bool here = i < all;
-            const int32_t beam = here ? pair / a.nparts : 0;
-            float2 c = make_float2(-CUDART_INF_F, 0.0f);
-            if (here) c = __ldcg(reinterpret_cast<const float2 *>(a.candidates + (first + pair) * a.room + (i - before)));
+            if (i >= all) continue;
+            const int32_t beam = pair / a.nparts;
+            const float2 c = __ldcg(reinterpret_cast<const float2 *>(a.candidates + (first + pair) * a.room + (i - before)));
             const double total = r.base[beam] + entering(c.x, r.top[beam]);
-            const bool kept = here && total >= bound && total > -CUDART_INF;
-            const uint32_t who = __ballot_sync(~0u, kept);
-            int32_t at = 0;
-            if (lane == 0 && who) at = atomicAdd(&counts[0], __popc(who));
-            at = __shfl_sync(~0u, at, 0) + __popc(who & ((1u << lane) - 1u));
-            if (kept && at < a.list_room) r.list[at] = Choice{ordered_double(total), rest_of(beam, c.x, __float_as_int(c.y))};
+            if (!(total >= bound && total > -CUDART_INF)) continue;
+            const int32_t at = atomicAdd(&counts[0], 1);
+            if (at < a.list_room) r.list.put(at, Choice{ordered_double(total), rest_of(beam, c.x, __float_as_int(c.y))});
         }
     }
     __syncthreads();
@@ -798,7 +813,7 @@ __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const Choos
     if (n <= kSortedAtOnce) return n;
     if (!(bound > -CUDART_INF)) {  // no row's part had k: from the least of the list on
         uint32_t least = ~0u;
-        for (int32_t i = threadIdx.x; i < n; i += blockDim.x) least = min(least, static_cast<uint32_t>(r.list[i].key >> 32));
+        for (int32_t i = threadIdx.x; i < n; i += blockDim.x) least = min(least, static_cast<uint32_t>(r.list.keys[i] >> 32));
         least = __reduce_min_sync(~0u, least);
         if (lane == 0) atomicMin(reinterpret_cast<uint32_t *>(&counts[1]), least);
         __syncthreads();
@@ -810,7 +825,7 @@ __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const Choos
     if (!(width > 1e-4f && width < 1e30f)) return n;
     static_assert(1e-4 > 16.0 * kRowError, "a bin is wider than what sums are off");
     const auto bin = [&](const Choice &c) { return min(kBins - 1, static_cast<int32_t>(static_cast<float>(c.total() - bound) * a_bin)); };
-    for (int32_t i = threadIdx.x; i < n; i += blockDim.x) atomicAdd(&r.places[bin(r.list[i])], 1);
+    for (int32_t i = threadIdx.x; i < n; i += blockDim.x) atomicAdd(&r.places[bin(r.list.at(i))], 1);
     __syncthreads();
     if (warp == 0) {  // the bin in which the k-th stands, counted from the last
         constexpr int kEach = kBins / 32;
@@ -833,10 +848,10 @@ __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const Choos
     const int32_t first_bin = counts[1] - 1;  // one bin more than is counted, wider than what sums are off
     for (int32_t i = threadIdx.x; i < kBins; i += blockDim.x) r.places[i] = 0;
     for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const Choice c = r.list[i];
+        const Choice c = r.list.at(i);
         if (bin(c) < first_bin) continue;
         const int32_t at = atomicAdd(&counts[0], 1);
-        if (at < kSorted) r.sorted[at] = c;
+        if (at < kSorted) r.sorted.put(at, c);
     }
     __syncthreads();
     *list = r.sorted, *sorted = r.list;
@@ -852,7 +867,7 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
     const int rank = choose_rank(), lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const int32_t request = blockIdx.x / kChooseBlocks;
     const ChooseRoom r(room, a, warps);
-    Choice *list = r.list, *sorted = r.sorted;
+    Choices list = r.list, sorted = r.sorted;
     int32_t n = 0;
     if (rank == 0) {
         for (int32_t i = threadIdx.x; i <= a.beams; i += blockDim.x) r.near[i] = 0;
@@ -887,8 +902,8 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
         if (n <= kSorted) {
             sort_list(list, sorted, n, r.places);
             for (int32_t i = threadIdx.x; i + 1 < n; i += blockDim.x) {
-                const Choice &p = sorted[i], &q = sorted[i + 1];
-                if (p.total() - q.total() <= 2.0 * kRowError && p.beam() != q.beam() && (i < a.k || sorted[a.k - 1].total() - p.total() <= 2.0 * kRowError))
+                const Choice p = sorted.at(i), q = sorted.at(i + 1);
+                if (p.total() - q.total() <= 2.0 * kRowError && p.beam() != q.beam() && (i < a.k || sorted.at(a.k - 1).total() - p.total() <= 2.0 * kRowError))
                     r.near[p.beam()] = r.near[q.beam()] = r.near[a.beams] = 1;
             }
             __syncthreads();
@@ -946,8 +961,8 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
                 if (warp == 0) take_best(a, r, request, false);
             } else {
                 for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
-                    Choice &c = list[i];
-                    c.key = ordered_double(r.base[c.beam()] + entering(c.x(), r.top[c.beam()]));
+                    const Choice c = list.at(i);
+                    list.keys[i] = ordered_double(r.base[c.beam()] + entering(c.x(), r.top[c.beam()]));
                 }
                 __syncthreads();
                 sort_list(list, sorted, n, r.places);
