@@ -401,7 +401,7 @@ __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads
     // The block's rows' pages follow one another in the list: a page a thread, its row found among theirs.
     const int32_t mine = a.t.rows - row0 < each ? a.t.rows - row0 : each;  // rows of this block, none or less behind the last
     if (mine > 0) {
-        const int64_t end = grown[mine - 1].rank + grown[mine - 1].pages;
+        const int64_t asked_for = grown[mine - 1].rank + grown[mine - 1].pages, end = asked_for < free ? asked_for : free;
         for (int64_t r = grown[0].rank + threadIdx.x; r < end; r += kClusterThreads) {
             int32_t lo = 0, hi = mine;  // ranks rise: the last row that begins at r or in front of it
             while (hi - lo > 1) {
@@ -616,6 +616,7 @@ int copy_pages(const cg_copy_job &j, const int32_t *count, bool early, cudaStrea
 }
 
 int check_copy(const cg_copy_job &j) {
+    if ((reinterpret_cast<uintptr_t>(j.pages_k) | reinterpret_cast<uintptr_t>(j.pages_v)) % 2) return CG_E_ALIGN;
     if (j.ncopies < 0 || j.nlayers < 0 || j.page_size <= 0 || j.heads <= 0 || j.head_size <= 0 || j.num_pages < 0 || j.num_pages > kMostPages) return CG_E_SHAPE;
     // offsets inside a page, and units of one copy, are 32-bit numbers
     if (static_cast<int64_t>(j.heads) * j.head_size > (1 << 28) || static_cast<int64_t>(j.page_size) * j.heads * j.head_size > (1 << 30) ||

@@ -277,6 +277,124 @@ def test_pages_and_lengths_that_do_not_fit():
     flagged()
 
 
+def test_as_many_rows_as_a_call_takes():
+    rows, pages, page = 4096, 30000, 4
+    rng = random.Random(7)
+    cache, table, lens, refs = layout(rng, rows, pages, page, 6, longest=20)
+    parents = [rng.randrange(rows) for _ in range(rows)]
+    got, got_lens, _ = paged.fork_pages(table, lens, numbers(parents), refs, page_size=page)
+    cache.table, cache.lens, _, lost = cache.fork(parents)
+    assert not lost and got.tolist() == cache.table and got_lens.tolist() == cache.lens and refs.tolist() == cache.refs
+    counts = [rng.choice([0, 1, 1, 2]) for _ in range(rows)]
+    starts = [0]
+    for c in counts:
+        starts.append(starts[-1] + c)
+    slots = paged.extend_pages(got, got_lens, refs, page, numbers(starts), starts[-1])
+    before = list(cache.lens)
+    want, without = cache_extend(cache, counts, starts)
+    assert slots.tolist() == want and got.tolist() == cache.table and got_lens.tolist() == cache.lens and refs.tolist() == cache.refs
+    assert without == [r for r in range(rows) if cache.lens[r] != before[r] + counts[r]]
+    if without:
+        with pytest.raises(RuntimeError):
+            paged.check_status()
+    paged.free_pages(got, got_lens, refs, page)
+    assert not refs.any()
+    paged.check_status()
+
+
+def cache_extend(cache, counts, starts):
+    """Cache.extend for many rows, without its sums over the rows in front."""
+    slots, without, free, rank = [-1] * starts[-1], [], cache.free(), 0
+    for r, c in enumerate(counts):
+        before, after = need(cache.lens[r], cache.page), need(cache.lens[r] + c, cache.page)
+        if after > len(cache.table[r]):
+            without.append(r)
+            continue
+        first, rank = rank, rank + after - before
+        if after > before and rank > len(free):
+            without.append(r)
+            continue
+        for j in range(before, after):
+            cache.table[r][j] = free[first + j - before]
+            cache.refs[cache.table[r][j]] = 1
+        for i in range(c):
+            place = cache.lens[r] + i
+            slots[starts[r] + i] = cache.table[r][place // cache.page] * cache.page + place % cache.page
+        cache.lens[r] += c
+    return slots, without
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_views_of_larger_arrays(offset):
+    """Tables that are columns of wider ones, counts and lengths that begin inside an array: what stands beside them stays."""
+    rng = random.Random(offset)
+    for pages in (300, 9001):
+        cache, table, lens, refs = layout(rng, 12, pages, 8, 9, longest=60)
+        wide, tight, counts = torch.full((12, 20), 777, dtype=torch.int32, device="cuda"), torch.full((30,), 777, dtype=torch.int32, device="cuda"), torch.full((pages + 9,), 777, dtype=torch.int32, device="cuda")
+        wide[:, offset:offset + 9], tight[offset:offset + 12], counts[offset:offset + pages] = table, lens, refs
+        table, lens, refs = wide[:, offset:offset + 9], tight[offset:offset + 12], counts[offset:offset + pages]
+        parents = [rng.randrange(12) for _ in range(12)]
+        out = torch.full((12, 17), 777, dtype=torch.int32, device="cuda"), torch.full((12,), 777, dtype=torch.int32, device="cuda")
+        got, got_lens, _ = paged.fork_pages(table, lens, numbers(parents), refs, page_size=8, out=(out[0][:, offset:offset + 9], out[1]))
+        cache.table, cache.lens, _, lost = cache.fork(parents)
+        assert not lost and got.tolist() == cache.table and got_lens.tolist() == cache.lens and refs.tolist() == cache.refs
+        assert (out[0][:, :offset] == 777).all() and (out[0][:, offset + 9:] == 777).all()
+        slots = paged.extend_pages(got, got_lens, refs, 8)
+        want, without = cache.extend([1] * 12, list(range(13)), 12)
+        assert slots.tolist() == want and got.tolist() == cache.table and refs.tolist() == cache.refs
+        places, _ = paged.compact_pages(got, got_lens, refs, page_size=8)
+        assert places.tolist() == cache.compact()[0] and got.tolist() == cache.table and refs.tolist() == cache.refs
+        paged.free_pages(got, got_lens, refs, 8, rows=numbers([2, 5]))
+        cache.give_back([2, 5])
+        assert refs.tolist() == cache.refs and got.tolist() == cache.table
+        for array, width in ((counts, pages), (tight, 12)):
+            assert (array[:offset] == 777).all() and (array[offset + width:] == 777).all()
+        assert (wide[:, :offset] == 777).all() and (wide[:, offset + 9:] == 777).all() and (out[0][:, offset + 9:] == 777).all()
+        if without:
+            with pytest.raises(RuntimeError):
+                paged.check_status()
+    paged.check_status()
+
+
+def test_layers_of_one_array():
+    """Keys and values that alternate in one array, layers and pages in any order of axes."""
+    rng = random.Random(2)
+    for axes in ((0, 1, 2, 3, 4, 5), (1, 2, 0, 3, 4, 5), (2, 0, 1, 4, 3, 5), (3, 0, 2, 1, 4, 5)):
+        sizes = (3, 2, 25, 6, 4, 16)  # layers, keys and values, pages, tokens, heads, values
+        array = torch.randint(-2 ** 15, 2 ** 15, [sizes[i] for i in axes], device="cuda", dtype=torch.int16).view(torch.bfloat16)
+        cache = array.permute([axes.index(i) for i in range(6)])
+        k, v = cache[:, 0], cache[:, 1]
+        order = rng.sample(range(25), 16)
+        n = [rng.randint(0, 6) for _ in range(8)]
+        moves = list(zip(order[:8], order[8:], n))
+        want = [moved(t, moves) for t in (k, v)]
+        paged.copy_pages(k, v, numbers(order[:8]), numbers(order[8:]), tokens=numbers(n))
+        assert torch.equal(bits(k), bits(want[0])) and torch.equal(bits(v), bits(want[1]))
+
+
+def test_without_the_host_module(monkeypatch):
+    """Through the general path: the same results, and the same errors as ever."""
+    from cachegen_b200 import _lib, _plain_calls
+    results = []
+    for plain in (False, True):
+        if plain:
+            monkeypatch.setattr(_lib, "_calls", _plain_calls)
+        rng = random.Random(3)
+        cache, table, lens, refs = layout(rng, 6, 90, 4, 9, longest=30)
+        _, (k, v) = pool(2, 90, 4, 2, 16)
+        got, got_lens, moves = paged.fork_pages(table, lens, numbers([0, 0, 1, 4, 4, 5]), refs, k, v)
+        slots = paged.extend_pages(got, got_lens, refs, 4, numbers([0, 2, 2, 9, 9, 10, 11]), 12)
+        single = paged.extend_pages(got, got_lens, refs, 4)
+        paged.free_pages(got, got_lens, refs, 4, rows=numbers([1, -1], torch.int64))
+        places, more = paged.compact_pages(got, got_lens, refs, k, v)
+        paged.copy_pages(k, v, numbers([3]), numbers([89]))
+        g = torch.Generator(device="cuda").manual_seed(1)
+        best = paged.beam_select(torch.randn((6, 999), generator=g, device="cuda"), -torch.arange(6.0, device="cuda").view(2, 3))
+        results.append([got, got_lens, moves, slots, single, places, more, refs, bits(k), bits(v), *best])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    paged.check_status()
+
+
 def test_nothing_to_do():
     e, refs, table = numbers([]), numbers([0, 1, 0]), torch.empty((0, 4), dtype=torch.int32, device="cuda")
     got, lens, moves = paged.fork_pages(table, e, e, refs, page_size=4)

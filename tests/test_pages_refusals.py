@@ -63,7 +63,7 @@ def test_copies_are_refused():
     L = _lib.lib()
     assert L.cg_copy_pages(None, None) == -1
     for given, code in (({"ncopies": -1}, -2), ({"nlayers": -1}, -2), ({"page_size": 0}, -2), ({"heads": 0}, -2), ({"head_size": 0}, -2), ({"num_pages": -1}, -2),
-                        ({"page_size": 1 << 20, "heads": 64}, -6), ({"nlayers": 1 << 30}, -6), ({"pages_k": None}, -1), ({"pages_v": None}, -1), ({"src": None}, -1), ({"dst": None}, -1)):
+                        ({"page_size": 1 << 20, "heads": 64}, -6), ({"pages_k": P + 1}, -5), ({"pages_v": P + 1}, -5), ({"nlayers": 1 << 30}, -6), ({"pages_k": None}, -1), ({"pages_v": None}, -1), ({"src": None}, -1), ({"dst": None}, -1)):
         assert L.cg_copy_pages(copy_job(**given), None) == code, given
     assert L.cg_copy_pages(copy_job(ncopies=0), None) == 0 and L.cg_copy_pages(copy_job(nlayers=0), None) == 0
 
