@@ -5,9 +5,9 @@
 // the lowest number, for rows in their order, so results do not depend on the order in which blocks run: counts change by atomic
 // additions, whose sum has no order, and everything else is decided from prefix sums.
 //
-// Work on tables is bound by latency: some hundred kilobytes, and a chain of a few dependent reads.  Prefix sums over all pages and rows
-// are made by one cluster, whose blocks tell one another their totals through distributed shared memory: one launch, and no second
-// pass over a grid.  Copies are bound by memory: 16 bytes a thread, four in flight.
+// Work on tables is bound by latency: some hundred kilobytes, and a chain of a few dependent reads.  Prefix sums over all pages and rows are made by one
+// block, or, of large caches, by one cluster, whose blocks tell one another their totals through distributed shared memory: one launch, and no second pass over a
+// grid.  Launches of one call start under those in front of them.  Copies are bound by memory: 16 bytes a thread, four in flight (1.1 GB moved in 181 us, 6.3 TB/s).
 #include "cg_common.cuh"
 
 namespace cg {
@@ -16,7 +16,7 @@ namespace {
 constexpr int kClusterBlocks = 8, kClusterThreads = 512, kClusterWarps = kClusterThreads / 32;
 constexpr int kRowThreads = 256, kRowColumns = 1024;  // of a block that works on a row of a table
 constexpr int kCopyThreads = 256, kCopyVectors = 4;
-constexpr int64_t kAlonePages = 8192;  // up to here, and with a row a thread, one block does: 2,600 pages and 8 rows extended in 9 us by eight blocks
+constexpr int64_t kAlonePages = 8192;  // up to here, and with a row a thread, one block does (8 rows in 2,600 pages extended: 6 us, by eight blocks 9 to 11)
 constexpr int32_t kSlotsTogether = 2 * kClusterBlocks * kClusterThreads;
 constexpr int64_t kMostPages = INT32_MAX - 1024;  // a warp counts on behind its last page
 
@@ -208,25 +208,22 @@ struct ForkArgs {
     int32_t nnew, wide, release;
 };
 
-// A block per row and 1,024 columns: the new row's entries, and the counts' changes.  Where a new row holds what the old one of its
-// place held, as rows of one request do in the context that they share, nothing changes and no atomic is issued.
-__global__ void __launch_bounds__(kRowThreads) fork_tables_kernel(const __grid_constant__ ForkArgs a) {
-    let_next_launch_start();
-    const int parts = (a.old.width + kRowColumns - 1) / kRowColumns > 0 ? (a.old.width + kRowColumns - 1) / kRowColumns : 1;
-    const int row = blockIdx.x / parts, column0 = (blockIdx.x - row * parts) * kRowColumns;
+// Columns column0 + first, + step .. below column1 of a row: the new row's entries, and the counts' changes.  Where a new row holds what the old one of its place
+// held, as rows of one request do in the context that they share, nothing changes and no atomic is issued.
+__device__ __forceinline__ void fork_row(const ForkArgs &a, int32_t row, int32_t column0, int32_t column1, int32_t first, int32_t step) {
     int64_t parent = -1;
     if (row < a.nnew) {
         parent = index_at(a.parents, row, a.wide);
         if (parent < -1 || parent >= a.old.rows) {
-            if (threadIdx.x == 0) note(a.old.status, CG_S_BAD_PAGE);
+            if (first == 0) note(a.old.status, CG_S_BAD_PAGE);
             parent = -1;
         }
     }
     const int32_t tokens = parent >= 0 ? length_of(a.old, static_cast<int>(parent)) : 0, need = pages_of(tokens, a.old.page_size);
     const int32_t had = a.release && row < a.old.rows ? pages_of(length_of(a.old, row), a.old.page_size) : 0;
-    if (row < a.nnew && column0 == 0 && threadIdx.x == 0) a.lens[row] = tokens;
+    if (row < a.nnew && column0 == 0 && first == 0) a.lens[row] = tokens;
     const int32_t last = tokens % a.old.page_size ? need - 1 : -1;  // the column of a page that is not full
-    for (int j = column0 + threadIdx.x; j < column0 + kRowColumns && j < a.old.width; j += kRowThreads) {
+    for (int32_t j = column0 + first; j < column1; j += step) {
         const int32_t now = j < need ? page_at(a.old, static_cast<int>(parent), j) : -1, before = j < had ? page_at(a.old, row, j) : -1;
         if (row < a.nnew) a.table[row * a.row + j] = now;
         if (now != before) {
@@ -236,14 +233,28 @@ __global__ void __launch_bounds__(kRowThreads) fork_tables_kernel(const __grid_c
         if (j == last && now >= 0) a.writers[now] = Writers{INT32_MAX, 0};  // the same from every row that does it
     }
 }
+// A block per row and 1,024 columns.
+__global__ void __launch_bounds__(kRowThreads) fork_tables_kernel(const __grid_constant__ ForkArgs a) {
+    let_next_launch_start();
+    const int parts = a.old.width > kRowColumns ? (a.old.width + kRowColumns - 1) / kRowColumns : 1;
+    const int row = blockIdx.x / parts, column0 = (blockIdx.x - row * parts) * kRowColumns;
+    fork_row(a, row, column0, min(a.old.width, column0 + kRowColumns), threadIdx.x, kRowThreads);
+}
 
 // One cluster, a row a thread.  A page that is not full may be written to by one row only: the first of the new rows that hold it
-// keeps it, if no other row does (it is counted more often than by these), and each of the rest gets a copy.
-template <int BLOCKS>
+// keeps it, if no other row does (it is counted more often than by these), and each of the rest gets a copy.  TABLES: small tables are made here
+// too, a warp a row, which saves a launch.
+template <int BLOCKS, bool TABLES>
 __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads) fork_writers_kernel(const __grid_constant__ ForkArgs a) {
     __shared__ Told told;
     let_next_launch_start();
-    wait_for_launch_before();
+    if (TABLES) {
+        const int32_t rows = a.release && a.old.rows > a.nnew ? a.old.rows : a.nnew;
+        for (int32_t row = threadIdx.x >> 5; row < rows; row += kClusterWarps) fork_row(a, row, 0, a.old.width, threadIdx.x & 31, 32);
+        __syncthreads();
+    } else {
+        wait_for_launch_before();
+    }
     const int32_t each = (a.nnew + BLOCKS - 1) / BLOCKS, row = cluster_rank<BLOCKS>() * each + threadIdx.x;
     const bool here = threadIdx.x < each && row < a.nnew;
     int32_t tokens = 0, page = -1, part = 0, column = 0;
@@ -432,8 +443,18 @@ struct CompactArgs {
     int32_t *table, *refs, *places, *moves;  // moves [2][num_pages / 2]
     int32_t *copies, *before_middle;
 };
-// One cluster.  With n pages held, those at n and behind go to the holes in front of n, the first to the first.
-template <int BLOCKS>
+__device__ __forceinline__ void compact_row(const CompactArgs &a, int32_t row, int32_t column0, int32_t column1, int32_t first, int32_t step) {
+    const int32_t need = pages_of(length_of(a.t, row), a.t.page_size);
+    for (int32_t j = column0 + first; j < column1 && j < need; j += step) {
+        const int32_t p = page_at(a.t, row, j);
+        if (p < 0) continue;
+        const int32_t to = __ldcg(a.places + p);
+        if (to >= 0) a.table[row * a.t.row + j] = to;
+        else note(a.t.status, CG_S_BAD_PAGE);  // a page that nobody holds
+    }
+}
+// One cluster.  With n pages held, those at n and behind go to the holes in front of n, the first to the first.  TABLES: as above.
+template <int BLOCKS, bool TABLES>
 __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads) compact_places_kernel(const __grid_constant__ CompactArgs a) {
     __shared__ Told told;
     let_next_launch_start();
@@ -481,20 +502,17 @@ __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kClusterThreads
         }
     }
     if (cluster_rank<BLOCKS>() == 0 && threadIdx.x == 0) *a.copies = made;
+    if (TABLES) {
+        __syncthreads();
+        for (int32_t row = threadIdx.x >> 5; row < a.t.rows; row += kClusterWarps) compact_row(a, row, 0, a.t.width, threadIdx.x & 31, 32);
+    }
 }
 __global__ void __launch_bounds__(kRowThreads) compact_tables_kernel(const __grid_constant__ CompactArgs a) {
     let_next_launch_start();
     wait_for_launch_before();
     const int parts = (a.t.width + kRowColumns - 1) / kRowColumns;
     const int row = blockIdx.x / parts, column0 = (blockIdx.x - row * parts) * kRowColumns;
-    const int32_t need = pages_of(length_of(a.t, row), a.t.page_size);
-    for (int j = column0 + threadIdx.x; j < column0 + kRowColumns && j < need; j += kRowThreads) {
-        const int32_t p = page_at(a.t, row, j);
-        if (p < 0) continue;
-        const int32_t to = __ldcg(a.places + p);
-        if (to >= 0) a.table[row * a.t.row + j] = to;
-        else note(a.t.status, CG_S_BAD_PAGE);  // a page that nobody holds
-    }
+    compact_row(a, row, column0, column0 + kRowColumns, threadIdx.x, kRowThreads);
 }
 
 // ---- copy ----------------------------------------------------------------------------------------------
@@ -638,6 +656,9 @@ Workspace workspace_of(int64_t num_pages) {
     return w;
 }
 
+// Whether one block goes through a table about as fast as a grid is launched: up to two steps a warp.
+bool few_entries(int64_t rows, int64_t width) { return rows * (width / 32 + 1) <= 2 * kClusterWarps; }
+
 enum What { kFork, kFree, kExtend, kCompact };
 
 int check_pages(const cg_pages_job *job, What what) {
@@ -699,12 +720,16 @@ extern "C" int cg_fork_pages(const cg_pages_job *job, const cg_copy_job *copy, v
     const int rows = j.release && j.nrows > j.nnew ? j.nrows : j.nnew, parts = j.width > kRowColumns ? (j.width + kRowColumns - 1) / kRowColumns : 1;
     if (rows == 0) return CG_OK;
     if (static_cast<int64_t>(rows) * parts > INT32_MAX) return CG_E_SHAPE;
-    if (const int rc = launch(fork_tables_kernel, dim3(rows * parts), kRowThreads, 0, false, st, a)) return rc;
-    if (j.nnew == 0) return CG_OK;
     const bool alone = j.num_pages <= kAlonePages && j.nnew <= kClusterThreads;
-    if (const int rc = alone ? launch(fork_writers_kernel<1>, dim3(1), kClusterThreads, 0, true, st, a)
-                             : launch(fork_writers_kernel<kClusterBlocks>, dim3(kClusterBlocks), kClusterThreads, 0, true, st, a))
-        return rc;
+    if (alone && few_entries(rows, j.width) && j.nnew) {
+        if (const int rc = launch(fork_writers_kernel<1, true>, dim3(1), kClusterThreads, 0, false, st, a)) return rc;
+    } else {
+        if (const int rc = launch(fork_tables_kernel, dim3(rows * parts), kRowThreads, 0, false, st, a)) return rc;
+        if (j.nnew == 0) return CG_OK;
+        if (const int rc = alone ? launch(fork_writers_kernel<1, false>, dim3(1), kClusterThreads, 0, true, st, a)
+                                 : launch(fork_writers_kernel<kClusterBlocks, false>, dim3(kClusterBlocks), kClusterThreads, 0, true, st, a))
+            return rc;
+    }
     if (!copy) return CG_OK;
     cg_copy_job c = *copy;
     c.src = j.moves, c.dst = j.moves + j.nnew, c.tokens = j.moves + 2 * static_cast<int64_t>(j.nnew);
@@ -754,13 +779,15 @@ extern "C" int cg_compact_pages(const cg_pages_job *job, const cg_copy_job *copy
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int32_t *const words = reinterpret_cast<int32_t *>(part_of(j, 0));
     CompactArgs a{table_of(j), j.table, j.refs, j.places, j.moves, words, words + 1};
-    if (const int rc = j.num_pages <= kAlonePages ? launch(compact_places_kernel<1>, dim3(1), kClusterThreads, 0, false, st, a)
-                                                      : launch(compact_places_kernel<kClusterBlocks>, dim3(kClusterBlocks), kClusterThreads, 0, false, st, a))
-        return rc;
-    if (j.nrows && j.width) {
+    const bool alone = j.num_pages <= kAlonePages, together = alone && few_entries(j.nrows, j.width);
+    const int rc = together ? launch(compact_places_kernel<1, true>, dim3(1), kClusterThreads, 0, false, st, a)
+                   : alone  ? launch(compact_places_kernel<1, false>, dim3(1), kClusterThreads, 0, false, st, a)
+                            : launch(compact_places_kernel<kClusterBlocks, false>, dim3(kClusterBlocks), kClusterThreads, 0, false, st, a);
+    if (rc) return rc;
+    if (!together && j.nrows && j.width) {
         const int64_t blocks = static_cast<int64_t>(j.nrows) * ((j.width + kRowColumns - 1) / kRowColumns);
         if (blocks > INT32_MAX) return CG_E_SHAPE;
-        if (const int rc = launch(compact_tables_kernel, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, true, st, a)) return rc;
+        if (const int rc2 = launch(compact_tables_kernel, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, true, st, a)) return rc2;
     }
     if (!copy) return CG_OK;
     cg_copy_job c = *copy;
