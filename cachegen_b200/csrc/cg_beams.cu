@@ -108,6 +108,21 @@ __device__ __forceinline__ double quick_log(double x) {
     const float m = static_cast<float>(__hiloint2double((high & 0xFFFFF) | 1023 << 20, __double2loint(x)));
     return ((high >> 20) - 1023) * 0.69314718055994531 + logf(m);
 }
+// A sum of numbers up to 1, to 2^-84 each, whose result does not depend on the order of additions: rows of the same logits in another order have the same.
+struct Wide {
+    uint64_t low, high;
+    __device__ __forceinline__ void add(const Wide &o) {
+        low += o.low;
+        high += o.high + (low < o.low);
+    }
+    static __device__ __forceinline__ Wide of(double x) {  // x = m 2^(e - 52), and m 2^(e + 32) is what counts 2^-84
+        const uint64_t u = static_cast<uint64_t>(__double_as_longlong(x)), m = (u & 0xFFFFFFFFFFFFFull) | 1ull << 52;
+        const int shift = static_cast<int>(u >> 52) - 1023 + 32;
+        if (shift > 0) return Wide{m << shift, m >> (64 - shift)};
+        return Wide{shift > -64 ? m >> -shift : 0, 0};
+    }
+    __device__ __forceinline__ double value() const { return (static_cast<double>(high) * 0x1p64 + static_cast<double>(low)) * 0x1p-84; }
+};
 // 2 to the power of a whole number that is not positive; 0 for what a float does not hold
 __device__ __forceinline__ float whole_power2(float n) { return n < -126.0f ? 0.0f : __int_as_float((127 + static_cast<int>(n)) << 23); }
 
@@ -540,9 +555,9 @@ __device__ __forceinline__ uint32_t word_of_block(const uint32_t *mine, int rank
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at_block(mine, rank)) : "memory");
     return v;
 }
-__device__ __forceinline__ double double_of_block(const double *mine, int rank) {
-    double v;
-    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at_block(mine, rank)) : "memory");
+__device__ __forceinline__ Wide wide_of_block(const Wide *mine, int rank) {
+    Wide v;
+    asm volatile("ld.shared::cluster.v2.u64 {%0, %1}, [%2];" : "=l"(v.low), "=l"(v.high) : "r"(at_block(mine, rank)) : "memory");
     return v;
 }
 
@@ -634,7 +649,8 @@ struct Choices {
 
 // How room in shared memory is divided; K beams, W warps
 struct ChooseRoom {
-    double *base, *sums;      // [K]: score - log sum exp(x - top); a block's share of a sum
+    double *base, *bounds;    // [K]: score - log sum exp(x - top); what k continuations of the row reach
+    Wide *wides, *of_warps;   // [K]: a block's share of a sum; [kMostChooseWarps]
     Choices list, sorted;     // [list_room], [kSorted]; in their place, where these are too small,
     uint64_t *best, *sorting; // [K][k], [W][sort_room]
     float *top;               // [K]
@@ -646,7 +662,7 @@ struct ChooseRoom {
         const size_t other = sizeof(uint64_t) * (static_cast<size_t>(a.beams) * a.k + static_cast<size_t>(warps) * a.sort_room);
         return (usual > other ? usual : other) + 15 & ~static_cast<size_t>(15);
     }
-    static size_t bytes(const BeamArgs &a, int warps) { return lists(a, warps) + a.beams * (2 * sizeof(double) + 3 * sizeof(float)) + sizeof(float) * (1 + kSorted); }
+    static size_t bytes(const BeamArgs &a, int warps) { return lists(a, warps) + a.beams * (sizeof(Wide) + 2 * sizeof(double) + 3 * sizeof(float)) + sizeof(float) * (1 + kSorted) + sizeof(Wide) * kMostChooseWarps; }
     __device__ ChooseRoom(char *at, const BeamArgs &a, int warps) {
         list.keys = reinterpret_cast<uint64_t *>(at);
         list.rests = list.keys + a.list_room;
@@ -654,9 +670,11 @@ struct ChooseRoom {
         sorted.rests = sorted.keys + kSorted;
         best = reinterpret_cast<uint64_t *>(at);
         sorting = best + static_cast<int64_t>(a.beams) * a.k;
-        base = reinterpret_cast<double *>(at + lists(a, warps));
-        sums = base + a.beams;
-        top = reinterpret_cast<float *>(sums + a.beams);
+        wides = reinterpret_cast<Wide *>(at + lists(a, warps));
+        of_warps = wides + a.beams;
+        base = reinterpret_cast<double *>(of_warps + kMostChooseWarps);
+        bounds = base + a.beams;
+        top = reinterpret_cast<float *>(bounds + a.beams);
         count = reinterpret_cast<int32_t *>(top + a.beams);
         near = reinterpret_cast<uint32_t *>(count + a.beams);
         places = reinterpret_cast<int32_t *>(near + a.beams + 1);
@@ -772,7 +790,7 @@ __device__ __forceinline__ void write_sorted(const BeamArgs &a, const Choices &s
 __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const ChooseRoom &r, int32_t request, int32_t *counts, Choices *list, Choices *sorted) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     double bound = -CUDART_INF;
-    for (int32_t i = 0; i < a.beams; ++i) bound = fmax(bound, r.sums[i]);
+    for (int32_t i = 0; i < a.beams; ++i) bound = fmax(bound, r.bounds[i]);
     bound -= 2.0 * kRowError;
     const int32_t pairs = a.beams * a.nparts;  // of a beam and a part of its row
     const int64_t first = static_cast<int64_t>(request) * pairs;
@@ -865,7 +883,6 @@ __device__ __forceinline__ int32_t gather_choices(const BeamArgs &a, const Choos
 template <int DT>
 __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostChooseWarps * 32) choose_kernel(const __grid_constant__ BeamArgs a) {
     extern __shared__ __align__(16) char room[];
-    __shared__ double warps_sums[kMostChooseWarps];
     __shared__ int32_t counts[2];
     const int rank = choose_rank(), lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const int32_t request = blockIdx.x / kChooseBlocks;
@@ -897,7 +914,7 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
                 const double base = any ? static_cast<double>(__ldg(a.scores + row)) - quick_log(sum) : -CUDART_INF;
                 r.top[i] = top;
                 r.base[i] = base;
-                r.sums[i] = any && least > -CUDART_INF_F ? base + entering(least, top) : -CUDART_INF;
+                r.bounds[i] = any && least > -CUDART_INF_F ? base + entering(least, top) : -CUDART_INF;
             }
         }
         __syncthreads();
@@ -932,32 +949,32 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
         for (int32_t i = 0; i < a.beams; ++i) {
             if (!word_of_block(r.near + i, 0)) continue;  // (the same for all threads)
             const float top = __uint_as_float(word_of_block(reinterpret_cast<const uint32_t *>(r.top + i), 0));
-            double sum = 0.0;
+            Wide sum{0, 0};
             if (top < CUDART_INF_F) {
                 const Row<DT> x(a, static_cast<int64_t>(request) * a.beams + i);
                 for (int32_t t = rank * blockDim.x + threadIdx.x; t < a.vocab; t += kChooseBlocks * blockDim.x) {
                     const float y = x.at(t);
-                    if (y > -CUDART_INF_F) sum += exp(static_cast<double>(y) - top);
+                    if (y > -CUDART_INF_F) sum.add(Wide::of(exp(static_cast<double>(y) - top)));
                 }
             }
 #pragma unroll
-            for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+            for (int d = 16; d; d /= 2) sum.add(Wide{__shfl_xor_sync(~0u, sum.low, d), __shfl_xor_sync(~0u, sum.high, d)});
             __syncthreads();
-            if (lane == 0) warps_sums[warp] = sum;
+            if (lane == 0) r.of_warps[warp] = sum;
             __syncthreads();
             if (threadIdx.x == 0) {
-                sum = 0.0;
-                for (int w = 0; w < warps; ++w) sum += warps_sums[w];
-                r.sums[i] = sum;
+                sum = Wide{0, 0};
+                for (int w = 0; w < warps; ++w) sum.add(r.of_warps[w]);
+                r.wides[i] = sum;
             }
         }
         cluster_barrier();
         if (rank == 0) {
             for (int32_t i = threadIdx.x; i < a.beams; i += blockDim.x) {
                 if (!r.near[i] || r.top[i] == CUDART_INF_F) continue;
-                double sum = 0.0;
-                for (int b = 0; b < kChooseBlocks; ++b) sum += double_of_block(r.sums + i, b);
-                r.base[i] = static_cast<double>(__ldg(a.scores + static_cast<int64_t>(request) * a.beams + i)) - log(sum);
+                Wide sum{0, 0};
+                for (int b = 0; b < kChooseBlocks; ++b) sum.add(wide_of_block(r.wides + i, b));
+                r.base[i] = static_cast<double>(__ldg(a.scores + static_cast<int64_t>(request) * a.beams + i)) - log(sum.value());
             }
             __syncthreads();
             if (n > kSorted) {
@@ -986,7 +1003,20 @@ Sizes sizes_of(const cg_beam_job &j, int sms) {
     const int per = j.dtype == kLogitF32 ? 4 : 8;
     const int64_t vectors = (static_cast<int64_t>(j.vocab) + 2 * (per - 1)) / per;  // a row may begin inside a vector
     const int64_t tiles = (vectors + kTileVectors - 1) / kTileVectors, rows = static_cast<int64_t>(j.nrequests) * j.beams, line = rows * tiles;
-    const int64_t blocks = static_cast<int64_t>(sms) * kRowBlocks, each = (line + blocks - 1) / blocks;
+    // Equal runs of the line cross the ends of rows, and every end of a part costs time.  Where whole rows, or equal parts of them, keep nearly all blocks busy they are what a
+    // block takes: 512 rows of 16 tiles by 512 blocks 32.7 us, by 586 with 14 tiles each 34.7; 256 rows of 17 tiles by 256 blocks 30.0, by 544 23.9.
+    const int64_t blocks = static_cast<int64_t>(sms) * kRowBlocks, nearly = blocks * 17 / 20;
+    int64_t each = (line + blocks - 1) / blocks;
+    if (rows <= blocks) {
+        for (int64_t parts = blocks / rows; parts >= 1 && rows * parts >= nearly; --parts)
+            if (tiles % parts == 0) {
+                each = tiles / parts;
+                break;
+            }
+    } else {
+        const int64_t of_block = (rows + blocks - 1) / blocks;
+        if ((rows + of_block - 1) / of_block >= nearly) each = of_block * tiles;
+    }
     if (line > INT32_MAX / 2 || each > INT32_MAX / 2) {
         z.total = -1;
         return z;

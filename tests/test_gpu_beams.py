@@ -112,6 +112,26 @@ def test_rows_whose_sums_are_nearly_the_same(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_the_same_logits_in_another_order(dtype):
+    """Their continuations are tied, and go to the lower beam, whatever the order of additions."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    for vocab in (2, 3, 10, 1000, 20011):
+        base = (2.0 * torch.randn(vocab, generator=g, device="cuda")).to(dtype)
+        rows_ = torch.stack([base[torch.randperm(vocab, generator=g, device="cuda")] for _ in range(8)])
+        scores, tokens, parents = paged.beam_select(rows_, torch.zeros((1, 8), device="cuda"), 16)
+        best_values = rows_.double().sort(dim=-1, descending=True).values[0]  # the same for all rows
+        at = 0
+        for value in best_values.unique(sorted=True).flip(0).tolist():
+            for beam in range(8):
+                for token in (rows_[beam].double() == value).nonzero()[:, 0].tolist():
+                    if at < min(16, 8 * vocab):
+                        assert (tokens[0, at].item(), parents[0, at].item()) == (token, beam), (vocab, at)
+                        at += 1
+        assert at == min(16, 8 * vocab)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_what_is_banned(dtype):
     low = torch.finfo(dtype).min
     for vocab in (40, 20000, 70001):
