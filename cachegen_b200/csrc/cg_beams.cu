@@ -2,10 +2,10 @@
 //     score[beam] + x[beam, token] - log sum_w exp x[beam, w],
 // in falling order, equal ones by beam and token.
 //
-// rows_kernel reads the logits once.  All rows' tiles of 16 KB stand in one line, and every block takes an equal run of it; what it has of one row is a
+// rows_kernel reads the logits once.  All rows' tiles of 16 KB stand in one line, and every block takes a run of it; what it has of one row is a
 // part.  A thread keeps its largest value and a sum of exponentials.  k of a part's logits reach the k-th largest of its threads' largest; what does not
 // reach it cannot be among the best, and the rest, little more than k, is read again and written down with its token.  Bound by memory (131 MB of 16-bit logits in
-// 34 us, 3.9 TB/s): of these, loads alone are 26, ends of parts, 2 us each and two a block, 6, and exponentials 2.  Blocks that take half as much have
+// 33 us, 4.0 TB/s): of these, loads alone are 26, ends of parts, 2 us each, 5, and exponentials 2.  Blocks that take half as much have
 // more ends: 39 us; tiles asked for two ahead, or through shared memory, leave room for fewer warps: 37 to 39.
 //
 // choose_kernel joins a row's parts, drops what is below a bound that k continuations of one row reach, and puts the rest in order.  Which of two rows'

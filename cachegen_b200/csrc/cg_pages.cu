@@ -609,9 +609,9 @@ bool vectors(const CopySide &s) {
     return reinterpret_cast<uintptr_t>(s.data) % 16 == 0 && s.layer % 8 == 0 && s.page % 8 == 0 && s.token % 8 == 0 && s.head % 8 == 0;
 }
 
-// count: how many copies there are, on the GPU, or nullptr: ncopies; early: the launch in front writes what is read here and has
-// let this one start
-int copy_pages(const cg_copy_job &j, const int32_t *count, bool early, cudaStream_t st) {
+// count: how many copies there are, on the GPU, or nullptr: ncopies; spread: they may well be as many; early: the launch in front writes what is read
+// here and has let this one start
+int copy_pages(const cg_copy_job &j, const int32_t *count, bool spread, bool early, cudaStream_t st) {
     if (j.ncopies == 0 || j.nlayers == 0 || j.page_size == 0) return CG_OK;
     CopyArgs a{};
     a.sides[0] = copy_side(j.pages_k, j.pages_k_strides, j.heads, j.head_size);
@@ -626,9 +626,10 @@ int copy_pages(const cg_copy_job &j, const int32_t *count, bool early, cudaStrea
     const int64_t parts = (pieces + kCopyThreads * kCopyVectors - 1) / (kCopyThreads * kCopyVectors), most = static_cast<int64_t>(sm_count()) * 8;
     const int64_t pages = 2 * static_cast<int64_t>(j.nlayers) * j.ncopies, slices = (4 * most + pages - 1) / pages, units = pages * (slices < parts ? slices : parts);
     a.slices = static_cast<int32_t>(slices < parts ? slices : parts);
-    // Where all copies are known to be there, more blocks than run at a time, so that those of short units make room for others (700 parts of pages: 197 us with as
-    // many as run, 181 so).
-    const int64_t blocks = count ? most : 16 * most;
+    // More blocks than run at a time make room for others as they end, so that units of unlike lengths are shared out evenly; blocks that find no unit cost a little
+    // (700 parts of pages: 197 us with as many blocks as run, 181 with sixteen times as many; a large cache compacted: 208, 195 with four times and 191 with sixteen;
+    // a fork, where few of the possible copies are there, is 2 us slower with four times and 10 with sixteen).
+    const int64_t blocks = most * (!count ? 16 : spread && units >= 8 * most ? 4 : 1);
     const dim3 grid(static_cast<unsigned>(units < blocks ? units : blocks));
     return vec ? launch(copy_pages_kernel<uint4>, grid, kCopyThreads, 0, early, st, a) : launch(copy_pages_kernel<uint16_t>, grid, kCopyThreads, 0, early, st, a);
 }
@@ -696,7 +697,7 @@ extern "C" int cg_copy_pages(const cg_copy_job *job, void *stream) {
     if (const int rc = check_copy(j)) return rc;
     if (j.ncopies == 0 || j.nlayers == 0) return CG_OK;
     if (!j.pages_k || !j.pages_v || !j.src || !j.dst) return CG_E_NULL;
-    return copy_pages(j, nullptr, false, static_cast<cudaStream_t>(stream));
+    return copy_pages(j, nullptr, true, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int cg_fork_pages(const cg_pages_job *job, const cg_copy_job *copy, void *stream) {
@@ -734,7 +735,7 @@ extern "C" int cg_fork_pages(const cg_pages_job *job, const cg_copy_job *copy, v
     cg_copy_job c = *copy;
     c.src = j.moves, c.dst = j.moves + j.nnew, c.tokens = j.moves + 2 * static_cast<int64_t>(j.nnew);
     c.wide = 0, c.ncopies = j.nnew, c.status = j.status;
-    return copy_pages(c, a.copies, true, st);
+    return copy_pages(c, a.copies, false, true, st);
 }
 
 extern "C" int cg_free_pages(const cg_pages_job *job, void *stream) {
@@ -793,5 +794,5 @@ extern "C" int cg_compact_pages(const cg_pages_job *job, const cg_copy_job *copy
     cg_copy_job c = *copy;
     c.src = j.moves, c.dst = j.moves + j.num_pages / 2, c.tokens = nullptr;
     c.wide = 0, c.ncopies = static_cast<int32_t>(j.num_pages / 2), c.status = j.status;
-    return copy_pages(c, a.copies, true, st);
+    return copy_pages(c, a.copies, true, true, st);
 }
