@@ -666,7 +666,8 @@ def extend_pages(page_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Te
     page_table, kv_lens and refs are brought up to date.
 
     Returns the tokens' slots (int64 [tokens]), as append_paged and decode_paged take them: -1 for tokens of no row, and for those of a row for which
-    no page is free or that its table has no room for; that row stays as it is, and check_status says so."""
+    no page is free or that its table has no room for; that row stays as it is, and check_status says so.  Behind a row that finds too few
+    free pages no other row that needs some finds any."""
     done = _lib.calls().extend_pages(page_table, kv_lens, refs, page_size, q_starts, tokens, _status_of(refs))
     if done is not None:
         return _finish(done, "extend_pages")
@@ -723,7 +724,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int = None) -> tu
     are in the order of their logits, whatever the scores lose of it.)
 
     Returns scores (float32), tokens and parents (int32), all [requests, k]; parents are rows of logits, as fork_pages takes them.  Scores are
-    compared in 64 bits and rounded once.  A beam whose score is not finite has no continuations, nor have logits of -infinity or NaN,
+    compared in 64 bits; what is returned is off by less than 5e-6 and its rounding.  A beam whose score is not finite has no continuations, nor have logits of -infinity or NaN,
     which weigh nothing; logits of +infinity share their row's weight.  Behind a request's last continuation stand -infinity, -1 and -1."""
     k = scores.shape[-1] if k is None and scores.dim() else k
     done = _lib.calls().beam_select(logits, scores, k)

@@ -571,7 +571,8 @@ int cg_paged_attention(const cg_attention_job *job_host, void *stream);
  * share nothing with the old ones'.
  * cg_free_pages: rows which[0 .. nnew) (-1: none; NULL: all rows) hold nothing any more: their lengths become 0, their entries -1.
  * cg_extend_pages: row r gets q_starts[r + 1] - q_starts[r] more tokens (int32 [nrows + 1], rising; NULL: one, and ntokens is nrows), with pages for them;
- * slots [ntokens]: where they belong, -1 for tokens of no row and of rows that find no place: those stay as they are.
+ * slots [ntokens]: where they belong, -1 for tokens of no row and of rows that find no place: those stay as they are (behind a row that finds
+ * too few free pages no other that needs some finds any).
  * cg_compact_pages: with n pages held, the held pages at n and behind move to the free places in front of n, the first to the first;
  * counts and the table follow.  places: int32 [num_pages]: where each page now is, -1 if it was free; moves: int32 [2, num_pages / 2]: from
  * and to, -1 behind the last.  copy as above.
@@ -621,7 +622,7 @@ int cg_compact_pages(const cg_pages_job *job_host, const cg_copy_job *copy_host,
  * continuations and weigh nothing; where there are logits of +infinity, these share their row's weight and the others are none.
  * out_scores (float32), tokens, parents (int32): [nrequests, k], parents as rows of logits; where a request has fewer than k
  * continuations, -infinity, -1, -1 behind them.  Continuations of one beam are compared by their logits, those of different beams in 64
- * bits; numbers are rounded once.
+ * bits; the scores written are off by less than 5e-6 and their rounding.
  * workspace: cg_beam_workspace(job) bytes (16-byte aligned), which calls on one stream may share.
  */
 #define CG_LOGITS_F32 2
