@@ -191,6 +191,23 @@ def test_compact(rows, pages, page, width, place):
     paged.check_status()
 
 
+@pytest.mark.parametrize("rows", [0, 3, 400])
+def test_compact_of_a_large_cache(rows):
+    """Copies by more blocks than run at a time, of which many, some or nearly all find nothing to do."""
+    rng = random.Random(rows)
+    pages, page = 12000, 2
+    cache, table, lens, refs = layout(rng, rows, pages, page, 20, share=0.0)
+    _, (k, v) = pool(2, pages, page, 1, 8)
+    before = k.clone(), v.clone()
+    places, moves = paged.compact_pages(table, lens, refs, k, v)
+    want, copies = cache.compact()
+    assert places.tolist() == want and refs.tolist() == cache.refs and table.tolist() == cache.table
+    assert moves[:, :len(copies)].tolist() == [[c[i] for c in copies] for i in range(2)] and (moves[:, len(copies):] == -1).all()
+    for t, b in zip((k, v), before):
+        assert torch.equal(bits(t), bits(moved(b, [(a, to, page) for a, to in copies])) if copies else bits(b))
+    paged.check_status()
+
+
 @pytest.mark.parametrize("heads,head,page", [(8, 128, 16), (1, 128, 16), (3, 40, 5), (2, 7, 3), (12, 96, 24), (32, 128, 128)])
 @pytest.mark.parametrize("fmt", ["vllm", "huggingface"])
 @pytest.mark.parametrize("part", [False, True])
