@@ -31,11 +31,13 @@ constexpr int kTilesPerPart = 16, kTileRoom = 512;         // a part's tiles, an
 constexpr int kChooseBlocks = 8;                           // of a request's cluster
 constexpr int kChooseWarps = 8, kMostChooseWarps = 16, kSorted = 512, kSortedAtOnce = 192, kBins = 256, kMostList = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kMostPlain = 32768.0f;                     // logits up to here are summed the quick way
+constexpr float kMostPlain = 32768.0f;                     // logits from -kMostPlain to here are summed the quick way
 // Relative error of a row's sum in 32 bits, and so the absolute one of its logarithm.  A term is 2 to the power y = x log2(e) - c, c whole and at most 9 below
 // the thread's largest: with u = top - x, y is at most 1.45 u + 9 and off by 2^-24 of itself, so the term by 2^-24 (u + 6.3).  u on average, weighted with
 // the terms, is below 17 for up to 2^24 tokens (n terms of one size u beside the largest weigh n u exp(-u) / (1 + n exp(-u))): 1.4e-6.  log2(e) is off by
-// 2^-26 of itself, which for the largest term is known and taken out; for the others 1.4e-8 u: 0.3e-6.  The power itself: 2^-22.  A thread's sum is 8 additions to each of
+// 2^-26 of itself, which for the largest term is known and taken out; for the others 1.4e-8 u: 0.3e-6.  A thread all of whose logits are below -kMostPlain takes
+// that instead of its largest: its terms are what they are, or 0, and weigh nothing, since the part's largest is above (or the part is summed again).  (Against
+// masks such as -1e10 c would be off by what is lost in x log2(e), some hundreds, and the power infinite.)  The power itself: 2^-22.  A thread's sum is 8 additions to each of
 // four accumulators, two to join them and one a tile, the warp's and the block's 8 more: 34 2^-24 or 2.1e-6, with factors that are whole powers of two.  Parts' sums are
 // taken to their largest, and joined, with two powers and a logarithm of 32 bits: 2^-21 and 2^-23.  In all below 1.4e-6 + 0.3e-6 + 0.3e-6 + 2.1e-6 + 0.6e-6.
 constexpr double kRowError = 5e-6;
@@ -417,8 +419,8 @@ __device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, Line<DT> &
         const float m = L::template most<4 * kVectors>(reinterpret_cast<const uint32_t *>(now));
         s.most[tile][tid] = m;
         top = fmaxf(top, m);
-        const float want = __fmul_rn(m, kLog2e);
-        if ((want > base + 8.0f || sum == 0.0f) && want > -CUDART_INF_F) {
+        const float want = fmaxf(__fmul_rn(m, kLog2e), -kMostPlain * kLog2e);
+        if (want > base + 8.0f || sum == 0.0f) {
             const float next = rintf(want);
             sum = sum == 0.0f ? 0.0f : __fmul_rn(sum, whole_power2(base - next));
             base = next;
@@ -437,7 +439,7 @@ __device__ __forceinline__ void do_part(const BeamArgs &a, Shared &s, Line<DT> &
         const float2 both = of_pair(pair_add(acc[0], acc[1]));
         sum = __fadd_rn(sum, __fadd_rn(both.x, both.y));
     }
-    const bool odd = (sum != sum && top > -CUDART_INF_F) || top > kMostPlain;
+    const bool odd = (!(sum < CUDART_INF_F) && top > -CUDART_INF_F) || top > kMostPlain;
     const uint32_t key = ordered(top);
     const float high = from_ordered(__reduce_max_sync(~0u, key));
     const float warp_base = from_ordered(__reduce_max_sync(~0u, sum > 0.0f ? ordered(base) : 0x00800000u));
