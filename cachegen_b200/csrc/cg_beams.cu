@@ -952,12 +952,10 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
             if (!word_of_block(r.near + i, 0)) continue;  // (the same for all threads)
             const float top = __uint_as_float(word_of_block(reinterpret_cast<const uint32_t *>(r.top + i), 0));
             Wide sum{0, 0};
-            if (top < CUDART_INF_F) {
-                const Row<DT> x(a, static_cast<int64_t>(request) * a.beams + i);
-                for (int32_t t = rank * blockDim.x + threadIdx.x; t < a.vocab; t += kChooseBlocks * blockDim.x) {
-                    const float y = x.at(t);
-                    if (y > -CUDART_INF_F) sum.add(Wide::of(exp(static_cast<double>(y) - top)));
-                }
+            const Row<DT> x(a, static_cast<int64_t>(request) * a.beams + i);
+            for (int32_t t = rank * blockDim.x + threadIdx.x; t < a.vocab; t += kChooseBlocks * blockDim.x) {
+                const float y = x.at(t);
+                if (top == CUDART_INF_F ? y == top : y > -CUDART_INF_F) sum.add(Wide::of(top == CUDART_INF_F ? 1.0 : exp(static_cast<double>(y) - top)));
             }
 #pragma unroll
             for (int d = 16; d; d /= 2) sum.add(Wide{__shfl_xor_sync(~0u, sum.low, d), __shfl_xor_sync(~0u, sum.high, d)});
@@ -973,7 +971,7 @@ __global__ void __cluster_dims__(kChooseBlocks, 1, 1) __launch_bounds__(kMostCho
         cluster_barrier();
         if (rank == 0) {
             for (int32_t i = threadIdx.x; i < a.beams; i += blockDim.x) {
-                if (!r.near[i] || r.top[i] == CUDART_INF_F) continue;
+                if (!r.near[i]) continue;
                 Wide sum{0, 0};
                 for (int b = 0; b < kChooseBlocks; ++b) sum.add(wide_of_block(r.wides + i, b));
                 r.base[i] = static_cast<double>(__ldg(a.scores + static_cast<int64_t>(request) * a.beams + i)) - log(sum.value());
