@@ -18,10 +18,10 @@ CG_S_STREAM_OVERFLOW, CG_S_BAD_LENGTHS, CG_S_BAD_SYMBOL, CG_S_COUNT_OVERFLOW, CG
 CG_S_BAD_PAGE, CG_S_TIMEOUT, CG_S_NO_PAGE = 32, 64, 128
 CG_MAX_REQUESTS = 4096
 CG_LOGITS_F32 = 2
-CG_MAX_BEAMS, CG_MAX_CHOICES, CG_MAX_BEAM_CHOICES, CG_MAX_VOCAB = 256, 128, 8192, 1 << 24
+CG_MAX_BEAMS, CG_MAX_CHOICES, CG_MAX_BEAM_CHOICES, CG_MAX_VOCAB, CG_MAX_BEAM_ROWS = 256, 128, 8192, 1 << 24, 1 << 20
 CG_TABLES_CDF, CG_TABLES_COUNTS, CG_TABLES_SPARSE = 0, 1, 2
 CG_LENGTHS_I32, CG_LENGTHS_U16 = 0, 1
-CG_E_CUDA = -8
+CG_E_CAPACITY, CG_E_CUDA = -6, -8
 
 
 def stream_capacity(ntokens):

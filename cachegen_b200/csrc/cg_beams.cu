@@ -1035,7 +1035,7 @@ int check_job(const cg_beam_job *job) {
     const cg_beam_job &j = *job;
     if (j.dtype != CG_F16 && j.dtype != CG_BF16 && j.dtype != kLogitF32) return CG_E_DTYPE;
     if (j.nrequests < 0 || j.beams <= 0 || j.vocab <= 0 || j.k <= 0 || j.vocab > CG_MAX_VOCAB) return CG_E_SHAPE;
-    if (j.beams > CG_MAX_BEAMS || j.k > CG_MAX_CHOICES || j.beams * j.k > CG_MAX_BEAM_CHOICES || static_cast<int64_t>(j.nrequests) * j.beams > (1 << 20))
+    if (j.beams > CG_MAX_BEAMS || j.k > CG_MAX_CHOICES || j.beams * j.k > CG_MAX_BEAM_CHOICES || static_cast<int64_t>(j.nrequests) * j.beams > CG_MAX_BEAM_ROWS)
         return CG_E_CAPACITY;
     return CG_OK;
 }

@@ -1012,7 +1012,7 @@ PyObject *beam_select(PyObject *, PyObject *const *a, Py_ssize_t n) {
     job.dtype = type == at::kFloat ? CG_LOGITS_F32 : code(type), job.row_stride = logits.stride(0);
     job.nrequests = static_cast<int32_t>(B), job.beams = static_cast<int32_t>(K), job.vocab = static_cast<int32_t>(V), job.k = static_cast<int32_t>(k);
     const int64_t need = beam_workspace(&job);
-    if (need < 0) return PyLong_FromLongLong(need);
+    if (need < 0) Py_RETURN_NONE;  // more than a call takes: the general path says what
     const at::Tensor workspace = make({need}, at::TensorOptions().dtype(at::kByte).device(dev));
     job.workspace = workspace.data_ptr(), job.workspace_bytes = need;
     const int rc = run(best_beams, job, dev);

@@ -744,6 +744,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int = None) -> tu
     _check(0 < K <= _lib.CG_MAX_BEAMS and 0 < k <= _lib.CG_MAX_CHOICES and K * k <= _lib.CG_MAX_BEAM_CHOICES,
            f"{k} of {K} beams' continuations: a call takes up to {_lib.CG_MAX_BEAMS} beams, {_lib.CG_MAX_CHOICES} choices and a product of {_lib.CG_MAX_BEAM_CHOICES}")
     _check(0 < V <= _lib.CG_MAX_VOCAB, f"a vocabulary has 1 to {_lib.CG_MAX_VOCAB} tokens, not {V}")
+    _check(B * K <= _lib.CG_MAX_BEAM_ROWS, f"at most {_lib.CG_MAX_BEAM_ROWS} rows of logits in a call, not {B * K}")
     out = torch.empty((B, k), dtype=torch.float32, device=dev)
     tokens, parents = (torch.empty((B, k), dtype=torch.int32, device=dev) for _ in range(2))
     job = _lib.BeamJob()
@@ -752,6 +753,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int = None) -> tu
     _set(job, nrequests=B, beams=K, vocab=V, k=k)
     with on_device(dev):
         need = _lib.lib().cg_beam_workspace(ctypes.byref(job))
+        _check(need != _lib.CG_E_CAPACITY, f"{B * K} rows of {V} logits are more than a call takes")
         _lib.check(min(need, 0), "beam_select")
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         job.workspace, job.workspace_bytes = workspace.data_ptr(), need

@@ -594,7 +594,8 @@ typedef struct cg_pages_job {
 /*
  * Page src[i] (int64 if wide, else int32) to page dst[i] of every layer's keys and values, or the first tokens[i] tokens of it (int32; NULL: all);
  * -1 in either: nothing.  No page is written to twice or read as well.  pages [nlayers, num_pages, page_size, heads, head_size] as above.
- * page_size * heads * head_size <= 2^30.
+ * heads * head_size <= 2^28, page_size * heads * head_size <= 2^30, and nlayers * (page_size * heads * head_size / 1024 + 1) <= 2^29 (the quotient
+ * rounded down).
  */
 typedef struct cg_copy_job {
     void *pages_k, *pages_v;
@@ -624,12 +625,15 @@ int cg_compact_pages(const cg_pages_job *job_host, const cg_copy_job *copy_host,
  * continuations, -infinity, -1, -1 behind them.  Continuations of one beam are compared by their logits, those of different beams in 64
  * bits; the scores written are off by less than 5e-6 and their rounding.
  * workspace: cg_beam_workspace(job) bytes (16-byte aligned), which calls on one stream may share.
+ * nrequests * beams <= CG_MAX_BEAM_ROWS, and all rows together, each as whole pieces of 16 KB (of addresses; rows may stand for the same memory), are
+ * below 2^30 pieces: CG_E_CAPACITY otherwise.
  */
 #define CG_LOGITS_F32 2
 #define CG_MAX_BEAMS 256
 #define CG_MAX_CHOICES 128
 #define CG_MAX_BEAM_CHOICES 8192 /* beams * k */
 #define CG_MAX_VOCAB (1 << 24)
+#define CG_MAX_BEAM_ROWS (1 << 20) /* nrequests * beams */
 typedef struct cg_beam_job {
     const void *logits;
     const float *scores;
