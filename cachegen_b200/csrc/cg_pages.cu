@@ -777,6 +777,8 @@ extern "C" int cg_compact_pages(const cg_pages_job *job, const cg_copy_job *copy
         if (copy->page_size != j.page_size || copy->num_pages != j.num_pages) return CG_E_SHAPE;
     }
     if (j.num_pages == 0) return CG_OK;
+    const int64_t blocks = static_cast<int64_t>(j.nrows) * ((static_cast<int64_t>(j.width) + kRowColumns - 1) / kRowColumns);  // of a grid over the table
+    if (blocks > INT32_MAX) return CG_E_SHAPE;  // before anything has moved
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int32_t *const words = reinterpret_cast<int32_t *>(part_of(j, 0));
     CompactArgs a{table_of(j), j.table, j.refs, j.places, j.moves, words, words + 1};
@@ -786,8 +788,6 @@ extern "C" int cg_compact_pages(const cg_pages_job *job, const cg_copy_job *copy
                             : launch(compact_places_kernel<kClusterBlocks, false>, dim3(kClusterBlocks), kClusterThreads, 0, false, st, a);
     if (rc) return rc;
     if (!together && j.nrows && j.width) {
-        const int64_t blocks = static_cast<int64_t>(j.nrows) * ((j.width + kRowColumns - 1) / kRowColumns);
-        if (blocks > INT32_MAX) return CG_E_SHAPE;
         if (const int rc2 = launch(compact_tables_kernel, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, true, st, a)) return rc2;
     }
     if (!copy) return CG_OK;
