@@ -813,7 +813,7 @@ struct Tables {
         return table.size(0) == rows && rows <= CG_MAX_REQUESTS && pages <= INT32_MAX - 1024;
     }
     bool fill(cg_pages_job *job, int64_t page_size) const {
-        if (page_size <= 0 || page_size > INT32_MAX || width > INT32_MAX / page_size) return false;
+        if (page_size <= 0 || page_size > INT32_MAX || width > INT32_MAX / page_size || width > INT32_MAX - 1024) return false;
         job->table = ints(table), job->kv_lens = ints(lens), job->refs = ints(refs), job->status = status.defined() ? ints(status) : nullptr;
         job->table_row = table.stride(0), job->num_pages = pages;
         job->nrows = static_cast<int32_t>(rows), job->width = static_cast<int32_t>(width), job->page_size = static_cast<int32_t>(page_size);

@@ -18,7 +18,7 @@ constexpr int kRowThreads = 256, kRowColumns = 1024;  // of a block that works o
 constexpr int kCopyThreads = 256, kCopyVectors = 4;
 constexpr int64_t kAlonePages = 8192;  // up to here, and with a row a thread, one block does (8 rows in 2,600 pages extended: 6 us, by eight blocks 9 to 11)
 constexpr int32_t kSlotsTogether = 2 * kClusterBlocks * kClusterThreads;
-constexpr int64_t kMostPages = INT32_MAX - 1024;  // a warp counts on behind its last page
+constexpr int64_t kMostPages = INT32_MAX - 1024;  // a warp counts on behind its last page, and a block behind its last column of a row
 
 struct Table {
     const int32_t *entries, *lens;
@@ -667,7 +667,7 @@ int check_pages(const cg_pages_job *job, What what) {
     const cg_pages_job &j = *job;
     if (j.nrows < 0 || j.width < 0 || j.page_size <= 0 || j.num_pages < 0 || j.num_pages > kMostPages || j.nnew < 0 || j.ntokens < 0) return CG_E_SHAPE;
     if (j.nrows > CG_MAX_REQUESTS || ((what == kFork || (what == kFree && j.which)) && j.nnew > CG_MAX_REQUESTS)) return CG_E_CAPACITY;
-    if (static_cast<int64_t>(j.width) * j.page_size > INT32_MAX) return CG_E_SHAPE;
+    if (static_cast<int64_t>(j.width) * j.page_size > INT32_MAX || j.width > kMostPages) return CG_E_SHAPE;
     if ((j.nrows && ((j.width && !j.table) || !j.kv_lens)) || (j.num_pages && !j.refs)) return CG_E_NULL;
     if (what == kFork && (!j.which || (j.width && !j.new_table) || !j.new_lens || !j.moves) && j.nnew) return CG_E_NULL;
     if (what == kExtend && ((!j.slots && j.ntokens) || (!j.q_starts && j.ntokens != j.nrows))) return j.q_starts || !j.slots ? CG_E_NULL : CG_E_SHAPE;
@@ -777,7 +777,7 @@ extern "C" int cg_compact_pages(const cg_pages_job *job, const cg_copy_job *copy
         if (copy->page_size != j.page_size || copy->num_pages != j.num_pages) return CG_E_SHAPE;
     }
     if (j.num_pages == 0) return CG_OK;
-    const int64_t blocks = static_cast<int64_t>(j.nrows) * ((static_cast<int64_t>(j.width) + kRowColumns - 1) / kRowColumns);  // of a grid over the table
+    const int64_t blocks = static_cast<int64_t>(j.nrows) * ((j.width + kRowColumns - 1) / kRowColumns);  // of a grid over the table
     if (blocks > INT32_MAX) return CG_E_SHAPE;  // before anything has moved
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int32_t *const words = reinterpret_cast<int32_t *>(part_of(j, 0));

@@ -519,7 +519,7 @@ def _tables(page_table, kv_lens, refs, page_size, device, written):
     _check(B <= _lib.CG_MAX_REQUESTS, f"at most {_lib.CG_MAX_REQUESTS} rows in a call")
     _check(page_size > 0, "pages must hold a token at least")
     W = page_table.shape[1]
-    _check(W * page_size < 2 ** 31, f"rows of {W} pages of {page_size} tokens are longer than a call takes")
+    _check(W * page_size < 2 ** 31 and W <= 2 ** 31 - 1025, f"rows of {W} pages of {page_size} tokens are longer than a call takes")
     job = _lib.PagesJob()
     job.table, job.kv_lens, job.refs, job.status = page_table.data_ptr(), kv_lens.data_ptr(), refs.data_ptr(), _address(_status_of(refs))
     job.table_row = page_table.stride(0)

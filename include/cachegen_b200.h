@@ -577,7 +577,7 @@ int cg_paged_attention(const cg_attention_job *job_host, void *stream);
  * counts and the table follow.  places: int32 [num_pages]: where each page now is, -1 if it was free; moves: int32 [2, num_pages / 2]: from
  * and to, -1 behind the last.  copy as above.
  * workspace: cg_pages_workspace(num_pages) bytes, 16-byte aligned, which calls on one stream may share (none for cg_free_pages).
- * nrows, nnew <= CG_MAX_REQUESTS, width * page_size < 2^31, num_pages <= 2^31 - 1025; for cg_fork_pages and cg_compact_pages, rows (the old or the
+ * nrows, nnew <= CG_MAX_REQUESTS, width * page_size < 2^31, width and num_pages <= 2^31 - 1025; for cg_fork_pages and cg_compact_pages, rows (the old or the
  * new ones, whichever are more) * ceil(width / 1024) < 2^31.
  */
 typedef struct cg_pages_job {
