@@ -725,7 +725,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int = None) -> tu
 
     Returns scores (float32), tokens and parents (int32), all [requests, k]; parents are rows of logits, as fork_pages takes them.  Scores are
     compared in 64 bits; what is returned is off by less than 5e-6 and its rounding.  A beam whose score is not finite has no continuations,
-    nor have logits of -infinity or NaN, which weigh nothing; logits of +infinity share their row's weight.  Behind a request's last continuation stand -infinity, -1 and -1."""
+    nor have logits of -infinity or NaN, which weigh nothing; logits of +infinity share their row's weight.  Behind a request's last continuation stand -infinity, -1 and -1.
+    A call takes up to 256 beams, 128 continuations, 8,192 of both multiplied, 2^24 tokens and 2^20 rows of logits."""
     k = scores.shape[-1] if k is None and scores.dim() else k
     done = _lib.calls().beam_select(logits, scores, k)
     if done is not None:
